@@ -312,6 +312,45 @@ int ckan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int6
                    double lr, double beta1, double beta2, double eps, double weight_decay,
                    void* stream);
 
+/* ---- mixture of experts: routing -------------------------------------------- */
+/* Rows of logits choose top_k of `experts` experts each.
+ *   s = softmax(l) or sigmoid(l);  key = s + bias (bias may be NULL).
+ *   An expert with logit -inf or NaN (or a NaN key) is not eligible: s = 0.
+ *   groups > 1: the experts are `groups` equal runs; a group's value is the sum of
+ *   its two largest keys (a missing or ineligible second counts 0), and only the
+ *   top_groups groups of largest value stay.
+ *   The top_k largest keys among them are chosen, in falling order.  Equal keys
+ *   or values: the lowest index first.
+ *   weights = scale * s_j / (sum of the chosen s + 1e-20) with renormalize,
+ *   scale * s_j without.  The bias moves the choice only, not the weights.
+ * A row with fewer than top_k eligible experts fills up with index -1, weight 0.
+ * No counterpart in the reference (its models are single layers and stacks). */
+typedef enum ckan_score {
+  CKAN_SCORE_SOFTMAX = 0,
+  CKAN_SCORE_SIGMOID = 1
+} ckan_score;
+
+typedef struct ckan_route_desc {
+  int64_t rows;         /* >= 0                                           */
+  int64_t logits_ld;    /* elements from a row of logits to the next      */
+  int32_t experts;      /* 1..512                                         */
+  int32_t top_k;        /* 1..64, at most the experts of top_groups groups */
+  int32_t score;        /* ckan_score                                     */
+  int32_t groups;       /* 1..64, divides experts                         */
+  int32_t top_groups;   /* 1..groups                                      */
+  int32_t renormalize;  /* 0 or 1                                         */
+  int32_t dtype;        /* ckan_dtype of logits and dlogits               */
+  float scale;
+} ckan_route_desc;
+
+/* weights [rows, top_k] fp32, indices [rows, top_k]; scores in fp32. */
+int ckan_route(const ckan_route_desc* desc, const void* logits, const float* bias, float* weights,
+               int64_t* indices, void* stream);
+/* dlogits [rows, experts] (dense rows, in the logits' dtype) from dweights
+ * [rows, top_k]; `indices` are ckan_route's.  No gradient goes through the choice. */
+int ckan_route_backward(const ckan_route_desc* desc, const void* logits, const int64_t* indices,
+                        const float* dweights, void* dlogits, void* stream);
+
 /* ---- resident multi-layer executor ---------------------------------------- */
 /* A stack of ChebyKAN layers (KANSequential, kan/layers/base.py:144-166)
  * trained in place on one GPU: the executor owns fp32 master coefficients,

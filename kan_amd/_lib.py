@@ -170,6 +170,32 @@ SIGNATURES.update({
     "ckan_exec_steps": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _vp]),
 })
 
+
+CKAN_SCORE_SOFTMAX = 0
+CKAN_SCORE_SIGMOID = 1
+
+
+class CkanRouteDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("logits_ld", ctypes.c_int64),
+        ("experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("score", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("top_groups", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+_proute = ctypes.POINTER(CkanRouteDesc)
+SIGNATURES.update({
+    "ckan_route": (ctypes.c_int, [_proute, _vp, _vp, _vp, _vp, _vp]),
+    "ckan_route_backward": (ctypes.c_int, [_proute, _vp, _vp, _vp, _vp, _vp]),
+})
+
 _lib = None
 _lock = threading.Lock()
 

@@ -1,0 +1,259 @@
+// Routing of rows to experts and its gradient (ckan_route, ckan_route_backward).
+//
+// A row of logits l[0..E) gives scores s (softmax or sigmoid), selection keys
+// s + bias, optionally a choice of whole groups of experts by the sum of their
+// two largest keys, the top_k largest keys among the kept groups (ties to the
+// lowest index), and the chosen experts' weights.  One wave takes one row: lane
+// j holds the J = ceil(E / 64) consecutive experts from j J on in registers, so
+// a row is read once and the lowest index among equal keys is the lowest lane's
+// lowest register.
+#include <float.h>
+#include <math.h>
+
+#include "ckan_kernels.hpp"
+#include "ckan_mix.hpp"
+
+namespace ckan {
+namespace {
+
+constexpr int kRowsPerBlock = 4;  // one wave a row
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
+  return v;
+}
+
+// The scores of a row in registers: s[q] of expert lane * J + q, 0 for an
+// expert that is not eligible (logit -inf or NaN) or past E.  The softmax's
+// exponentials are summed in 64 bits and the sum rounded once to 32: the score
+// of an expert then does not depend on the order of the sum, and keys that are
+// near one another compare the same way wherever the row is computed.
+template <int J>
+__device__ __forceinline__ void row_scores(const float (&l)[J], int softmax, float (&s)[J]) {
+  if (softmax) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < J; ++q) m = fmaxf(m, l[q]);
+    m = fmaxf(wave_max(m), -FLT_MAX);
+    double sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < J; ++q) {
+      s[q] = expf(l[q] - m);
+      sum += (double)s[q];
+    }
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) sum += __shfl_xor(sum, w);
+    const float total = (float)sum;
+#pragma unroll
+    for (int q = 0; q < J; ++q) s[q] = total > 0.0f ? s[q] / total : 0.0f;
+  } else {
+#pragma unroll
+    for (int q = 0; q < J; ++q) s[q] = 1.0f / (1.0f + expf(-l[q]));
+  }
+}
+
+template <int J, typename T>
+__device__ __forceinline__ void row_logits(const T* row, int E, int lane, float (&l)[J]) {
+#pragma unroll
+  for (int q = 0; q < J; ++q) {
+    const int e = lane * J + q;
+    const float v = e < E ? (float)row[e] : -INFINITY;
+    l[q] = v > -INFINITY ? v : -INFINITY;  // NaN: not eligible
+  }
+}
+
+template <int J, typename T>
+__global__ __launch_bounds__(64 * kRowsPerBlock) void k_route(RouteArgs a) {
+  extern __shared__ float sm[];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + wave;
+  if (row >= a.rows) return;  // no block-wide barrier below: each wave keeps to its own LDS
+  float l[J], s[J], key[J];
+  row_logits<J>((const T*)a.logits + row * a.ld, a.E, lane, l);
+  row_scores<J>(l, a.softmax, s);
+#pragma unroll
+  for (int q = 0; q < J; ++q) {
+    const int e = lane * J + q;
+    float k = -INFINITY;
+    if (l[q] > -INFINITY) {
+      k = a.bias ? s[q] + a.bias[e] : s[q];
+      k = k > -INFINITY ? k : -INFINITY;  // a NaN bias: not eligible
+    }
+    key[q] = k;
+  }
+  if (a.groups > 1) {
+    // lane (g, u) of LG lanes a group takes every LG-th key of group g for the
+    // group's two largest, then the lanes of a group merge theirs
+    float* keys = sm + wave * (64 * J + 64);
+    float* kept = keys + 64 * J;
+#pragma unroll
+    for (int q = 0; q < J; ++q) keys[lane * J + q] = key[q];
+    __builtin_amdgcn_wave_barrier();
+    const int G = a.groups, size = a.E / G;
+    int LG = 64;
+    while (LG * G > 64) LG >>= 1;
+    const int g = lane / LG, u = lane % LG;
+    float b1 = -INFINITY, b2 = -INFINITY;
+    if (g < G)
+      for (int e = u; e < size; e += LG) {
+        const float k = keys[g * size + e];
+        b2 = fmaxf(b2, fminf(b1, k));
+        b1 = fmaxf(b1, k);
+      }
+    for (int w = 1; w < LG; w <<= 1) {
+      const float o1 = __shfl_xor(b1, w), o2 = __shfl_xor(b2, w);
+      b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+      b1 = fmaxf(b1, o1);
+    }
+    const float value = b1 + (b2 > -INFINITY ? b2 : 0.0f);
+    int ahead = 0;  // groups before this one in the order of the choice
+    for (int h = 0; h < G; ++h) {
+      const float v = __shfl(value, h * LG);
+      ahead += v > value || (v == value && h < g);
+    }
+    if (g < G && u == 0) kept[g] = ahead < a.top_groups ? 1.0f : 0.0f;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < J; ++q) {
+      const int e = lane * J + q;
+      if (e < a.E && kept[e / size] == 0.0f) key[q] = -INFINITY;
+    }
+  }
+  // top_k rounds: the largest key left, then its lowest index
+  int mine = -1;      // lane j: the j-th chosen expert
+  float chosen = 0.0f;
+  for (int j = 0; j < a.top_k; ++j) {
+    float best = key[0];
+#pragma unroll
+    for (int q = 1; q < J; ++q) best = fmaxf(best, key[q]);
+    best = wave_max(best);
+    if (!(best > -INFINITY)) break;  // uniform: no eligible expert is left
+    int at = J;
+    float score = 0.0f;
+#pragma unroll
+    for (int q = J - 1; q >= 0; --q)
+      if (key[q] == best) {
+        at = q;
+        score = s[q];
+      }
+    const int from = __ffsll((unsigned long long)__ballot(at < J)) - 1;
+    const int e = __shfl(lane * J + at, from);
+    score = __shfl(score, from);
+    if (lane == j) {
+      mine = e;
+      chosen = score;
+    }
+    if (lane == from) {
+#pragma unroll
+      for (int q = 0; q < J; ++q)
+        if (q == at) key[q] = -INFINITY;
+    }
+  }
+  float w = chosen;
+  if (a.renormalize) w = chosen / (wave_sum(chosen) + kRouteEps);
+  if (a.scale != 1.0f) w *= a.scale;
+  if (lane < a.top_k) {
+    a.weights[row * a.top_k + lane] = w;
+    a.indices[row * a.top_k + lane] = mine;
+  }
+}
+
+// dlogits of a row from the chosen experts' weight gradients.  The scores are
+// computed again from the logits (reading them twice costs less than keeping a
+// [rows, E] tensor).  With r = sum over the chosen of s ds: softmax
+// dl = s (ds - r), sigmoid dl = s (1 - s) ds, ds being 0 off the chosen.
+template <int J, typename T>
+__global__ __launch_bounds__(64 * kRowsPerBlock) void k_route_backward(RouteArgs a) {
+  extern __shared__ float sm[];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + wave;
+  if (row >= a.rows) return;
+  float* lds = sm + wave * (64 * J);
+  float l[J], s[J];
+  row_logits<J>((const T*)a.logits + row * a.ld, a.E, lane, l);
+  row_scores<J>(l, a.softmax, s);
+#pragma unroll
+  for (int q = 0; q < J; ++q) lds[lane * J + q] = s[q];
+  __builtin_amdgcn_wave_barrier();
+  int64_t e = -1;
+  float sj = 0.0f, dw = 0.0f;
+  if (lane < a.top_k) {
+    e = a.indices[row * a.top_k + lane];
+    if (e >= 0 && e < a.E) {
+      sj = lds[e];
+      dw = a.dweights[row * a.top_k + lane];
+    } else {
+      e = -1;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  float ds, r = 0.0f;
+  if (a.renormalize) {
+    const float total = wave_sum(sj) + kRouteEps;
+    const float mean = wave_sum(dw * sj) / total;
+    ds = a.scale * (dw - mean) / total;
+    r = a.scale * mean * (kRouteEps / total);  // sum s ds, of which total leaves this
+  } else {
+    ds = a.scale * dw;
+    r = wave_sum(sj * ds);
+  }
+  // the chosen experts' ds to the lanes that hold them
+#pragma unroll
+  for (int q = 0; q < J; ++q) lds[lane * J + q] = 0.0f;
+  __builtin_amdgcn_wave_barrier();
+  if (e >= 0) lds[e] = ds;
+  __builtin_amdgcn_wave_barrier();
+  T* out = (T*)a.dlogits + row * a.E;
+#pragma unroll
+  for (int q = 0; q < J; ++q) {
+    const int i = lane * J + q;
+    if (i >= a.E) continue;
+    const float d = lds[i];
+    float v;
+    if (a.softmax) {
+      v = s[q] * (d - r);
+    } else {
+      // s (1 - s) without the cancellation of 1 - s near s = 1
+      const float x = expf(-fabsf(l[q]));
+      v = l[q] > -INFINITY ? x / ((1.0f + x) * (1.0f + x)) * d : 0.0f;
+    }
+    out[i] = (T)v;
+  }
+}
+
+template <typename T>
+void launch_typed(const RouteArgs& a, bool backward, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(a.rows, kRowsPerBlock)), block(64 * kRowsPerBlock);
+  const int J = (a.E + 63) / 64;
+#define CKAN_ROUTE_CASE(N)                                                                     \
+  if (J <= N) {                                                                                \
+    const size_t lds = (size_t)kRowsPerBlock * (64 * N + (backward ? 0 : 64)) * sizeof(float); \
+    if (backward)                                                                              \
+      hipLaunchKernelGGL((k_route_backward<N, T>), grid, block, lds, st, a);                   \
+    else                                                                                       \
+      hipLaunchKernelGGL((k_route<N, T>), grid, block, a.groups > 1 ? lds : 0, st, a);         \
+    return;                                                                                    \
+  }
+  CKAN_ROUTE_CASE(1)
+  CKAN_ROUTE_CASE(2)
+  CKAN_ROUTE_CASE(4)
+  CKAN_ROUTE_CASE(8)
+#undef CKAN_ROUTE_CASE
+}
+
+}  // namespace
+
+void launch_route(const RouteArgs& a, bool backward, hipStream_t st) {
+  if (a.bf16)
+    launch_typed<__bf16>(a, backward, st);
+  else
+    launch_typed<float>(a, backward, st);
+}
+
+}  // namespace ckan

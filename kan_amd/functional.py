@@ -529,3 +529,6 @@ def jacobian(x: torch.Tensor, coeffs: torch.Tensor, spec, affine=None) -> torch.
     _lib.check(lib.ckan_jacobian(desc, _spec_ref(spec), x32.data_ptr(), c.data_ptr(),
                                  jac.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(x.device)))
     return jac
+
+
+from .mixture import route  # noqa: E402  (a public operator of this namespace)
