@@ -351,6 +351,42 @@ int ckan_route(const ckan_route_desc* desc, const void* logits, const float* bia
 int ckan_route_backward(const ckan_route_desc* desc, const void* logits, const int64_t* indices,
                         const float* dweights, void* dlogits, void* stream);
 
+/* ---- orthogonalised updates ---------------------------------------------------- */
+/* Newton-Schulz orthogonalisation of a batch of matrices G [rows, cols]:
+ *   X = G / (|G|_F + eps), then `steps` times
+ *   X = a X + (b A + c A^2) X with A = X X^T (X^T X for rows > cols).
+ * Products run on two fp16 planes an operand (22 bits) with fp32 sums; the
+ * norm is summed in fp64.  The coefficients' B = b A + c A^2 has to stay below 15 for
+ * singular values in [0, 1] over all steps (checked on the host).
+ * Element (r, col) of matrix i lies at i batch_stride + r row_stride +
+ * (col / inner) outer_stride + (col % inner) inner_stride elements; inner divides
+ * cols.  An ordinary matrix has inner = 1 and its column stride in outer_stride.  A
+ * ChebyKAN layer's coefficients [in, out, D] as [out, in D], the matrix by which
+ * the basis values act on the outputs, have inner = D, row_stride = D,
+ * outer_stride = out D, inner_stride = 1.  Replaces nothing in the reference, whose
+ * training loop uses torch's optimizers (README.md:59-69). */
+typedef struct ckan_ortho_desc {
+  int64_t batch_stride, row_stride, outer_stride, inner_stride;
+  int32_t batch;       /* 0..65535                                       */
+  int32_t rows, cols;  /* >= 1; the smaller at most 16384                */
+  int32_t inner;       /* >= 1, divides cols                             */
+  int32_t steps;       /* 0..100                                         */
+  int32_t dtype;       /* ckan_dtype of in and out; fp32 for the Muon step */
+  float a, b, c, eps;  /* eps >= 0                                       */
+} ckan_ortho_desc;
+
+size_t ckan_orthogonalize_workspace_bytes(const ckan_ortho_desc* desc);
+/* out = the orthogonalised in; both in the descriptor's layout (they may be the same). */
+int ckan_orthogonalize(const ckan_ortho_desc* desc, const void* in, void* out, void* ws, size_t ws_bytes,
+                       void* stream);
+/* One step of Muon on parameters p with gradient g and momentum buf (fp32, all in
+ * the descriptor's layout, p and buf updated in place):
+ *   buf = momentum buf + (1 - momentum) g
+ *   u = nesterov ? (1 - momentum) g + momentum buf : buf
+ *   p = (1 - lr weight_decay) p - lr scale O(u),   O the orthogonalisation above. */
+int ckan_muon_step(const ckan_ortho_desc* desc, float* p, const float* g, float* buf, float lr, float momentum,
+                   float weight_decay, float scale, int nesterov, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- resident multi-layer executor ---------------------------------------- */
 /* A stack of ChebyKAN layers (KANSequential, kan/layers/base.py:144-166)
  * trained in place on one GPU: the executor owns fp32 master coefficients,

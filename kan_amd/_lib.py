@@ -196,6 +196,34 @@ SIGNATURES.update({
     "ckan_route_backward": (ctypes.c_int, [_proute, _vp, _vp, _vp, _vp, _vp]),
 })
 
+
+class CkanOrthoDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch_stride", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64),
+        ("inner_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("cols", ctypes.c_int32),
+        ("inner", ctypes.c_int32),
+        ("steps", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+_portho = ctypes.POINTER(CkanOrthoDesc)
+SIGNATURES.update({
+    "ckan_orthogonalize_workspace_bytes": (_sz, [_portho]),
+    "ckan_orthogonalize": (ctypes.c_int, [_portho, _vp, _vp, _vp, _sz, _vp]),
+    "ckan_muon_step": (ctypes.c_int, [_portho, _vp, _vp, _vp, _f32, _f32, _f32, _f32, ctypes.c_int,
+                                      _vp, _sz, _vp]),
+})
+
 _lib = None
 _lock = threading.Lock()
 

@@ -68,9 +68,112 @@ int route_args(const ckan_route_desc* d, RouteArgs* a) {
   return CKAN_OK;
 }
 
+// The largest |b s^2 + c s^4| that the iteration's matrix B can reach from
+// singular values in [0, 1], over all steps, by sampling the interval.
+double ortho_reach(const ckan_ortho_desc* d) {
+  double top = 1.0, most = 0.0;
+  for (int s = 0; s < d->steps && most < 1e6; ++s) {
+    double next = 0.0;
+    for (int i = 0; i <= 1024; ++i) {
+      const double x = top * i / 1024, y = x * x, bv = d->b * y + d->c * y * y;
+      most = fmax(most, fabs(bv));
+      next = fmax(next, fabs(x * (d->a + bv)));
+    }
+    top = fmax(next, 1e-30);
+  }
+  return fmax(most, 2.0 * top * top);  // A = X X^T has to fit with it
+}
+
+int ortho_check(const ckan_ortho_desc* d) {
+  if (!d) return fail(CKAN_ERR_INVALID_ARG, "ortho desc is NULL");
+  if (d->batch < 0 || d->batch > 65535)
+    return fail(CKAN_ERR_INVALID_ARG, "batch must lie in [0, 65535] (got %d)", d->batch);
+  if (d->rows < 1 || d->cols < 1)
+    return fail(CKAN_ERR_INVALID_ARG, "rows and cols must be >= 1 (got %d, %d)", d->rows, d->cols);
+  const int m = d->rows < d->cols ? d->rows : d->cols, n = d->rows < d->cols ? d->cols : d->rows;
+  if (m > 16384) return fail(CKAN_ERR_UNSUPPORTED, "the smaller dimension above 16384 is not supported (got %d)", m);
+  if (n > (1 << 24)) return fail(CKAN_ERR_UNSUPPORTED, "dimensions above 2^24 are not supported (got %d)", n);
+  if (d->inner < 1 || d->cols % d->inner)
+    return fail(CKAN_ERR_INVALID_ARG, "inner must divide cols %d (got %d)", d->cols, d->inner);
+  if (d->batch_stride < 0 || d->row_stride < 0 || d->outer_stride < 0 || d->inner_stride < 0)
+    return fail(CKAN_ERR_INVALID_ARG, "strides must be >= 0");
+  if (d->steps < 0 || d->steps > 100) return fail(CKAN_ERR_INVALID_ARG, "steps must lie in [0, 100] (got %d)", d->steps);
+  if (d->dtype != CKAN_DTYPE_F32 && d->dtype != CKAN_DTYPE_BF16)
+    return fail(CKAN_ERR_INVALID_ARG, "unknown dtype %d", d->dtype);
+  if (!isfinite(d->a) || !isfinite(d->b) || !isfinite(d->c) || !(d->eps >= 0.0f) || !isfinite(d->eps))
+    return fail(CKAN_ERR_INVALID_ARG, "the coefficients and eps must be finite, eps >= 0");
+  if (!(ortho_reach(d) < 15.0))
+    return fail(CKAN_ERR_UNSUPPORTED, "coefficients (%g, %g, %g) leave the products' range within %d steps", d->a,
+                d->b, d->c, d->steps);
+  return CKAN_OK;
+}
+
+OrthoArgs ortho_args(const ckan_ortho_desc* d) {
+  OrthoArgs a{};
+  a.batch = d->batch;
+  a.rows = d->rows;
+  a.cols = d->cols;
+  a.steps = d->steps;
+  a.a = d->a;
+  a.b = d->b;
+  a.c = d->c;
+  a.eps = d->eps;
+  a.bf16 = d->dtype == CKAN_DTYPE_BF16;
+  a.view = MatView{d->batch_stride, d->row_stride, d->outer_stride, d->inner_stride, d->inner};
+  return a;
+}
+
+int ortho_ws(const ckan_ortho_desc* d, void* ws, size_t ws_bytes) {
+  const size_t need = ortho_workspace_bytes(d->batch, d->rows, d->cols);
+  if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!ws || !is_al16(ws)) return fail(CKAN_ERR_INVALID_ARG, "workspace is NULL or not 16-byte aligned");
+  return CKAN_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t ckan_orthogonalize_workspace_bytes(const ckan_ortho_desc* desc) {
+  return ortho_check(desc) ? 0 : ortho_workspace_bytes(desc->batch, desc->rows, desc->cols);
+}
+
+int ckan_orthogonalize(const ckan_ortho_desc* desc, const void* in, void* out, void* ws, size_t ws_bytes,
+                       void* stream) {
+  if (const int rc = ortho_check(desc)) return rc;
+  if (desc->batch == 0) return CKAN_OK;
+  if (!in || !out) return fail(CKAN_ERR_INVALID_ARG, "orthogonalize: NULL pointer");
+  if (const int rc = ortho_ws(desc, ws, ws_bytes)) return rc;
+  OrthoArgs a = ortho_args(desc);
+  a.in = in;
+  a.out = out;
+  launch_ortho(a, ws, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("orthogonalize");
+}
+
+int ckan_muon_step(const ckan_ortho_desc* desc, float* p, const float* g, float* buf, float lr, float momentum,
+                   float weight_decay, float scale, int nesterov, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = ortho_check(desc)) return rc;
+  if (desc->dtype != CKAN_DTYPE_F32) return fail(CKAN_ERR_INVALID_ARG, "muon_step: fp32 only");
+  if (!(momentum >= 0.0f && momentum < 1.0f))
+    return fail(CKAN_ERR_INVALID_ARG, "momentum must lie in [0, 1) (got %g)", momentum);
+  if (!isfinite(lr) || !isfinite(weight_decay) || !isfinite(scale))
+    return fail(CKAN_ERR_INVALID_ARG, "lr, weight_decay and scale must be finite");
+  if (desc->batch == 0) return CKAN_OK;
+  if (!p || !g || !buf) return fail(CKAN_ERR_INVALID_ARG, "muon_step: NULL pointer");
+  if (const int rc = ortho_ws(desc, ws, ws_bytes)) return rc;
+  OrthoArgs a = ortho_args(desc);
+  a.p = p;
+  a.g = g;
+  a.buf = buf;
+  a.lr = lr;
+  a.momentum = momentum;
+  a.decay = weight_decay;
+  a.scale = scale;
+  a.nesterov = nesterov != 0;
+  launch_ortho(a, ws, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("muon_step");
+}
 
 int ckan_route(const ckan_route_desc* desc, const void* logits, const float* bias, float* weights,
                int64_t* indices, void* stream) {

@@ -531,4 +531,6 @@ def jacobian(x: torch.Tensor, coeffs: torch.Tensor, spec, affine=None) -> torch.
     return jac
 
 
-from .mixture import route  # noqa: E402  (a public operator of this namespace)
+# public operators of this namespace that live in modules of their own
+from .mixture import route  # noqa: E402
+from .orthogonal import orthogonalize  # noqa: E402

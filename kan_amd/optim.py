@@ -1,8 +1,9 @@
-"""Fused SGD and Adam steps for device parameters.
+"""Fused SGD and Adam steps for device parameters, and Muon for matrices.
 
-Both follow torch.optim's single-tensor update order (torch/optim/sgd.py,
+SGD and Adam follow torch.optim's single-tensor update order (torch/optim/sgd.py,
 torch/optim/adam.py), which the reference's training loop uses
-(README.md:58-66), and run as one HIP kernel per parameter tensor.  Only
+(README.md:58-66), and run as one HIP kernel per parameter tensor.  Muon's
+update is the orthogonalised momentum of each coefficient matrix.  Only
 fp32 contiguous ROCm-device parameters are accepted.
 """
 from __future__ import annotations
@@ -13,6 +14,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
+from .orthogonal import NS_COEFFICIENTS, matrix_shape, muon_step_
 
 
 def _check_param(p: torch.Tensor) -> None:
@@ -97,4 +99,48 @@ class Adam(torch.optim.Optimizer):
                     float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]),
                     _lib.stream_ptr(p.device)))
                 increment_version(p)  # written through its pointer (see SGD.step)
+        return loss
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum orthogonalised by Newton-Schulz products (``muon_step_``).
+
+    Takes [rows, cols] weights, ChebyKAN coefficients [in, out, degree+1] (each as
+    the matrix [out, in (degree+1)]) and experts' [E, in, out, degree+1]; anything
+    else raises ValueError at construction: give biases and gains to another
+    optimizer."""
+
+    def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5,
+                 coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7):
+        if lr < 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"Invalid momentum: {momentum}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, coefficients=coefficients, eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                matrix_shape(p.shape)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                _check_param(p)
+                st = self.state[p]
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p)
+                buf = st["momentum_buffer"]
+                if buf.device != p.device or not buf.is_contiguous():
+                    st["momentum_buffer"] = buf = buf.to(p.device, torch.float32).contiguous()
+                muon_step_(p, p.grad.contiguous(), buf, lr=group["lr"], momentum=group["momentum"],
+                           nesterov=group["nesterov"], weight_decay=group["weight_decay"],
+                           steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
         return loss

@@ -64,3 +64,37 @@ def route_backward(logits, idx, dw, score="softmax", renormalize=True, scale=1.0
     if score == "sigmoid":
         return ds * s * (1 - s)
     return s * (ds - (s * ds).sum(1, keepdims=True))
+
+
+def orthogonalize(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Newton-Schulz by its definition on one matrix [rows, cols]."""
+    a, b, c = coefficients
+    x = np.asarray(g, dtype=np.float64)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    x = x / (np.sqrt((x * x).sum()) + eps)
+    for _ in range(steps):
+        gram = x @ x.T
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    return x.T if tall else x
+
+
+def coeff_matrix(c):
+    """[in, out, D] coefficients as [out, in D]."""
+    c = np.asarray(c)
+    return c.transpose(1, 0, 2).reshape(c.shape[1], -1)
+
+
+def muon_step(p, g, buf, lr, momentum=0.95, nesterov=True, weight_decay=0.0, **kw):
+    """(p, buf) after a step; p a matrix [rows, cols] or coefficients [in, out, D]."""
+    p, g, buf = (np.asarray(v, dtype=np.float64) for v in (p, g, buf))
+    buf = momentum * buf + (1 - momentum) * g
+    u = (1 - momentum) * g + momentum * buf if nesterov else buf
+    if p.ndim == 3:
+        i, o, d = p.shape
+        up = orthogonalize(coeff_matrix(u), **kw).reshape(o, i, d).transpose(1, 0, 2)
+        ratio = o / (i * d)
+    else:
+        up = orthogonalize(u, **kw)
+        ratio = p.shape[0] / p.shape[1]
+    return p * (1 - lr * weight_decay) - lr * np.sqrt(max(1.0, ratio)) * up, buf
