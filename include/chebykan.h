@@ -351,6 +351,40 @@ int ckan_route(const ckan_route_desc* desc, const void* logits, const float* bia
 int ckan_route_backward(const ckan_route_desc* desc, const void* logits, const int64_t* indices,
                         const float* dweights, void* dlogits, void* stream);
 
+/* ---- mixture of experts: the experts' products -------------------------------------- */
+/* y[t] = sum_j w[t, j] f_e(x[t]) with e = indices[t, j] and expert e's ChebyKAN layer
+ *   f_e(x)[o] = sum_{i, d} T_d(tanh x_i) C[e, i, o, d]   (kan/layers/chebykan.py:64-67).
+ * x [rows, in], y [rows, out], coeffs [experts, in, out, degree + 1] in `dtype`,
+ * weights [rows, top_k] in `wdtype`, indices int64 [rows, top_k].  A slot whose index
+ * lies outside [0, experts) has no expert: it adds nothing and its weight's
+ * gradient is 0.  A row may name an expert twice.
+ * fp32 tensors are computed on two fp16 planes an operand (22 bits), bf16 ones on
+ * one (11 bits); sums, tanh and the basis recurrence are in fp32.
+ * `saved` (ckan_experts_saved_bytes) carries the sorted slots, tanh values, expert
+ * outputs and packed coefficients from the forward to its backward; NULL where no
+ * backward follows.  Buffers need 16-byte alignment. */
+typedef struct ckan_experts_desc {
+  int64_t rows;      /* >= 0; rows * top_k at most 2^29            */
+  int32_t experts;   /* 1..512                                     */
+  int32_t top_k;     /* 1..64                                      */
+  int32_t in_dim;    /* 1..65536                                   */
+  int32_t out_dim;   /* 1..65536                                   */
+  int32_t degree;    /* 1..16                                      */
+  int32_t dtype;     /* ckan_dtype of x, coeffs, y, dy, dx, dcoeffs */
+  int32_t wdtype;    /* ckan_dtype of weights and dweights         */
+} ckan_experts_desc;
+
+size_t ckan_experts_saved_bytes(const ckan_experts_desc* desc);
+/* Workspace of the forward (backward == 0; without_saved != 0 when saved is NULL) or the backward. */
+size_t ckan_experts_workspace_bytes(const ckan_experts_desc* desc, int backward, int without_saved);
+int ckan_experts_forward(const ckan_experts_desc* desc, const void* x, const void* coeffs, const int64_t* indices,
+                         const void* weights, void* y, void* saved, void* ws, size_t ws_bytes, void* stream);
+/* dx [rows, in], dcoeffs (as coeffs; zero for experts without rows), dweights
+ * [rows, top_k] from dy [rows, out]; each may be NULL. */
+int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices, const void* weights, void* saved,
+                          const void* dy, void* dx, void* dcoeffs, void* dweights, void* ws, size_t ws_bytes,
+                          void* stream);
+
 /* ---- orthogonalised updates ---------------------------------------------------- */
 /* Newton-Schulz orthogonalisation of a batch of matrices G [rows, cols]:
  *   X = G / (|G|_F + eps), then `steps` times

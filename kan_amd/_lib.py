@@ -197,6 +197,28 @@ SIGNATURES.update({
 })
 
 
+class CkanExpertsDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("out_dim", ctypes.c_int32),
+        ("degree", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("wdtype", ctypes.c_int32),
+    ]
+
+
+_pexperts = ctypes.POINTER(CkanExpertsDesc)
+SIGNATURES.update({
+    "ckan_experts_saved_bytes": (_sz, [_pexperts]),
+    "ckan_experts_workspace_bytes": (_sz, [_pexperts, ctypes.c_int, ctypes.c_int]),
+    "ckan_experts_forward": (ctypes.c_int, [_pexperts, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ckan_experts_backward": (ctypes.c_int, [_pexperts, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+})
+
+
 class CkanOrthoDesc(ctypes.Structure):
     _fields_ = [
         ("batch_stride", ctypes.c_int64),

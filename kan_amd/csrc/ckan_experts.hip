@@ -1,0 +1,849 @@
+// The products of a mixture of ChebyKAN experts, forward and backward.
+//
+//   y[t] = sum_j w[t, j] f_e(x[t]),  e = idx[t, j],  f_e(x) = sum_{i, d} T_d(tanh x_i) C_e[i, :, d].
+//
+// The slots (t, j) are sorted by expert on the device, each expert's run padded to
+// 32 rows, so one launch a product covers every expert and nothing is read back
+// by the host.  All three products run on fp16 planes (ckan_planes.hpp): one
+// plane for bf16 tensors (the basis values then carry 11 bits, more than a bf16
+// result), two for fp32.  fp16's range is met by one power-of-two scale an
+// expert for the coefficients and one for the upstream gradients; the basis
+// values lie in [-1, 1].
+//
+//   forward  z[row, o] = sum_k phi[row, k] Cf[o, k]: phi is made in registers from
+//            the row's tanh values, k = (input, degree 1..P); T_0 is a bias.
+//   dx       per row and input the degrees' sums over o of g[row, o] d C[i, o, d]
+//            stand in separate accumulators; the epilogue weights them by
+//            U_{d-1}(t) (1 - t^2).
+//   dC       sum over rows of T_d(t) g: phi is made into LDS, k = the rows.
+#include <float.h>
+#include <math.h>
+
+#include "ckan_mix.hpp"
+#include "ckan_planes.hpp"
+
+namespace ckan {
+
+ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bool bf16, bool wbf16) {
+  ExpertsPlan p{};
+  p.T = T;
+  p.S = T * k;
+  p.E = E;
+  p.k = k;
+  p.I = I;
+  p.O = O;
+  p.deg = deg;
+  p.D = deg + 1;
+  p.P = deg <= 4 ? 4 : deg <= 8 ? 8 : 16;
+  p.NP = bf16 ? 1 : 2;
+  p.bf16 = bf16;
+  p.wbf16 = wbf16;
+  p.Ip = (int)round_up(I, 32);
+  p.Op = (int)round_up(O, 32);
+  p.R = round_up(p.S + (int64_t)31 * (E < p.S ? E : p.S), 128) + 128;
+  p.tiles = (int)(ceil_div(p.S, 128) + (E < p.S ? E : p.S));
+  p.plan_chunk = round_up(ceil_div(p.S, kPlanBlocks), kPlanThreads);
+  p.plan_blocks = (int)ceil_div(p.S, p.plan_chunk);
+  p.grad_blocks = ceil_div(p.R, 32) < kGradBlocks ? ceil_div(p.R, 32) : kGradBlocks;
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off = align256(off + n);
+    return at;
+  };
+  p.off_off = take((size_t)(E + 1) * 4);
+  p.tok_off = take((size_t)p.R * 4);
+  p.slot_off = take((size_t)p.R * 4);
+  p.row_off = take((size_t)p.S * 4);
+  p.tiles_off = take((size_t)p.tiles * 8);
+  p.scale_off = take((size_t)E * 4);
+  p.t_off = take((size_t)p.T * p.Ip * 4);
+  p.z_off = take((size_t)p.R * O * 4);
+  p.cb_off = take((size_t)E * p.Ip * deg * p.Op * 2 * p.NP);
+  p.saved_bytes = off;
+  off = 0;
+  p.bias_parts = (int)ceil_div(p.Ip, 256);
+  p.hist_off = take((size_t)p.plan_blocks * E * 4);
+  p.cmax_off = take((size_t)E * kMaxParts * 4);
+  p.cf_off = take((size_t)E * p.Op * p.Ip * p.P * 2 * p.NP);
+  p.bias_off = take((size_t)p.bias_parts * E * p.Op * 4);
+  p.fwd_bytes = off;
+  off = 0;
+  p.gmax_off = take((size_t)p.grad_blocks * E * 4);
+  p.gscale_off = take((size_t)E * 4);
+  p.gr_off = take((size_t)p.R * p.Op * 2 * p.NP);
+  p.gt_off = take((size_t)p.R * p.Op * 2 * p.NP);
+  p.gsum_off = take((size_t)(p.R / 32) * p.Op * 4);
+  p.dxs_off = take((size_t)p.R * I * 4);
+  p.bwd_bytes = off;
+  return p;
+}
+
+namespace {
+
+// ---- the plan: slots sorted by expert ----------------------------------------
+
+__device__ __forceinline__ int slot_expert(const ExpertsArgs& a, int64_t s) {
+  const int64_t e = a.indices[s];
+  return e >= 0 && e < a.p.E ? (int)e : -1;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_plan_count(ExpertsArgs a) {
+  __shared__ int count[kExpertsMax];
+  const ExpertsPlan& p = a.p;
+  for (int e = threadIdx.x; e < p.E; e += kPlanThreads) count[e] = 0;
+  __syncthreads();
+  const int64_t s0 = blockIdx.x * p.plan_chunk;
+  for (int64_t s = s0 + threadIdx.x; s < s0 + p.plan_chunk && s < p.S; s += kPlanThreads) {
+    const int e = slot_expert(a, s);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  int* hist = (int*)(a.ws + p.hist_off) + (size_t)blockIdx.x * p.E;
+  for (int e = threadIdx.x; e < p.E; e += kPlanThreads) hist[e] = count[e];
+}
+
+// Each block scans the counts again (a few kilobytes from the L2) instead of
+// waiting for a launch that does, then places its own slots: within a wave
+// by the lanes before it of the same expert (one ballot a bit of the number),
+// among the waves of the block by their counts.  The order within an expert is
+// the slots' order, whatever the blocks' timing.
+__global__ __launch_bounds__(kPlanThreads) void k_plan_place(ExpertsArgs a) {
+  constexpr int kWaves = kPlanThreads / 64;
+  __shared__ int next[kExpertsMax], scan[2][kExpertsMax], wave_count[kWaves][kExpertsMax];
+  const ExpertsPlan& p = a.p;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int* hist = (const int*)(a.ws + p.hist_off);
+  int total = 0, before = 0;
+  if (tid < p.E)
+    for (int b = 0; b < p.plan_blocks; ++b) {
+      const int h = hist[(size_t)b * p.E + tid];
+      total += h;
+      if (b < (int)blockIdx.x) before += h;
+    }
+  const int padded = (total + 31) / 32 * 32, ntiles = (total + 127) / 128;
+  int sum[2] = {padded, ntiles};  // inclusive sums over the experts of rows and of tiles
+  for (int which = 0; which < 2; ++which) {
+    if (tid < kExpertsMax) scan[0][tid] = tid < p.E ? sum[which] : 0;
+    __syncthreads();
+    int cur = 0;
+    for (int w = 1; w < p.E; w <<= 1) {
+      if (tid < kExpertsMax) scan[cur ^ 1][tid] = scan[cur][tid] + (tid >= w ? scan[cur][tid - w] : 0);
+      __syncthreads();
+      cur ^= 1;
+    }
+    if (tid < p.E) sum[which] = scan[cur][tid];
+    __syncthreads();
+  }
+  int* off = (int*)(a.saved + p.off_off);
+  int* tok = (int*)(a.saved + p.tok_off);
+  int* slot = (int*)(a.saved + p.slot_off);
+  int* row = (int*)(a.saved + p.row_off);
+  if (tid < p.E) {
+    next[tid] = sum[0] - padded + before;
+    if (blockIdx.x == 0) {
+      off[tid + 1] = sum[0];
+      if (tid == 0) off[0] = 0;
+      for (int r = sum[0] - padded + total; r < sum[0]; ++r) tok[r] = slot[r] = -1;
+      int2* tiles = (int2*)(a.saved + p.tiles_off);
+      for (int i = 0; i < ntiles; ++i) tiles[sum[1] - ntiles + i] = make_int2(tid, sum[0] - padded + i * 128);
+      if (tid == p.E - 1)
+        for (int i = sum[1]; i < p.tiles; ++i) tiles[i] = make_int2(-1, 0);
+    }
+  }
+  const int64_t s0 = blockIdx.x * p.plan_chunk;
+  for (int64_t s = s0; s < s0 + p.plan_chunk && s < p.S; s += kPlanThreads) {
+    for (int e = lane; e < p.E; e += 64) wave_count[wave][e] = 0;
+    __syncthreads();
+    const int64_t mine = s + tid;
+    const int e = mine < p.S ? slot_expert(a, mine) : -1;
+    unsigned long long same = __ballot(e >= 0);
+    for (int bit = 1; bit < p.E; bit <<= 1) {
+      const unsigned long long has = __ballot(e & bit);
+      same &= (e & bit) ? has : ~has;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    if (e >= 0 && rank == 0) wave_count[wave][e] = __popcll(same);
+    __syncthreads();
+    if (tid < p.E) {
+      int at = next[tid];
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = wave_count[w][tid];
+        wave_count[w][tid] = at;
+        at += c;
+      }
+      next[tid] = at;
+    }
+    __syncthreads();
+    if (mine < p.S) {
+      int r = -1;
+      if (e >= 0) {
+        r = wave_count[wave][e] + rank;
+        tok[r] = (int)(mine / p.k);
+        slot[r] = (int)mine;
+      }
+      row[mine] = r;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- tanh, scales, packed coefficients ----------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_experts_tanh(ExpertsArgs a) {
+  const ExpertsPlan& p = a.p;
+  float* t = (float*)(a.saved + p.t_off);
+  const int64_t n = p.T * p.Ip;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
+    const int64_t r = q / p.Ip;
+    const int i = (int)(q - r * p.Ip);
+    t[q] = i < p.I ? tanhf((float)((const T*)a.x)[r * p.I + i]) : 0.0f;
+  }
+}
+
+// The power of two that brings a largest magnitude m into [2^(e-1), 2^e).
+__device__ __forceinline__ float range_scale(float m, int e) {
+  if (!(m > 0.0f)) return 1.0f;
+  int x;
+  frexpf(m, &x);
+  x = e - x;
+  return ldexpf(1.0f, x > 126 ? 126 : x < -126 ? -126 : x);
+}
+__device__ __forceinline__ float finite_abs(float v) {
+  const float m = fabsf(v);
+  return m <= FLT_MAX ? m : 0.0f;  // infinities and NaN pass through the planes as they are
+}
+__device__ __forceinline__ float block_max_256(float v, float* red) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_experts_cmax(ExpertsArgs a) {
+  __shared__ float red[4];
+  const ExpertsPlan& p = a.p;
+  const int e = blockIdx.y;
+  const int64_t n = (int64_t)p.I * p.O * p.D;
+  const T* c = (const T*)a.coeffs + e * n;
+  float m = 0.0f;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)kMaxParts * 256)
+    m = fmaxf(m, finite_abs((float)c[q]));
+  m = block_max_256(m, red);
+  if (threadIdx.x == 0) ((float*)(a.ws + p.cmax_off))[e * kMaxParts + blockIdx.x] = m;
+}
+
+// Inputs a stage of the forward takes, and its k-blocks (see k_experts_fwd).
+template <int NP, int P> struct FwdStage {
+  static constexpr int KS = NP == 2 && P < 16 ? 2 : 4;
+  static constexpr int IN = KS * 16 / P;
+};
+
+// Cf: the forward's operand, rows o, k in stages of IN inputs: half g of a lane
+// pair holds inputs g IN/2.., P degrees each, eight values a k-block.  Cb: the dx
+// operand, rows i and k = o for each degree d, scaled by d.  And the sums over the
+// inputs of the T_0 coefficients.  A block takes 32 outputs and 256 inputs of an
+// expert, 16 inputs at a time through LDS.
+template <typename T, int NP, int P>
+__global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backward) {
+  extern __shared__ float sm[];
+  using FS = FwdStage<NP, P>;
+  const ExpertsPlan& p = a.p;
+  const int e = blockIdx.z, ob = blockIdx.y, tid = threadIdx.x;
+  const int D = p.D, W = 32 * D + 1;  // a row of the tile: 32 outputs, D coefficients each
+  const float* cmax = (const float*)(a.ws + p.cmax_off) + e * kMaxParts;
+  float m = 0.0f;
+  for (int i = 0; i < kMaxParts; ++i) m = fmaxf(m, cmax[i]);
+  // d C with d <= 16 has to fit too: the largest |C| below 2^11
+  const float scale = range_scale(m, 11);
+  if (blockIdx.x == 0 && ob == 0 && tid == 0) ((float*)(a.saved + p.scale_off))[e] = scale;
+  const T* C = (const T*)a.coeffs + (int64_t)e * p.I * p.O * D;
+  char* cf = a.ws + p.cf_off + (size_t)e * p.Op * p.Ip * P * 2 * NP;
+  char* cb = a.saved + p.cb_off + (size_t)e * p.Ip * p.deg * p.Op * 2 * NP;
+  const int KBf = p.Ip * P / 16, KBo = p.Op / 16;
+  const int o0 = ob * 32, no = p.O - o0 < 32 ? p.O - o0 : 32;
+  float bias = 0.0f;
+  const int i_end = (int)(blockIdx.x + 1) * 256 < p.Ip ? (int)(blockIdx.x + 1) * 256 : p.Ip;
+  for (int i0 = blockIdx.x * 256; i0 < i_end; i0 += 16) {
+    __syncthreads();
+    for (int q = tid; q < 16 * 32 * D; q += 256) {
+      const int i = q / (32 * D), f = q - i * 32 * D;
+      sm[i * W + f] = i0 + i < p.I && f < no * D ? (float)C[((int64_t)(i0 + i) * p.O + o0) * D + f] : 0.0f;
+    }
+    __syncthreads();
+    if (tid < 32)
+      for (int i = 0; i < 16; ++i) bias += sm[i * W + tid * D];
+    // Cf: P k-blocks of 64 lanes
+    for (int q = tid; q < 64 * P; q += 256) {
+      const int lane = q & 63, kb = q >> 6;  // k-block of the 16 inputs
+      const int stage = kb / FS::KS, j = kb % FS::KS;
+      float v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const int u = j * 8 + s;
+        const int i = stage * FS::IN + (lane >> 5) * (FS::IN / 2) + u / P, d = u % P + 1;
+        v[s] = d < D ? scale * sm[i * W + (lane & 31) * D + d] : 0.0f;
+      }
+      const Planes8<NP> f = to_planes8<NP>(v);
+      char* dst = cf + (((size_t)ob * KBf + i0 * P / 16 + kb) * NP) * kPlaneBytes + lane * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(dst + k * kPlaneBytes) = f.p[k];
+    }
+    // Cb: for each degree 16 rows (half a row block) x 4 groups of 8 outputs
+    if (backward)
+      for (int q = tid; q < 64 * p.deg; q += 256) {
+        const int i = q & 15, k8 = (q >> 4) & 3, d = (q >> 6) + 1;
+        float v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v[s] = (float)d * scale * sm[i * W + (k8 * 8 + s) * D + d];
+        const Planes8<NP> f = to_planes8<NP>(v);
+        const int row = i0 + i;
+        char* dst = cb + (((((size_t)(row >> 5) * p.deg + d - 1) * KBo) + ob * 2 + (k8 >> 1)) * NP) * kPlaneBytes +
+                    ((row & 31) + 32 * (k8 & 1)) * 16;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) *(f16x8_t*)(dst + k * kPlaneBytes) = f.p[k];
+      }
+  }
+  if (tid < 32) ((float*)(a.ws + p.bias_off))[((size_t)blockIdx.x * p.E + e) * p.Op + o0 + tid] = bias;
+}
+
+// ---- forward ------------------------------------------------------------------
+
+// 128 rows x 64 FN columns a block, four waves of 64 x 32 FN.  Each stage copies the
+// rows' tanh values of IN inputs (gathered by token) and KS k-blocks of Cf to LDS;
+// a wave makes its rows' basis values in registers, eight values of one or two
+// inputs a lane and k-block.
+template <int NP, int P, int FN>
+__global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
+  extern __shared__ char lds[];
+  using FS = FwdStage<NP, P>;
+  constexpr int KS = FS::KS, IN = FS::IN, TB = IN * 4;  // bytes of a row's tanh values a stage
+  constexpr int kT = 128 * TB, kTChunks = kT / 1024, kB = 2 * FN * KS * NP;  // 1 KiB chunks
+  constexpr int kStage = kT + kB * kPlaneBytes;
+  const ExpertsPlan& p = a.p;
+  const int cols = (p.O + 64 * FN - 1) / (64 * FN);
+  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[blockIdx.x / cols];
+  if (tile.x < 0) return;
+  const int e = tile.x, row0 = tile.y, cb = blockIdx.x % cols;
+  const int end = ((const int*)(a.saved + p.off_off))[e + 1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave >> 1, wn = wave & 1, g = lane >> 5;
+  const int* tok = (const int*)(a.saved + p.tok_off);
+  const float* t = (const float*)(a.saved + p.t_off);
+  const int KB = p.Ip * P / 16, nst = KB / KS, nb = p.Op / 32;
+  const char* cf = a.ws + p.cf_off + (size_t)e * p.Op * p.Ip * P * 2 * NP;
+  const size_t pitch = (size_t)KB * NP * kPlaneBytes;
+  const uint32_t l0 = lds_address(lds);
+  // this wave's tanh copies: chunk c holds 1024 / TB rows, 16 bytes a lane
+  constexpr int kTPer = (kTChunks + 3) / 4;
+  const float* tsrc[kTPer];
+#pragma unroll
+  for (int i = 0; i < kTPer; ++i) {
+    const int c = i * 4 + wave;
+    const int byte = c * 1024 + lane * 16, r = row0 + byte / TB;
+    int k = c < kTChunks && r < end ? tok[r] : 0;
+    if (k < 0) k = 0;  // a pad row: any values, its results are not stored
+    tsrc[i] = t + (int64_t)k * p.Ip + byte % TB / 4;
+  }
+  auto copy = [&](int s, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < kTPer; ++i)
+      if (i * 4 + wave < kTChunks) dma16v(tsrc[i] + s * IN, at + (i * 4 + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < kB / 4; ++i) {
+      const int c = i * 4 + wave;
+      int rb = cb * 2 * FN + c / (KS * NP);
+      rb = rb < nb ? rb : nb - 1;  // past the outputs: any, not stored
+      dma16s(cf + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + kT + c * kPlaneBytes);
+    }
+  };
+  f32x16_t acc[2][FN] = {};
+  copy(0, l0);
+  for (int s = 0; s < nst; ++s) {
+    wait_vm<0>();
+    wait_lds();
+    block_barrier();
+    if (s + 1 < nst) copy(s + 1, l0 + ((s + 1) & 1) * kStage);
+    const char* buf = lds + (s & 1) * kStage;
+    float tv[2][IN / 2], pa[2], pb[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int q = 0; q < IN / 2; ++q)
+        tv[m][q] = ((const float*)(buf + (wm * 64 + m * 32 + (lane & 31)) * TB + g * (TB / 2)))[q];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      f16x8_t fa[2][NP], fb[FN][NP];
+#pragma unroll
+      for (int n = 0; n < FN; ++n)
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+          fb[n][q] = lds_frag(buf + kT + (((wn * FN + n) * KS + k) * NP + q) * kPlaneBytes, lane);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int d = (k * 8 + u) % P;  // T_{d+1} of input (k 8 + u) / P
+          const float x = tv[m][(k * 8 + u) / P];
+          if (d == 0) {
+            pa[m] = 1.0f;
+            pb[m] = x;
+          } else {
+            const float c = fmaf(x + x, pb[m], -pa[m]);
+            pa[m] = pb[m];
+            pb[m] = c;
+          }
+          v[u] = pb[m];
+        }
+        const Planes8<NP> f = to_planes8<NP>(v);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) fa[m][q] = f.p[q];
+      }
+      mfma_planes<NP, NP, 2, FN>(fa, fb, acc);
+    }
+  }
+  const float inv = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
+  const float* bias = (const float*)(a.ws + p.bias_off);
+  float* z = (float*)(a.saved + p.z_off);
+#pragma unroll
+  for (int n = 0; n < FN; ++n) {
+    const int o = (cb * 2 * FN + wn * FN + n) * 32 + (lane & 31);
+    if (o >= p.O) continue;
+    float b = 0.0f;
+    for (int k = 0; k < p.bias_parts; ++k) b += bias[((size_t)k * p.E + e) * p.Op + o];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int r = row0 + wm * 64 + m * 32 + acc_row(q, g);
+        if (r < end) z[(size_t)r * p.O + o] = fmaf(acc[m][n][q], inv, b);
+      }
+  }
+}
+
+__device__ __forceinline__ float load_weight(const ExpertsArgs& a, int64_t s) {
+  return a.p.wbf16 ? (float)((const __bf16*)a.weights)[s] : ((const float*)a.weights)[s];
+}
+
+// out[t, c] = sum over the token's kept slots of (weight) src[row, c], in slot order.
+template <typename T, bool WEIGHTED>
+__global__ __launch_bounds__(256) void k_experts_gather(ExpertsArgs a, const float* src, void* out, int width) {
+  const ExpertsPlan& p = a.p;
+  const int* row = (const int*)(a.saved + p.row_off);
+  const int64_t n = p.T * width;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
+    const int64_t t = q / width;
+    const int c = (int)(q - t * width);
+    float v = 0.0f;
+    for (int j = 0; j < p.k; ++j) {
+      const int r = row[t * p.k + j];
+      if (r >= 0) v += WEIGHTED ? load_weight(a, t * p.k + j) * src[(size_t)r * width + c] : src[(size_t)r * width + c];
+    }
+    ((T*)out)[q] = (T)v;
+  }
+}
+
+// ---- backward -------------------------------------------------------------------
+
+// dweights of each slot, and the largest |w dy| of each expert (by blocks).
+template <typename T>
+__global__ __launch_bounds__(256) void k_experts_dweights(ExpertsArgs a) {
+  __shared__ float gmax[kExpertsMax];
+  const ExpertsPlan& p = a.p;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int e = threadIdx.x; e < p.E; e += 256) gmax[e] = 0.0f;
+  __syncthreads();
+  const int* off = (const int*)(a.saved + p.off_off);
+  const int* slot = (const int*)(a.saved + p.slot_off);
+  const int* row = (const int*)(a.saved + p.row_off);
+  const float* z = (const float*)(a.saved + p.z_off);
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < off[p.E]; r += (int64_t)gridDim.x * 4) {
+    const int s = slot[r];
+    if (s < 0) continue;
+    const T* dy = (const T*)a.dy + (int64_t)(s / p.k) * p.O;
+    float dot = 0.0f, m = 0.0f;
+    for (int o = lane; o < p.O; o += 64) {
+      const float v = (float)dy[o];
+      dot = fmaf(v, z[(size_t)r * p.O + o], dot);
+      m = fmaxf(m, finite_abs(v));
+    }
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      dot += __shfl_xor(dot, w);
+      m = fmaxf(m, __shfl_xor(m, w));
+    }
+    if (lane == 0) {
+      if (a.dweights) {
+        if (p.wbf16)
+          ((__bf16*)a.dweights)[s] = (__bf16)dot;
+        else
+          ((float*)a.dweights)[s] = dot;
+      }
+      const int e = (int)a.indices[s];
+      m = finite_abs(m * load_weight(a, s));
+      atomicMax((unsigned*)&gmax[e], __float_as_uint(m));  // non-negative floats order as integers
+    }
+  }
+  if (a.dweights)
+    for (int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x; s < p.S; s += (int64_t)gridDim.x * 256)
+      if (row[s] < 0) {
+        if (p.wbf16)
+          ((__bf16*)a.dweights)[s] = (__bf16)0.0f;
+        else
+          ((float*)a.dweights)[s] = 0.0f;
+      }
+  __syncthreads();
+  float* out = (float*)(a.ws + p.gmax_off) + (size_t)blockIdx.x * p.E;
+  for (int e = threadIdx.x; e < p.E; e += 256) out[e] = gmax[e];
+}
+
+__device__ __forceinline__ int row_expert(const int* off, int E, int r) {
+  int lo = 0, hi = E;  // the last e with off[e] <= r
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= r)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  while (lo + 1 < E && off[lo + 1] <= r) ++lo;
+  return lo;
+}
+
+// g = w dy (scaled) of 32 rows x 64 outputs in both operand forms: rows = slots and
+// k = o for dx, rows = o and k = slots for dC; and the rows' sum for each output.
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
+  __shared__ float tile[32][65], red[4];
+  const ExpertsPlan& p = a.p;
+  const int* off = (const int*)(a.saved + p.off_off);
+  const int rb = blockIdx.x, o0 = blockIdx.y * 64, tid = threadIdx.x;
+  if (rb * 32 >= off[p.E]) return;
+  const int e = row_expert(off, p.E, rb * 32);
+  const float* gmax = (const float*)(a.ws + p.gmax_off);
+  float m = 0.0f;
+  for (int b = tid; b < (int)p.grad_blocks; b += 256) m = fmaxf(m, gmax[(size_t)b * p.E + e]);
+  m = block_max_256(m, red);
+  const float scale = range_scale(m, 14);
+  if (rb * 32 == off[e] && blockIdx.y == 0 && tid == 0) ((float*)(a.ws + p.gscale_off))[e] = scale;
+  const int* slot = (const int*)(a.saved + p.slot_off);
+  for (int q = tid; q < 32 * 64; q += 256) {
+    const int r = q >> 6, o = o0 + (q & 63), s = slot[rb * 32 + r];
+    float v = 0.0f;
+    if (s >= 0 && o < p.O) v = load_weight(a, s) * (float)((const T*)a.dy)[(int64_t)(s / p.k) * p.O + o];
+    tile[r][q & 63] = v;
+  }
+  __syncthreads();
+  if (tid < 64 && o0 + tid < p.Op) {
+    float sum = 0.0f;
+    for (int r = 0; r < 32; ++r) sum += tile[r][tid];
+    ((float*)(a.ws + p.gsum_off))[(size_t)rb * p.Op + o0 + tid] = sum;
+  }
+  float v[8];
+  const int KBo = p.Op / 16;
+  {  // rows = slots: 32 rows x 8 groups of 8 outputs
+    const int r = tid & 31, k8 = tid >> 5, o = o0 + k8 * 8;
+    if (o < p.Op) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = scale * tile[r][k8 * 8 + j];
+      const Planes8<NP> f = to_planes8<NP>(v);
+      char* d = a.ws + p.gr_off + (((size_t)rb * KBo + (o >> 4)) * NP) * kPlaneBytes + (r + 32 * (k8 & 1)) * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f.p[k];
+    }
+  }
+  {  // rows = o: 64 rows x 4 groups of 8 slots
+    const int oo = tid & 63, k8 = tid >> 6, o = o0 + oo;
+    if (o < p.Op) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = scale * tile[k8 * 8 + j][oo];
+      const Planes8<NP> f = to_planes8<NP>(v);
+      const int KBr = (int)(p.R / 16);
+      char* d = a.ws + p.gt_off + (((size_t)(o >> 5) * KBr + rb * 2 + (k8 >> 1)) * NP) * kPlaneBytes +
+                ((o & 31) + 32 * (k8 & 1)) * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f.p[k];
+    }
+  }
+}
+
+// dx of 128 rows x 64 inputs a block, waves of 64 rows x 32 inputs: four degrees a
+// pass over the outputs stand in four accumulator fragments; between passes only
+// their weighted sum is kept.
+template <int NP>
+__global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
+  extern __shared__ char lds[];
+  typedef NtTile<NP, NP, 2, 2, 2, 4, 2, 2> Tile;
+  const ExpertsPlan& p = a.p;
+  const int cols = (p.Ip + 63) / 64;
+  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[blockIdx.x / cols];
+  if (tile.x < 0) return;
+  const int e = tile.x, row0 = tile.y, ib0 = blockIdx.x % cols * 2;
+  const int end = ((const int*)(a.saved + p.off_off))[e + 1];
+  const int KB = p.Op / 16, nib = p.Ip / 32;
+  const size_t pitch = (size_t)KB * NP * kPlaneBytes;
+  const char* cbase = a.saved + p.cb_off + (size_t)e * p.Ip * p.deg * p.Op * 2 * NP;
+  const RowBlocks A{a.ws + p.gr_off + (row0 >> 5) * pitch, pitch};
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
+  const int i = (ib0 + (wave & 1)) * 32 + (lane & 31);
+  const int* tok = (const int*)(a.saved + p.tok_off);
+  const float* t = (const float*)(a.saved + p.t_off);
+  float dx[2][16] = {};
+  for (int d0 = 0; d0 < p.deg; d0 += 4) {
+    f32x16_t acc[2][4] = {};
+    Tile::run(A, [&](int r) {
+      int ib = ib0 + (r >> 2), d = d0 + (r & 3);
+      ib = ib < nib ? ib : nib - 1;     // past the inputs or degrees: any, not used
+      d = d < p.deg ? d : p.deg - 1;
+      return cbase + ((size_t)ib * p.deg + d) * pitch;
+    }, 0, KB / 2, lds, acc);
+    const int nd = p.deg - d0 < 4 ? p.deg - d0 : 4;
+    if (i < p.I) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int r = row0 + (wave >> 1) * 64 + m * 32 + acc_row(q, g);
+          if (r >= end) continue;
+          const int k = tok[r];
+          const float x = k >= 0 ? t[(int64_t)k * p.Ip + i] : 0.0f, x2 = x + x;
+          float ua = 0.0f, ub = 1.0f;  // U_{-1}, U_0
+          for (int d = 0; d < d0; ++d) {
+            const float c = fmaf(x2, ub, -ua);
+            ua = ub;
+            ub = c;
+          }
+          float s = 0.0f;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            if (d < nd) s = fmaf(acc[m][d][q], ub, s);
+            const float c = fmaf(x2, ub, -ua);
+            ua = ub;
+            ub = c;
+          }
+          dx[m][q] = fmaf(s, 1.0f - x * x, dx[m][q]);
+        }
+    }
+  }
+  if (i >= p.I) return;
+  const float ic = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
+  const float ig = 1.0f / ((const float*)(a.ws + p.gscale_off))[e];
+  float* out = (float*)(a.ws + p.dxs_off);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int r = row0 + (wave >> 1) * 64 + m * 32 + acc_row(q, g);
+      if (r < end) out[(size_t)r * p.I + i] = dx[m][q] * ic * ig;
+    }
+}
+
+// dC of 32 inputs x 8 degrees x 128 outputs of an expert a block; waves of 32 inputs x
+// 4 degrees x 64 outputs.  A stage is 32 rows: each thread makes four degrees of
+// eight rows of one input into LDS for the next stage while the matrix
+// instructions work on this one.
+template <typename T, int NP>
+__global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
+  extern __shared__ char lds[];
+  constexpr int KS = 2, kA = 8 * KS * NP, kB = 4 * KS * NP;  // 1 KiB chunks of a stage
+  constexpr int kStage = (kA + kB) * kPlaneBytes;
+  const ExpertsPlan& p = a.p;
+  const int nob = (p.O + 127) / 128, nib = p.Ip / 32, ndc = (p.deg + 7) / 8;
+  int id = blockIdx.x;
+  const int ob = id % nob;
+  id /= nob;
+  const int ib = id % nib;
+  id /= nib;
+  const int dc = id % ndc, e = id / ndc;
+  const int* off = (const int*)(a.saved + p.off_off);
+  const int row0 = off[e], nst = (off[e + 1] - row0) / 32;
+  const int* tok = (const int*)(a.saved + p.tok_off);
+  const float* t = (const float*)(a.saved + p.t_off);
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wd = wave >> 1, wo = wave & 1;
+  const uint32_t l0 = lds_address(lds);
+  const int KBr = (int)(p.R / 16), nb = p.Op / 32;
+  const size_t pitch = (size_t)KBr * NP * kPlaneBytes;
+  const char* gt = a.ws + p.gt_off + ((size_t)(row0 / 16) * NP) * kPlaneBytes;
+  // the making thread's input, row group and degrees
+  const int mi = tid & 31, mr = (tid >> 5) & 3, mh = tid >> 7;
+  const float* tcol = t + ib * 32 + mi;
+  float tv[8];
+  auto load_t = [&](int s) {
+    const int* tk = tok + row0 + s * 32 + mr * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = tk[j];
+      tv[j] = k >= 0 ? tcol[(int64_t)k * p.Ip] : 0.0f;
+    }
+  };
+  auto make = [&](char* buf) {
+    float ta[8], tb[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ta[j] = 1.0f;
+      tb[j] = tv[j];
+    }
+    // T_{d1-1}, T_{d1} for the thread's first degree d1 = dc 8 + mh 4 + 1
+    for (int d = 0; d < dc * 8 + mh * 4; ++d)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = fmaf(tv[j] + tv[j], tb[j], -ta[j]);
+        ta[j] = tb[j];
+        tb[j] = c;
+      }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const Planes8<NP> f = to_planes8<NP>(tb);
+      char* dst = buf + (((mh * 4 + d) * KS + (mr >> 1)) * NP) * kPlaneBytes + (mi + 32 * (mr & 1)) * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(dst + k * kPlaneBytes) = f.p[k];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = fmaf(tv[j] + tv[j], tb[j], -ta[j]);
+        ta[j] = tb[j];
+        tb[j] = c;
+      }
+    }
+  };
+  auto copy = [&](int s, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < kB / 4; ++i) {
+      const int c = i * 4 + wave;
+      int rb = ob * 4 + c / (KS * NP);
+      rb = rb < nb ? rb : nb - 1;
+      dma16s(gt + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + (kA + c) * kPlaneBytes);
+    }
+  };
+  f32x16_t acc[4][2] = {};
+  if (nst > 0) {
+    copy(0, l0);
+    load_t(0);
+    make(lds);
+    if (nst > 1) load_t(1);
+  }
+  for (int s = 0; s < nst; ++s) {
+    wait_vm<0>();
+    wait_lds();
+    block_barrier();
+    if (s + 1 < nst) {
+      copy(s + 1, l0 + ((s + 1) & 1) * kStage);
+      make(lds + ((s + 1) & 1) * kStage);
+      if (s + 2 < nst) load_t(s + 2);
+    }
+    const char* buf = lds + (s & 1) * kStage;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      f16x8_t fa[4][NP], fb[2][NP];
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+          fa[m][q] = lds_frag(buf + (((wd * 4 + m) * KS + k) * NP + q) * kPlaneBytes, lane);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+          fb[n][q] = lds_frag(buf + (kA + ((wo * 2 + n) * KS + k) * NP + q) * kPlaneBytes, lane);
+      mfma_planes<NP, NP, 4, 2>(fa, fb, acc);
+    }
+  }
+  const float inv = nst > 0 ? 1.0f / ((const float*)(a.ws + p.gscale_off))[e] : 1.0f;
+  const float* gsum = (const float*)(a.ws + p.gsum_off);
+  T* out = (T*)a.dcoeffs + (int64_t)e * p.I * p.O * p.D;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int o = ob * 128 + wo * 64 + n * 32 + (lane & 31);
+    if (o >= p.O) continue;
+    float s0 = 0.0f;  // T_0: the same for every input
+    if (dc == 0 && wd == 0)
+      for (int s = 0; s < nst; ++s) s0 += gsum[(size_t)(row0 / 32 + s) * p.Op + o];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int i = ib * 32 + acc_row(q, g);
+      if (i >= p.I) continue;
+      T* dst = out + ((int64_t)i * p.O + o) * p.D;
+      if (dc == 0 && wd == 0) dst[0] = (T)s0;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int d = dc * 8 + wd * 4 + m + 1;
+        if (d <= p.deg) dst[d] = (T)(acc[m][n][q] * inv);
+      }
+    }
+  }
+}
+
+int grid_for(int64_t n) { return (int)(ceil_div(n, 256) < 4096 ? ceil_div(n, 256) : 4096); }
+
+template <typename T, int NP, int P>
+void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
+  const ExpertsPlan& p = a.p;
+  hipLaunchKernelGGL(k_plan_count, dim3(p.plan_blocks), dim3(kPlanThreads), 0, st, a);
+  hipLaunchKernelGGL(k_plan_place, dim3(p.plan_blocks), dim3(kPlanThreads), 0, st, a);
+  hipLaunchKernelGGL((k_experts_tanh<T>), dim3(grid_for(p.T * p.Ip)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_experts_cmax<T>), dim3(kMaxParts, p.E), dim3(256), 0, st, a);
+  const size_t pack_lds = (size_t)16 * (32 * p.D + 1) * sizeof(float);
+  hipLaunchKernelGGL((k_experts_pack<T, NP, P>), dim3(p.bias_parts, p.Op / 32, p.E), dim3(256), pack_lds, st, a, keep);
+  constexpr int FN = 4;
+  using FS = FwdStage<NP, P>;
+  constexpr int lds = 2 * (128 * FS::IN * 4 + 2 * FN * FS::KS * NP * kPlaneBytes);
+  static std::atomic<uint32_t> done;
+  ensure_lds_limit((const void*)k_experts_fwd<NP, P, FN>, lds, done);
+  const int cols = (p.O + 64 * FN - 1) / (64 * FN);
+  hipLaunchKernelGGL((k_experts_fwd<NP, P, FN>), dim3((unsigned)(p.tiles * cols)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((k_experts_gather<T, true>), dim3(grid_for(p.T * p.O)), dim3(256), 0, st, a,
+                     (const float*)(a.saved + p.z_off), a.y, p.O);
+}
+
+template <typename T, int NP>
+void backward_typed(const ExpertsArgs& a, hipStream_t st) {
+  const ExpertsPlan& p = a.p;
+  hipLaunchKernelGGL((k_experts_dweights<T>), dim3((unsigned)p.grad_blocks), dim3(256), 0, st, a);
+  if (!a.dx && !a.dcoeffs) return;
+  hipLaunchKernelGGL((k_experts_gpack<T, NP>), dim3((unsigned)(p.R / 32), (p.Op + 63) / 64), dim3(256), 0, st, a);
+  if (a.dx) {
+    constexpr int lds = NtTile<NP, NP, 2, 2, 2, 4, 2, 2>::kLdsBytes;
+    static std::atomic<uint32_t> done;
+    ensure_lds_limit((const void*)k_experts_dx<NP>, lds, done);
+    hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)(p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_experts_gather<T, false>), dim3(grid_for(p.T * p.I)), dim3(256), 0, st, a,
+                       (const float*)(a.ws + p.dxs_off), a.dx, p.I);
+  }
+  if (a.dcoeffs) {
+    constexpr int lds = 2 * (8 + 4) * 2 * NP * kPlaneBytes;
+    static std::atomic<uint32_t> done;
+    ensure_lds_limit((const void*)k_experts_dc<T, NP>, lds, done);
+    const unsigned blocks = (unsigned)p.E * ((p.deg + 7) / 8) * (p.Ip / 32) * ((p.O + 127) / 128);
+    hipLaunchKernelGGL((k_experts_dc<T, NP>), dim3(blocks), dim3(256), lds, st, a);
+  }
+}
+
+}  // namespace
+
+void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st) {
+  if (a.p.bf16) {
+    if (a.p.P == 4) forward_typed<__bf16, 1, 4>(a, keep, st);
+    if (a.p.P == 8) forward_typed<__bf16, 1, 8>(a, keep, st);
+    if (a.p.P == 16) forward_typed<__bf16, 1, 16>(a, keep, st);
+  } else {
+    if (a.p.P == 4) forward_typed<float, 2, 4>(a, keep, st);
+    if (a.p.P == 8) forward_typed<float, 2, 8>(a, keep, st);
+    if (a.p.P == 16) forward_typed<float, 2, 16>(a, keep, st);
+  }
+}
+
+void launch_experts_backward(const ExpertsArgs& a, hipStream_t st) {
+  if (a.p.bf16)
+    backward_typed<__bf16, 1>(a, st);
+  else
+    backward_typed<float, 2>(a, st);
+}
+
+}  // namespace ckan

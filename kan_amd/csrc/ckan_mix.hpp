@@ -50,6 +50,51 @@ struct OrthoArgs {
   float lr, momentum, decay, scale;
   int nesterov;
 };
+// ---- ChebyKAN experts (ckan_experts.hip) ---------------------------------------
+constexpr int kExpertsMax = 512;       // a thread of the plan's scan an expert
+constexpr int kExpertsMaxDegree = 16;
+constexpr int kExpertsMaxTopK = 64;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBlocks = 256;       // at most: a block's share of the slots grows past that
+constexpr int kMaxParts = 32;          // blocks an expert that look for its largest coefficient
+constexpr int kGradBlocks = 1024;      // blocks that look for the largest upstream gradients
+
+// Sizes and the layout of the buffers.  "Rows" are the kept slots sorted by expert,
+// each expert's run padded to a multiple of 32; "slots" are the T top_k entries of
+// the caller's indices.
+struct ExpertsPlan {
+  int64_t T, S;        // tokens, slots
+  int E, k, I, O, deg, D;
+  int P;               // degrees a forward reduction group holds (deg padded to 4, 8 or 16)
+  int NP;              // fp16 planes an operand: 1 for bf16 tensors, 2 for fp32
+  bool bf16, wbf16;
+  int Ip;              // I padded to 32: pitch of the tanh cache, inputs of the packs
+  int Op;              // O padded to 32
+  int64_t R;           // rows allocated (a multiple of 128)
+  int tiles;           // 128-row tiles at most
+  int plan_blocks;
+  int64_t plan_chunk;  // slots a plan block takes (a multiple of kPlanThreads)
+  int64_t grad_blocks;
+  // saved from the forward to the backward
+  size_t off_off, tok_off, slot_off, row_off, tiles_off, scale_off, t_off, z_off, cb_off, saved_bytes;
+  // forward workspace
+  size_t hist_off, cmax_off, cf_off, bias_off, fwd_bytes;
+  // backward workspace
+  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, dxs_off, bwd_bytes;
+  int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
+};
+ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bool bf16, bool wbf16);
+
+struct ExpertsArgs {
+  ExpertsPlan p;
+  const void *x, *coeffs, *weights, *dy;
+  const int64_t* indices;
+  void *y, *dx, *dcoeffs, *dweights;
+  char *saved, *ws;
+};
+void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st);
+void launch_experts_backward(const ExpertsArgs& a, hipStream_t st);
+
 size_t ortho_workspace_bytes(int batch, int rows, int cols);
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st);
 

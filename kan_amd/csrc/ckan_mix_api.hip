@@ -68,6 +68,38 @@ int route_args(const ckan_route_desc* d, RouteArgs* a) {
   return CKAN_OK;
 }
 
+int experts_check(const ckan_experts_desc* d) {
+  if (!d) return fail(CKAN_ERR_INVALID_ARG, "experts desc is NULL");
+  if (d->rows < 0) return fail(CKAN_ERR_INVALID_ARG, "rows must be >= 0 (got %lld)", (long long)d->rows);
+  if (d->experts < 1 || d->top_k < 1 || d->in_dim < 1 || d->out_dim < 1)
+    return fail(CKAN_ERR_INVALID_ARG, "experts, top_k, in_dim and out_dim must be >= 1 (got %d, %d, %d, %d)", d->experts,
+                d->top_k, d->in_dim, d->out_dim);
+  if (d->degree < 0) return fail(CKAN_ERR_INVALID_ARG, "degree must be >= 0 (got %d)", d->degree);
+  if (d->dtype != CKAN_DTYPE_F32 && d->dtype != CKAN_DTYPE_BF16) return fail(CKAN_ERR_INVALID_ARG, "unknown dtype %d", d->dtype);
+  if (d->wdtype != CKAN_DTYPE_F32 && d->wdtype != CKAN_DTYPE_BF16)
+    return fail(CKAN_ERR_INVALID_ARG, "unknown weights dtype %d", d->wdtype);
+  if (d->experts > kExpertsMax) return fail(CKAN_ERR_UNSUPPORTED, "experts above %d are not supported (got %d)", kExpertsMax, d->experts);
+  if (d->top_k > kExpertsMaxTopK) return fail(CKAN_ERR_UNSUPPORTED, "top_k above %d is not supported (got %d)", kExpertsMaxTopK, d->top_k);
+  if (d->degree < 1 || d->degree > kExpertsMaxDegree)
+    return fail(CKAN_ERR_UNSUPPORTED, "experts have degree 1 to %d (got %d)", kExpertsMaxDegree, d->degree);
+  if (d->in_dim > 65536 || d->out_dim > 65536)
+    return fail(CKAN_ERR_UNSUPPORTED, "in_dim and out_dim above 65536 are not supported (got %d, %d)", d->in_dim, d->out_dim);
+  if (d->rows > ((int64_t)1 << 29) / d->top_k)
+    return fail(CKAN_ERR_UNSUPPORTED, "rows * top_k above 2^29 is not supported");
+  return CKAN_OK;
+}
+
+ExpertsPlan experts_plan(const ckan_experts_desc* d) {
+  return make_experts_plan(d->rows, d->experts, d->top_k, d->in_dim, d->out_dim, d->degree,
+                           d->dtype == CKAN_DTYPE_BF16, d->wdtype == CKAN_DTYPE_BF16);
+}
+
+// Without a saved buffer its parts that the forward itself needs (all before the
+// packed dx operand) lead the workspace.
+size_t experts_fwd_ws(const ExpertsPlan& p, bool without_saved) {
+  return p.fwd_bytes + (without_saved ? p.cb_off : 0);
+}
+
 // The largest |b s^2 + c s^4| that the iteration's matrix B can reach from
 // singular values in [0, 1], over all steps, by sampling the interval.
 double ortho_reach(const ckan_ortho_desc* d) {
@@ -133,6 +165,66 @@ int ortho_ws(const ckan_ortho_desc* d, void* ws, size_t ws_bytes) {
 }  // namespace
 
 extern "C" {
+
+size_t ckan_experts_saved_bytes(const ckan_experts_desc* desc) {
+  return experts_check(desc) || desc->rows == 0 ? 0 : experts_plan(desc).saved_bytes;
+}
+
+size_t ckan_experts_workspace_bytes(const ckan_experts_desc* desc, int backward, int without_saved) {
+  if (experts_check(desc) || desc->rows == 0) return 0;
+  const ExpertsPlan p = experts_plan(desc);
+  return backward ? p.bwd_bytes : experts_fwd_ws(p, without_saved != 0);
+}
+
+int ckan_experts_forward(const ckan_experts_desc* desc, const void* x, const void* coeffs, const int64_t* indices,
+                         const void* weights, void* y, void* saved, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = experts_check(desc)) return rc;
+  if (desc->rows == 0) return CKAN_OK;
+  if (!x || !coeffs || !indices || !weights || !y) return fail(CKAN_ERR_INVALID_ARG, "experts_forward: NULL pointer");
+  ExpertsArgs a{};
+  a.p = experts_plan(desc);
+  const size_t need = experts_fwd_ws(a.p, !saved);
+  if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "experts forward workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!ws || !is_al16(ws) || !is_al16(saved))
+    return fail(CKAN_ERR_INVALID_ARG, "experts_forward: workspace is NULL, or workspace or saved not 16-byte aligned");
+  a.x = x;
+  a.coeffs = coeffs;
+  a.indices = indices;
+  a.weights = weights;
+  a.y = y;
+  a.saved = saved ? (char*)saved : (char*)ws;
+  a.ws = (char*)ws + (saved ? 0 : a.p.cb_off);
+  launch_experts_forward(a, saved != nullptr, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("experts_forward");
+}
+
+int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices, const void* weights, void* saved,
+                          const void* dy, void* dx, void* dcoeffs, void* dweights, void* ws, size_t ws_bytes,
+                          void* stream) {
+  if (const int rc = experts_check(desc)) return rc;
+  if (desc->rows == 0) {
+    if (dcoeffs) return fail(CKAN_ERR_INVALID_ARG, "experts_backward: no rows, the caller fills dcoeffs with zeros");
+    return CKAN_OK;
+  }
+  if (!dx && !dcoeffs && !dweights) return CKAN_OK;
+  if (!indices || !weights || !saved || !dy) return fail(CKAN_ERR_INVALID_ARG, "experts_backward: NULL pointer");
+  ExpertsArgs a{};
+  a.p = experts_plan(desc);
+  if (ws_bytes < a.p.bwd_bytes)
+    return fail(CKAN_ERR_WORKSPACE, "experts backward workspace too small: %zu < %zu bytes", ws_bytes, a.p.bwd_bytes);
+  if (!ws || !is_al16(ws) || !is_al16(saved))
+    return fail(CKAN_ERR_INVALID_ARG, "experts_backward: workspace is NULL, or workspace or saved not 16-byte aligned");
+  a.indices = indices;
+  a.weights = weights;
+  a.dy = dy;
+  a.dx = dx;
+  a.dcoeffs = dcoeffs;
+  a.dweights = dweights;
+  a.saved = (char*)saved;
+  a.ws = (char*)ws;
+  launch_experts_backward(a, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("experts_backward");
+}
 
 size_t ckan_orthogonalize_workspace_bytes(const ckan_ortho_desc* desc) {
   return ortho_check(desc) ? 0 : ortho_workspace_bytes(desc->batch, desc->rows, desc->cols);

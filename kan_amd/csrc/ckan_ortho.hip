@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
   const char* x = xr + b * p.xr_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(x + tm * 4 * pitch, pitch, x + tn * 4 * pitch, pitch, kb0, kbs / 2, lds, acc);
+  Tile22::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / 2, lds, acc);
   float* out = part + ((size_t)split * p.batch + b) * p.part_elems;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_poly(OrthoPlan p, const char* 
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
   const char* x = A + b * p.a_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(x + tm * 4 * pitch, pitch, x + tn * 4 * pitch, pitch, 0, KB / 2, lds, acc);
+  Tile22::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0, KB / 2, lds, acc);
   char* out = B + b * p.a_bytes;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
   const char* x = xc + b * p.xc_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(B + b * p.a_bytes + tm * 4 * pitch, pitch, x + tn * 4 * pitch, pitch, 0, KB / 2, lds, acc);
+  Tile22::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0, KB / 2, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   constexpr int kPitch = (kTile + 8) * 2;  // bytes of a row of the LDS tile
   char* plane1 = lds + kTile * kPitch;

@@ -29,6 +29,15 @@ typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
 
 constexpr int kPlaneBytes = 1024;
 
+// A value in a register that the compiler does not see through.  The planes need
+// it: h = fp16(a b) and l = fp16(a b - h) from one expression may be contracted
+// differently (h in a mixed-precision multiply that rounds once, a b in l twice),
+// and then h + l misses the value by an fp16 ulp of h.
+__device__ __forceinline__ float opaque(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 // The 8 values of a lane in planes (round to nearest even each).
 template <int NP> struct Planes8 { f16x8_t p[NP]; };
 template <int NP>
@@ -36,9 +45,10 @@ __device__ __forceinline__ Planes8<NP> to_planes8(const float* v) {
   Planes8<NP> f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const _Float16 h = (_Float16)v[j];
+    const float x = NP == 2 ? opaque(v[j]) : v[j];
+    const _Float16 h = (_Float16)x;
     f.p[0][j] = h;
-    if constexpr (NP == 2) f.p[1][j] = (_Float16)(v[j] - (float)h);
+    if constexpr (NP == 2) f.p[1][j] = (_Float16)(x - (float)h);
   }
   return f;
 }
@@ -48,9 +58,10 @@ __device__ __forceinline__ Planes4<NP> to_planes4(const float* v) {
   Planes4<NP> f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const _Float16 h = (_Float16)v[j];
+    const float x = NP == 2 ? opaque(v[j]) : v[j];
+    const _Float16 h = (_Float16)x;
     f.p[0][j] = h;
-    if constexpr (NP == 2) f.p[1][j] = (_Float16)(v[j] - (float)h);
+    if constexpr (NP == 2) f.p[1][j] = (_Float16)(x - (float)h);
   }
   return f;
 }
@@ -86,6 +97,23 @@ __device__ __forceinline__ f16x8_t lds_frag(const char* base, int lane) {
   return *reinterpret_cast<const f16x8_t*>(base + lane * 16);
 }
 
+// The LDS address that a copy takes for a generic pointer into shared memory.
+__device__ __forceinline__ uint32_t lds_address(char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p;
+}
+// A 16-byte-per-lane copy from per-lane addresses: lane l's 16 bytes at src land at
+// LDS byte lds + 16 l (lds wave-uniform); counted in vmcnt, like dma16s.
+__device__ __forceinline__ void dma16v(const void* src, uint32_t lds) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l) : "memory", "m0");
+}
+// The address of row block r of an operand whose row blocks lie `pitch` bytes apart.
+struct RowBlocks {
+  const char* base;
+  size_t pitch;
+  __device__ const char* operator()(int r) const { return base + r * pitch; }
+};
+
 // Waits until at most N of the wave's vector memory operations are in flight.
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -109,17 +137,18 @@ struct NtTile {
 
   // Copies stage kb.. of both operands: the 1 KiB chunks in LDS order, chunk c by
   // wave c % kWaves (row block, then k-block and plane, both contiguous in memory).
-  __device__ static void copy(const char* A, size_t pa, const char* B, size_t pb, int kb, uint32_t lds,
-                              int wave, int lane) {
+  // A(r) and B(r) give the address of the tile's r-th row block.
+  template <typename SrcA, typename SrcB>
+  __device__ static void copy(const SrcA& A, const SrcB& B, int kb, uint32_t lds, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int c = i * kWaves + wave;
       const char* src;
       if (c < kChunksA) {
-        src = A + (size_t)(c / (KS * NA)) * pa + ((size_t)kb * NA + c % (KS * NA)) * kPlaneBytes;
+        src = A(c / (KS * NA)) + ((size_t)kb * NA + c % (KS * NA)) * kPlaneBytes;
       } else {
         const int d = c - kChunksA;
-        src = B + (size_t)(d / (KS * NB)) * pb + ((size_t)kb * NB + d % (KS * NB)) * kPlaneBytes;
+        src = B(d / (KS * NB)) + ((size_t)kb * NB + d % (KS * NB)) * kPlaneBytes;
       }
       dma16s(src, lane * 16, lds + c * kPlaneBytes);
     }
@@ -143,17 +172,18 @@ struct NtTile {
     }
   }
 
-  // acc += the product over the nst stages from k-block kb0 on.  A and B point at
-  // the tile's first row block, pa and pb are bytes from one row block to the
-  // next.  Ends with every wave past its last LDS read.
-  __device__ static void run(const char* A, size_t pa, const char* B, size_t pb, int kb0, int nst, char* lds,
+  // acc += the product over the nst stages from k-block kb0 on.  A and B give the
+  // addresses of the tile's row blocks.  Ends with every wave past its last LDS
+  // read.
+  template <typename SrcA, typename SrcB>
+  __device__ static void run(const SrcA& A, const SrcB& B, int kb0, int nst, char* lds,
                              f32x16_t (&acc)[FM][FN]) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave / WN, wn = wave % WN;
-    const uint32_t l0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const uint32_t l0 = lds_address(lds);
 #pragma unroll
     for (int s = 0; s < NBUF - 1; ++s)
-      if (s < nst) copy(A, pa, B, pb, kb0 + s * KS, l0 + s * kStageBytes, wave, lane);
+      if (s < nst) copy(A, B, kb0 + s * KS, l0 + s * kStageBytes, wave, lane);
     int cur = 0;
     for (int s = 0; s < nst; ++s) {
       // stage s has landed when only the later stages' copies are in flight
@@ -168,7 +198,7 @@ struct NtTile {
       if (nxt < nst) {
         int at = cur + NBUF - 1;
         if (at >= NBUF) at -= NBUF;
-        copy(A, pa, B, pb, kb0 + nxt * KS, l0 + at * kStageBytes, wave, lane);
+        copy(A, B, kb0 + nxt * KS, l0 + at * kStageBytes, wave, lane);
       }
       compute(lds + cur * kStageBytes, wm, wn, lane, acc);
       if (++cur == NBUF) cur = 0;

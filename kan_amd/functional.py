@@ -532,5 +532,5 @@ def jacobian(x: torch.Tensor, coeffs: torch.Tensor, spec, affine=None) -> torch.
 
 
 # public operators of this namespace that live in modules of their own
-from .mixture import route  # noqa: E402
+from .mixture import kan_experts, route  # noqa: E402
 from .orthogonal import orthogonalize  # noqa: E402

@@ -98,3 +98,31 @@ def muon_step(p, g, buf, lr, momentum=0.95, nesterov=True, weight_decay=0.0, **k
         up = orthogonalize(u, **kw)
         ratio = p.shape[0] / p.shape[1]
     return p * (1 - lr * weight_decay) - lr * np.sqrt(max(1.0, ratio)) * up, buf
+
+
+def cheb(t, degree):
+    """T_0..T_degree and their derivatives in t, in a last dimension (t away from +-1)."""
+    theta = np.arccos(t)[..., None]
+    n = np.arange(degree + 1)
+    return np.cos(n * theta), n * np.sin(n * theta) / np.sin(theta)
+
+
+def kan_experts(x, coeffs, indices, weights, dy=None):
+    """y, and with dy also (dx, dcoeffs, dweights), one slot at a time."""
+    x, coeffs, weights = (np.asarray(v, dtype=np.float64) for v in (x, coeffs, weights))
+    experts, _, out, dd = coeffs.shape
+    t = np.tanh(x)
+    basis, slope = cheb(t, dd - 1)
+    y = np.zeros((x.shape[0], out))
+    dx, dc, dw = np.zeros_like(x), np.zeros_like(coeffs), np.zeros_like(weights)
+    for (r, j), e in np.ndenumerate(np.asarray(indices)):
+        if not 0 <= e < experts:
+            continue
+        z = np.einsum("id,iod->o", basis[r], coeffs[e])
+        y[r] += weights[r, j] * z
+        if dy is not None:
+            dw[r, j] = z @ dy[r]
+            g = weights[r, j] * np.asarray(dy[r], dtype=np.float64)
+            dc[e] += basis[r][:, None, :] * g[None, :, None]
+            dx[r] += np.einsum("iod,o,id->i", coeffs[e], g, slope[r]) * (1 - t[r] ** 2)
+    return y if dy is None else (y, dx, dc, dw)
