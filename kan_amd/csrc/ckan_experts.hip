@@ -76,6 +76,19 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.gsum_off = take((size_t)(p.R / 32) * p.Op * 4);
   p.dxs_off = take((size_t)p.R * I * 4);
   p.bwd_bytes = off;
+  // Streaming: up to 16 slots an expert on average.  Its blocks read the coefficients
+  // as they lie, once for 8 rows; the tile path reads them twice and packs them
+  // before its products start.
+  const int64_t active = E < p.S ? E : p.S, oc = ceil_div(O, 64);
+  p.stream = p.S <= kStreamMaxSlots && p.S <= 16 * active;
+  int64_t chunks = ceil_div(8 * kNumCUs, active * oc);
+  if (chunks > ceil_div(I, 16)) chunks = ceil_div(I, 16);
+  if (chunks < ceil_div(I, kStreamInputs)) chunks = ceil_div(I, kStreamInputs);
+  p.chunk_inputs = (int)round_up(ceil_div(I, chunks), 4);
+  if (p.chunk_inputs > kStreamInputs) p.chunk_inputs = kStreamInputs;
+  p.chunks = (int)ceil_div(I, p.chunk_inputs);
+  p.part_off = 0;
+  p.stream_bytes = p.stream ? align256((size_t)p.chunks * p.S * O * 4) : 0;
   return p;
 }
 
@@ -780,6 +793,185 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
   }
 }
 
+// ---- forward of few slots ---------------------------------------------------------
+
+// The D coefficients of lane o of one input's row [O, D], through a bounds-checked
+// buffer (lanes past O read zeros).  bf16 rows may begin, and coefficients lie, on
+// odd halves of a dword: the dwords that cover them are read and shifted.
+template <int D>
+__device__ __forceinline__ void stream_load(const float* row, int bytes, int o, uint32_t (&w)[D]) {
+  const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(row, bytes);
+  constexpr int kQ = D / 4 * 4;
+#pragma unroll
+  for (int v = 0; v < kQ; v += 4) {
+    const u32x4_t q = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (o * D + v) * 4, 0, 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[v + j] = q[j];
+  }
+#pragma unroll
+  for (int v = kQ; v < D; ++v) w[v] = __builtin_amdgcn_raw_buffer_load_b32(rs, (o * D + v) * 4, 0, 0);
+}
+template <int D> struct StreamRow {  // dwords a lane holds of an input
+  static constexpr int kF32 = D, kBf16 = D % 2 ? (D + 1) / 2 : D / 2;
+};
+template <int D>
+__device__ __forceinline__ void stream_load(const __bf16* row, int bytes, int o, uint32_t (&w)[StreamRow<D>::kBf16]) {
+  const uintptr_t at = (uintptr_t)row;
+  const int odd = (int)(at & 2);
+  const __amdgpu_buffer_rsrc_t rs = buffer_rsrc((const void*)(at & ~(uintptr_t)3), (bytes + odd + 3) & ~3);
+  const int byte = o * D * 2 + odd;
+  constexpr int N = StreamRow<D>::kBf16, kQ = N / 4 * 4;
+#pragma unroll
+  for (int v = 0; v < kQ; v += 4) {
+    const u32x4_t q = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (byte & ~3) + v * 4, 0, 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[v + j] = q[j];
+  }
+#pragma unroll
+  for (int v = kQ; v < N; ++v) w[v] = __builtin_amdgcn_raw_buffer_load_b32(rs, (byte & ~3) + v * 4, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ void stream_unpack(const float*, int, const uint32_t (&w)[D], float (&c)[D]) {
+#pragma unroll
+  for (int d = 0; d < D; ++d) c[d] = __uint_as_float(w[d]);
+}
+// D odd: D + 1 halves cover the D coefficients from either half of the first dword.
+template <int D>
+__device__ __forceinline__ void stream_unpack(const __bf16* row, int o, const uint32_t (&w)[StreamRow<D>::kBf16],
+                                              float (&c)[D]) {
+  const bool odd = D % 2 && ((((uintptr_t)row & 2) + o * D * 2) & 2);
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    const float lo = __uint_as_float(d & 1 ? w[d / 2] & 0xffff0000u : w[d / 2] << 16);
+    if constexpr (D % 2) {
+      const float hi = __uint_as_float(d & 1 ? w[(d + 1) / 2] << 16 : w[d / 2] & 0xffff0000u);
+      c[d] = odd ? hi : lo;
+    } else {
+      c[d] = lo;
+    }
+  }
+}
+
+// part[chunk, slot, o] = the slot's expert output over one chunk of inputs.  A block
+// takes one expert, 64 outputs (a lane each) and a chunk; it finds its expert's
+// slots itself, makes the basis values of up to 8 rows in LDS (read as
+// broadcasts), and its four waves stream the chunk's coefficients.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_experts_stream(ExpertsArgs a) {
+  constexpr int kDeg = D - 1, kW = (kDeg + 3) / 4 * 4, kU = 4;
+  constexpr int kN = sizeof(T) == 4 ? StreamRow<D>::kF32 : StreamRow<D>::kBf16;
+  __shared__ int slots[kStreamMaxSlots], counts[4];
+  __shared__ __align__(16) float basis[kStreamInputs * kStreamRows * kW];
+  __shared__ float red[4][kStreamRows][64];
+  const ExpertsPlan& p = a.p;
+  const int oc = (p.O + 63) / 64;
+  int id = blockIdx.x;
+  const int chunk = id % p.chunks;
+  id /= p.chunks;
+  const int o = id % oc * 64 + (threadIdx.x & 63), e = id / oc;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  int n = 0;
+  for (int s0 = 0; s0 < (int)p.S; s0 += 256) {
+    const int s = s0 + tid;
+    const bool mine = s < (int)p.S && a.indices[s] == e;
+    const unsigned long long has = __ballot(mine);
+    if (lane == 0) counts[wave] = __popcll(has);
+    __syncthreads();
+    int at = n;
+    for (int w = 0; w < wave; ++w) at += counts[w];
+    if (mine) slots[at + __popcll(has & ((1ull << lane) - 1))] = s;
+    n += counts[0] + counts[1] + counts[2] + counts[3];
+    __syncthreads();
+  }
+  const int i0 = chunk * p.chunk_inputs, ni = p.I - i0 < p.chunk_inputs ? p.I - i0 : p.chunk_inputs;
+  const T* C = (const T*)a.coeffs + ((int64_t)e * p.I + i0) * p.O * D;
+  const int row_elems = p.O * D;
+  float* part = (float*)(a.ws + p.part_off) + (size_t)chunk * p.S * p.O;
+  for (int r0 = 0; r0 < n; r0 += kStreamRows) {
+    const int nr = n - r0 < kStreamRows ? n - r0 : kStreamRows;
+    for (int q = tid; q < ni * nr; q += 256) {
+      const int r = q / ni, i = q - r * ni;
+      const float t = tanhf((float)((const T*)a.x)[(int64_t)(slots[r0 + r] / p.k) * p.I + i0 + i]);
+      float* b = basis + (i * kStreamRows + r) * kW;
+      float ta = 1.0f, tb = t;
+#pragma unroll
+      for (int d = 0; d < kDeg; ++d) {
+        b[d] = tb;
+        const float tc = fmaf(t + t, tb, -ta);
+        ta = tb;
+        tb = tc;
+      }
+    }
+    __syncthreads();
+    float acc[kStreamRows] = {};
+    for (int i = wave; i < ni; i += 4 * kU) {
+      uint32_t w[kU][kN];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (i + 4 * u < ni) stream_load<D>(C + (int64_t)(i + 4 * u) * row_elems, row_elems * (int)sizeof(T), o, w[u]);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (i + 4 * u >= ni) break;
+        float c[D];
+        stream_unpack<D>(C + (int64_t)(i + 4 * u) * row_elems, o, w[u], c);
+        const float* b = basis + (i + 4 * u) * kStreamRows * kW;
+#pragma unroll
+        for (int r = 0; r < kStreamRows; ++r) {
+          if (r >= nr) break;
+          float s = c[0];
+#pragma unroll
+          for (int d = 0; d < kDeg; ++d) s = fmaf(c[d + 1], b[r * kW + d], s);
+          acc[r] += s;
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kStreamRows; ++r) red[wave][r][lane] = acc[r];
+    __syncthreads();
+    for (int r = wave; r < nr; r += 4)
+      if (o < p.O)
+        part[(size_t)slots[r0 + r] * p.O + o] = (red[0][r][lane] + red[1][r][lane]) + (red[2][r][lane] + red[3][r][lane]);
+    __syncthreads();
+  }
+}
+
+// y from the chunks' partial sums.
+template <typename T>
+__global__ __launch_bounds__(256) void k_experts_stream_sum(ExpertsArgs a) {
+  const ExpertsPlan& p = a.p;
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= p.T * p.O) return;
+  const int64_t t = q / p.O;
+  const int o = (int)(q - t * p.O);
+  const float* part = (const float*)(a.ws + p.part_off);
+  float v = 0.0f;
+  for (int j = 0; j < p.k; ++j) {
+    const int64_t s = t * p.k + j;
+    if (slot_expert(a, s) < 0) continue;
+    float z = 0.0f;
+#pragma unroll 8
+    for (int c = 0; c < p.chunks; ++c) z += part[((size_t)c * p.S + s) * p.O + o];
+    v += load_weight(a, s) * z;
+  }
+  ((T*)a.y)[q] = (T)v;
+}
+
+template <typename T>
+void stream_typed(const ExpertsArgs& a, hipStream_t st) {
+  const ExpertsPlan& p = a.p;
+  const dim3 grid((unsigned)(p.chunks * ((p.O + 63) / 64) * p.E)), block(256);
+  switch (p.D) {
+#define CKAN_STREAM_CASE(N) \
+  case N: hipLaunchKernelGGL((k_experts_stream<T, N>), grid, block, 0, st, a); break;
+    CKAN_STREAM_CASE(2) CKAN_STREAM_CASE(3) CKAN_STREAM_CASE(4) CKAN_STREAM_CASE(5) CKAN_STREAM_CASE(6)
+    CKAN_STREAM_CASE(7) CKAN_STREAM_CASE(8) CKAN_STREAM_CASE(9) CKAN_STREAM_CASE(10) CKAN_STREAM_CASE(11)
+    CKAN_STREAM_CASE(12) CKAN_STREAM_CASE(13) CKAN_STREAM_CASE(14) CKAN_STREAM_CASE(15) CKAN_STREAM_CASE(16)
+    CKAN_STREAM_CASE(17)
+#undef CKAN_STREAM_CASE
+  }
+  hipLaunchKernelGGL((k_experts_stream_sum<T>), dim3((unsigned)ceil_div(p.T * p.O, 256)), block, 0, st, a);
+}
+
 int grid_for(int64_t n) { return (int)(ceil_div(n, 256) < 4096 ? ceil_div(n, 256) : 4096); }
 
 template <typename T, int NP, int P>
@@ -837,6 +1029,13 @@ void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st) {
     if (a.p.P == 8) forward_typed<float, 2, 8>(a, keep, st);
     if (a.p.P == 16) forward_typed<float, 2, 16>(a, keep, st);
   }
+}
+
+void launch_experts_stream(const ExpertsArgs& a, hipStream_t st) {
+  if (a.p.bf16)
+    stream_typed<__bf16>(a, st);
+  else
+    stream_typed<float>(a, st);
 }
 
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st) {

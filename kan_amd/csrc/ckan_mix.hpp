@@ -82,7 +82,14 @@ struct ExpertsPlan {
   // backward workspace
   size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, dxs_off, bwd_bytes;
   int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
+  // the streaming forward (few slots): input chunks, inputs a chunk, partial sums
+  bool stream;
+  int chunks, chunk_inputs;
+  size_t part_off, stream_bytes;
 };
+constexpr int kStreamMaxSlots = 1024;  // a block keeps its expert's slots in LDS
+constexpr int kStreamInputs = 64;      // inputs whose basis values a block holds at once
+constexpr int kStreamRows = 8;         // rows a pass over the coefficients serves
 ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bool bf16, bool wbf16);
 
 struct ExpertsArgs {
@@ -93,6 +100,8 @@ struct ExpertsArgs {
   char *saved, *ws;
 };
 void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st);
+// The forward without a backward of few slots (p.stream).
+void launch_experts_stream(const ExpertsArgs& a, hipStream_t st);
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st);
 
 size_t ortho_workspace_bytes(int batch, int rows, int cols);

@@ -97,6 +97,7 @@ ExpertsPlan experts_plan(const ckan_experts_desc* d) {
 // Without a saved buffer its parts that the forward itself needs (all before the
 // packed dx operand) lead the workspace.
 size_t experts_fwd_ws(const ExpertsPlan& p, bool without_saved) {
+  if (without_saved && p.stream) return p.stream_bytes;
   return p.fwd_bytes + (without_saved ? p.cb_off : 0);
 }
 
@@ -187,11 +188,18 @@ int ckan_experts_forward(const ckan_experts_desc* desc, const void* x, const voi
   if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "experts forward workspace too small: %zu < %zu bytes", ws_bytes, need);
   if (!ws || !is_al16(ws) || !is_al16(saved))
     return fail(CKAN_ERR_INVALID_ARG, "experts_forward: workspace is NULL, or workspace or saved not 16-byte aligned");
+  if (!is_al16(x) || !is_al16(coeffs) || !is_al16(y))
+    return fail(CKAN_ERR_INVALID_ARG, "experts_forward: x, coeffs and y must be 16-byte aligned");
   a.x = x;
   a.coeffs = coeffs;
   a.indices = indices;
   a.weights = weights;
   a.y = y;
+  if (!saved && a.p.stream) {
+    a.ws = (char*)ws;
+    launch_experts_stream(a, reinterpret_cast<hipStream_t>(stream));
+    return check_launch("experts_forward");
+  }
   a.saved = saved ? (char*)saved : (char*)ws;
   a.ws = (char*)ws + (saved ? 0 : a.p.cb_off);
   launch_experts_forward(a, saved != nullptr, reinterpret_cast<hipStream_t>(stream));
@@ -214,6 +222,8 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
     return fail(CKAN_ERR_WORKSPACE, "experts backward workspace too small: %zu < %zu bytes", ws_bytes, a.p.bwd_bytes);
   if (!ws || !is_al16(ws) || !is_al16(saved))
     return fail(CKAN_ERR_INVALID_ARG, "experts_backward: workspace is NULL, or workspace or saved not 16-byte aligned");
+  if (!is_al16(dy) || !is_al16(dx) || !is_al16(dcoeffs))
+    return fail(CKAN_ERR_INVALID_ARG, "experts_backward: dy, dx and dcoeffs must be 16-byte aligned");
   a.indices = indices;
   a.weights = weights;
   a.dy = dy;

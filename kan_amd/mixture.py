@@ -35,6 +35,12 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
         raise RuntimeError(f"{name} must be float32 or bfloat16, got {t.dtype}") from None
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous at a 16-byte aligned address, as the library's vector loads need it."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class RouteFunction(torch.autograd.Function):
     """(weights, indices) of ``route``; differentiable in the logits."""
 
@@ -135,7 +141,7 @@ class ExpertsFunction(torch.autograd.Function):
         if not (need_x or need_c or need_w):
             return None, None, None, None, None
         dev = dy.device
-        dy = dy.to(dtype).contiguous()
+        dy = _aligned(dy.to(dtype))
         dx = torch.empty(xs, dtype=dtype, device=dev) if need_x else None
         dw = torch.empty(weights.shape, dtype=weights.dtype, device=dev) if need_w else None
         if desc.rows == 0:
@@ -181,7 +187,7 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
         raise RuntimeError(f"indices and weights must be [{x.shape[0]}, top_k], got {tuple(indices.shape)} and "
                            f"{tuple(weights.shape)}")
     desc = _lib.CkanExpertsDesc(x.shape[0], experts, indices.shape[1], in_dim, out_dim, dd - 1, code, wcode)
-    x, coeffs, indices, weights = (t.contiguous() for t in (x, coeffs, indices, weights))
+    x, coeffs, indices, weights = _aligned(x), _aligned(coeffs), indices.contiguous(), weights.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or coeffs.requires_grad or weights.requires_grad):
         return ExpertsFunction.apply(x, coeffs, weights, indices, desc)
     return _experts_forward(x, coeffs, indices, weights, desc, keep=False)[0]

@@ -48,14 +48,16 @@ def test_workspace_and_pointers():
     d = _desc()
     need, need_b = lib.ckan_experts_workspace_bytes(d, 0, 0), lib.ckan_experts_workspace_bytes(d, 1, 0)
     alone = lib.ckan_experts_workspace_bytes(d, 0, 1)
-    assert alone > need > 0 and need_b > 0 and lib.ckan_experts_saved_bytes(d) > 0
+    assert alone > 0 and need > 0 and need_b > 0 and lib.ckan_experts_saved_bytes(d) > 0
     inv, ws = _lib.CKAN_ERR_INVALID_ARG, _lib.CKAN_ERR_WORKSPACE
     assert lib.ckan_experts_forward(d, 256, 256, 256, 256, 256, 256, 256, need - 1, None) == ws
     assert lib.ckan_experts_forward(d, 256, 256, 256, 256, 256, None, 256, alone - 1, None) == ws
     assert lib.ckan_experts_forward(d, None, 256, 256, 256, 256, None, 256, alone, None) == inv
     assert lib.ckan_experts_forward(d, 256, 256, 256, 256, 256, 264, 256, need, None) == inv
     assert lib.ckan_experts_forward(d, 256, 256, 256, 256, 256, None, None, alone, None) == inv
+    assert lib.ckan_experts_forward(d, 256, 260, 256, 256, 256, None, 256, alone, None) == inv
     assert lib.ckan_experts_backward(d, 256, 256, 256, 256, 256, 256, 256, 256, need_b - 1, None) == ws
+    assert lib.ckan_experts_backward(d, 256, 256, 256, 258, 256, 256, 256, 256, need_b, None) == inv
     assert lib.ckan_experts_backward(d, 256, 256, None, 256, 256, 256, 256, 256, need_b, None) == inv
     assert lib.ckan_experts_backward(d, 256, 256, 256, 256, None, None, None, None, 0, None) == _lib.CKAN_OK
     z = _desc(rows=0)

@@ -186,6 +186,13 @@ def test_layouts_streams_partial_gradients_and_repeats():
     y = kan_amd.functional.kan_experts(xs.cuda()[:, 10:34], c.permute(3, 0, 1, 2).contiguous().cuda().permute(1, 2, 3, 0),
                                        idx.t().contiguous().cuda().t(), w.t().contiguous().cuda().t())
     assert torch.equal(y, base[0])
+    # contiguous tensors at addresses that no vector load can take
+    off = torch.zeros(150 * 24 + 1)
+    off[1:] = x.reshape(-1)
+    offc = torch.zeros(c.numel() + 1)
+    offc[1:] = c.reshape(-1)
+    y = kan_amd.functional.kan_experts(off.cuda()[1:].view(150, 24), offc.cuda()[1:].view(c.shape), idx.cuda(), w.cuda())
+    assert torch.equal(y, base[0])
     # another stream
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -208,6 +215,27 @@ def test_layouts_streams_partial_gradients_and_repeats():
     assert y.shape == (0, 40)
     y.sum().backward()
     assert (cd.grad == 0).all() and e.grad.shape == (0, 24)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("degree", [1, 2, 3, 5, 7, 8, 10, 11, 13, 14, 15, 16])
+def test_few_slots(degree, dtype):
+    """The streaming forward: odd output counts put bf16 rows on odd halves of a dword."""
+    def edit(x, c, idx, w, dy):
+        idx = idx.clone()
+        idx[0] = -1
+        idx[1:20, 0] = 1  # more rows of one expert than a pass over its coefficients serves
+        return x, c, idx, w, dy
+
+    _compare(21, 67, 77, degree, 3, 2, dtype, seed=degree, edit=edit)
+
+
+def test_streaming_and_tile_forwards_agree():
+    """The same rows through calls of few slots and one of many."""
+    x, c, idx, w, _ = (v.cuda() for v in _inputs(700, 130, 200, 8, 4, 2, torch.float32, 11))
+    whole = kan_amd.functional.kan_experts(x, c, idx, w)
+    parts = torch.cat([kan_amd.functional.kan_experts(x[r:r + 7], c, idx[r:r + 7], w[r:r + 7]) for r in range(0, 700, 7)])
+    assert ((whole - parts).norm() / whole.norm()).item() <= 2 * TOL[torch.float32]
 
 
 def test_one_expert_is_the_layer():
