@@ -62,7 +62,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.cb_off = take((size_t)E * p.Ip * deg * p.Op * 2 * p.NP);
   p.saved_bytes = off;
   off = 0;
-  p.bias_parts = (int)ceil_div(p.Ip, 256);
+  p.bias_parts = (int)ceil_div(p.Ip, kPackInputs);
   p.hist_off = take((size_t)p.plan_blocks * E * 4);
   p.cmax_off = take((size_t)E * kMaxParts * 4);
   p.cf_off = take((size_t)E * p.Op * p.Ip * p.P * 2 * p.NP);
@@ -74,6 +74,8 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.gr_off = take((size_t)p.R * p.Op * 2 * p.NP);
   p.gt_off = take((size_t)p.R * p.Op * 2 * p.NP);
   p.gsum_off = take((size_t)(p.R / 32) * p.Op * 4);
+  p.gtot_off = take((size_t)E * p.Op * 4);
+  p.ts_off = take((size_t)p.R * p.Ip * 4);
   p.dxs_off = take((size_t)p.R * I * 4);
   p.bwd_bytes = off;
   // Streaming: up to 16 slots an expert on average.  Its blocks read the coefficients
@@ -237,18 +239,76 @@ __device__ __forceinline__ float block_max_256(float v, float* red) {
   return v;
 }
 
+// Sixteen bytes of T as floats: 8 bf16 or 4 fp32 values.
+template <typename T> struct Vec16 { static constexpr int N = 16 / (int)sizeof(T); };
+__device__ __forceinline__ void widen(u32x4_t q, float (&v)[4], const float*) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(q[j]);
+}
+__device__ __forceinline__ void widen(u32x4_t q, float (&v)[8], const __bf16*) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(q[j] << 16);
+    v[2 * j + 1] = __uint_as_float(q[j] & 0xffff0000u);
+  }
+}
+
+// The largest finite |C| of each expert by blocks; four 16-byte loads in flight a
+// thread (2-byte loads took 450 us for 151 MB where these take 35).
 template <typename T>
 __global__ __launch_bounds__(256) void k_experts_cmax(ExpertsArgs a) {
   __shared__ float red[4];
+  constexpr int N = Vec16<T>::N;
   const ExpertsPlan& p = a.p;
   const int e = blockIdx.y;
   const int64_t n = (int64_t)p.I * p.O * p.D;
   const T* c = (const T*)a.coeffs + e * n;
+  // the elements before the expert's first 16-byte boundary and past its last
+  int64_t head = ((16 - ((uintptr_t)c & 15)) & 15) / sizeof(T);
+  if (head > n) head = n;
+  const int64_t nv = (n - head) / N, step = (int64_t)kMaxParts * 256;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const u32x4_t* q = (const u32x4_t*)(c + head);
   float m = 0.0f;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)kMaxParts * 256)
-    m = fmaxf(m, finite_abs((float)c[q]));
+  for (int64_t i = first; i < nv; i += 4 * step) {
+    u32x4_t w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * step < nv) w[u] = q[i + u * step];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * step < nv) {
+        float v[N];
+        widen(w[u], v, c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, finite_abs(v[j]));
+      }
+  }
+  if (first < head) m = fmaxf(m, finite_abs((float)c[first]));
+  if (head + nv * N + first < n) m = fmaxf(m, finite_abs((float)c[head + nv * N + first]));
   m = block_max_256(m, red);
   if (threadIdx.x == 0) ((float*)(a.ws + p.cmax_off))[e * kMaxParts + blockIdx.x] = m;
+}
+
+// Blocks are spread over the eight XCDs in turn; this gives XCD x the x-th eighth of
+// the work, so that blocks which share operands share an L2.  Returns n or more
+// for the blocks of the round-up.
+__device__ __forceinline__ int xcd_chunk(int block, int n) {
+  const int per = (n + 7) / 8;
+  const int v = (block & 7) * per + (block >> 3);
+  return (block >> 3) < per ? v : n;
+}
+int xcd_grid(int64_t n) { return (int)((n + 7) / 8 * 8); }
+
+// (tile, column block) of a product's block: 16 tiles go through one column block
+// before the next, so the 64 blocks that an XCD runs at once read about four
+// column blocks of the packed coefficients and 16 tiles of rows.
+__device__ __forceinline__ void tile_and_column(int v, int tiles, int cols, int& tile, int& col) {
+  constexpr int G = 16;
+  const int group = v / (G * cols), in = v - group * G * cols;
+  const int size = tiles - group * G < G ? tiles - group * G : G;
+  col = in / size;
+  tile = group * G + in - col * size;
 }
 
 // Inputs a stage of the forward takes, and its k-blocks (see k_experts_fwd).
@@ -260,35 +320,64 @@ template <int NP, int P> struct FwdStage {
 // Cf: the forward's operand, rows o, k in stages of IN inputs: half g of a lane
 // pair holds inputs g IN/2.., P degrees each, eight values a k-block.  Cb: the dx
 // operand, rows i and k = o for each degree d, scaled by d.  And the sums over the
-// inputs of the T_0 coefficients.  A block takes 32 outputs and 256 inputs of an
-// expert, 16 inputs at a time through LDS.
-template <typename T, int NP, int P>
+// inputs of the T_0 coefficients.  A block takes 32 outputs and kPackInputs inputs of
+// an expert, 16 inputs at a time through LDS, the next 16 inputs' loads in flight
+// meanwhile.
+template <typename T, int NP, int P, bool VEC>
 __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backward) {
   extern __shared__ float sm[];
+  __shared__ float red[4];
   using FS = FwdStage<NP, P>;
+  constexpr int N = VEC ? Vec16<T>::N : 1;
+  constexpr int kLoads = 16 * 32 * 17 / N / 256 + 1;  // at degree 16
   const ExpertsPlan& p = a.p;
   const int e = blockIdx.z, ob = blockIdx.y, tid = threadIdx.x;
   const int D = p.D, W = 32 * D + 1;  // a row of the tile: 32 outputs, D coefficients each
   const float* cmax = (const float*)(a.ws + p.cmax_off) + e * kMaxParts;
-  float m = 0.0f;
-  for (int i = 0; i < kMaxParts; ++i) m = fmaxf(m, cmax[i]);
   // d C with d <= 16 has to fit too: the largest |C| below 2^11
-  const float scale = range_scale(m, 11);
+  const float scale = range_scale(block_max_256(cmax[tid % kMaxParts], red), 11);
   if (blockIdx.x == 0 && ob == 0 && tid == 0) ((float*)(a.saved + p.scale_off))[e] = scale;
   const T* C = (const T*)a.coeffs + (int64_t)e * p.I * p.O * D;
   char* cf = a.ws + p.cf_off + (size_t)e * p.Op * p.Ip * P * 2 * NP;
   char* cb = a.saved + p.cb_off + (size_t)e * p.Ip * p.deg * p.Op * 2 * NP;
   const int KBf = p.Ip * P / 16, KBo = p.Op / 16;
   const int o0 = ob * 32, no = p.O - o0 < 32 ? p.O - o0 : 32;
+  const int vrow = 32 * D / N, loads = (16 * vrow + 255) / 256;  // vectors of an input, of a thread
   float bias = 0.0f;
-  const int i_end = (int)(blockIdx.x + 1) * 256 < p.Ip ? (int)(blockIdx.x + 1) * 256 : p.Ip;
-  for (int i0 = blockIdx.x * 256; i0 < i_end; i0 += 16) {
+  const int i_end = (int)(blockIdx.x + 1) * kPackInputs < p.Ip ? (int)(blockIdx.x + 1) * kPackInputs : p.Ip;
+  u32x4_t w[VEC ? kLoads : 1];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      if (u >= loads) break;
+      const int q = tid + u * 256, i = q / vrow, f = (q - i * vrow) * N;
+      w[u] = u32x4_t{0, 0, 0, 0};
+      if (i < 16 && i0 + i < p.I && f < no * D) w[u] = *(const u32x4_t*)(C + ((int64_t)(i0 + i) * p.O + o0) * D + f);
+    }
+  };
+  if constexpr (VEC) load(blockIdx.x * kPackInputs);
+  for (int i0 = blockIdx.x * kPackInputs; i0 < i_end; i0 += 16) {
     __syncthreads();
-    for (int q = tid; q < 16 * 32 * D; q += 256) {
-      const int i = q / (32 * D), f = q - i * 32 * D;
-      sm[i * W + f] = i0 + i < p.I && f < no * D ? (float)C[((int64_t)(i0 + i) * p.O + o0) * D + f] : 0.0f;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        if (u >= loads) break;
+        const int q = tid + u * 256, i = q / vrow, f = (q - i * vrow) * N;
+        if (i >= 16) continue;
+        float v[N];
+        widen(w[u], v, C);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sm[i * W + f + j] = v[j];
+      }
+    } else {
+      for (int q = tid; q < 16 * 32 * D; q += 256) {
+        const int i = q / (32 * D), f = q - i * 32 * D;
+        sm[i * W + f] = i0 + i < p.I && f < no * D ? (float)C[((int64_t)(i0 + i) * p.O + o0) * D + f] : 0.0f;
+      }
     }
     __syncthreads();
+    if constexpr (VEC)
+      if (i0 + 16 < i_end) load(i0 + 16);
     if (tid < 32)
       for (int i = 0; i < 16; ++i) bias += sm[i * W + tid * D];
     // Cf: P k-blocks of 64 lanes
@@ -339,10 +428,13 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   constexpr int kT = 128 * TB, kTChunks = kT / 1024, kB = 2 * FN * KS * NP;  // 1 KiB chunks
   constexpr int kStage = kT + kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
-  const int cols = (p.O + 64 * FN - 1) / (64 * FN);
-  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[blockIdx.x / cols];
+  const int cols = (p.O + 64 * FN - 1) / (64 * FN), v = xcd_chunk(blockIdx.x, p.tiles * cols);
+  if (v >= p.tiles * cols) return;
+  int ti, cb;
+  tile_and_column(v, p.tiles, cols, ti, cb);
+  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
   if (tile.x < 0) return;
-  const int e = tile.x, row0 = tile.y, cb = blockIdx.x % cols;
+  const int e = tile.x, row0 = tile.y;
   const int end = ((const int*)(a.saved + p.off_off))[e + 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave >> 1, wn = wave & 1, g = lane >> 5;
@@ -594,10 +686,13 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
   extern __shared__ char lds[];
   typedef NtTile<NP, NP, 2, 2, 2, 4, 2, 2> Tile;
   const ExpertsPlan& p = a.p;
-  const int cols = (p.Ip + 63) / 64;
-  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[blockIdx.x / cols];
+  const int cols = (p.Ip + 63) / 64, v = xcd_chunk(blockIdx.x, p.tiles * cols);
+  if (v >= p.tiles * cols) return;
+  int ti, cb;
+  tile_and_column(v, p.tiles, cols, ti, cb);
+  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
   if (tile.x < 0) return;
-  const int e = tile.x, row0 = tile.y, ib0 = blockIdx.x % cols * 2;
+  const int e = tile.x, row0 = tile.y, ib0 = cb * 2;
   const int end = ((const int*)(a.saved + p.off_off))[e + 1];
   const int KB = p.Op / 16, nib = p.Ip / 32;
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
@@ -607,7 +702,18 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
   const int i = (ib0 + (wave & 1)) * 32 + (lane & 31);
   const int* tok = (const int*)(a.saved + p.tok_off);
   const float* t = (const float*)(a.saved + p.t_off);
-  float dx[2][16] = {};
+  // every tanh value of the epilogue, asked for before the products (32 loads in
+  // flight; one at a time behind a branch they took longer than the products)
+  float x[2][16], dx[2][16] = {};
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      int r = row0 + (wave >> 1) * 64 + m * 32 + acc_row(q, g);
+      r = r < end ? r : end - 1;
+      const int k = tok[r];
+      x[m][q] = t[(int64_t)(k >= 0 ? k : 0) * p.Ip + (i < p.Ip ? i : p.Ip - 1)];
+    }
   for (int d0 = 0; d0 < p.deg; d0 += 4) {
     f32x16_t acc[2][4] = {};
     Tile::run(A, [&](int r) {
@@ -617,32 +723,27 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
       return cbase + ((size_t)ib * p.deg + d) * pitch;
     }, 0, KB / 2, lds, acc);
     const int nd = p.deg - d0 < 4 ? p.deg - d0 : 4;
-    if (i < p.I) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int r = row0 + (wave >> 1) * 64 + m * 32 + acc_row(q, g);
-          if (r >= end) continue;
-          const int k = tok[r];
-          const float x = k >= 0 ? t[(int64_t)k * p.Ip + i] : 0.0f, x2 = x + x;
-          float ua = 0.0f, ub = 1.0f;  // U_{-1}, U_0
-          for (int d = 0; d < d0; ++d) {
-            const float c = fmaf(x2, ub, -ua);
-            ua = ub;
-            ub = c;
-          }
-          float s = 0.0f;
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            if (d < nd) s = fmaf(acc[m][d][q], ub, s);
-            const float c = fmaf(x2, ub, -ua);
-            ua = ub;
-            ub = c;
-          }
-          dx[m][q] = fmaf(s, 1.0f - x * x, dx[m][q]);
+      for (int q = 0; q < 16; ++q) {
+        const float x2 = x[m][q] + x[m][q];
+        float ua = 0.0f, ub = 1.0f;  // U_{-1}, U_0
+        for (int d = 0; d < d0; ++d) {
+          const float c = fmaf(x2, ub, -ua);
+          ua = ub;
+          ub = c;
         }
-    }
+        float s = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          if (d < nd) s = fmaf(acc[m][d][q], ub, s);
+          const float c = fmaf(x2, ub, -ua);
+          ua = ub;
+          ub = c;
+        }
+        dx[m][q] = fmaf(s, 1.0f - x[m][q] * x[m][q], dx[m][q]);
+      }
   }
   if (i >= p.I) return;
   const float ic = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
@@ -657,27 +758,67 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
     }
 }
 
-// dC of 32 inputs x 8 degrees x 128 outputs of an expert a block; waves of 32 inputs x
-// 4 degrees x 64 outputs.  A stage is 32 rows: each thread makes four degrees of
-// eight rows of one input into LDS for the next stage while the matrix
-// instructions work on this one.
-template <typename T, int NP>
-__global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
-  extern __shared__ char lds[];
-  constexpr int KS = 2, kA = 8 * KS * NP, kB = 4 * KS * NP;  // 1 KiB chunks of a stage
-  constexpr int kStage = (kA + kB) * kPlaneBytes;
+// The T_0 column of dC: each expert's sum of g over its rows, from the row blocks'
+// sums; four running sums a column, eight loads in flight.
+__global__ __launch_bounds__(256) void k_experts_gsum(ExpertsArgs a) {
+  __shared__ float red[4][64];
   const ExpertsPlan& p = a.p;
-  const int nob = (p.O + 127) / 128, nib = p.Ip / 32, ndc = (p.deg + 7) / 8;
-  int id = blockIdx.x;
+  const int* off = (const int*)(a.saved + p.off_off);
+  const int e = blockIdx.x, o = blockIdx.y * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const float* src = (const float*)(a.ws + p.gsum_off) + o;
+  float s = 0.0f;
+  if (o < p.Op) {
+#pragma unroll 8
+    for (int rb = off[e] / 32 + w; rb < off[e + 1] / 32; rb += 4) s += src[(size_t)rb * p.Op];
+  }
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && o < p.Op)
+    ((float*)(a.ws + p.gtot_off))[(size_t)e * p.Op + o] =
+        (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// The rows' tanh values in the order that dC reads them: for 32 inputs and 32 rows one
+// run of [4 row groups][32 inputs][8 rows], zeros for pad rows.
+__global__ __launch_bounds__(256) void k_experts_tsort(ExpertsArgs a) {
+  __shared__ float tile[32][33];
+  const ExpertsPlan& p = a.p;
+  const int rb = blockIdx.x, ib = blockIdx.y, tid = threadIdx.x;
+  if (rb * 32 >= ((const int*)(a.saved + p.off_off))[p.E]) return;
+  const int* tok = (const int*)(a.saved + p.tok_off) + rb * 32;
+  const float* t = (const float*)(a.saved + p.t_off) + ib * 32;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = u * 8 + (tid >> 5), k = tok[r];
+    tile[r][tid & 31] = k >= 0 ? t[(int64_t)k * p.Ip + (tid & 31)] : 0.0f;
+  }
+  __syncthreads();
+  f32x4_t v;
+  const int g = tid >> 6, i = (tid >> 1) & 31, h = tid & 1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = tile[g * 8 + h * 4 + j][i];
+  ((f32x4_t*)(a.ws + p.ts_off))[((size_t)ib * (p.R / 32) + rb) * 256 + tid] = v;
+}
+
+// dC of NI x 32 inputs x DB degrees x 128 outputs of an expert a block (NI DB = 8 row
+// blocks); waves of 4 row blocks x 64 outputs.  A stage is 32 rows.  The tanh
+// values and g arrive by copies; each thread makes the basis values of 32 (row,
+// degree) pairs of one input into LDS for the next stage while the matrix
+// instructions work on this one.
+template <typename T, int NP, int DB>
+__global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
+  extern __shared__ char lds[];
+  constexpr int KS = 2, NI = 8 / DB, kA = 8 * KS * NP, kB = 4 * KS * NP, kT = 4 * NI;  // 1 KiB chunks of a stage
+  constexpr int kBAt = 2 * kA * kPlaneBytes, kTAt = kBAt + 2 * kB * kPlaneBytes;
+  const ExpertsPlan& p = a.p;
+  const int nob = (p.O + 127) / 128, nib = p.Ip / 32, nbi = (nib + NI - 1) / NI;
+  int id = xcd_chunk(blockIdx.x, p.E * nbi * nob);
+  if (id >= p.E * nbi * nob) return;
   const int ob = id % nob;
   id /= nob;
-  const int ib = id % nib;
-  id /= nib;
-  const int dc = id % ndc, e = id / ndc;
+  const int ib0 = id % nbi * NI, e = id / nbi;
   const int* off = (const int*)(a.saved + p.off_off);
   const int row0 = off[e], nst = (off[e + 1] - row0) / 32;
-  const int* tok = (const int*)(a.saved + p.tok_off);
-  const float* t = (const float*)(a.saved + p.t_off);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wd = wave >> 1, wo = wave & 1;
@@ -685,111 +826,151 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
   const int KBr = (int)(p.R / 16), nb = p.Op / 32;
   const size_t pitch = (size_t)KBr * NP * kPlaneBytes;
   const char* gt = a.ws + p.gt_off + ((size_t)(row0 / 16) * NP) * kPlaneBytes;
-  // the making thread's input, row group and degrees
-  const int mi = tid & 31, mr = (tid >> 5) & 3, mh = tid >> 7;
-  const float* tcol = t + ib * 32 + mi;
-  float tv[8];
-  auto load_t = [&](int s) {
-    const int* tk = tok + row0 + s * 32 + mr * 8;
+  const char* ts = a.ws + p.ts_off + ((size_t)(row0 / 32)) * 4096;
+  // the making thread's input, and its rows: DB 8: four rows of a group of eight,
+  // DB 4: the whole group
+  const int mq = DB == 8 ? tid >> 1 : tid;
+  const int mi = mq & 31, mr = (mq >> 5) & 3, mib = mq >> 7, mh = DB == 8 ? tid & 1 : 0;
+  constexpr int MR = DB == 8 ? 4 : 8;
+  auto make = [&](int s) {
+    const float* src = (const float*)(lds + kTAt + (s & 1) * kT * kPlaneBytes) + ((mib * 4 + mr) * 32 + mi) * 8 + mh * 4;
+    float tv[MR], ta[MR], tb[MR];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = tk[j];
-      tv[j] = k >= 0 ? tcol[(int64_t)k * p.Ip] : 0.0f;
-    }
-  };
-  auto make = [&](char* buf) {
-    float ta[8], tb[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < MR; ++j) {
+      tv[j] = src[j];
       ta[j] = 1.0f;
       tb[j] = tv[j];
     }
-    // T_{d1-1}, T_{d1} for the thread's first degree d1 = dc 8 + mh 4 + 1
-    for (int d = 0; d < dc * 8 + mh * 4; ++d)
+    if (d0) {  // 8: T_8 and T_9 by products, T_{m+n} = 2 T_m T_n - T_{m-n}
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = fmaf(tv[j] + tv[j], tb[j], -ta[j]);
-        ta[j] = tb[j];
-        tb[j] = c;
+      for (int j = 0; j < MR; ++j) {
+        const float x = tv[j], t2 = fmaf(x + x, x, -1.0f), t3 = fmaf(x + x, t2, -x), t4 = fmaf(t2 + t2, t2, -1.0f);
+        ta[j] = fmaf(t4 + t4, t4, -1.0f);
+        tb[j] = fmaf(t4 + t4, fmaf(t2 + t2, t3, -x), -x);
+      }
+    }
+    char* dst = lds + (s & 1) * kA * kPlaneBytes + (mi + 32 * (mr & 1)) * 16 + mh * 8;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      char* at = dst + ((((mib * DB + d) * KS + (mr >> 1)) * NP)) * kPlaneBytes;
+      if constexpr (MR == 8) {
+        const Planes8<NP> f = to_planes8<NP>(tb);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) *(f16x8_t*)(at + k * kPlaneBytes) = f.p[k];
+      } else {
+        const Planes4<NP> f = to_planes4<NP>(tb);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) *(f16x4_t*)(at + k * kPlaneBytes) = f.p[k];
       }
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const Planes8<NP> f = to_planes8<NP>(tb);
-      char* dst = buf + (((mh * 4 + d) * KS + (mr >> 1)) * NP) * kPlaneBytes + (mi + 32 * (mr & 1)) * 16;
-#pragma unroll
-      for (int k = 0; k < NP; ++k) *(f16x8_t*)(dst + k * kPlaneBytes) = f.p[k];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < MR; ++j) {
         const float c = fmaf(tv[j] + tv[j], tb[j], -ta[j]);
         ta[j] = tb[j];
         tb[j] = c;
       }
     }
   };
-  auto copy = [&](int s, uint32_t at) {
+  auto copy_g = [&](int s) {
 #pragma unroll
     for (int i = 0; i < kB / 4; ++i) {
       const int c = i * 4 + wave;
       int rb = ob * 4 + c / (KS * NP);
       rb = rb < nb ? rb : nb - 1;
-      dma16s(gt + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + (kA + c) * kPlaneBytes);
+      dma16s(gt + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16,
+             l0 + kBAt + ((s & 1) * kB + c) * kPlaneBytes);
+    }
+  };
+  auto copy_t = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < kT / 4; ++i) {
+      int ib = ib0 + i;
+      ib = ib < nib ? ib : nib - 1;
+      dma16s(ts + ((size_t)ib * (p.R / 32) + s) * 4096 + wave * 1024, lane * 16,
+             l0 + kTAt + ((s & 1) * kT + i * 4 + wave) * kPlaneBytes);
     }
   };
   f32x16_t acc[4][2] = {};
   if (nst > 0) {
-    copy(0, l0);
-    load_t(0);
-    make(lds);
-    if (nst > 1) load_t(1);
+    copy_t(0);
+    copy_g(0);
+    if (nst > 1) copy_t(1);
+    wait_vm<0>();
+    block_barrier();
+    make(0);
   }
   for (int s = 0; s < nst; ++s) {
     wait_vm<0>();
     wait_lds();
     block_barrier();
-    if (s + 1 < nst) {
-      copy(s + 1, l0 + ((s + 1) & 1) * kStage);
-      make(lds + ((s + 1) & 1) * kStage);
-      if (s + 2 < nst) load_t(s + 2);
-    }
-    const char* buf = lds + (s & 1) * kStage;
+    if (s + 1 < nst) copy_g(s + 1);
+    if (s + 2 < nst) copy_t(s + 2);  // over stage s, which was made from before the barrier
+    if (s + 1 < nst) make(s + 1);
+    const char* buf = lds + (s & 1) * kA * kPlaneBytes;
+    const char* bufb = lds + kBAt + (s & 1) * kB * kPlaneBytes;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       f16x8_t fa[4][NP], fb[2][NP];
 #pragma unroll
       for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-          fa[m][q] = lds_frag(buf + (((wd * 4 + m) * KS + k) * NP + q) * kPlaneBytes, lane);
+        for (int q = 0; q < NP; ++q) fa[m][q] = lds_frag(buf + (((wd * 4 + m) * KS + k) * NP + q) * kPlaneBytes, lane);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-          fb[n][q] = lds_frag(buf + (kA + ((wo * 2 + n) * KS + k) * NP + q) * kPlaneBytes, lane);
+        for (int q = 0; q < NP; ++q) fb[n][q] = lds_frag(bufb + (((wo * 2 + n) * KS + k) * NP + q) * kPlaneBytes, lane);
       mfma_planes<NP, NP, 4, 2>(fa, fb, acc);
     }
   }
+  // The tile leaves through LDS, 8 inputs (of each row block) at a time, so that an
+  // input's coefficients of 128 outputs are stored as they lie in memory.
+  wait_lds();
+  block_barrier();
+  const int nd = p.deg - d0 < DB ? p.deg - d0 : DB, lead = d0 == 0 ? 1 : 0, w = nd + lead;  // columns here, T_0 first
+  const int no = p.O - ob * 128 < 128 ? p.O - ob * 128 : 128;
   const float inv = nst > 0 ? 1.0f / ((const float*)(a.ws + p.gscale_off))[e] : 1.0f;
-  const float* gsum = (const float*)(a.ws + p.gsum_off);
+  const float* gtot = (const float*)(a.ws + p.gtot_off) + (size_t)e * p.Op + ob * 128;
   T* out = (T*)a.dcoeffs + (int64_t)e * p.I * p.O * p.D;
+  float* tile = (float*)lds;  // [NI][8][128][w]
+  const bool whole = w == p.D && (int64_t)p.O * p.D % 4 == 0 && no * w % 4 == 0;
+  const int wib = DB == 8 ? 0 : wd, wd1 = DB == 8 ? wd * 4 : 0;  // the wave's row block of inputs, its degrees
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int o = ob * 128 + wo * 64 + n * 32 + (lane & 31);
-    if (o >= p.O) continue;
-    float s0 = 0.0f;  // T_0: the same for every input
-    if (dc == 0 && wd == 0)
-      for (int s = 0; s < nst; ++s) s0 += gsum[(size_t)(row0 / 32 + s) * p.Op + o];
+  for (int h = 0; h < 4; ++h) {
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int i = ib * 32 + acc_row(q, g);
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (wd1 + m < nd)
+            tile[((wib * 8 + g * 4 + j) * 128 + wo * 64 + n * 32 + (lane & 31)) * w + lead + wd1 + m] = acc[m][n][h * 4 + j] * inv;
+    if (lead)
+      for (int q = tid; q < NI * 8 * 128; q += 256) tile[q * w] = (q & 127) < no ? gtot[q & 127] : 0.0f;
+    __syncthreads();
+    for (int r = wave; r < NI * 8; r += 4) {
+      const int i = (ib0 + (r >> 3)) * 32 + 8 * h + (r & 7);
       if (i >= p.I) continue;
-      T* dst = out + ((int64_t)i * p.O + o) * p.D;
-      if (dc == 0 && wd == 0) dst[0] = (T)s0;
+      const float* src = tile + r * 128 * w;
+      T* dst = out + ((int64_t)i * p.O + ob * 128) * p.D;
+      if (whole) {
+        for (int q = lane * 4; q < no * w; q += 256) {
+          const f32x4_t v = *(const f32x4_t*)(src + q);
+          if constexpr (sizeof(T) == 4) {
+            *(f32x4_t*)(dst + q) = v;
+          } else {
+            bf16x4_t b;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int d = dc * 8 + wd * 4 + m + 1;
-        if (d <= p.deg) dst[d] = (T)(acc[m][n][q] * inv);
+            for (int j = 0; j < 4; ++j) b[j] = (__bf16)v[j];
+            *(bf16x4_t*)(dst + q) = b;
+          }
+        }
+      } else {
+        for (int q = lane; q < no * w; q += 64) {
+          const int o = q / w;
+          dst[(int64_t)o * p.D + d0 + (1 - lead) + q - o * w] = (T)src[q];
+        }
       }
     }
+    __syncthreads();
   }
 }
 
@@ -982,16 +1163,31 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
   hipLaunchKernelGGL((k_experts_tanh<T>), dim3(grid_for(p.T * p.Ip)), dim3(256), 0, st, a);
   hipLaunchKernelGGL((k_experts_cmax<T>), dim3(kMaxParts, p.E), dim3(256), 0, st, a);
   const size_t pack_lds = (size_t)16 * (32 * p.D + 1) * sizeof(float);
-  hipLaunchKernelGGL((k_experts_pack<T, NP, P>), dim3(p.bias_parts, p.Op / 32, p.E), dim3(256), pack_lds, st, a, keep);
+  const dim3 pack_grid(p.bias_parts, p.Op / 32, p.E);
+  // 16-byte loads where every input's row of coefficients begins at such a boundary
+  if (p.O * p.D % Vec16<T>::N == 0)
+    hipLaunchKernelGGL((k_experts_pack<T, NP, P, true>), pack_grid, dim3(256), pack_lds, st, a, keep);
+  else
+    hipLaunchKernelGGL((k_experts_pack<T, NP, P, false>), pack_grid, dim3(256), pack_lds, st, a, keep);
   constexpr int FN = 4;
   using FS = FwdStage<NP, P>;
   constexpr int lds = 2 * (128 * FS::IN * 4 + 2 * FN * FS::KS * NP * kPlaneBytes);
   static std::atomic<uint32_t> done;
   ensure_lds_limit((const void*)k_experts_fwd<NP, P, FN>, lds, done);
   const int cols = (p.O + 64 * FN - 1) / (64 * FN);
-  hipLaunchKernelGGL((k_experts_fwd<NP, P, FN>), dim3((unsigned)(p.tiles * cols)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((k_experts_fwd<NP, P, FN>), dim3(xcd_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
   hipLaunchKernelGGL((k_experts_gather<T, true>), dim3(grid_for(p.T * p.O)), dim3(256), 0, st, a,
                      (const float*)(a.saved + p.z_off), a.y, p.O);
+}
+
+template <typename T, int NP, int DB>
+void launch_dc(const ExpertsArgs& a, int d0, hipStream_t st) {
+  constexpr int NI = 8 / DB, ring = 2 * ((8 + 4) * 2 * NP + 4 * NI) * kPlaneBytes;
+  constexpr int tile = NI * 8 * 128 * (DB + 1) * 4, lds = ring > tile ? ring : tile;
+  static std::atomic<uint32_t> done;
+  ensure_lds_limit((const void*)k_experts_dc<T, NP, DB>, lds, done);
+  const int64_t blocks = (int64_t)a.p.E * ceil_div(a.p.Ip / 32, NI) * ceil_div(a.p.O, 128);
+  hipLaunchKernelGGL((k_experts_dc<T, NP, DB>), dim3(xcd_grid(blocks)), dim3(256), lds, st, a, d0);
 }
 
 template <typename T, int NP>
@@ -1004,16 +1200,17 @@ void backward_typed(const ExpertsArgs& a, hipStream_t st) {
     constexpr int lds = NtTile<NP, NP, 2, 2, 2, 4, 2, 2>::kLdsBytes;
     static std::atomic<uint32_t> done;
     ensure_lds_limit((const void*)k_experts_dx<NP>, lds, done);
-    hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)(p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_experts_dx<NP>), dim3(xcd_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
     hipLaunchKernelGGL((k_experts_gather<T, false>), dim3(grid_for(p.T * p.I)), dim3(256), 0, st, a,
                        (const float*)(a.ws + p.dxs_off), a.dx, p.I);
   }
   if (a.dcoeffs) {
-    constexpr int lds = 2 * (8 + 4) * 2 * NP * kPlaneBytes;
-    static std::atomic<uint32_t> done;
-    ensure_lds_limit((const void*)k_experts_dc<T, NP>, lds, done);
-    const unsigned blocks = (unsigned)p.E * ((p.deg + 7) / 8) * (p.Ip / 32) * ((p.O + 127) / 128);
-    hipLaunchKernelGGL((k_experts_dc<T, NP>), dim3(blocks), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(k_experts_gsum, dim3(p.E, (p.Op + 63) / 64), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_experts_tsort, dim3((unsigned)(p.R / 32), p.Ip / 32), dim3(256), 0, st, a);
+    // runs of 8 degrees, and of 4 where no more are left
+    int d0 = 0;
+    for (; p.deg - d0 > 4; d0 += 8) launch_dc<T, NP, 8>(a, d0, st);
+    if (d0 < p.deg) launch_dc<T, NP, 4>(a, d0, st);
   }
 }
 

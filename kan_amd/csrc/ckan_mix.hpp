@@ -56,7 +56,8 @@ constexpr int kExpertsMaxDegree = 16;
 constexpr int kExpertsMaxTopK = 64;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBlocks = 256;       // at most: a block's share of the slots grows past that
-constexpr int kMaxParts = 32;          // blocks an expert that look for its largest coefficient
+constexpr int kMaxParts = 128;         // blocks an expert that look for its largest coefficient
+constexpr int kPackInputs = 128;       // inputs a block of the pack takes
 constexpr int kGradBlocks = 1024;      // blocks that look for the largest upstream gradients
 
 // Sizes and the layout of the buffers.  "Rows" are the kept slots sorted by expert,
@@ -80,7 +81,7 @@ struct ExpertsPlan {
   // forward workspace
   size_t hist_off, cmax_off, cf_off, bias_off, fwd_bytes;
   // backward workspace
-  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, dxs_off, bwd_bytes;
+  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bwd_bytes;
   int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
   // the streaming forward (few slots): input chunks, inputs a chunk, partial sums
   bool stream;
