@@ -56,6 +56,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.slot_off = take((size_t)p.R * 4);
   p.row_off = take((size_t)p.S * 4);
   p.tiles_off = take((size_t)p.tiles * 8);
+  p.order_off = take((size_t)E * 4);
   p.scale_off = take((size_t)E * 4);
   p.t_off = take((size_t)p.T * p.Ip * 4);
   p.z_off = take((size_t)p.R * O * 4);
@@ -137,6 +138,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_place(ExpertsArgs a) {
       if (b < (int)blockIdx.x) before += h;
     }
   const int padded = (total + 31) / 32 * 32, ntiles = (total + 127) / 128;
+  if (blockIdx.x == 0) {  // the experts by falling row count
+    if (tid < p.E) next[tid] = total;
+    __syncthreads();
+    if (tid < p.E) {
+      int ahead = 0;
+      for (int e = 0; e < p.E; ++e) ahead += next[e] > total || (next[e] == total && e < tid);
+      ((int*)(a.saved + p.order_off))[ahead] = tid;
+    }
+    __syncthreads();
+  }
   int sum[2] = {padded, ntiles};  // inclusive sums over the experts of rows and of tiles
   for (int which = 0; which < 2; ++which) {
     if (tid < kExpertsMax) scan[0][tid] = tid < p.E ? sum[which] : 0;
@@ -298,7 +309,7 @@ __device__ __forceinline__ int xcd_chunk(int block, int n) {
   const int v = (block & 7) * per + (block >> 3);
   return (block >> 3) < per ? v : n;
 }
-int xcd_grid(int64_t n) { return (int)((n + 7) / 8 * 8); }
+int64_t xcd_grid(int64_t n) { return (n + 7) / 8 * 8; }
 
 // (tile, column block) of a product's block: 16 tiles go through one column block
 // before the next, so the 64 blocks that an XCD runs at once read about four
@@ -311,10 +322,16 @@ __device__ __forceinline__ void tile_and_column(int v, int tiles, int cols, int&
   tile = group * G + in - col * size;
 }
 
-// Inputs a stage of the forward takes, and its k-blocks (see k_experts_fwd).
+// The forward's stages: KS k-blocks, the IN inputs that they hold, and the ring of
+// LDS buffers.  One plane: short stages, three ahead (the copies of a stage take
+// longer than its products); two planes: a stage's products take three times as
+// long and one ahead is enough.  FN: column fragments a wave, so that two blocks'
+// rings share a CU.
 template <int NP, int P> struct FwdStage {
-  static constexpr int KS = NP == 2 && P < 16 ? 2 : 4;
+  static constexpr int KS = P == 16 ? 4 : 2;
   static constexpr int IN = KS * 16 / P;
+  static constexpr int NBUF = NP == 1 && P < 16 ? 4 : 2;
+  static constexpr int FN = NP == 2 && P == 16 ? 2 : 4;
 };
 
 // Cf: the forward's operand, rows o, k in stages of IN inputs: half g of a lane
@@ -420,12 +437,13 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
 // rows' tanh values of IN inputs (gathered by token) and KS k-blocks of Cf to LDS;
 // a wave makes its rows' basis values in registers, eight values of one or two
 // inputs a lane and k-block.
-template <int NP, int P, int FN>
+template <int NP, int P>
 __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   extern __shared__ char lds[];
   using FS = FwdStage<NP, P>;
-  constexpr int KS = FS::KS, IN = FS::IN, TB = IN * 4;  // bytes of a row's tanh values a stage
-  constexpr int kT = 128 * TB, kTChunks = kT / 1024, kB = 2 * FN * KS * NP;  // 1 KiB chunks
+  constexpr int KS = FS::KS, IN = FS::IN, NBUF = FS::NBUF, FN = FS::FN;
+  constexpr int TB = IN * 4;  // bytes of a row's tanh values a stage
+  constexpr int kT = 128 * TB, kB = 2 * FN * KS * NP;  // bytes, 1 KiB chunks
   constexpr int kStage = kT + kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
   const int cols = (p.O + 64 * FN - 1) / (64 * FN), v = xcd_chunk(blockIdx.x, p.tiles * cols);
@@ -444,21 +462,21 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   const char* cf = a.ws + p.cf_off + (size_t)e * p.Op * p.Ip * P * 2 * NP;
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const uint32_t l0 = lds_address(lds);
-  // this wave's tanh copies: chunk c holds 1024 / TB rows, 16 bytes a lane
-  constexpr int kTPer = (kTChunks + 3) / 4;
+  // this wave's tanh copies: its 32 rows of the tile, 16 bytes a lane (half the lanes
+  // where a row has 16), the same count for every wave
+  constexpr int kTPer = (32 * TB + 1023) / 1024;
   const float* tsrc[kTPer];
 #pragma unroll
   for (int i = 0; i < kTPer; ++i) {
-    const int c = i * 4 + wave;
-    const int byte = c * 1024 + lane * 16, r = row0 + byte / TB;
-    int k = c < kTChunks && r < end ? tok[r] : 0;
+    const int byte = i * 1024 + lane * 16, r = row0 + wave * 32 + byte / TB % 32;
+    int k = r < end ? tok[r] : 0;
     if (k < 0) k = 0;  // a pad row: any values, its results are not stored
     tsrc[i] = t + (int64_t)k * p.Ip + byte % TB / 4;
   }
   auto copy = [&](int s, uint32_t at) {
 #pragma unroll
     for (int i = 0; i < kTPer; ++i)
-      if (i * 4 + wave < kTChunks) dma16v(tsrc[i] + s * IN, at + (i * 4 + wave) * 1024);
+      if (32 * TB >= 1024 || lane * 16 < 32 * TB) dma16v(tsrc[i] + s * IN, at + wave * 32 * TB + i * 1024);
 #pragma unroll
     for (int i = 0; i < kB / 4; ++i) {
       const int c = i * 4 + wave;
@@ -467,14 +485,22 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
       dma16s(cf + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + kT + c * kPlaneBytes);
     }
   };
+  constexpr int kPer = kTPer + kB / 4;  // copies a wave and stage
   f32x16_t acc[2][FN] = {};
-  copy(0, l0);
+#pragma unroll
+  for (int s = 0; s < NBUF - 1; ++s)
+    if (s < nst) copy(s, l0 + s * kStage);
+  int cur = 0;
   for (int s = 0; s < nst; ++s) {
-    wait_vm<0>();
+    if (NBUF > 2 && nst - 1 - s >= NBUF - 2)
+      wait_vm<kPer * (NBUF - 2)>();
+    else
+      wait_vm<0>();
     wait_lds();
     block_barrier();
-    if (s + 1 < nst) copy(s + 1, l0 + ((s + 1) & 1) * kStage);
-    const char* buf = lds + (s & 1) * kStage;
+    if (s + NBUF - 1 < nst) copy(s + NBUF - 1, l0 + (cur == 0 ? NBUF - 1 : cur - 1) * kStage);
+    const char* buf = lds + cur * kStage;
+    if (++cur == NBUF) cur = 0;
     float tv[2][IN / 2], pa[2], pb[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -681,10 +707,13 @@ __global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
 // dx of 128 rows x 64 inputs a block, waves of 64 rows x 32 inputs: four degrees a
 // pass over the outputs stand in four accumulator fragments; between passes only
 // their weighted sum is kept.
+template <int NP> using DxTile = NtTile<NP, NP, 2, 2, 2, 4, NP == 1 ? 2 : 1, 3>;  // 72 KiB of LDS
+
 template <int NP>
 __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
   extern __shared__ char lds[];
-  typedef NtTile<NP, NP, 2, 2, 2, 4, 2, 2> Tile;
+  typedef DxTile<NP> Tile;
+  constexpr int KS = Tile::kStageBlocks;
   const ExpertsPlan& p = a.p;
   const int cols = (p.Ip + 63) / 64, v = xcd_chunk(blockIdx.x, p.tiles * cols);
   if (v >= p.tiles * cols) return;
@@ -721,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
       ib = ib < nib ? ib : nib - 1;     // past the inputs or degrees: any, not used
       d = d < p.deg ? d : p.deg - 1;
       return cbase + ((size_t)ib * p.deg + d) * pitch;
-    }, 0, KB / 2, lds, acc);
+    }, 0, KB / KS, lds, acc);
     const int nd = p.deg - d0 < 4 ? p.deg - d0 : 4;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -812,11 +841,13 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
   constexpr int kBAt = 2 * kA * kPlaneBytes, kTAt = kBAt + 2 * kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
   const int nob = (p.O + 127) / 128, nib = p.Ip / 32, nbi = (nib + NI - 1) / NI;
-  int id = xcd_chunk(blockIdx.x, p.E * nbi * nob);
-  if (id >= p.E * nbi * nob) return;
-  const int ob = id % nob;
-  id /= nob;
-  const int ib0 = id % nbi * NI, e = id / nbi;
+  // Every XCD takes an eighth of each expert's blocks (whole columns of outputs, so
+  // that they share g in its L2), the experts with most rows first: one expert an
+  // XCD left the seven others waiting for the largest.
+  const int per = (nbi * nob + 7) / 8, turn = (blockIdx.x >> 3) / per;
+  const int id = ((blockIdx.x + turn) & 7) * per + (blockIdx.x >> 3) % per;
+  if (id >= nbi * nob) return;
+  const int ob = id % nob, ib0 = id / nob * NI, e = ((const int*)(a.saved + p.order_off))[turn];
   const int* off = (const int*)(a.saved + p.off_off);
   const int row0 = off[e], nst = (off[e + 1] - row0) / 32;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
@@ -1169,13 +1200,12 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
     hipLaunchKernelGGL((k_experts_pack<T, NP, P, true>), pack_grid, dim3(256), pack_lds, st, a, keep);
   else
     hipLaunchKernelGGL((k_experts_pack<T, NP, P, false>), pack_grid, dim3(256), pack_lds, st, a, keep);
-  constexpr int FN = 4;
   using FS = FwdStage<NP, P>;
-  constexpr int lds = 2 * (128 * FS::IN * 4 + 2 * FN * FS::KS * NP * kPlaneBytes);
+  constexpr int lds = FS::NBUF * (128 * FS::IN * 4 + 2 * FS::FN * FS::KS * NP * kPlaneBytes);
   static std::atomic<uint32_t> done;
-  ensure_lds_limit((const void*)k_experts_fwd<NP, P, FN>, lds, done);
-  const int cols = (p.O + 64 * FN - 1) / (64 * FN);
-  hipLaunchKernelGGL((k_experts_fwd<NP, P, FN>), dim3(xcd_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
+  ensure_lds_limit((const void*)k_experts_fwd<NP, P>, lds, done);
+  const int cols = (p.O + 64 * FS::FN - 1) / (64 * FS::FN);
+  hipLaunchKernelGGL((k_experts_fwd<NP, P>), dim3((unsigned)xcd_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
   hipLaunchKernelGGL((k_experts_gather<T, true>), dim3(grid_for(p.T * p.O)), dim3(256), 0, st, a,
                      (const float*)(a.saved + p.z_off), a.y, p.O);
 }
@@ -1186,8 +1216,8 @@ void launch_dc(const ExpertsArgs& a, int d0, hipStream_t st) {
   constexpr int tile = NI * 8 * 128 * (DB + 1) * 4, lds = ring > tile ? ring : tile;
   static std::atomic<uint32_t> done;
   ensure_lds_limit((const void*)k_experts_dc<T, NP, DB>, lds, done);
-  const int64_t blocks = (int64_t)a.p.E * ceil_div(a.p.Ip / 32, NI) * ceil_div(a.p.O, 128);
-  hipLaunchKernelGGL((k_experts_dc<T, NP, DB>), dim3(xcd_grid(blocks)), dim3(256), lds, st, a, d0);
+  const int64_t blocks = a.p.E * xcd_grid(ceil_div(a.p.Ip / 32, NI) * ceil_div(a.p.O, 128));
+  hipLaunchKernelGGL((k_experts_dc<T, NP, DB>), dim3((unsigned)blocks), dim3(256), lds, st, a, d0);
 }
 
 template <typename T, int NP>
@@ -1197,10 +1227,10 @@ void backward_typed(const ExpertsArgs& a, hipStream_t st) {
   if (!a.dx && !a.dcoeffs) return;
   hipLaunchKernelGGL((k_experts_gpack<T, NP>), dim3((unsigned)(p.R / 32), (p.Op + 63) / 64), dim3(256), 0, st, a);
   if (a.dx) {
-    constexpr int lds = NtTile<NP, NP, 2, 2, 2, 4, 2, 2>::kLdsBytes;
+    constexpr int lds = DxTile<NP>::kLdsBytes;
     static std::atomic<uint32_t> done;
     ensure_lds_limit((const void*)k_experts_dx<NP>, lds, done);
-    hipLaunchKernelGGL((k_experts_dx<NP>), dim3(xcd_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)xcd_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
     hipLaunchKernelGGL((k_experts_gather<T, false>), dim3(grid_for(p.T * p.I)), dim3(256), 0, st, a,
                        (const float*)(a.ws + p.dxs_off), a.dx, p.I);
   }

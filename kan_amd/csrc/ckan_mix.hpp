@@ -77,7 +77,7 @@ struct ExpertsPlan {
   int64_t plan_chunk;  // slots a plan block takes (a multiple of kPlanThreads)
   int64_t grad_blocks;
   // saved from the forward to the backward
-  size_t off_off, tok_off, slot_off, row_off, tiles_off, scale_off, t_off, z_off, cb_off, saved_bytes;
+  size_t off_off, tok_off, slot_off, row_off, tiles_off, order_off, scale_off, t_off, z_off, cb_off, saved_bytes;
   // forward workspace
   size_t hist_off, cmax_off, cf_off, bias_off, fwd_bytes;
   // backward workspace

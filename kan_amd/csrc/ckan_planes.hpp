@@ -127,7 +127,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // stages ahead, one barrier a stage.
 template <int NA, int NB, int WM, int WN, int FM, int FN, int KS, int NBUF>
 struct NtTile {
-  static constexpr int kWaves = WM * WN;
+  static constexpr int kWaves = WM * WN, kStageBlocks = KS;
   static constexpr int kRA = WM * FM, kRB = WN * FN;
   static constexpr int kChunksA = kRA * KS * NA, kChunks = kChunksA + kRB * KS * NB;
   static constexpr int kStageBytes = kChunks * kPlaneBytes;
