@@ -51,7 +51,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
     off = align256(off + n);
     return at;
   };
-  p.off_off = take((size_t)(E + 1) * 4);
+  p.off_off = take((size_t)(E + 2) * 4);
   p.tok_off = take((size_t)p.R * 4);
   p.slot_off = take((size_t)p.R * 4);
   p.row_off = take((size_t)p.S * 4);
@@ -68,6 +68,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.cmax_off = take((size_t)E * kMaxParts * 4);
   p.cf_off = take((size_t)E * p.Op * p.Ip * p.P * 2 * p.NP);
   p.bias_off = take((size_t)p.bias_parts * E * p.Op * 4);
+  p.fpart_off = take((size_t)512 * 128 * 256 * 4);
   p.fwd_bytes = off;
   off = 0;
   p.gmax_off = take((size_t)p.grad_blocks * E * 4);
@@ -78,6 +79,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.gtot_off = take((size_t)E * p.Op * 4);
   p.ts_off = take((size_t)p.R * p.Ip * 4);
   p.dxs_off = take((size_t)p.R * I * 4);
+  p.bpart_off = take((size_t)512 * 128 * 64 * 4);
   p.bwd_bytes = off;
   // Streaming: up to 16 slots an expert on average.  Its blocks read the coefficients
   // as they lie, once for 8 rows; the tile path reads them twice and packs them
@@ -173,8 +175,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_place(ExpertsArgs a) {
       for (int r = sum[0] - padded + total; r < sum[0]; ++r) tok[r] = slot[r] = -1;
       int2* tiles = (int2*)(a.saved + p.tiles_off);
       for (int i = 0; i < ntiles; ++i) tiles[sum[1] - ntiles + i] = make_int2(tid, sum[0] - padded + i * 128);
-      if (tid == p.E - 1)
-        for (int i = sum[1]; i < p.tiles; ++i) tiles[i] = make_int2(-1, 0);
+      if (tid == p.E - 1) off[p.E + 1] = sum[1];
     }
   }
   const int64_t s0 = blockIdx.x * p.plan_chunk;
@@ -301,15 +302,46 @@ __global__ __launch_bounds__(256) void k_experts_cmax(ExpertsArgs a) {
   if (threadIdx.x == 0) ((float*)(a.ws + p.cmax_off))[e * kMaxParts + blockIdx.x] = m;
 }
 
-// Blocks are spread over the eight XCDs in turn; this gives XCD x the x-th eighth of
-// the work, so that blocks which share operands share an L2.  Returns n or more
-// for the blocks of the round-up.
-__device__ __forceinline__ int xcd_chunk(int block, int n) {
-  const int per = (n + 7) / 8;
-  const int v = (block & 7) * per + (block >> 3);
-  return (block >> 3) < per ? v : n;
-}
 int64_t xcd_grid(int64_t n) { return (n + 7) / 8 * 8; }
+
+// The share of a product over W equal output tiles that a block takes.  Blocks are
+// spread over the eight XCDs in turn; XCD x gets the x-th eighth of the tiles, so that
+// blocks which share operands share an L2.  64 blocks run on an XCD at once: its
+// tiles past the last whole round of 64 are each split along k into up to
+// kMaxSplits parts (few tiles altogether are the same case), whose partial
+// results a second launch sums in order.  528 tiles in 512 places took the time of
+// two whole rounds.
+constexpr int kMaxSplits = 8, kXcdBlocks = 64;
+struct Share {
+  int v;            // the tile; -1: none
+  int part, parts;  // this block's part of its k
+  int place;        // of the partial result among kXcdBlocks of the XCD
+};
+__device__ __forceinline__ Share split_rule(int xcd, int W, int& full, int& rest, int& parts) {
+  const int per = (W + 7) / 8, n = W - xcd * per < per ? W - xcd * per : per;
+  full = n > 0 ? n / kXcdBlocks * kXcdBlocks : 0;
+  rest = n > 0 ? n - full : 0;
+  parts = rest ? kXcdBlocks / rest : 1;
+  parts = parts < kMaxSplits ? parts : kMaxSplits;
+  return Share{xcd * per, 0, 1, 0};
+}
+__device__ __forceinline__ Share block_share(int block, int W) {
+  int full, rest, parts;
+  Share s = split_rule(block & 7, W, full, rest, parts);
+  const int j = block >> 3;
+  if (j < full) {
+    s.v += j;
+  } else if (j - full < rest * parts) {
+    s.place = j - full;
+    s.part = s.place % parts;
+    s.parts = parts;
+    s.v += full + s.place / parts;
+  } else {
+    s.v = -1;
+  }
+  return s;
+}
+int64_t share_grid(int64_t most) { return 8 * (ceil_div(most, 8) + kXcdBlocks); }
 
 // (tile, column block) of a product's block: 16 tiles go through one column block
 // before the next, so the 64 blocks that an XCD runs at once read about four
@@ -446,19 +478,20 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   constexpr int kT = 128 * TB, kB = 2 * FN * KS * NP;  // bytes, 1 KiB chunks
   constexpr int kStage = kT + kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
-  const int cols = (p.O + 64 * FN - 1) / (64 * FN), v = xcd_chunk(blockIdx.x, p.tiles * cols);
-  if (v >= p.tiles * cols) return;
+  const int cols = (p.O + 64 * FN - 1) / (64 * FN), tiles = ((const int*)(a.saved + p.off_off))[p.E + 1];
+  const Share share = block_share(blockIdx.x, tiles * cols);
+  if (share.v < 0) return;
   int ti, cb;
-  tile_and_column(v, p.tiles, cols, ti, cb);
+  tile_and_column(share.v, tiles, cols, ti, cb);
   const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
-  if (tile.x < 0) return;
   const int e = tile.x, row0 = tile.y;
   const int end = ((const int*)(a.saved + p.off_off))[e + 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave >> 1, wn = wave & 1, g = lane >> 5;
   const int* tok = (const int*)(a.saved + p.tok_off);
   const float* t = (const float*)(a.saved + p.t_off);
-  const int KB = p.Ip * P / 16, nst = KB / KS, nb = p.Op / 32;
+  const int KB = p.Ip * P / 16, nb = p.Op / 32;
+  const int s0 = KB / KS * share.part / share.parts, nst = KB / KS * (share.part + 1) / share.parts - s0;
   const char* cf = a.ws + p.cf_off + (size_t)e * p.Op * p.Ip * P * 2 * NP;
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const uint32_t l0 = lds_address(lds);
@@ -476,13 +509,13 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   auto copy = [&](int s, uint32_t at) {
 #pragma unroll
     for (int i = 0; i < kTPer; ++i)
-      if (32 * TB >= 1024 || lane * 16 < 32 * TB) dma16v(tsrc[i] + s * IN, at + wave * 32 * TB + i * 1024);
+      if (32 * TB >= 1024 || lane * 16 < 32 * TB) dma16v(tsrc[i] + (s0 + s) * IN, at + wave * 32 * TB + i * 1024);
 #pragma unroll
     for (int i = 0; i < kB / 4; ++i) {
       const int c = i * 4 + wave;
       int rb = cb * 2 * FN + c / (KS * NP);
       rb = rb < nb ? rb : nb - 1;  // past the outputs: any, not stored
-      dma16s(cf + rb * pitch + ((size_t)s * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + kT + c * kPlaneBytes);
+      dma16s(cf + rb * pitch + ((size_t)(s0 + s) * KS * NP + c % (KS * NP)) * kPlaneBytes, lane * 16, at + kT + c * kPlaneBytes);
     }
   };
   constexpr int kPer = kTPer + kB / 4;  // copies a wave and stage
@@ -540,6 +573,17 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
     }
   }
   const float inv = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
+  if (share.parts > 1) {
+    float* part = (float*)(a.ws + p.fpart_off) + ((size_t)(blockIdx.x & 7) * kXcdBlocks + share.place) * 128 * 256;
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+          part[(wm * 64 + m * 32 + acc_row(q, g)) * 256 + (wn * FN + n) * 32 + (lane & 31)] = acc[m][n][q] * inv;
+    return;
+  }
   const float* bias = (const float*)(a.ws + p.bias_off);
   float* z = (float*)(a.saved + p.z_off);
 #pragma unroll
@@ -555,6 +599,42 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
         const int r = row0 + wm * 64 + m * 32 + acc_row(q, g);
         if (r < end) z[(size_t)r * p.O + o] = fmaf(acc[m][n][q], inv, b);
       }
+  }
+}
+
+// The tiles that block_share split: the sum of their parts, in order.  dx: the
+// inputs' gradients of 64 columns a tile, or the forward's outputs of `width`
+// columns and their bias.  A block sums 8 rows.
+template <bool DX>
+__global__ __launch_bounds__(256) void k_experts_parts(ExpertsArgs a, int width) {
+  const ExpertsPlan& p = a.p;
+  const int n = DX ? p.I : p.O, cols = ((DX ? p.Ip : p.O) + width - 1) / width;
+  const int tiles = ((const int*)(a.saved + p.off_off))[p.E + 1];
+  const int xcd = blockIdx.x & 7, u = blockIdx.x >> 3;
+  int full, rest, parts;
+  const Share s = split_rule(xcd, tiles * cols, full, rest, parts);
+  if (u >= rest || parts < 2) return;
+  int ti, cb;
+  tile_and_column(s.v + full + u, tiles, cols, ti, cb);
+  const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
+  const int end = ((const int*)(a.saved + p.off_off))[tile.x + 1];
+  const int pitch = DX ? 64 : 256;
+  const float* part = (const float*)(a.ws + (DX ? p.bpart_off : p.fpart_off)) +
+                      ((size_t)xcd * kXcdBlocks + u * parts) * 128 * pitch;
+  float* out = (float*)(DX ? a.ws + p.dxs_off : a.saved + p.z_off);
+  for (int q = threadIdx.x; q < 8 * width; q += 256) {
+    const int r = blockIdx.y * 8 + q / width, c = q % width, col = cb * width + c;
+    if (tile.y + r >= end || col >= n) continue;
+    float v = 0.0f;
+    if constexpr (!DX) {
+      const float* bias = (const float*)(a.ws + p.bias_off);
+      for (int k = 0; k < p.bias_parts; ++k) v += bias[((size_t)k * p.E + tile.x) * p.Op + col];
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMaxSplits; ++k)
+      if (k < parts) sum += part[(size_t)k * 128 * pitch + r * pitch + c];
+    out[(size_t)(tile.y + r) * n + col] = sum + v;
   }
 }
 
@@ -715,15 +795,16 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
   typedef DxTile<NP> Tile;
   constexpr int KS = Tile::kStageBlocks;
   const ExpertsPlan& p = a.p;
-  const int cols = (p.Ip + 63) / 64, v = xcd_chunk(blockIdx.x, p.tiles * cols);
-  if (v >= p.tiles * cols) return;
+  const int cols = (p.Ip + 63) / 64, tiles = ((const int*)(a.saved + p.off_off))[p.E + 1];
+  const Share share = block_share(blockIdx.x, tiles * cols);
+  if (share.v < 0) return;
   int ti, cb;
-  tile_and_column(v, p.tiles, cols, ti, cb);
+  tile_and_column(share.v, tiles, cols, ti, cb);
   const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
-  if (tile.x < 0) return;
   const int e = tile.x, row0 = tile.y, ib0 = cb * 2;
   const int end = ((const int*)(a.saved + p.off_off))[e + 1];
   const int KB = p.Op / 16, nib = p.Ip / 32;
+  const int s0 = KB / KS * share.part / share.parts, nst = KB / KS * (share.part + 1) / share.parts - s0;
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const char* cbase = a.saved + p.cb_off + (size_t)e * p.Ip * p.deg * p.Op * 2 * NP;
   const RowBlocks A{a.ws + p.gr_off + (row0 >> 5) * pitch, pitch};
@@ -750,7 +831,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
       ib = ib < nib ? ib : nib - 1;     // past the inputs or degrees: any, not used
       d = d < p.deg ? d : p.deg - 1;
       return cbase + ((size_t)ib * p.deg + d) * pitch;
-    }, 0, KB / KS, lds, acc);
+    }, s0 * KS, nst, lds, acc);
     const int nd = p.deg - d0 < 4 ? p.deg - d0 : 4;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -774,9 +855,18 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
         dx[m][q] = fmaf(s, 1.0f - x[m][q] * x[m][q], dx[m][q]);
       }
   }
-  if (i >= p.I) return;
   const float ic = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
   const float ig = 1.0f / ((const float*)(a.ws + p.gscale_off))[e];
+  if (share.parts > 1) {
+    float* part = (float*)(a.ws + p.bpart_off) + ((size_t)(blockIdx.x & 7) * kXcdBlocks + share.place) * 128 * 64;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int q = 0; q < 16; ++q)
+        part[((wave >> 1) * 64 + m * 32 + acc_row(q, g)) * 64 + (wave & 1) * 32 + (lane & 31)] = dx[m][q] * ic * ig;
+    return;
+  }
+  if (i >= p.I) return;
   float* out = (float*)(a.ws + p.dxs_off);
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -1205,7 +1295,8 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
   static std::atomic<uint32_t> done;
   ensure_lds_limit((const void*)k_experts_fwd<NP, P>, lds, done);
   const int cols = (p.O + 64 * FS::FN - 1) / (64 * FS::FN);
-  hipLaunchKernelGGL((k_experts_fwd<NP, P>), dim3((unsigned)xcd_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((k_experts_fwd<NP, P>), dim3((unsigned)share_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((k_experts_parts<false>), dim3(8 * kXcdBlocks, 16), dim3(256), 0, st, a, 64 * FS::FN);
   hipLaunchKernelGGL((k_experts_gather<T, true>), dim3(grid_for(p.T * p.O)), dim3(256), 0, st, a,
                      (const float*)(a.saved + p.z_off), a.y, p.O);
 }
@@ -1230,7 +1321,9 @@ void backward_typed(const ExpertsArgs& a, hipStream_t st) {
     constexpr int lds = DxTile<NP>::kLdsBytes;
     static std::atomic<uint32_t> done;
     ensure_lds_limit((const void*)k_experts_dx<NP>, lds, done);
-    hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)xcd_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)share_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds,
+                       st, a);
+    hipLaunchKernelGGL((k_experts_parts<true>), dim3(8 * kXcdBlocks, 16), dim3(256), 0, st, a, 64);
     hipLaunchKernelGGL((k_experts_gather<T, false>), dim3(grid_for(p.T * p.I)), dim3(256), 0, st, a,
                        (const float*)(a.ws + p.dxs_off), a.dx, p.I);
   }

@@ -79,9 +79,9 @@ struct ExpertsPlan {
   // saved from the forward to the backward
   size_t off_off, tok_off, slot_off, row_off, tiles_off, order_off, scale_off, t_off, z_off, cb_off, saved_bytes;
   // forward workspace
-  size_t hist_off, cmax_off, cf_off, bias_off, fwd_bytes;
+  size_t hist_off, cmax_off, cf_off, bias_off, fpart_off, fwd_bytes;
   // backward workspace
-  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bwd_bytes;
+  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bpart_off, bwd_bytes;
   int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
   // the streaming forward (few slots): input chunks, inputs a chunk, partial sums
   bool stream;
