@@ -44,7 +44,6 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.tiles = (int)(ceil_div(p.S, 128) + (E < p.S ? E : p.S));
   p.plan_chunk = round_up(ceil_div(p.S, kPlanBlocks), kPlanThreads);
   p.plan_blocks = (int)ceil_div(p.S, p.plan_chunk);
-  p.grad_blocks = ceil_div(p.R, 32) < kGradBlocks ? ceil_div(p.R, 32) : kGradBlocks;
   size_t off = 0;
   auto take = [&](size_t n) {
     const size_t at = off;
@@ -71,7 +70,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.fpart_off = take((size_t)512 * 128 * 256 * 4);
   p.fwd_bytes = off;
   off = 0;
-  p.gmax_off = take((size_t)p.grad_blocks * E * 4);
+  p.gmax_off = take((size_t)(p.R / 32) * 4);
   p.gscale_off = take((size_t)E * 4);
   p.gr_off = take((size_t)p.R * p.Op * 2 * p.NP);
   p.gt_off = take((size_t)p.R * p.Op * 2 * p.NP);
@@ -217,16 +216,72 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_place(ExpertsArgs a) {
 
 // ---- tanh, scales, packed coefficients ----------------------------------------
 
+// Sixteen bytes of T as floats: 8 bf16 or 4 fp32 values.
+template <typename T> struct Vec16 { static constexpr int N = 16 / (int)sizeof(T); };
+__device__ __forceinline__ void widen(u32x4_t q, float (&v)[4], const float*) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(q[j]);
+}
+__device__ __forceinline__ void widen(u32x4_t q, float (&v)[8], const __bf16*) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(q[j] << 16);
+    v[2 * j + 1] = __uint_as_float(q[j] & 0xffff0000u);
+  }
+}
+
+// Four consecutive values of a row, from a vector load where every row begins at a
+// multiple of four values (n the row's length, the values past it zeros).
+__device__ __forceinline__ f32x4_t load4(const float* row, int c, int n, bool vec) {
+  if (vec) return *(const f32x4_t*)(row + c);
+  f32x4_t v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = c + j < n ? row[c + j] : 0.0f;
+  return v;
+}
+__device__ __forceinline__ f32x4_t load4(const __bf16* row, int c, int n, bool vec) {
+  f32x4_t v;
+  if (vec) {
+    const bf16x4_t b = *(const bf16x4_t*)(row + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)b[j];
+    return v;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = c + j < n ? (float)row[c + j] : 0.0f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int c, int n, bool vec, f32x4_t v) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      *(f32x4_t*)(row + c) = v;
+    } else {
+      bf16x4_t b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = (__bf16)v[j];
+      *(bf16x4_t*)(row + c) = b;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < n) row[c + j] = (T)v[j];
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void k_experts_tanh(ExpertsArgs a) {
   const ExpertsPlan& p = a.p;
-  float* t = (float*)(a.saved + p.t_off);
-  const int64_t n = p.T * p.Ip;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
-    const int64_t r = q / p.Ip;
-    const int i = (int)(q - r * p.Ip);
-    t[q] = i < p.I ? tanhf((float)((const T*)a.x)[r * p.I + i]) : 0.0f;
-  }
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = p.Ip / 4;
+  const int64_t r = q / per;
+  if (r >= p.T) return;
+  const int i = (int)(q - r * per) * 4;
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (i < p.I) v = load4((const T*)a.x + r * p.I, i, p.I, p.I % 4 == 0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = tanhf(v[j]);
+  *(f32x4_t*)((float*)(a.saved + p.t_off) + r * p.Ip + i) = v;
 }
 
 // The power of two that brings a largest magnitude m into [2^(e-1), 2^e).
@@ -249,20 +304,6 @@ __device__ __forceinline__ float block_max_256(float v, float* red) {
   v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   __syncthreads();
   return v;
-}
-
-// Sixteen bytes of T as floats: 8 bf16 or 4 fp32 values.
-template <typename T> struct Vec16 { static constexpr int N = 16 / (int)sizeof(T); };
-__device__ __forceinline__ void widen(u32x4_t q, float (&v)[4], const float*) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(q[j]);
-}
-__device__ __forceinline__ void widen(u32x4_t q, float (&v)[8], const __bf16*) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = __uint_as_float(q[j] << 16);
-    v[2 * j + 1] = __uint_as_float(q[j] & 0xffff0000u);
-  }
 }
 
 // The largest finite |C| of each expert by blocks; four 16-byte loads in flight a
@@ -602,9 +643,9 @@ __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   }
 }
 
-// The tiles that block_share split: the sum of their parts, in order.  dx: the
-// inputs' gradients of 64 columns a tile, or the forward's outputs of `width`
-// columns and their bias.  A block sums 8 rows.
+// The tiles that block_share split: the sum of their parts, in order, four columns a
+// thread.  dx: the inputs' gradients of 64 columns a tile; else the forward's outputs
+// of `width` columns and their bias.
 template <bool DX>
 __global__ __launch_bounds__(256) void k_experts_parts(ExpertsArgs a, int width) {
   const ExpertsPlan& p = a.p;
@@ -619,99 +660,118 @@ __global__ __launch_bounds__(256) void k_experts_parts(ExpertsArgs a, int width)
   const int2 tile = ((const int2*)(a.saved + p.tiles_off))[ti];
   const int end = ((const int*)(a.saved + p.off_off))[tile.x + 1];
   const int pitch = DX ? 64 : 256;
+  const int r = (blockIdx.y * 256 + threadIdx.x) / (width / 4), c = (int)threadIdx.x % (width / 4) * 4, col = cb * width + c;
+  if (tile.y + r >= end || col >= n) return;
   const float* part = (const float*)(a.ws + (DX ? p.bpart_off : p.fpart_off)) +
-                      ((size_t)xcd * kXcdBlocks + u * parts) * 128 * pitch;
-  float* out = (float*)(DX ? a.ws + p.dxs_off : a.saved + p.z_off);
-  for (int q = threadIdx.x; q < 8 * width; q += 256) {
-    const int r = blockIdx.y * 8 + q / width, c = q % width, col = cb * width + c;
-    if (tile.y + r >= end || col >= n) continue;
-    float v = 0.0f;
-    if constexpr (!DX) {
-      const float* bias = (const float*)(a.ws + p.bias_off);
-      for (int k = 0; k < p.bias_parts; ++k) v += bias[((size_t)k * p.E + tile.x) * p.Op + col];
-    }
-    float sum = 0.0f;
+                      ((size_t)xcd * kXcdBlocks + u * parts) * 128 * pitch + r * pitch + c;
+  f32x4_t w[kMaxSplits], v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < kMaxSplits; ++k)
-      if (k < parts) sum += part[(size_t)k * 128 * pitch + r * pitch + c];
-    out[(size_t)(tile.y + r) * n + col] = sum + v;
+  for (int k = 0; k < kMaxSplits; ++k)
+    if (k < parts) w[k] = *(const f32x4_t*)(part + (size_t)k * 128 * pitch);
+  if constexpr (!DX) {
+    const float* bias = (const float*)(a.ws + p.bias_off) + (size_t)tile.x * p.Op + col;  // padded to 32 columns
+#pragma unroll 4
+    for (int k = 0; k < p.bias_parts; ++k) {
+      const f32x4_t b = *(const f32x4_t*)(bias + (size_t)k * p.E * p.Op);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += b[j];
+    }
   }
+#pragma unroll
+  for (int k = 0; k < kMaxSplits; ++k)
+    if (k < parts)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += w[k][j];
+  store4((float*)(DX ? a.ws + p.dxs_off : a.saved + p.z_off) + (size_t)(tile.y + r) * n, col, n, n % 4 == 0, v);
 }
 
 __device__ __forceinline__ float load_weight(const ExpertsArgs& a, int64_t s) {
   return a.p.wbf16 ? (float)((const __bf16*)a.weights)[s] : ((const float*)a.weights)[s];
 }
 
-// out[t, c] = sum over the token's kept slots of (weight) src[row, c], in slot order.
+// out[t, c] = sum over the token's kept slots of (weight) src[row, c], in slot order;
+// four columns a thread.
 template <typename T, bool WEIGHTED>
 __global__ __launch_bounds__(256) void k_experts_gather(ExpertsArgs a, const float* src, void* out, int width) {
   const ExpertsPlan& p = a.p;
   const int* row = (const int*)(a.saved + p.row_off);
-  const int64_t n = p.T * width;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
-    const int64_t t = q / width;
-    const int c = (int)(q - t * width);
-    float v = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
-      const int r = row[t * p.k + j];
-      if (r >= 0) v += WEIGHTED ? load_weight(a, t * p.k + j) * src[(size_t)r * width + c] : src[(size_t)r * width + c];
-    }
-    ((T*)out)[q] = (T)v;
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = (width + 3) / 4;
+  const int64_t t = q / per;
+  if (t >= p.T) return;
+  const int c = (int)(q - t * per) * 4;
+  const bool vec = width % 4 == 0;
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+  for (int j = 0; j < p.k; ++j) {
+    const int r = row[t * p.k + j];
+    const float w = WEIGHTED ? load_weight(a, t * p.k + j) : 1.0f;
+    if (r < 0) continue;
+    const f32x4_t z = load4(src + (size_t)r * width, c, width, vec);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = WEIGHTED ? fmaf(w, z[u], v[u]) : v[u] + z[u];
   }
+  store4((T*)out + t * width, c, width, vec, v);
 }
 
 // ---- backward -------------------------------------------------------------------
 
-// dweights of each slot, and the largest |w dy| of each expert (by blocks).
+// dweights of each slot, and the largest |w dy| of each block of 32 rows; 16 waves a
+// block, two rows each.
 template <typename T>
-__global__ __launch_bounds__(256) void k_experts_dweights(ExpertsArgs a) {
-  __shared__ float gmax[kExpertsMax];
+__global__ __launch_bounds__(1024) void k_experts_dweights(ExpertsArgs a) {
+  __shared__ float most[16];
   const ExpertsPlan& p = a.p;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int e = threadIdx.x; e < p.E; e += 256) gmax[e] = 0.0f;
-  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rb = blockIdx.x;
   const int* off = (const int*)(a.saved + p.off_off);
   const int* slot = (const int*)(a.saved + p.slot_off);
   const int* row = (const int*)(a.saved + p.row_off);
   const float* z = (const float*)(a.saved + p.z_off);
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < off[p.E]; r += (int64_t)gridDim.x * 4) {
-    const int s = slot[r];
-    if (s < 0) continue;
-    const T* dy = (const T*)a.dy + (int64_t)(s / p.k) * p.O;
-    float dot = 0.0f, m = 0.0f;
-    for (int o = lane; o < p.O; o += 64) {
-      const float v = (float)dy[o];
-      dot = fmaf(v, z[(size_t)r * p.O + o], dot);
-      m = fmaxf(m, finite_abs(v));
-    }
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      dot += __shfl_xor(dot, w);
-      m = fmaxf(m, __shfl_xor(m, w));
-    }
-    if (lane == 0) {
-      if (a.dweights) {
-        if (p.wbf16)
-          ((__bf16*)a.dweights)[s] = (__bf16)dot;
-        else
-          ((float*)a.dweights)[s] = dot;
-      }
-      const int e = (int)a.indices[s];
-      m = finite_abs(m * load_weight(a, s));
-      atomicMax((unsigned*)&gmax[e], __float_as_uint(m));  // non-negative floats order as integers
-    }
-  }
-  if (a.dweights)
-    for (int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x; s < p.S; s += (int64_t)gridDim.x * 256)
+  if (a.dweights)  // slots without an expert
+    for (int64_t s = (int64_t)rb * 1024 + threadIdx.x; s < p.S; s += (int64_t)gridDim.x * 1024)
       if (row[s] < 0) {
         if (p.wbf16)
           ((__bf16*)a.dweights)[s] = (__bf16)0.0f;
         else
           ((float*)a.dweights)[s] = 0.0f;
       }
+  if (rb * 32 >= off[p.E]) return;
+  const bool vec = p.O % 4 == 0;
+  float dot[2] = {}, m[2] = {};
+  int s[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) s[h] = slot[rb * 32 + wave * 2 + h];
+  for (int o = lane * 4; o < p.O; o += 256)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (s[h] < 0) continue;
+      const f32x4_t d = load4((const T*)a.dy + (int64_t)(s[h] / p.k) * p.O, o, p.O, vec);
+      const f32x4_t v = load4(z + (size_t)(rb * 32 + wave * 2 + h) * p.O, o, p.O, vec);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dot[h] = fmaf(d[j], v[j], dot[h]);
+        m[h] = fmaxf(m[h], finite_abs(d[j]));
+      }
+    }
+  float big = 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (s[h] < 0) continue;
+    const float sum = wave_sum(dot[h]);
+    big = fmaxf(big, finite_abs(wave_max(m[h]) * load_weight(a, s[h])));
+    if (lane == 0 && a.dweights) {
+      if (p.wbf16)
+        ((__bf16*)a.dweights)[s[h]] = (__bf16)sum;
+      else
+        ((float*)a.dweights)[s[h]] = sum;
+    }
+  }
+  if (lane == 0) most[wave] = big;
   __syncthreads();
-  float* out = (float*)(a.ws + p.gmax_off) + (size_t)blockIdx.x * p.E;
-  for (int e = threadIdx.x; e < p.E; e += 256) out[e] = gmax[e];
+  if (wave == 0) {
+    const float v = wave_max(lane < 16 ? most[lane] : 0.0f);
+    if (lane == 0) ((float*)(a.ws + p.gmax_off))[rb] = v;
+  }
 }
 
 __device__ __forceinline__ int row_expert(const int* off, int E, int r) {
@@ -739,16 +799,22 @@ __global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
   const int e = row_expert(off, p.E, rb * 32);
   const float* gmax = (const float*)(a.ws + p.gmax_off);
   float m = 0.0f;
-  for (int b = tid; b < (int)p.grad_blocks; b += 256) m = fmaxf(m, gmax[(size_t)b * p.E + e]);
+  for (int b = off[e] / 32 + tid; b < off[e + 1] / 32; b += 256) m = fmaxf(m, gmax[b]);
   m = block_max_256(m, red);
   const float scale = range_scale(m, 14);
   if (rb * 32 == off[e] && blockIdx.y == 0 && tid == 0) ((float*)(a.ws + p.gscale_off))[e] = scale;
   const int* slot = (const int*)(a.saved + p.slot_off);
-  for (int q = tid; q < 32 * 64; q += 256) {
-    const int r = q >> 6, o = o0 + (q & 63), s = slot[rb * 32 + r];
-    float v = 0.0f;
-    if (s >= 0 && o < p.O) v = load_weight(a, s) * (float)((const T*)a.dy)[(int64_t)(s / p.k) * p.O + o];
-    tile[r][q & 63] = v;
+  {  // eight values a thread
+    const int r = tid >> 3, c = (tid & 7) * 8, s = slot[rb * 32 + r];
+    const float w = s >= 0 ? load_weight(a, s) : 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int o = o0 + c + h * 4;
+      f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (s >= 0 && o < p.O) v = load4((const T*)a.dy + (int64_t)(s / p.k) * p.O, o, p.O, p.O % 4 == 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tile[r][c + h * 4 + j] = s >= 0 ? w * v[j] : 0.0f;
+    }
   }
   __syncthreads();
   if (tid < 64 && o0 + tid < p.Op) {
@@ -1274,14 +1340,12 @@ void stream_typed(const ExpertsArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_experts_stream_sum<T>), dim3((unsigned)ceil_div(p.T * p.O, 256)), block, 0, st, a);
 }
 
-int grid_for(int64_t n) { return (int)(ceil_div(n, 256) < 4096 ? ceil_div(n, 256) : 4096); }
-
 template <typename T, int NP, int P>
 void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
   const ExpertsPlan& p = a.p;
   hipLaunchKernelGGL(k_plan_count, dim3(p.plan_blocks), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL(k_plan_place, dim3(p.plan_blocks), dim3(kPlanThreads), 0, st, a);
-  hipLaunchKernelGGL((k_experts_tanh<T>), dim3(grid_for(p.T * p.Ip)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_experts_tanh<T>), dim3((unsigned)ceil_div(p.T * (p.Ip / 4), 256)), dim3(256), 0, st, a);
   hipLaunchKernelGGL((k_experts_cmax<T>), dim3(kMaxParts, p.E), dim3(256), 0, st, a);
   const size_t pack_lds = (size_t)16 * (32 * p.D + 1) * sizeof(float);
   const dim3 pack_grid(p.bias_parts, p.Op / 32, p.E);
@@ -1296,8 +1360,8 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
   ensure_lds_limit((const void*)k_experts_fwd<NP, P>, lds, done);
   const int cols = (p.O + 64 * FS::FN - 1) / (64 * FS::FN);
   hipLaunchKernelGGL((k_experts_fwd<NP, P>), dim3((unsigned)share_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
-  hipLaunchKernelGGL((k_experts_parts<false>), dim3(8 * kXcdBlocks, 16), dim3(256), 0, st, a, 64 * FS::FN);
-  hipLaunchKernelGGL((k_experts_gather<T, true>), dim3(grid_for(p.T * p.O)), dim3(256), 0, st, a,
+  hipLaunchKernelGGL((k_experts_parts<false>), dim3(8 * kXcdBlocks, 8 * FS::FN), dim3(256), 0, st, a, 64 * FS::FN);
+  hipLaunchKernelGGL((k_experts_gather<T, true>), dim3((unsigned)ceil_div(p.T * ((p.O + 3) / 4), 256)), dim3(256), 0, st, a,
                      (const float*)(a.saved + p.z_off), a.y, p.O);
 }
 
@@ -1314,7 +1378,7 @@ void launch_dc(const ExpertsArgs& a, int d0, hipStream_t st) {
 template <typename T, int NP>
 void backward_typed(const ExpertsArgs& a, hipStream_t st) {
   const ExpertsPlan& p = a.p;
-  hipLaunchKernelGGL((k_experts_dweights<T>), dim3((unsigned)p.grad_blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_experts_dweights<T>), dim3((unsigned)(p.R / 32)), dim3(1024), 0, st, a);
   if (!a.dx && !a.dcoeffs) return;
   hipLaunchKernelGGL((k_experts_gpack<T, NP>), dim3((unsigned)(p.R / 32), (p.Op + 63) / 64), dim3(256), 0, st, a);
   if (a.dx) {
@@ -1323,8 +1387,8 @@ void backward_typed(const ExpertsArgs& a, hipStream_t st) {
     ensure_lds_limit((const void*)k_experts_dx<NP>, lds, done);
     hipLaunchKernelGGL((k_experts_dx<NP>), dim3((unsigned)share_grid((int64_t)p.tiles * ((p.Ip + 63) / 64))), dim3(256), lds,
                        st, a);
-    hipLaunchKernelGGL((k_experts_parts<true>), dim3(8 * kXcdBlocks, 16), dim3(256), 0, st, a, 64);
-    hipLaunchKernelGGL((k_experts_gather<T, false>), dim3(grid_for(p.T * p.I)), dim3(256), 0, st, a,
+    hipLaunchKernelGGL((k_experts_parts<true>), dim3(8 * kXcdBlocks, 8), dim3(256), 0, st, a, 64);
+    hipLaunchKernelGGL((k_experts_gather<T, false>), dim3((unsigned)ceil_div(p.T * ((p.I + 3) / 4), 256)), dim3(256), 0, st, a,
                        (const float*)(a.ws + p.dxs_off), a.dx, p.I);
   }
   if (a.dcoeffs) {

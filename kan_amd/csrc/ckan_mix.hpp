@@ -5,6 +5,17 @@
 
 namespace ckan {
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
+  return v;
+}
+
 // ---- routing (ckan_route.hip) -----------------------------------------------
 constexpr int kRouteMaxExperts = 512;  // 8 experts a lane
 constexpr int kRouteMaxTopK = 64;      // lane j holds the j-th chosen expert
@@ -58,7 +69,6 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanBlocks = 256;       // at most: a block's share of the slots grows past that
 constexpr int kMaxParts = 128;         // blocks an expert that look for its largest coefficient
 constexpr int kPackInputs = 128;       // inputs a block of the pack takes
-constexpr int kGradBlocks = 1024;      // blocks that look for the largest upstream gradients
 
 // Sizes and the layout of the buffers.  "Rows" are the kept slots sorted by expert,
 // each expert's run padded to a multiple of 32; "slots" are the T top_k entries of
@@ -75,7 +85,6 @@ struct ExpertsPlan {
   int tiles;           // 128-row tiles at most
   int plan_blocks;
   int64_t plan_chunk;  // slots a plan block takes (a multiple of kPlanThreads)
-  int64_t grad_blocks;
   // saved from the forward to the backward
   size_t off_off, tok_off, slot_off, row_off, tiles_off, order_off, scale_off, t_off, z_off, cb_off, saved_bytes;
   // forward workspace

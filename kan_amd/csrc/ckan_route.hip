@@ -18,17 +18,6 @@ namespace {
 
 constexpr int kRowsPerBlock = 4;  // one wave a row
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
-  return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
-  return v;
-}
-
 // The scores of a row in registers: s[q] of expert lane * J + q, 0 for an
 // expert that is not eligible (logit -inf or NaN) or past E.  The softmax's
 // exponentials are summed in 64 bits and the sum rounded once to 32: the score
