@@ -390,11 +390,14 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
  *   X = G / (|G|_F + eps), then `steps` times
  *   X = a X + (b A + c A^2) X with A = X X^T (X^T X for rows > cols).
  * Products run on two fp16 planes an operand (22 bits) with fp32 sums; the
- * norm is summed in fp64.  The coefficients' B = b A + c A^2 has to stay below 15 for
- * singular values in [0, 1] over all steps (checked on the host).
+ * norm is summed in fp64.  bf16 matrices take the iteration in powers of X X^T (the
+ * same up to far less than their own rounding).  |b A + c A^2| and |a + b A + c A^2|
+ * have to stay below 15 for singular values in [0, 1] over all steps (checked on
+ * the host).
  * Element (r, col) of matrix i lies at i batch_stride + r row_stride +
  * (col / inner) outer_stride + (col % inner) inner_stride elements; inner divides
- * cols.  An ordinary matrix has inner = 1 and its column stride in outer_stride.  A
+ * cols, and the strides have to make each matrix dense: row-major, column-major or, with
+ * inner > 1, [cols / inner, rows, inner].  An ordinary matrix has inner = 1 and its column stride in outer_stride.  A
  * ChebyKAN layer's coefficients [in, out, D] as [out, in D], the matrix by which
  * the basis values act on the outputs, have inner = D, row_stride = D,
  * outer_stride = out D, inner_stride = 1.  Replaces nothing in the reference, whose

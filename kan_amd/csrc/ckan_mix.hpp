@@ -114,7 +114,7 @@ void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st);
 void launch_experts_stream(const ExpertsArgs& a, hipStream_t st);
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st);
 
-size_t ortho_workspace_bytes(int batch, int rows, int cols);
+size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16);
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st);
 
 }  // namespace ckan

@@ -101,15 +101,15 @@ size_t experts_fwd_ws(const ExpertsPlan& p, bool without_saved) {
   return p.fwd_bytes + (without_saved ? p.cb_off : 0);
 }
 
-// The largest |b s^2 + c s^4| that the iteration's matrix B can reach from
-// singular values in [0, 1], over all steps, by sampling the interval.
+// The largest |b s^2 + c s^4| and |a + b s^2 + c s^4|, the iteration's matrices, that
+// singular values in [0, 1] can reach over all steps, by sampling the interval.
 double ortho_reach(const ckan_ortho_desc* d) {
   double top = 1.0, most = 0.0;
   for (int s = 0; s < d->steps && most < 1e6; ++s) {
     double next = 0.0;
     for (int i = 0; i <= 1024; ++i) {
       const double x = top * i / 1024, y = x * x, bv = d->b * y + d->c * y * y;
-      most = fmax(most, fabs(bv));
+      most = fmax(most, fmax(fabs(bv), fabs(d->a + bv)));
       next = fmax(next, fabs(x * (d->a + bv)));
     }
     top = fmax(next, 1e-30);
@@ -130,6 +130,13 @@ int ortho_check(const ckan_ortho_desc* d) {
     return fail(CKAN_ERR_INVALID_ARG, "inner must divide cols %d (got %d)", d->cols, d->inner);
   if (d->batch_stride < 0 || d->row_stride < 0 || d->outer_stride < 0 || d->inner_stride < 0)
     return fail(CKAN_ERR_INVALID_ARG, "strides must be >= 0");
+  const bool rows_first = d->inner == 1 && d->outer_stride == 1 && d->row_stride == d->cols;
+  const bool cols_first = d->inner == 1 && d->row_stride == 1 && d->outer_stride == d->rows;
+  const bool coeffs = d->inner > 1 && d->inner_stride == 1 && d->row_stride == d->inner &&
+                      d->outer_stride == (int64_t)d->rows * d->inner;
+  const bool vector = d->inner == 1 && (d->rows == 1 || d->cols == 1) && (d->rows == 1 ? d->outer_stride : d->row_stride) == 1;
+  if (!rows_first && !cols_first && !coeffs && !vector)
+    return fail(CKAN_ERR_UNSUPPORTED, "the matrices have to be dense: row-major, column-major or [cols / inner, rows, inner]");
   if (d->steps < 0 || d->steps > 100) return fail(CKAN_ERR_INVALID_ARG, "steps must lie in [0, 100] (got %d)", d->steps);
   if (d->dtype != CKAN_DTYPE_F32 && d->dtype != CKAN_DTYPE_BF16)
     return fail(CKAN_ERR_INVALID_ARG, "unknown dtype %d", d->dtype);
@@ -157,7 +164,7 @@ OrthoArgs ortho_args(const ckan_ortho_desc* d) {
 }
 
 int ortho_ws(const ckan_ortho_desc* d, void* ws, size_t ws_bytes) {
-  const size_t need = ortho_workspace_bytes(d->batch, d->rows, d->cols);
+  const size_t need = ortho_workspace_bytes(d->batch, d->rows, d->cols, d->dtype == CKAN_DTYPE_BF16);
   if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", ws_bytes, need);
   if (!ws || !is_al16(ws)) return fail(CKAN_ERR_INVALID_ARG, "workspace is NULL or not 16-byte aligned");
   return CKAN_OK;
@@ -237,7 +244,7 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
 }
 
 size_t ckan_orthogonalize_workspace_bytes(const ckan_ortho_desc* desc) {
-  return ortho_check(desc) ? 0 : ortho_workspace_bytes(desc->batch, desc->rows, desc->cols);
+  return ortho_check(desc) ? 0 : ortho_workspace_bytes(desc->batch, desc->rows, desc->cols, desc->dtype == CKAN_DTYPE_BF16);
 }
 
 int ckan_orthogonalize(const ckan_ortho_desc* desc, const void* in, void* out, void* ws, size_t ws_bytes,

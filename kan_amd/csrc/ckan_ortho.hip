@@ -4,11 +4,21 @@
 // A = X X^T.  m = the smaller, n = the larger dimension; the matrix is taken
 // with its m-side as rows (the iteration of the transpose is the transpose).
 //
-// The products run on two fp16 planes (ckan_planes.hpp), all values scaled by
-// 2^12: |X| and |A| stay below 1.5 and |b A + c A^2| below 7, far inside fp16's
-// range, and the planes keep 22 bits of entries down to 2^-15 of the largest.
-// X is held twice, as the operand with rows m and k = n (Xr, for A = X X^T) and
-// as the operand with rows n and k = m (Xc, for the product with X).
+// The products run on fp16 planes (ckan_planes.hpp), X and A scaled by 2^12: |X| and
+// |A| stay below 1.5 and |b A + c A^2| below 7, far inside fp16's range, and two
+// planes keep 22 bits of entries down to 2^-15 of the largest.
+//
+// fp32 matrices take the iteration as it is written, on two planes.  X is held
+// twice, as the operand with rows m and k = n (Xr, for A = X X^T) and as the one
+// with rows n and k = m (Xc, for the product with X).
+//
+// bf16 matrices take it in the m x m domain.  Every factor is a polynomial in A_0:
+//   P_s = a I + b A_s + c A_s^2,   A_{s+1} = P_s A_s P_s,   Q = P_4 P_3 P_2 P_1 P_0,
+// and the result is Q X0: two products with the long side instead of fifteen, and X0,
+// scaled by a power of two, is exact in one plane.  Errors of A count more this way,
+// those of small singular values by 3.4^2 a step (up to 1.5e-4 of the result for a
+// spectrum over four decades, 1e-5 for a gradient's), which bf16's 2e-3 hides and
+// fp32's 1e-6 would not.
 #include "ckan_mix.hpp"
 #include "ckan_planes.hpp"
 
@@ -23,16 +33,21 @@ constexpr int kTile = 128;
 struct OrthoPlan {
   int batch, m, n;
   bool tall;           // rows > cols: m runs along the columns
+  bool bf16;
+  int np;              // planes of X
   int m32, n32;        // k extents
   int m128, n128;      // row extents
   int splits, kb_per_split;
-  size_t norm_off, xr_off, xc_off[2], part_off, a_off, b_off, bytes;
+  float qscale;        // bf16: the scale of Q's planes
+  size_t norm_off, xr_off, xc_off[2], part_off, mm_off[5], bytes;
   size_t xr_bytes, xc_bytes, a_bytes, part_elems;  // a matrix
 };
 
-OrthoPlan make_ortho_plan(int batch, int rows, int cols) {
+OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   OrthoPlan p{};
   p.batch = batch;
+  p.bf16 = bf16;
+  p.np = bf16 ? 1 : 2;
   p.tall = rows > cols;
   p.m = p.tall ? cols : rows;
   p.n = p.tall ? rows : cols;
@@ -50,8 +65,8 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols) {
   if (splits < 1) splits = 1;
   p.kb_per_split = (int)round_up(ceil_div(kb, splits), 2);
   p.splits = (int)ceil_div(kb, p.kb_per_split);
-  p.xr_bytes = (size_t)p.m128 * p.n32 * 4;
-  p.xc_bytes = (size_t)p.n128 * p.m32 * 4;
+  p.xr_bytes = (size_t)p.m128 * p.n32 * 2 * p.np;
+  p.xc_bytes = (size_t)p.n128 * p.m32 * 2 * p.np;
   p.a_bytes = (size_t)p.m128 * p.m32 * 4;
   p.part_elems = (size_t)p.m128 * p.m128;
   size_t off = 0;
@@ -60,13 +75,12 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols) {
     off = align256(off + n);
     return at;
   };
-  p.norm_off = take((size_t)batch * kNormBlocks * sizeof(double));
+  p.norm_off = take((size_t)batch * (kNormBlocks + 1) * sizeof(double));
   p.xr_off = take(p.xr_bytes * batch);
   p.xc_off[0] = take(p.xc_bytes * batch);
-  p.xc_off[1] = take(p.xc_bytes * batch);
+  p.xc_off[1] = bf16 ? 0 : take(p.xc_bytes * batch);
   p.part_off = take(p.part_elems * batch * p.splits * sizeof(float));
-  p.a_off = take(p.a_bytes * batch);
-  p.b_off = take(p.a_bytes * batch);
+  for (int i = 0; i < (bf16 ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
   p.bytes = off;
   return p;
 }
@@ -87,33 +101,63 @@ __device__ __forceinline__ float entry(const OrthoArgs& a, int64_t at) {
 }
 
 // Sums of squares in 64 bits, kNormBlocks partials a matrix; Muon's momentum is
-// updated on the way (buf = mu buf + (1 - mu) g).  Element order follows memory:
-// inner, then rows, then outer columns where a view has an inner dimension.
+// updated on the way (buf = mu buf + (1 - mu) g).  A matrix is dense in memory, so
+// its elements are read as they lie, 16 bytes a load, four loads in flight.
 __global__ __launch_bounds__(256) void k_ortho_norm(OrthoArgs a, double* part) {
   const int b = blockIdx.y;
-  const int64_t total = (int64_t)a.rows * a.cols;
-  const int inner = a.view.inner;
+  const int64_t total = (int64_t)a.rows * a.cols, step = (int64_t)kNormBlocks * 256;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, base = b * a.view.sb;
   double s = 0.0;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)kNormBlocks * 256) {
-    int64_t at;
-    if (inner == 1) {
-      const int64_t r = e / a.cols;
-      at = b * a.view.sb + r * a.view.sr + (e - r * a.cols) * a.view.so;
-    } else {  // (outer column, row, inner)
-      const int64_t q = e / inner, i = q / a.rows;
-      at = b * a.view.sb + (q - i * a.rows) * a.view.sr + i * a.view.so + (e - q * inner) * a.view.si;
-    }
-    float v;
+  auto one = [&](int64_t e) {
     if (a.in) {
-      v = entry(a, at);
+      const float v = entry(a, base + e);
+      s += (double)v * v;
     } else {
-      const float g = a.g[at];
-      const float nb = fmaf(a.momentum, a.buf[at], (1.0f - a.momentum) * g);
-      a.buf[at] = nb;
-      v = muon_dir(g, nb, a);
+      const float g = a.g[base + e], nb = fmaf(a.momentum, a.buf[base + e], (1.0f - a.momentum) * g);
+      a.buf[base + e] = nb;
+      const float v = muon_dir(g, nb, a);
+      s += (double)v * v;
     }
-    s += (double)v * v;
+  };
+  const int N = a.in && a.bf16 ? 8 : 4;
+  const void* src = a.in ? (a.bf16 ? (const void*)((const __bf16*)a.in + base) : (const void*)((const float*)a.in + base))
+                         : (const void*)(a.g + base);
+  // vectors where the matrix (and Muon's momentum) begin at a 16-byte boundary
+  const int64_t nv = (((uintptr_t)src | (a.in ? 0 : (uintptr_t)(a.buf + base))) & 15) ? 0 : total / N;
+  for (int64_t i = first; i < nv; i += 4 * step) {
+    u32x4_t w[4], m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * step < nv) {
+        w[u] = ((const u32x4_t*)src)[i + u * step];
+        if (!a.in) m[u] = ((const u32x4_t*)(a.buf + base))[i + u * step];
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i + u * step >= nv) continue;
+      if (a.in && a.bf16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = __uint_as_float(w[u][j] << 16), y = __uint_as_float(w[u][j] & 0xffff0000u);
+          s += (double)x * x;
+          s += (double)y * y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v = __uint_as_float(w[u][j]);
+          if (!a.in) {
+            const float nb = fmaf(a.momentum, __uint_as_float(m[u][j]), (1.0f - a.momentum) * v);
+            m[u][j] = __float_as_uint(nb);
+            v = muon_dir(v, nb, a);
+          }
+          s += (double)v * v;
+        }
+        if (!a.in) ((u32x4_t*)(a.buf + base))[i + u * step] = m[u];
+      }
+    }
   }
+  for (int64_t e = nv * N + first; e < total; e += step) one(e);
   __shared__ double red[256];
   red[threadIdx.x] = s;
   __syncthreads();
@@ -124,31 +168,54 @@ __global__ __launch_bounds__(256) void k_ortho_norm(OrthoArgs a, double* part) {
   if (threadIdx.x == 0) part[b * kNormBlocks + blockIdx.x] = red[0];
 }
 
-// X0 in both operand forms: one block a 64 x 64 tile (m x n), through LDS.
-__global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, const double* part, char* xr,
-                                                    char* xc) {
+__device__ __forceinline__ double norm_sum(const double* part, int b, double* red) {
+  red[threadIdx.x] = part[b * kNormBlocks + threadIdx.x];
+  __syncthreads();
+  for (int w = 128; w > 0; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  return red[0];
+}
+
+// X0 in both operand forms: one block a 64 x 64 tile (m x n), through LDS.  In one
+// plane the scale is a power of two and what it leaves, a factor in [1, 2), goes to
+// rest[b]: the matrix is then X0 / rest exactly.
+template <int NP>
+__global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, const double* part, double* rest,
+                                                    char* xr, char* xc) {
   __shared__ float tile[64][65];
   __shared__ double red[256];
   const int b = blockIdx.z, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tid = threadIdx.x;
-  red[tid] = part[b * kNormBlocks + tid];
-  __syncthreads();
-  for (int w = 128; w > 0; w >>= 1) {
-    if (tid < w) red[tid] += red[tid + w];
-    __syncthreads();
+  float f = kS / ((float)sqrt(norm_sum(part, b, red)) + a.eps);
+  if constexpr (NP == 1) {
+    int x;
+    frexpf(f, &x);
+    const float two = ldexpf(1.0f, x - 1);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) rest[b] = (double)(f / two);
+    f = two;
   }
-  const float f = kS / ((float)sqrt(red[0]) + a.eps);
-  // memory runs along n for an ordinary matrix with rows m, along m for the
-  // transposed, and along (row, inner) for a view with an inner dimension
-  for (int e = tid; e < 64 * 64; e += 256) {
-    int mi = e >> 6, ni = e & 63;
-    if (p.tall || a.view.inner != 1) {
-      mi = e & 63;
-      ni = e >> 6;
+  if (a.view.inner != 1 && !p.tall) {
+    // memory runs along (row, inner column): 64 rows of each outer column in the tile
+    const int D = a.view.inner, i0 = n0 / D, i1 = (n0 + 63) / D;
+    for (int q = tid; q < 64 * 64; q += 256) tile[q >> 6][q & 63] = 0.0f;
+    __syncthreads();
+    for (int q = tid; q < (i1 - i0 + 1) * 64 * D; q += 256) {
+      const int i = q / (64 * D), in = q - i * 64 * D, r = in / D, c = (i0 + i) * D + in - r * D;
+      if (c < n0 || c >= n0 + 64 || c >= p.n || m0 + r >= p.m) continue;
+      tile[r][c - n0] = f * entry(a, b * a.view.sb + (int64_t)(m0 + r) * a.view.sr + (int64_t)(i0 + i) * a.view.so +
+                                         (int64_t)(in - r * D) * a.view.si);
     }
-    const int m = m0 + mi, n = n0 + ni;
-    float v = 0.0f;
-    if (m < p.m && n < p.n) v = f * entry(a, p.tall ? view_at(a.view, b, n, m) : view_at(a.view, b, m, n));
-    tile[mi][ni] = v;
+  } else {
+    // memory runs along n for an ordinary matrix with rows m, along m for a transposed one
+    const bool along_m = p.tall == (a.view.so == 1 || a.view.inner != 1);
+    for (int e = tid; e < 64 * 64; e += 256) {
+      const int mi = along_m ? e & 63 : e >> 6, ni = along_m ? e >> 6 : e & 63;
+      const int m = m0 + mi, n = n0 + ni;
+      float v = 0.0f;
+      if (m < p.m && n < p.n) v = f * entry(a, p.tall ? view_at(a.view, b, n, m) : view_at(a.view, b, m, n));
+      tile[mi][ni] = v;
+    }
   }
   __syncthreads();
   // 64 rows x 8 groups of 8 k of each form: 512 lanes' values, two a thread
@@ -159,28 +226,30 @@ __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, co
     if (m0 + r < p.m128 && n0 + k8 * 8 < p.n32) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = tile[r][k8 * 8 + j];
-      const Planes8<2> f8 = to_planes8<2>(v);
+      const Planes8<NP> f8 = to_planes8<NP>(v);
       const int row = m0 + r, kb = (n0 + k8 * 8) >> 4, g = k8 & 1;
-      char* d = xr + b * p.xr_bytes + ((size_t)(row >> 5) * (p.n32 / 16) + kb) * 2 * kPlaneBytes + ((row & 31) + 32 * g) * 16;
-      *(f16x8_t*)d = f8.p[0];
-      *(f16x8_t*)(d + kPlaneBytes) = f8.p[1];
+      char* d = xr + b * p.xr_bytes + ((size_t)(row >> 5) * (p.n32 / 16) + kb) * NP * kPlaneBytes + ((row & 31) + 32 * g) * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f8.p[k];
     }
     if (n0 + r < p.n128 && m0 + k8 * 8 < p.m32) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = tile[k8 * 8 + j][r];
-      const Planes8<2> f8 = to_planes8<2>(v);
+      const Planes8<NP> f8 = to_planes8<NP>(v);
       const int row = n0 + r, kb = (m0 + k8 * 8) >> 4, g = k8 & 1;
-      char* d = xc + b * p.xc_bytes + ((size_t)(row >> 5) * (p.m32 / 16) + kb) * 2 * kPlaneBytes + ((row & 31) + 32 * g) * 16;
-      *(f16x8_t*)d = f8.p[0];
-      *(f16x8_t*)(d + kPlaneBytes) = f8.p[1];
+      char* d = xc + b * p.xc_bytes + ((size_t)(row >> 5) * (p.m32 / 16) + kb) * NP * kPlaneBytes + ((row & 31) + 32 * g) * 16;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f8.p[k];
     }
   }
 }
 
-typedef NtTile<2, 2, 2, 2, 2, 2, 2, 2> Tile22;  // 128 x 128, 64 KiB of LDS
+template <int NP> using GramTile = NtTile<NP, NP, 2, 2, 2, 2, 2, NP == 1 ? 4 : 2>;  // 128 x 128, 64 KiB of LDS
+typedef GramTile<2> Tile22;
 
 // Partial sums of A = X X^T (scale kS^2): the tiles on and below the diagonal,
 // each stored with its mirror image, k split over blocks.
+template <int NP>
 __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* xr, float* part) {
   extern __shared__ char lds[];
   const int T = p.m128 / kTile, pairs = T * (T + 1) / 2;
@@ -193,10 +262,10 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
   const int tn = pair - tm * (tm + 1) / 2;
   const int KB = p.n32 / 16, kb0 = split * p.kb_per_split;
   const int kbs = KB - kb0 < p.kb_per_split ? KB - kb0 : p.kb_per_split;
-  const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
+  const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const char* x = xr + b * p.xr_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / 2, lds, acc);
+  GramTile<NP>::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / 2, lds, acc);
   float* out = part + ((size_t)split * p.batch + b) * p.part_elems;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -218,69 +287,126 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
 }
 
 // A in planes from the partial sums: a thread a row and 8 k.
-__global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, char* A) {
+__global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, const double* rest, char* A) {
   const int b = blockIdx.y;
   const int k8s = p.m32 / 8;
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (q >= (int64_t)p.m128 * k8s) return;
   const int k8 = (int)(q % k8s), row = (int)(q / k8s);
+  const float f = p.bf16 ? (float)(rest[b] * rest[b]) * kInvS : kInvS;
   float v[8] = {};
   if (row < p.m) {
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
       const float* src = part + ((size_t)s * p.batch + b) * p.part_elems + (size_t)row * p.m128 + k8 * 8;
+      const f32x4_t lo = *(const f32x4_t*)src, hi = *(const f32x4_t*)(src + 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += src[j];
+      for (int j = 0; j < 4; ++j) {
+        v[j] += lo[j];
+        v[4 + j] += hi[j];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k8 * 8 + j < p.m ? v[j] * kInvS : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = k8 * 8 + j < p.m ? v[j] * f : 0.0f;
   }
-  const Planes8<2> f = to_planes8<2>(v);
+  const Planes8<2> o = to_planes8<2>(v);
   char* d = A + b * p.a_bytes + ((size_t)(row >> 5) * (p.m32 / 16) + (k8 >> 1)) * 2 * kPlaneBytes + ((row & 31) + 32 * (k8 & 1)) * 16;
-  *(f16x8_t*)d = f.p[0];
-  *(f16x8_t*)(d + kPlaneBytes) = f.p[1];
+  *(f16x8_t*)d = o.p[0];
+  *(f16x8_t*)(d + kPlaneBytes) = o.p[1];
 }
 
 // The 8-byte half of a lane's planes that an accumulator quad (4 consecutive
 // rows of the product) is in the operand whose k runs along those rows.
+template <int NP>
 __device__ __forceinline__ size_t quad_at(int row, int k, int KB) {
-  return ((size_t)(row >> 5) * KB + (k >> 4)) * 2 * kPlaneBytes + ((row & 31) + 32 * ((k >> 3) & 1)) * 16 + (k & 4) * 2;
+  return ((size_t)(row >> 5) * KB + (k >> 4)) * NP * kPlaneBytes + ((row & 31) + 32 * ((k >> 3) & 1)) * 16 + (k & 4) * 2;
 }
 
-// B = b A + c A^2 (A symmetric: A A = A A^T); B is symmetric too, so the product's
-// rows are stored as the operand's k.
-__global__ __launch_bounds__(256, 2) void k_ortho_poly(OrthoPlan p, const char* A, char* B, float cb, float cc) {
+// One product of m x m matrices: out = alpha L R^T + beta R + gamma I in planes (out2
+// the same times `two`).  All of them are symmetric, polynomials in one matrix, so
+// the product's rows are stored as the operand's k.
+struct MmJob {
+  const char *l, *r;
+  char *out, *out2;
+  float alpha, beta, gamma, two;
+};
+struct MmJobs { MmJob j[2]; };
+
+// 64 x 64 tiles (128 x 128 ones leave most CUs without a block at these sizes), waves
+// of 32 x 32, stages of 4 k-blocks two ahead.
+typedef NtTile<2, 2, 2, 2, 1, 1, 2, 4> MmTile;  // 64 KiB of LDS
+
+__global__ __launch_bounds__(256, 2) void k_ortho_mm(OrthoPlan p, MmJobs jobs) {
   extern __shared__ char lds[];
-  const int T = p.m128 / kTile, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T), tm = t / T, tn = t % T;
+  const MmJob& j = jobs.j[blockIdx.y];
+  const int T = (p.m32 + 63) / 64, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T), tm = t / T, tn = t % T;
   const int KB = p.m32 / 16;
-  const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
-  const char* x = A + b * p.a_bytes;
-  f32x16_t acc[2][2] = {};
-  Tile22::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0, KB / 2, lds, acc);
-  char* out = B + b * p.a_bytes;
+  const size_t pitch = (size_t)KB * 2 * kPlaneBytes, at0 = b * p.a_bytes;
+  f32x16_t acc[1][1] = {};
+  MmTile::run(RowBlocks{j.l + at0 + tm * 2 * pitch, pitch}, RowBlocks{j.r + at0 + tn * 2 * pitch, pitch}, 0, KB / 2, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
+  const int row0 = tm * 64 + (wave >> 1) * 32, col = tn * 64 + (wave & 1) * 32 + (lane & 31);
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int q = 0; q < 4; ++q) {
+    const int k = row0 + 8 * q + 4 * g;
+    if (k >= p.m32) continue;
+    const size_t at = at0 + quad_at<2>(col, k, KB);
+    float v[4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int row0 = tm * kTile + (wave >> 1) * 64 + m * 32, col = tn * kTile + (wave & 1) * 64 + n * 32 + (lane & 31);
+    for (int i = 0; i < 4; ++i) v[i] = j.alpha * acc[0][0][q * 4 + i] + (k + i == col ? j.gamma : 0.0f);
+    if (j.beta != 0.0f) {
+      const f16x4_t h = *(const f16x4_t*)(j.r + at), l = *(const f16x4_t*)(j.r + at + kPlaneBytes);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int k = row0 + 8 * q + 4 * g;
-        if (k >= p.m32) continue;
-        const size_t at = quad_at(col, k, KB);
-        const f16x4_t h = *(const f16x4_t*)(x + at), l = *(const f16x4_t*)(x + at + kPlaneBytes);
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = cb * ((float)h[j] + (float)l[j]) + cc * (acc[m][n][q * 4 + j] * kInvS);
-          if (k + j >= p.m || col >= p.m) v[j] = 0.0f;
-        }
-        const Planes4<2> f = to_planes4<2>(v);
-        *(f16x4_t*)(out + at) = f.p[0];
-        *(f16x4_t*)(out + at + kPlaneBytes) = f.p[1];
-      }
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(j.beta, (float)h[i] + (float)l[i], v[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k + i >= p.m || col >= p.m) v[i] = 0.0f;
+    Planes4<2> f = to_planes4<2>(v);
+    *(f16x4_t*)(j.out + at) = f.p[0];
+    *(f16x4_t*)(j.out + at + kPlaneBytes) = f.p[1];
+    if (j.out2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] *= j.two;
+      f = to_planes4<2>(v);
+      *(f16x4_t*)(j.out2 + at) = f.p[0];
+      *(f16x4_t*)(j.out2 + at + kPlaneBytes) = f.p[1];
+    }
+  }
 }
+
+__device__ __forceinline__ void put(const OrthoArgs& a, int64_t e, float o) {
+  if (!a.in)
+    a.p[e] = fmaf(-a.lr * a.scale, o, a.p[e] * (1.0f - a.lr * a.decay));
+  else if (a.bf16)
+    ((__bf16*)a.out)[e] = (__bf16)o;
+  else
+    ((float*)a.out)[e] = o;
+}
+
+// A 128 x 128 tile of the result, staged in LDS as [n][m] (pitch 129), to where it
+// belongs: along (row, inner) for a view with an inner dimension and rows m, else
+// along whichever of m and n lies contiguous.
+__device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p, const float* tile, int b, int m0, int n0) {
+  constexpr int W = kTile + 1;
+  if (a.view.inner != 1 && !p.tall) {
+    const int D = a.view.inner, i0 = n0 / D, i1 = (n0 + kTile - 1) / D;
+    for (int q = threadIdx.x; q < (i1 - i0 + 1) * kTile * D; q += 256) {
+      const int i = q / (kTile * D), in = q - i * kTile * D, r = in / D, d = in - r * D, c = (i0 + i) * D + d;
+      if (c < n0 || c >= n0 + kTile || c >= p.n || m0 + r >= p.m) continue;
+      put(a, b * a.view.sb + (int64_t)(m0 + r) * a.view.sr + (int64_t)(i0 + i) * a.view.so + (int64_t)d * a.view.si,
+          tile[(c - n0) * W + r]);
+    }
+    return;
+  }
+  const bool along_m = p.tall == (a.view.so == 1 || a.view.inner != 1);
+  for (int q = threadIdx.x; q < kTile * kTile; q += 256) {
+    const int mi = along_m ? q % kTile : q / kTile, ni = along_m ? q / kTile : q % kTile;
+    if (m0 + mi < p.m && n0 + ni < p.n)
+      put(a, p.tall ? view_at(a.view, b, n0 + ni, m0 + mi) : view_at(a.view, b, m0 + mi, n0 + ni), tile[ni * W + mi]);
+  }
+}
+constexpr int kPutLds = kTile * (kTile + 1) * 4;
 
 // X' = a X + B X.  The product's rows are m, its columns n: an accumulator quad is 4
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
@@ -311,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
       for (int q = 0; q < 4; ++q) {
         const int r = r0 + 8 * q + 4 * g, k = tm * kTile + r;
         float v[4] = {};
-        const size_t at = quad_at(col, k, KB);
+        const size_t at = quad_at<2>(col, k, KB);
         if (k < p.m32) {
           const f16x4_t h = *(const f16x4_t*)(x + at), l = *(const f16x4_t*)(x + at + kPlaneBytes);
 #pragma unroll
@@ -320,17 +446,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
         }
         if (last) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (k + j >= p.m || col >= p.n) continue;
-            const float o = v[j] * kInvS;
-            const int64_t e = p.tall ? view_at(a.view, b, col, k + j) : view_at(a.view, b, k + j, col);
-            if (!a.in)
-              a.p[e] = fmaf(-a.lr * a.scale, o, a.p[e] * (1.0f - a.lr * a.decay));
-            else if (a.bf16)
-              ((__bf16*)a.out)[e] = (__bf16)o;
-            else
-              ((float*)a.out)[e] = o;
-          }
+          for (int j = 0; j < 4; ++j) ((float*)lds)[c * (kTile + 1) + r + j] = v[j] * kInvS;
           continue;
         }
         const Planes4<2> f = to_planes4<2>(v);
@@ -346,8 +462,11 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
         }
       }
     }
-  if (last) return;
   __syncthreads();
+  if (last) {
+    put_tile(a, p, (const float*)lds, b, tm * kTile, tn * kTile);
+    return;
+  }
   // Xr: 128 rows x 16 groups of 8 k, 8 a thread
   const int KBr = p.n32 / 16;
 #pragma unroll
@@ -361,64 +480,132 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   }
 }
 
-constexpr int kUpdateLds = 2 * kTile * (kTile + 8) * 2 > Tile22::kLdsBytes ? 2 * kTile * (kTile + 8) * 2 : Tile22::kLdsBytes;
+constexpr int max3(int a, int b, int c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
+constexpr int kUpdateLds = max3(2 * kTile * (kTile + 8) * 2, Tile22::kLdsBytes, kPutLds);
+
+// The bf16 result Q X0: Q in two planes (scale qscale), X0 / rest in one.
+typedef NtTile<2, 1, 2, 2, 2, 2, 2, 3> ApplyTile;  // 72 KiB of LDS
+__global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p, const char* Q, const char* xc,
+                                                        const double* rest) {
+  extern __shared__ char lds[];
+  const int TM = p.m128 / kTile, TN = p.n128 / kTile;
+  int id = blockIdx.x;
+  const int tm = id % TM;
+  id /= TM;
+  const int tn = id % TN, b = id / TN;
+  const int KB = p.m32 / 16;
+  const size_t pq = (size_t)KB * 2 * kPlaneBytes, px = (size_t)KB * kPlaneBytes;
+  f32x16_t acc[2][2] = {};
+  ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0, KB / 2,
+                 lds, acc);
+  const float f = (float)rest[b] * kInvS / p.qscale;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int q = 0; q < 16; ++q)
+        ((float*)lds)[((wave & 1) * 64 + n * 32 + (lane & 31)) * (kTile + 1) + (wave >> 1) * 64 + m * 32 + acc_row(q, g)] =
+            acc[m][n][q] * f;
+  __syncthreads();
+  put_tile(a, p, (const float*)lds, b, tm * kTile, tn * kTile);
+}
+constexpr int kApplyLds = ApplyTile::kLdsBytes > kPutLds ? ApplyTile::kLdsBytes : kPutLds;
 
 // steps == 0: the normalised matrix itself.
 __global__ __launch_bounds__(256) void k_ortho_scale(OrthoArgs a, const double* part) {
   __shared__ double red[256];
-  const int b = blockIdx.y, tid = threadIdx.x;
-  red[tid] = part[b * kNormBlocks + tid];
-  __syncthreads();
-  for (int w = 128; w > 0; w >>= 1) {
-    if (tid < w) red[tid] += red[tid + w];
-    __syncthreads();
-  }
-  const float f = (float)sqrt(red[0]) + a.eps;
+  const int b = blockIdx.y;
+  const float f = (float)sqrt(norm_sum(part, b, red)) + a.eps;
   const int64_t total = (int64_t)a.rows * a.cols;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + tid; e < total; e += (int64_t)gridDim.x * 256) {
-    const int r = (int)(e / a.cols), c = (int)(e % a.cols);
-    const int64_t at = view_at(a.view, b, r, c);
-    const float o = entry(a, at) / f;
-    if (!a.in)
-      a.p[at] = fmaf(-a.lr * a.scale, o, a.p[at] * (1.0f - a.lr * a.decay));
-    else if (a.bf16)
-      ((__bf16*)a.out)[at] = (__bf16)o;
-    else
-      ((float*)a.out)[at] = o;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256)
+    put(a, b * a.view.sb + e, entry(a, b * a.view.sb + e) / f);
+}
+
+// The largest value of Q that singular values in [0, 1] give, by sampling.
+float largest_q(const OrthoArgs& a) {
+  double most = 0.0;
+  for (int i = 0; i <= 1024; ++i) {
+    double x = i / 1024.0, q = 1.0;
+    for (int s = 0; s < a.steps; ++s) {
+      const double f = a.a + a.b * x * x + a.c * x * x * x * x;
+      q *= f;
+      x *= f;
+      most = fmax(most, fabs(q));
+    }
   }
+  return (float)most;
 }
 
 }  // namespace
 
-size_t ortho_workspace_bytes(int batch, int rows, int cols) { return make_ortho_plan(batch, rows, cols).bytes; }
+size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16) {
+  return make_ortho_plan(batch, rows, cols, bf16).bytes;
+}
 
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
-  const OrthoPlan p = make_ortho_plan(a.batch, a.rows, a.cols);
+  OrthoPlan p = make_ortho_plan(a.batch, a.rows, a.cols, a.bf16 != 0);
   char* w = (char*)ws;
-  double* norm = (double*)(w + p.norm_off);
-  char *xr = w + p.xr_off, *A = w + p.a_off, *B = w + p.b_off;
+  double *norm = (double*)(w + p.norm_off), *rest = norm + (size_t)a.batch * kNormBlocks;
+  char* xr = w + p.xr_off;
   char* xc[2] = {w + p.xc_off[0], w + p.xc_off[1]};
   float* part = (float*)(w + p.part_off);
-  static std::atomic<uint32_t> done[3];
-  ensure_lds_limit((const void*)k_ortho_gram, Tile22::kLdsBytes, done[0]);
-  ensure_lds_limit((const void*)k_ortho_poly, Tile22::kLdsBytes, done[1]);
-  ensure_lds_limit((const void*)k_ortho_update, kUpdateLds, done[2]);
+  char* mm[5];
+  for (int i = 0; i < 5; ++i) mm[i] = w + p.mm_off[i];
+  static std::atomic<uint32_t> done[5];
+  ensure_lds_limit((const void*)k_ortho_gram<1>, GramTile<1>::kLdsBytes, done[0]);
+  ensure_lds_limit((const void*)k_ortho_gram<2>, GramTile<2>::kLdsBytes, done[1]);
+  ensure_lds_limit((const void*)k_ortho_mm, MmTile::kLdsBytes, done[2]);
+  ensure_lds_limit((const void*)k_ortho_update, kUpdateLds, done[3]);
+  ensure_lds_limit((const void*)k_ortho_apply, kApplyLds, done[4]);
   hipLaunchKernelGGL(k_ortho_norm, dim3(kNormBlocks, a.batch), dim3(256), 0, st, a, norm);
   if (a.steps == 0) {
     hipLaunchKernelGGL(k_ortho_scale, dim3(kNormBlocks, a.batch), dim3(256), 0, st, a, norm);
     return;
   }
-  hipLaunchKernelGGL(k_ortho_pack, dim3(p.n128 / 64, p.m128 / 64, a.batch), dim3(256), 0, st, a, p, norm, xr, xc[0]);
-  const int T = p.m128 / kTile, TN = p.n128 / kTile;
-  for (int s = 0; s < a.steps; ++s) {
-    hipLaunchKernelGGL(k_ortho_gram, dim3(a.batch * (T * (T + 1) / 2) * p.splits), dim3(256), Tile22::kLdsBytes, st, p,
-                       xr, part);
-    hipLaunchKernelGGL(k_ortho_gram_sum, dim3((unsigned)ceil_div((int64_t)p.m128 * (p.m32 / 8), 256), a.batch),
-                       dim3(256), 0, st, p, part, A);
-    hipLaunchKernelGGL(k_ortho_poly, dim3(a.batch * T * T), dim3(256), Tile22::kLdsBytes, st, p, A, B, a.b, a.c);
-    hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), dim3(256), kUpdateLds, st, a, p, B, xc[s & 1],
-                       xc[(s + 1) & 1], xr, s == a.steps - 1);
+  const dim3 pack_grid(p.n128 / 64, p.m128 / 64, a.batch), block(256);
+  const int T = p.m128 / kTile, TN = p.n128 / kTile, T64 = (p.m32 + 63) / 64;
+  const dim3 gram_grid(a.batch * (T * (T + 1) / 2) * p.splits);
+  const dim3 sum_grid((unsigned)ceil_div((int64_t)p.m128 * (p.m32 / 8), 256), a.batch);
+  auto products = [&](const MmJob& one, const MmJob* two) {
+    MmJobs jobs{{one, two ? *two : one}};
+    hipLaunchKernelGGL(k_ortho_mm, dim3(a.batch * T64 * T64, two ? 2 : 1), block, MmTile::kLdsBytes, st, p, jobs);
+  };
+  if (!p.bf16) {
+    hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
+    for (int s = 0; s < a.steps; ++s) {
+      hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::kLdsBytes, st, p, xr, part);
+      hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
+      products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f}, nullptr);
+      hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), block, kUpdateLds, st, a, p, mm[1], xc[s & 1], xc[(s + 1) & 1],
+                         xr, s == a.steps - 1);
+    }
+    return;
   }
+  // |Q| below 2^14 in its planes
+  int x;
+  frexpf(largest_q(a), &x);
+  p.qscale = ldexpf(1.0f, 14 - x > 12 ? 12 : 14 - x);
+  hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
+  hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::kLdsBytes, st, p, xr, part);
+  hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
+  char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
+  for (int s = 0; s < a.steps; ++s) {
+    const bool last = s == a.steps - 1;
+    products(MmJob{A, A, P, s == 0 ? Q : nullptr, a.c * kInvS, a.b, a.a * kS, p.qscale * kInvS}, nullptr);
+    const MmJob pa{P, A, W, nullptr, kInvS, 0.0f, 0.0f, 0.0f}, qp{Q, P, Qn, nullptr, kInvS, 0.0f, 0.0f, 0.0f};
+    if (s == 0) {
+      if (!last) products(pa, nullptr);
+    } else {
+      products(qp, last ? nullptr : &pa);
+      char* q = Q;
+      Q = Qn;
+      Qn = q;
+    }
+    if (!last) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);
+  }
+  hipLaunchKernelGGL(k_ortho_apply, dim3(a.batch * T * TN), block, kApplyLds, st, a, p, Q, xc[0], rest);
 }
 
 }  // namespace ckan
