@@ -35,7 +35,7 @@ struct OrthoPlan {
   bool tall;           // rows > cols: m runs along the columns
   bool bf16;
   int np;              // planes of X
-  int m32, n32;        // k extents
+  int mk, n32;         // k extents: m in whole stages of the m x m products, n in 32
   int m128, n128;      // row extents
   int splits, kb_per_split;
   float qscale;        // bf16: the scale of Q's planes
@@ -51,23 +51,23 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   p.tall = rows > cols;
   p.m = p.tall ? cols : rows;
   p.n = p.tall ? rows : cols;
-  p.m32 = (int)round_up(p.m, 32);
+  p.mk = (int)round_up(p.m, 64);
   p.n32 = (int)round_up(p.n, 32);
   p.m128 = (int)round_up(p.m, kTile);
   p.n128 = (int)round_up(p.n, kTile);
-  // A = X X^T has few tiles and a long k: enough splits of k to give every CU a
-  // block, none shorter than 256 (16 k-blocks)
+  // A = X X^T has few tiles and a long k: splits of k up to two blocks a CU (320 blocks
+  // of 8 x [512, 4608] took 54 us, 480 take 37), none shorter than 256 (16 k-blocks)
   const int T = p.m128 / kTile;
   const int64_t tiles = (int64_t)batch * T * (T + 1) / 2;
-  int64_t splits = ceil_div(kNumCUs, tiles);
+  int64_t splits = 2 * kNumCUs / tiles;
   const int kb = p.n32 / 16;
   if (splits > kb / 16) splits = kb / 16;
   if (splits < 1) splits = 1;
   p.kb_per_split = (int)round_up(ceil_div(kb, splits), 2);
   p.splits = (int)ceil_div(kb, p.kb_per_split);
   p.xr_bytes = (size_t)p.m128 * p.n32 * 2 * p.np;
-  p.xc_bytes = (size_t)p.n128 * p.m32 * 2 * p.np;
-  p.a_bytes = (size_t)p.m128 * p.m32 * 4;
+  p.xc_bytes = (size_t)p.n128 * p.mk * 2 * p.np;
+  p.a_bytes = (size_t)p.m128 * p.mk * 4;
   p.part_elems = (size_t)p.m128 * p.m128;
   size_t off = 0;
   auto take = [&](size_t n) {
@@ -103,61 +103,63 @@ __device__ __forceinline__ float entry(const OrthoArgs& a, int64_t at) {
 // Sums of squares in 64 bits, kNormBlocks partials a matrix; Muon's momentum is
 // updated on the way (buf = mu buf + (1 - mu) g).  A matrix is dense in memory, so
 // its elements are read as they lie, 16 bytes a load, four loads in flight.
+enum NormKind { kNormF32, kNormBf16, kNormMuon };
+template <int KIND>
 __global__ __launch_bounds__(256) void k_ortho_norm(OrthoArgs a, double* part) {
+  constexpr int N = KIND == kNormBf16 ? 8 : 4;
   const int b = blockIdx.y;
   const int64_t total = (int64_t)a.rows * a.cols, step = (int64_t)kNormBlocks * 256;
   const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, base = b * a.view.sb;
+  const char* src = (KIND == kNormMuon ? (const char*)a.g : (const char*)a.in) + base * (16 / N);
+  float* buf = a.buf + base;
   double s = 0.0;
-  auto one = [&](int64_t e) {
-    if (a.in) {
-      const float v = entry(a, base + e);
-      s += (double)v * v;
-    } else {
-      const float g = a.g[base + e], nb = fmaf(a.momentum, a.buf[base + e], (1.0f - a.momentum) * g);
-      a.buf[base + e] = nb;
-      const float v = muon_dir(g, nb, a);
-      s += (double)v * v;
-    }
+  auto muon = [&](float g, float& m) {
+    m = fmaf(a.momentum, m, (1.0f - a.momentum) * g);
+    const float v = muon_dir(g, m, a);
+    s += (double)v * v;
   };
-  const int N = a.in && a.bf16 ? 8 : 4;
-  const void* src = a.in ? (a.bf16 ? (const void*)((const __bf16*)a.in + base) : (const void*)((const float*)a.in + base))
-                         : (const void*)(a.g + base);
   // vectors where the matrix (and Muon's momentum) begin at a 16-byte boundary
-  const int64_t nv = (((uintptr_t)src | (a.in ? 0 : (uintptr_t)(a.buf + base))) & 15) ? 0 : total / N;
+  const uintptr_t at = (uintptr_t)src | (KIND == kNormMuon ? (uintptr_t)buf : 0);
+  const int64_t nv = at & 15 ? 0 : total / N;
   for (int64_t i = first; i < nv; i += 4 * step) {
     u32x4_t w[4], m[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (i + u * step < nv) {
         w[u] = ((const u32x4_t*)src)[i + u * step];
-        if (!a.in) m[u] = ((const u32x4_t*)(a.buf + base))[i + u * step];
+        if constexpr (KIND == kNormMuon) m[u] = ((const u32x4_t*)buf)[i + u * step];
       }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (i + u * step >= nv) continue;
-      if (a.in && a.bf16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (KIND == kNormBf16) {
           const float x = __uint_as_float(w[u][j] << 16), y = __uint_as_float(w[u][j] & 0xffff0000u);
           s += (double)x * x;
           s += (double)y * y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v = __uint_as_float(w[u][j]);
-          if (!a.in) {
-            const float nb = fmaf(a.momentum, __uint_as_float(m[u][j]), (1.0f - a.momentum) * v);
-            m[u][j] = __float_as_uint(nb);
-            v = muon_dir(v, nb, a);
-          }
+        } else if constexpr (KIND == kNormF32) {
+          const float v = __uint_as_float(w[u][j]);
           s += (double)v * v;
+        } else {
+          float nb = __uint_as_float(m[u][j]);
+          muon(__uint_as_float(w[u][j]), nb);
+          m[u][j] = __float_as_uint(nb);
         }
-        if (!a.in) ((u32x4_t*)(a.buf + base))[i + u * step] = m[u];
       }
+      if constexpr (KIND == kNormMuon) ((u32x4_t*)buf)[i + u * step] = m[u];
     }
   }
-  for (int64_t e = nv * N + first; e < total; e += step) one(e);
+  for (int64_t e = nv * N + first; e < total; e += step) {
+    if constexpr (KIND == kNormMuon) {
+      float nb = buf[e];
+      muon(((const float*)src)[e], nb);
+      buf[e] = nb;
+    } else {
+      const float v = entry(a, base + e);
+      s += (double)v * v;
+    }
+  }
   __shared__ double red[256];
   red[threadIdx.x] = s;
   __syncthreads();
@@ -232,12 +234,12 @@ __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, co
 #pragma unroll
       for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f8.p[k];
     }
-    if (n0 + r < p.n128 && m0 + k8 * 8 < p.m32) {
+    if (n0 + r < p.n128 && m0 + k8 * 8 < p.mk) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = tile[k8 * 8 + j][r];
       const Planes8<NP> f8 = to_planes8<NP>(v);
       const int row = n0 + r, kb = (m0 + k8 * 8) >> 4, g = k8 & 1;
-      char* d = xc + b * p.xc_bytes + ((size_t)(row >> 5) * (p.m32 / 16) + kb) * NP * kPlaneBytes + ((row & 31) + 32 * g) * 16;
+      char* d = xc + b * p.xc_bytes + ((size_t)(row >> 5) * (p.mk / 16) + kb) * NP * kPlaneBytes + ((row & 31) + 32 * g) * 16;
 #pragma unroll
       for (int k = 0; k < NP; ++k) *(f16x8_t*)(d + k * kPlaneBytes) = f8.p[k];
     }
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const char* x = xr + b * p.xr_bytes;
   f32x16_t acc[2][2] = {};
-  GramTile<NP>::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / 2, lds, acc);
+  GramTile<NP>::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / GramTile<NP>::kStageBlocks, lds, acc);
   float* out = part + ((size_t)split * p.batch + b) * p.part_elems;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
 // A in planes from the partial sums: a thread a row and 8 k.
 __global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, const double* rest, char* A) {
   const int b = blockIdx.y;
-  const int k8s = p.m32 / 8;
+  const int k8s = p.mk / 8;
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (q >= (int64_t)p.m128 * k8s) return;
   const int k8 = (int)(q % k8s), row = (int)(q / k8s);
@@ -310,7 +312,7 @@ __global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float
     for (int j = 0; j < 8; ++j) v[j] = k8 * 8 + j < p.m ? v[j] * f : 0.0f;
   }
   const Planes8<2> o = to_planes8<2>(v);
-  char* d = A + b * p.a_bytes + ((size_t)(row >> 5) * (p.m32 / 16) + (k8 >> 1)) * 2 * kPlaneBytes + ((row & 31) + 32 * (k8 & 1)) * 16;
+  char* d = A + b * p.a_bytes + ((size_t)(row >> 5) * (p.mk / 16) + (k8 >> 1)) * 2 * kPlaneBytes + ((row & 31) + 32 * (k8 & 1)) * 16;
   *(f16x8_t*)d = o.p[0];
   *(f16x8_t*)(d + kPlaneBytes) = o.p[1];
 }
@@ -333,27 +335,31 @@ struct MmJob {
 struct MmJobs { MmJob j[2]; };
 
 // 64 x 64 tiles (128 x 128 ones leave most CUs without a block at these sizes), waves
-// of 32 x 32, stages of 4 k-blocks two ahead.
-typedef NtTile<2, 2, 2, 2, 1, 1, 2, 4> MmTile;  // 64 KiB of LDS
+// of 32 x 32 with three accumulators.
+typedef NtTile<2, 2, 2, 2, 1, 1, 4, 2, 3> MmTile;  // 64 KiB of LDS
 
 __global__ __launch_bounds__(256, 2) void k_ortho_mm(OrthoPlan p, MmJobs jobs) {
   extern __shared__ char lds[];
   const MmJob& j = jobs.j[blockIdx.y];
-  const int T = (p.m32 + 63) / 64, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T), tm = t / T, tn = t % T;
-  const int KB = p.m32 / 16;
+  const int T = p.mk / 64, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T), tm = t / T, tn = t % T;
+  const int KB = p.mk / 16;
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes, at0 = b * p.a_bytes;
-  f32x16_t acc[1][1] = {};
-  MmTile::run(RowBlocks{j.l + at0 + tm * 2 * pitch, pitch}, RowBlocks{j.r + at0 + tn * 2 * pitch, pitch}, 0, KB / 2, lds, acc);
+  f32x16_t acc[3][1] = {};
+  MmTile::run(RowBlocks{j.l + at0 + tm * 2 * pitch, pitch}, RowBlocks{j.r + at0 + tn * 2 * pitch, pitch}, 0,
+              KB / MmTile::kStageBlocks, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   const int row0 = tm * 64 + (wave >> 1) * 32, col = tn * 64 + (wave & 1) * 32 + (lane & 31);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int k = row0 + 8 * q + 4 * g;
-    if (k >= p.m32) continue;
+    if (k >= p.mk) continue;
     const size_t at = at0 + quad_at<2>(col, k, KB);
     float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = j.alpha * acc[0][0][q * 4 + i] + (k + i == col ? j.gamma : 0.0f);
+    for (int i = 0; i < 4; ++i) {
+      const float s = (acc[0][0][q * 4 + i] + acc[1][0][q * 4 + i]) + acc[2][0][q * 4 + i];
+      v[i] = j.alpha * s + (k + i == col ? j.gamma : 0.0f);
+    }
     if (j.beta != 0.0f) {
       const f16x4_t h = *(const f16x4_t*)(j.r + at), l = *(const f16x4_t*)(j.r + at + kPlaneBytes);
 #pragma unroll
@@ -375,35 +381,63 @@ __global__ __launch_bounds__(256, 2) void k_ortho_mm(OrthoPlan p, MmJobs jobs) {
   }
 }
 
-__device__ __forceinline__ void put(const OrthoArgs& a, int64_t e, float o) {
-  if (!a.in)
-    a.p[e] = fmaf(-a.lr * a.scale, o, a.p[e] * (1.0f - a.lr * a.decay));
-  else if (a.bf16)
-    ((__bf16*)a.out)[e] = (__bf16)o;
-  else
-    ((float*)a.out)[e] = o;
+// N results o[] to elements e[] (negative: none); Muon's N parameters are asked for
+// before any of them is needed.
+template <int N>
+__device__ __forceinline__ void put(const OrthoArgs& a, const int64_t (&e)[N], const float (&o)[N]) {
+  if (!a.in) {
+    float old[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) old[u] = e[u] >= 0 ? a.p[e[u]] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (e[u] >= 0) a.p[e[u]] = fmaf(-a.lr * a.scale, o[u], old[u] * (1.0f - a.lr * a.decay));
+  } else if (a.bf16) {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (e[u] >= 0) ((__bf16*)a.out)[e[u]] = (__bf16)o[u];
+  } else {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (e[u] >= 0) ((float*)a.out)[e[u]] = o[u];
+  }
 }
 
 // A 128 x 128 tile of the result, staged in LDS as [n][m] (pitch 129), to where it
 // belongs: along (row, inner) for a view with an inner dimension and rows m, else
 // along whichever of m and n lies contiguous.
 __device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p, const float* tile, int b, int m0, int n0) {
-  constexpr int W = kTile + 1;
+  constexpr int W = kTile + 1, U = 8;
+  int64_t e[U];
+  float o[U];
   if (a.view.inner != 1 && !p.tall) {
     const int D = a.view.inner, i0 = n0 / D, i1 = (n0 + kTile - 1) / D;
-    for (int q = threadIdx.x; q < (i1 - i0 + 1) * kTile * D; q += 256) {
-      const int i = q / (kTile * D), in = q - i * kTile * D, r = in / D, d = in - r * D, c = (i0 + i) * D + d;
-      if (c < n0 || c >= n0 + kTile || c >= p.n || m0 + r >= p.m) continue;
-      put(a, b * a.view.sb + (int64_t)(m0 + r) * a.view.sr + (int64_t)(i0 + i) * a.view.so + (int64_t)d * a.view.si,
-          tile[(c - n0) * W + r]);
+    for (int in = threadIdx.x; in < kTile * D; in += 256) {
+      const int r = in / D, d = in - r * D;
+      const int64_t at = b * a.view.sb + (int64_t)(m0 + r) * a.view.sr + (int64_t)d * a.view.si;
+      for (int i = i0; i <= i1; i += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = (i + u) * D + d;
+          const bool here = i + u <= i1 && c >= n0 && c < n0 + kTile && c < p.n && m0 + r < p.m;
+          e[u] = here ? at + (int64_t)(i + u) * a.view.so : -1;
+          o[u] = here ? tile[(c - n0) * W + r] : 0.0f;
+        }
+        put<U>(a, e, o);
+      }
     }
     return;
   }
   const bool along_m = p.tall == (a.view.so == 1 || a.view.inner != 1);
-  for (int q = threadIdx.x; q < kTile * kTile; q += 256) {
-    const int mi = along_m ? q % kTile : q / kTile, ni = along_m ? q / kTile : q % kTile;
-    if (m0 + mi < p.m && n0 + ni < p.n)
-      put(a, p.tall ? view_at(a.view, b, n0 + ni, m0 + mi) : view_at(a.view, b, m0 + mi, n0 + ni), tile[ni * W + mi]);
+  for (int q = threadIdx.x; q < kTile * kTile; q += 256 * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int f = q + u * 256, mi = along_m ? f % kTile : f / kTile, ni = along_m ? f / kTile : f % kTile;
+      const bool here = m0 + mi < p.m && n0 + ni < p.n;
+      e[u] = !here ? -1 : p.tall ? view_at(a.view, b, n0 + ni, m0 + mi) : view_at(a.view, b, m0 + mi, n0 + ni);
+      o[u] = tile[ni * W + mi];
+    }
+    put<U>(a, e, o);
   }
 }
 constexpr int kPutLds = kTile * (kTile + 1) * 4;
@@ -419,11 +453,12 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   const int tm = id % TM;
   id /= TM;
   const int tn = id % TN, b = id / TN;
-  const int KB = p.m32 / 16;
+  const int KB = p.mk / 16;
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
   const char* x = xc + b * p.xc_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0, KB / 2, lds, acc);
+  Tile22::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0,
+              KB / Tile22::kStageBlocks, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   constexpr int kPitch = (kTile + 8) * 2;  // bytes of a row of the LDS tile
   char* plane1 = lds + kTile * kPitch;
@@ -438,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
         const int r = r0 + 8 * q + 4 * g, k = tm * kTile + r;
         float v[4] = {};
         const size_t at = quad_at<2>(col, k, KB);
-        if (k < p.m32) {
+        if (k < p.mk) {
           const f16x4_t h = *(const f16x4_t*)(x + at), l = *(const f16x4_t*)(x + at + kPlaneBytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -450,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
           continue;
         }
         const Planes4<2> f = to_planes4<2>(v);
-        if (k < p.m32) {
+        if (k < p.mk) {
           char* d = xc_new + b * p.xc_bytes + at;
           *(f16x4_t*)d = f.p[0];
           *(f16x4_t*)(d + kPlaneBytes) = f.p[1];
@@ -493,11 +528,11 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
   const int tm = id % TM;
   id /= TM;
   const int tn = id % TN, b = id / TN;
-  const int KB = p.m32 / 16;
+  const int KB = p.mk / 16;
   const size_t pq = (size_t)KB * 2 * kPlaneBytes, px = (size_t)KB * kPlaneBytes;
   f32x16_t acc[2][2] = {};
-  ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0, KB / 2,
-                 lds, acc);
+  ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0,
+                 KB / ApplyTile::kStageBlocks, lds, acc);
   const float f = (float)rest[b] * kInvS / p.qscale;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -520,7 +555,11 @@ __global__ __launch_bounds__(256) void k_ortho_scale(OrthoArgs a, const double* 
   const float f = (float)sqrt(norm_sum(part, b, red)) + a.eps;
   const int64_t total = (int64_t)a.rows * a.cols;
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256)
-    put(a, b * a.view.sb + e, entry(a, b * a.view.sb + e) / f);
+  {
+    const int64_t at[1] = {b * a.view.sb + e};
+    const float o[1] = {entry(a, at[0]) / f};
+    put<1>(a, at, o);
+  }
 }
 
 // The largest value of Q that singular values in [0, 1] give, by sampling.
@@ -559,15 +598,21 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   ensure_lds_limit((const void*)k_ortho_mm, MmTile::kLdsBytes, done[2]);
   ensure_lds_limit((const void*)k_ortho_update, kUpdateLds, done[3]);
   ensure_lds_limit((const void*)k_ortho_apply, kApplyLds, done[4]);
-  hipLaunchKernelGGL(k_ortho_norm, dim3(kNormBlocks, a.batch), dim3(256), 0, st, a, norm);
+  const dim3 norm_grid(kNormBlocks, a.batch);
+  if (!a.in)
+    hipLaunchKernelGGL(k_ortho_norm<kNormMuon>, norm_grid, dim3(256), 0, st, a, norm);
+  else if (a.bf16)
+    hipLaunchKernelGGL(k_ortho_norm<kNormBf16>, norm_grid, dim3(256), 0, st, a, norm);
+  else
+    hipLaunchKernelGGL(k_ortho_norm<kNormF32>, norm_grid, dim3(256), 0, st, a, norm);
   if (a.steps == 0) {
     hipLaunchKernelGGL(k_ortho_scale, dim3(kNormBlocks, a.batch), dim3(256), 0, st, a, norm);
     return;
   }
   const dim3 pack_grid(p.n128 / 64, p.m128 / 64, a.batch), block(256);
-  const int T = p.m128 / kTile, TN = p.n128 / kTile, T64 = (p.m32 + 63) / 64;
+  const int T = p.m128 / kTile, TN = p.n128 / kTile, T64 = p.mk / 64;
   const dim3 gram_grid(a.batch * (T * (T + 1) / 2) * p.splits);
-  const dim3 sum_grid((unsigned)ceil_div((int64_t)p.m128 * (p.m32 / 8), 256), a.batch);
+  const dim3 sum_grid((unsigned)ceil_div((int64_t)p.m128 * (p.mk / 8), 256), a.batch);
   auto products = [&](const MmJob& one, const MmJob* two) {
     MmJobs jobs{{one, two ? *two : one}};
     hipLaunchKernelGGL(k_ortho_mm, dim3(a.batch * T64 * T64, two ? 2 : 1), block, MmTile::kLdsBytes, st, p, jobs);

@@ -71,26 +71,28 @@ __device__ __forceinline__ f32x16_t mfma16(f16x8_t a, f16x8_t b, f32x16_t c) {
 }
 
 // acc[m][n] += a[m] b[n] for FM x FN fragments of one k-block; the small plane
-// products first.
-template <int NA, int NB, int FM, int FN>
+// products first.  With NC = 3 accumulators each of the three plane products has its
+// own: a wave of one fragment would otherwise wait for each instruction's result.
+template <int NA, int NB, int FM, int FN, int NC = 1>
 __device__ __forceinline__ void mfma_planes(const f16x8_t (&a)[FM][NA], const f16x8_t (&b)[FN][NB],
-                                            f32x16_t (&acc)[FM][FN]) {
+                                            f32x16_t (&acc)[NC * FM][FN]) {
   if constexpr (NA == 2) {
 #pragma unroll
     for (int m = 0; m < FM; ++m)
 #pragma unroll
       for (int n = 0; n < FN; ++n) acc[m][n] = mfma16(a[m][1], b[n][0], acc[m][n]);
   }
+  constexpr int k1 = NC == 3 ? FM : 0, k2 = NC == 3 ? 2 * FM : 0;
   if constexpr (NB == 2) {
 #pragma unroll
     for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int n = 0; n < FN; ++n) acc[m][n] = mfma16(a[m][0], b[n][1], acc[m][n]);
+      for (int n = 0; n < FN; ++n) acc[k1 + m][n] = mfma16(a[m][0], b[n][1], acc[k1 + m][n]);
   }
 #pragma unroll
   for (int m = 0; m < FM; ++m)
 #pragma unroll
-    for (int n = 0; n < FN; ++n) acc[m][n] = mfma16(a[m][0], b[n][0], acc[m][n]);
+    for (int n = 0; n < FN; ++n) acc[k2 + m][n] = mfma16(a[m][0], b[n][0], acc[k2 + m][n]);
 }
 
 __device__ __forceinline__ f16x8_t lds_frag(const char* base, int lane) {
@@ -125,7 +127,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // fragments of 32 x 32; A tile of WM FM row blocks, B tile of WN FN.  Stages of
 // KS k-blocks go through a ring of NBUF LDS buffers by direct copies, NBUF - 1
 // stages ahead, one barrier a stage.
-template <int NA, int NB, int WM, int WN, int FM, int FN, int KS, int NBUF>
+template <int NA, int NB, int WM, int WN, int FM, int FN, int KS, int NBUF, int NC = 1>
 struct NtTile {
   static constexpr int kWaves = WM * WN, kStageBlocks = KS;
   static constexpr int kRA = WM * FM, kRB = WN * FN;
@@ -154,7 +156,7 @@ struct NtTile {
     }
   }
 
-  __device__ static void compute(const char* buf, int wm, int wn, int lane, f32x16_t (&acc)[FM][FN]) {
+  __device__ static void compute(const char* buf, int wm, int wn, int lane, f32x16_t (&acc)[NC * FM][FN]) {
     const char* a = buf + wm * FM * KS * NA * kPlaneBytes;
     const char* b = buf + (kChunksA + wn * FN * KS * NB) * kPlaneBytes;
 #pragma unroll
@@ -168,7 +170,7 @@ struct NtTile {
       for (int n = 0; n < FN; ++n)
 #pragma unroll
         for (int p = 0; p < NB; ++p) fb[n][p] = lds_frag(b + ((n * KS + k) * NB + p) * kPlaneBytes, lane);
-      mfma_planes<NA, NB, FM, FN>(fa, fb, acc);
+      mfma_planes<NA, NB, FM, FN, NC>(fa, fb, acc);
     }
   }
 
@@ -177,7 +179,7 @@ struct NtTile {
   // read.
   template <typename SrcA, typename SrcB>
   __device__ static void run(const SrcA& A, const SrcB& B, int kb0, int nst, char* lds,
-                             f32x16_t (&acc)[FM][FN]) {
+                             f32x16_t (&acc)[NC * FM][FN]) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave / WN, wn = wave % WN;
     const uint32_t l0 = lds_address(lds);
