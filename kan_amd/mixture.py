@@ -6,9 +6,10 @@ Tensors on the CPU are rejected: there is no CPU path.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Any, Dict, Optional, Tuple
 
 import torch
+import torch.nn as nn
 
 from . import _lib
 
@@ -191,3 +192,82 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
     if torch.is_grad_enabled() and (x.requires_grad or coeffs.requires_grad or weights.requires_grad):
         return ExpertsFunction.apply(x, coeffs, weights, indices, desc)
     return _experts_forward(x, coeffs, indices, weights, desc, keep=False)[0]
+
+
+class MixtureKANLayer(nn.Module):
+    """A mixture of ChebyKAN layers: each row goes to ``top_k`` of ``experts`` layers of
+    ``ChebyKANLayer(input_dim, output_dim, degree)`` (kan/layers/chebykan.py:21-51), chosen
+    and weighted by a linear gate through ``route``, computed by ``kan_experts``.
+
+    Parameters: ``gate`` [experts, input_dim] and ``cheby_coeffs`` [experts, input_dim,
+    output_dim, degree+1], each expert initialised as the layer is.  ``compute``: 'fp32'
+    or 'bf16' (the experts' operands and outputs are bf16, the gate and the choice stay
+    fp32; the output is fp32, as a ChebyKANLayer's).
+
+    With ``balance``, a per-expert bias steers the choice, not the weights:
+    ``update_balance`` moves it towards experts that got fewer rows than the mean."""
+
+    def __init__(self, input_dim: int, output_dim: int, degree: int, experts: int, top_k: int = 2, *,
+                 score: str = "softmax", groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+                 scale: float = 1.0, balance: bool = False, init_scale: Optional[float] = None,
+                 compute: str = "fp32"):
+        super().__init__()
+        if score not in _SCORES:
+            raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+        if compute not in ("fp32", "bf16"):
+            raise ValueError(f"compute must be 'fp32' or 'bf16', got {compute!r}")
+        if not 1 <= degree <= 16:
+            raise ValueError(f"experts have degree 1 to 16, got {degree}")
+        if groups < 1 or experts % groups or not 1 <= top_groups <= groups:
+            raise ValueError(f"groups must divide experts and hold top_groups: got {experts} experts, {groups} "
+                             f"groups, {top_groups} kept")
+        if not 1 <= top_k <= experts // groups * top_groups:
+            raise ValueError(f"top_k must lie in [1, {experts // groups * top_groups}], got {top_k}")
+        self.input_dim, self.output_dim, self.degree = input_dim, output_dim, degree
+        self.experts, self.top_k, self.score = experts, top_k, score
+        self.groups, self.top_groups = groups, top_groups
+        self.renormalize, self.scale, self.compute = renormalize, scale, compute
+        self.gate = nn.Parameter(torch.empty(experts, input_dim))
+        self.cheby_coeffs = nn.Parameter(torch.empty(experts, input_dim, output_dim, degree + 1))
+        nn.init.normal_(self.gate, mean=0.0, std=input_dim ** -0.5)
+        nn.init.normal_(self.cheby_coeffs, mean=0.0, std=init_scale or 1.0 / (input_dim * (degree + 1)))
+        self.register_buffer("balance_bias", torch.zeros(experts) if balance else None)
+        self._last_indices: Optional[torch.Tensor] = None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        x = x.reshape(-1, self.input_dim).to(torch.float32)
+        weights, indices = route(x @ self.gate.t(), self.top_k, score=self.score, bias=self.balance_bias,
+                                 groups=self.groups, top_groups=self.top_groups, renormalize=self.renormalize,
+                                 scale=self.scale)
+        self._last_indices = indices if self.balance_bias is not None else None
+        if self.compute == "fp32":
+            return kan_experts(x, self.cheby_coeffs, indices, weights)
+        y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights.bfloat16())
+        return y.to(torch.float32)
+
+    @torch.no_grad()
+    def update_balance(self, speed: float = 1e-3) -> None:
+        """Moves the balance bias of each expert by ``speed``, up where the last forward
+        gave it fewer rows than the mean and down where more."""
+        if self.balance_bias is None:
+            raise RuntimeError("the layer was built without balance=True")
+        if self._last_indices is None:
+            raise RuntimeError("update_balance needs a forward first")
+        idx = self._last_indices.reshape(-1)
+        load = torch.zeros(self.experts + 1, device=idx.device)
+        load.scatter_add_(0, torch.where(idx >= 0, idx, self.experts), torch.ones_like(idx, dtype=load.dtype))
+        load = load[:-1]
+        self.balance_bias.add_(speed * torch.sign(load.mean() - load))
+
+    def get_coefficients(self) -> torch.Tensor:
+        return self.cheby_coeffs
+
+    def get_analytical_form(self) -> Dict[str, Any]:
+        return {"type": "MixtureKANLayer", "input_dim": self.input_dim, "output_dim": self.output_dim,
+                "degree": self.degree, "experts": self.experts, "top_k": self.top_k, "basis": "chebyshev",
+                "gate": self.gate.detach().cpu().numpy(),
+                "coefficients": self.cheby_coeffs.detach().cpu().numpy()}
+
+    def extra_repr(self) -> str:
+        return (f"input_dim={self.input_dim}, output_dim={self.output_dim}, degree={self.degree}, "
+                f"experts={self.experts}, top_k={self.top_k}, score={self.score}")
