@@ -334,32 +334,51 @@ struct MmJob {
 };
 struct MmJobs { MmJob j[2]; };
 
-// 64 x 64 tiles (128 x 128 ones leave most CUs without a block at these sizes), waves
-// of 32 x 32 with three accumulators.
-typedef NtTile<2, 2, 2, 2, 1, 1, 4, 2, 3> MmTile;  // 64 KiB of LDS
+// 64 x 64 tiles (128 x 128 ones leave most CUs without a block at these sizes): one
+// block a CU, so kMmGroups groups of four waves divide a stage's k-blocks to have
+// work while others wait.
+constexpr int kMmGroups = 2;
+typedef NtTile<2, 2, 2, 2, 1, 1, 4, 2, 3, kMmGroups> MmTile;  // 64 KiB of LDS
 
-__global__ __launch_bounds__(256, 2) void k_ortho_mm(OrthoPlan p, MmJobs jobs) {
+__global__ __launch_bounds__(256 * kMmGroups) void k_ortho_mm(OrthoPlan p, MmJobs jobs) {
   extern __shared__ char lds[];
   const MmJob& j = jobs.j[blockIdx.y];
-  const int T = p.mk / 64, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T), tm = t / T, tn = t % T;
+  const int T = p.mk / 64, b = blockIdx.x / (T * T), t = blockIdx.x % (T * T);
+  int tm = t / T, tn = t % T;
+  if (T % 4 == 0) {
+    // a patch of T/2 x T/4 tiles an XCD: 3/4 of the operands through its L2, where rows
+    // of tiles in turn take 9/8 and more
+    const int x = t & 7, u = t >> 3;
+    tm = (x >> 2) * (T / 2) + u / (T / 4);
+    tn = (x & 3) * (T / 4) + u % (T / 4);
+  }
   const int KB = p.mk / 16;
   const size_t pitch = (size_t)KB * 2 * kPlaneBytes, at0 = b * p.a_bytes;
   f32x16_t acc[3][1] = {};
   MmTile::run(RowBlocks{j.l + at0 + tm * 2 * pitch, pitch}, RowBlocks{j.r + at0 + tn * 2 * pitch, pitch}, 0,
               KB / MmTile::kStageBlocks, lds, acc);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
-  const int row0 = tm * 64 + (wave >> 1) * 32, col = tn * 64 + (wave & 1) * 32 + (lane & 31);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5, quad = wave & 3, group = wave >> 2;
+  f32x16_t sum;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) sum[q] = (acc[0][0][q] + acc[1][0][q]) + acc[2][0][q];
+  float* share = (float*)lds;  // the later groups' sums
+  if (group > 0)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) share[(((group - 1) * 4 + quad) * 16 + q) * 64 + lane] = sum[q];
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int s = 0; s < kMmGroups - 1; ++s)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) sum[q] += share[((s * 4 + quad) * 16 + q) * 64 + lane];
+  const int row0 = tm * 64 + (quad >> 1) * 32, col = tn * 64 + (quad & 1) * 32 + (lane & 31);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int k = row0 + 8 * q + 4 * g;
-    if (k >= p.mk) continue;
     const size_t at = at0 + quad_at<2>(col, k, KB);
     float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float s = (acc[0][0][q * 4 + i] + acc[1][0][q * 4 + i]) + acc[2][0][q * 4 + i];
-      v[i] = j.alpha * s + (k + i == col ? j.gamma : 0.0f);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = j.alpha * sum[q * 4 + i] + (k + i == col ? j.gamma : 0.0f);
     if (j.beta != 0.0f) {
       const f16x4_t h = *(const f16x4_t*)(j.r + at), l = *(const f16x4_t*)(j.r + at + kPlaneBytes);
 #pragma unroll
@@ -615,7 +634,8 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   const dim3 sum_grid((unsigned)ceil_div((int64_t)p.m128 * (p.mk / 8), 256), a.batch);
   auto products = [&](const MmJob& one, const MmJob* two) {
     MmJobs jobs{{one, two ? *two : one}};
-    hipLaunchKernelGGL(k_ortho_mm, dim3(a.batch * T64 * T64, two ? 2 : 1), block, MmTile::kLdsBytes, st, p, jobs);
+    hipLaunchKernelGGL(k_ortho_mm, dim3(a.batch * T64 * T64, two ? 2 : 1), dim3(256 * kMmGroups), MmTile::kLdsBytes, st, p,
+                       jobs);
   };
   if (!p.bf16) {
     hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);

@@ -123,13 +123,15 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// One block's tile of C = A B^T over stored operands: WM x WN waves (4), each FM x FN
+// One block's tile of C = A B^T over stored operands: WM x WN waves, each FM x FN
 // fragments of 32 x 32; A tile of WM FM row blocks, B tile of WN FN.  Stages of
 // KS k-blocks go through a ring of NBUF LDS buffers by direct copies, NBUF - 1
-// stages ahead, one barrier a stage.
-template <int NA, int NB, int WM, int WN, int FM, int FN, int KS, int NBUF, int NC = 1>
+// stages ahead, one barrier a stage.  WK > 1: that many groups of waves take a share
+// of each stage's k-blocks and leave their sums to the caller.
+template <int NA, int NB, int WM, int WN, int FM, int FN, int KS, int NBUF, int NC = 1, int WK = 1>
 struct NtTile {
-  static constexpr int kWaves = WM * WN, kStageBlocks = KS;
+  static constexpr int kWaves = WM * WN * WK, kStageBlocks = KS;
+  static_assert(KS % WK == 0, "k-blocks divide among the groups");
   static constexpr int kRA = WM * FM, kRB = WN * FN;
   static constexpr int kChunksA = kRA * KS * NA, kChunks = kChunksA + kRB * KS * NB;
   static constexpr int kStageBytes = kChunks * kPlaneBytes;
@@ -156,11 +158,12 @@ struct NtTile {
     }
   }
 
-  __device__ static void compute(const char* buf, int wm, int wn, int lane, f32x16_t (&acc)[NC * FM][FN]) {
+  __device__ static void compute(const char* buf, int wm, int wn, int wk, int lane, f32x16_t (&acc)[NC * FM][FN]) {
     const char* a = buf + wm * FM * KS * NA * kPlaneBytes;
     const char* b = buf + (kChunksA + wn * FN * KS * NB) * kPlaneBytes;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
+    for (int u = 0; u < KS / WK; ++u) {
+      const int k = wk * (KS / WK) + u;
       f16x8_t fa[FM][NA], fb[FN][NB];
 #pragma unroll
       for (int m = 0; m < FM; ++m)
@@ -181,7 +184,7 @@ struct NtTile {
   __device__ static void run(const SrcA& A, const SrcB& B, int kb0, int nst, char* lds,
                              f32x16_t (&acc)[NC * FM][FN]) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int wm = wave / WN, wn = wave % WN;
+    const int wk = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
     const uint32_t l0 = lds_address(lds);
 #pragma unroll
     for (int s = 0; s < NBUF - 1; ++s)
@@ -202,7 +205,7 @@ struct NtTile {
         if (at >= NBUF) at -= NBUF;
         copy(A, B, kb0 + nxt * KS, l0 + at * kStageBytes, wave, lane);
       }
-      compute(lds + cur * kStageBytes, wm, wn, lane, acc);
+      compute(lds + cur * kStageBytes, wm, wn, wk, lane, acc);
       if (++cur == NBUF) cur = 0;
     }
     wait_lds();

@@ -6,6 +6,7 @@ Tensors on the CPU are rejected: there is no CPU path.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Any, Dict, Optional, Tuple
 
 import torch
@@ -36,40 +37,57 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
         raise RuntimeError(f"{name} must be float32 or bfloat16, got {t.dtype}") from None
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _stream(device: torch.device) -> int:
+    """hipStream_t of torch's current stream, without building a Stream object (2 us)."""
+    return _raw_stream(device.index) if _raw_stream is not None else _lib.stream_ptr(device)
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for the library's launches; nothing to do when it is."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t contiguous at a 16-byte aligned address, as the library's vector loads need it."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _route_forward(logits, bias, desc):
+    dev = logits.device
+    w = torch.empty(desc.rows, desc.top_k, dtype=torch.float32, device=dev)
+    idx = torch.empty(desc.rows, desc.top_k, dtype=torch.int64, device=dev)
+    with _on(dev):
+        _lib.check(_lib.load().ckan_route(desc, logits.data_ptr(), _lib.ptr(bias), w.data_ptr(), idx.data_ptr(),
+                                          _stream(dev)))
+    return w, idx
+
+
 class RouteFunction(torch.autograd.Function):
-    """(weights, indices) of ``route``; differentiable in the logits."""
+    """The weights of ``route``, differentiable in the logits; the indices go by the
+    side (``out``): an output more costs the autograd engine 4 us a step."""
 
     @staticmethod
-    def forward(ctx, logits: torch.Tensor, bias: Optional[torch.Tensor], desc):
-        rows = logits.shape[0]
-        w = torch.empty(rows, desc.top_k, dtype=torch.float32, device=logits.device)
-        idx = torch.empty(rows, desc.top_k, dtype=torch.int64, device=logits.device)
-        with torch.cuda.device(logits.device):
-            _lib.check(_lib.load().ckan_route(desc, logits.data_ptr(), _lib.ptr(bias), w.data_ptr(),
-                                              idx.data_ptr(), _lib.stream_ptr(logits.device)))
-        ctx.save_for_backward(logits, idx)
-        ctx.mark_non_differentiable(idx)
-        ctx.desc = desc
-        return w, idx
+    def forward(ctx, logits: torch.Tensor, bias: Optional[torch.Tensor], desc, out: list):
+        w, idx = _route_forward(logits, bias, desc)
+        ctx.save_for_backward(logits)
+        ctx.desc, ctx.idx = desc, idx
+        out.append(idx)
+        return w
 
     @staticmethod
-    def backward(ctx, dw: torch.Tensor, _didx):
-        logits, idx = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            return None, None, None
-        dw = dw.to(torch.float32).contiguous()
-        dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        with torch.cuda.device(logits.device):
-            _lib.check(_lib.load().ckan_route_backward(
-                ctx.desc, logits.data_ptr(), idx.data_ptr(), dw.data_ptr(), dl.data_ptr(),
-                _lib.stream_ptr(logits.device)))
-        return dl, None, None
+    def backward(ctx, dw: torch.Tensor):
+        logits, = ctx.saved_tensors
+        if dw.dtype != torch.float32 or not dw.is_contiguous():
+            dw = dw.to(torch.float32).contiguous()
+        dl = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        # the engine runs a node on its device and stream
+        _lib.check(_lib.load().ckan_route_backward(ctx.desc, logits.data_ptr(), ctx.idx.data_ptr(), dw.data_ptr(),
+                                                   dl.data_ptr(), _stream(dl.device)))
+        return dl, None, None, None
 
 
 def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
@@ -103,7 +121,10 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     desc = _lib.CkanRouteDesc(logits.shape[0], max(logits.stride(0), experts), experts, int(top_k),
                               _SCORES[score], int(groups), int(top_groups), int(bool(renormalize)),
                               code, float(scale))
-    return RouteFunction.apply(logits, bias, desc)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out: list = []
+        return RouteFunction.apply(logits, bias, desc, out), out[0]
+    return _route_forward(logits, bias, desc)
 
 
 def _experts_forward(x, coeffs, indices, weights, desc, keep):
@@ -111,14 +132,14 @@ def _experts_forward(x, coeffs, indices, weights, desc, keep):
     lib, dev = _lib.load(), x.device
     y = torch.empty(desc.rows, desc.out_dim, dtype=x.dtype, device=dev)
     nbytes = lib.ckan_experts_workspace_bytes(desc, 0, int(not keep))
-    with torch.cuda.device(dev):
+    with _on(dev):
         # both from torch's allocator on the current stream: reused by it in stream order
         saved = (torch.empty(max(lib.ckan_experts_saved_bytes(desc), 256), dtype=torch.uint8, device=dev)
                  if keep else None)
         ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
         _lib.check(lib.ckan_experts_forward(desc, x.data_ptr(), coeffs.data_ptr(), indices.data_ptr(),
                                             weights.data_ptr(), y.data_ptr(), _lib.ptr(saved), ws.data_ptr(), nbytes,
-                                            _lib.stream_ptr(dev)))
+                                            _stream(dev)))
     return y, saved
 
 
@@ -150,11 +171,11 @@ class ExpertsFunction(torch.autograd.Function):
         dc = torch.empty(cs, dtype=dtype, device=dev) if need_c else None
         lib = _lib.load()
         nbytes = lib.ckan_experts_workspace_bytes(desc, 1, 0)
-        with torch.cuda.device(dev):
-            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-            _lib.check(lib.ckan_experts_backward(desc, indices.data_ptr(), weights.data_ptr(), saved.data_ptr(),
-                                                 dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dc), _lib.ptr(dw), ws.data_ptr(),
-                                                 nbytes, _lib.stream_ptr(dev)))
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+        # the engine runs a node on its device and stream
+        _lib.check(lib.ckan_experts_backward(desc, indices.data_ptr(), weights.data_ptr(), saved.data_ptr(),
+                                             dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dc), _lib.ptr(dw), ws.data_ptr(),
+                                             nbytes, _stream(dev)))
         return dx, dc, dw, None, None
 
 
