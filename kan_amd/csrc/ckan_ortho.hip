@@ -180,6 +180,11 @@ __device__ __forceinline__ double norm_sum(const double* part, int b, double* re
   return red[0];
 }
 
+// Whether memory runs along m: the columns of a tall matrix in row-major order, the
+// rows of a wide one in column-major order.
+__device__ __forceinline__ bool runs_along_m(const OrthoArgs& a, const OrthoPlan& p) {
+  return p.tall == (a.view.so == 1 || a.view.inner != 1);
+}
 // X0 in both operand forms: one block a 64 x 64 tile (m x n), through LDS.  In one
 // plane the scale is a power of two and what it leaves, a factor in [1, 2), goes to
 // rest[b]: the matrix is then X0 / rest exactly.
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, co
     }
   } else {
     // memory runs along n for an ordinary matrix with rows m, along m for a transposed one
-    const bool along_m = p.tall == (a.view.so == 1 || a.view.inner != 1);
+    const bool along_m = runs_along_m(a, p);
     for (int e = tid; e < 64 * 64; e += 256) {
       const int mi = along_m ? e & 63 : e >> 6, ni = along_m ? e >> 6 : e & 63;
       const int m = m0 + mi, n = n0 + ni;
@@ -400,66 +405,98 @@ __global__ __launch_bounds__(256 * kMmGroups) void k_ortho_mm(OrthoPlan p, MmJob
   }
 }
 
-// N results o[] to elements e[] (negative: none); Muon's N parameters are asked for
-// before any of them is needed.
-template <int N>
-__device__ __forceinline__ void put(const OrthoArgs& a, const int64_t (&e)[N], const float (&o)[N]) {
-  if (!a.in) {
-    float old[N];
-#pragma unroll
-    for (int u = 0; u < N; ++u) old[u] = e[u] >= 0 ? a.p[e[u]] : 0.0f;
-#pragma unroll
-    for (int u = 0; u < N; ++u)
-      if (e[u] >= 0) a.p[e[u]] = fmaf(-a.lr * a.scale, o[u], old[u] * (1.0f - a.lr * a.decay));
-  } else if (a.bf16) {
-#pragma unroll
-    for (int u = 0; u < N; ++u)
-      if (e[u] >= 0) ((__bf16*)a.out)[e[u]] = (__bf16)o[u];
-  } else {
-#pragma unroll
-    for (int u = 0; u < N; ++u)
-      if (e[u] >= 0) ((float*)a.out)[e[u]] = o[u];
-  }
+// Muon's parameter from its old value and the update.
+__device__ __forceinline__ float muon_param(const OrthoArgs& a, float old, float o) {
+  return fmaf(-a.lr * a.scale, o, old * (1.0f - a.lr * a.decay));
+}
+__device__ __forceinline__ void put(const OrthoArgs& a, int64_t e, float o) {
+  if (!a.in)
+    a.p[e] = muon_param(a, a.p[e], o);
+  else if (a.bf16)
+    ((__bf16*)a.out)[e] = (__bf16)o;
+  else
+    ((float*)a.out)[e] = o;
 }
 
-// A 128 x 128 tile of the result, staged in LDS as [n][m] (pitch 129), to where it
-// belongs: along (row, inner) for a view with an inner dimension and rows m, else
-// along whichever of m and n lies contiguous.
+// Where entry (m, n) of a 128 x 128 result tile is staged in LDS: the direction in
+// which it is stored is the contiguous one, except for a view with an inner
+// dimension, whose outer columns are gathered at an odd pitch.
+constexpr int kPutPitch = kTile + 4;
+__device__ __forceinline__ int tile_at(bool along_m, bool gathered, int m, int n) {
+  return gathered ? n * (kTile + 1) + m : along_m ? n * kPutPitch + m : m * kPutPitch + n;
+}
+
+// The staged tile to where it belongs.  Four elements a thread and step along the
+// contiguous direction, in one access where the addresses allow; one element at a
+// time cost the apply launch 40 of its 77 us.
 __device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p, const float* tile, int b, int m0, int n0) {
-  constexpr int W = kTile + 1, U = 8;
-  int64_t e[U];
-  float o[U];
   if (a.view.inner != 1 && !p.tall) {
+    constexpr int U = 8;
     const int D = a.view.inner, i0 = n0 / D, i1 = (n0 + kTile - 1) / D;
     for (int in = threadIdx.x; in < kTile * D; in += 256) {
       const int r = in / D, d = in - r * D;
+      if (m0 + r >= p.m) continue;
       const int64_t at = b * a.view.sb + (int64_t)(m0 + r) * a.view.sr + (int64_t)d * a.view.si;
       for (int i = i0; i <= i1; i += U) {
+        float old[U];  // Muon's parameters, asked for before any of them is needed
+        if (!a.in)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = (i + u) * D + d;
+            if (i + u <= i1 && c >= n0 && c < n0 + kTile && c < p.n) old[u] = a.p[at + (int64_t)(i + u) * a.view.so];
+          }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int c = (i + u) * D + d;
-          const bool here = i + u <= i1 && c >= n0 && c < n0 + kTile && c < p.n && m0 + r < p.m;
-          e[u] = here ? at + (int64_t)(i + u) * a.view.so : -1;
-          o[u] = here ? tile[(c - n0) * W + r] : 0.0f;
+          if (i + u > i1 || c < n0 || c >= n0 + kTile || c >= p.n) continue;
+          const float o = tile[tile_at(false, true, r, c - n0)];
+          const int64_t e = at + (int64_t)(i + u) * a.view.so;
+          if (!a.in)
+            a.p[e] = muon_param(a, old[u], o);
+          else
+            put(a, e, o);
         }
-        put<U>(a, e, o);
       }
     }
     return;
   }
-  const bool along_m = p.tall == (a.view.so == 1 || a.view.inner != 1);
-  for (int q = threadIdx.x; q < kTile * kTile; q += 256 * U) {
+  const bool along_m = runs_along_m(a, p);
+  const int c0 = along_m ? m0 : n0, r0 = along_m ? n0 : m0, cn = along_m ? p.m : p.n, rn = along_m ? p.n : p.m;
+  // stride of the slow direction; the fast one is 1 (or `inner` runs of a tall view)
+  const int64_t slow = p.tall == along_m ? a.view.sr : a.view.so;
+  const int64_t base = b * a.view.sb + r0 * slow;
+  const bool vec = a.view.inner == 1 && slow % 4 == 0 && (a.view.sb % 4 == 0 || p.batch == 1) &&
+                   (((uintptr_t)(a.in ? a.out : (void*)a.p)) & 15) == 0;
+#pragma unroll 4
+  for (int q = threadIdx.x; q < kTile * kTile / 4; q += 256) {
+    const int r = q / (kTile / 4), c = q % (kTile / 4) * 4;
+    if (r0 + r >= rn || c0 + c >= cn) continue;
+    const f32x4_t v = *(const f32x4_t*)(tile + r * kPutPitch + c);
+    if (vec && c0 + c + 4 <= cn) {
+      const int64_t e = base + r * slow + c0 + c;
+      if (!a.in) {
+        f32x4_t w = *(const f32x4_t*)(a.p + e);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int f = q + u * 256, mi = along_m ? f % kTile : f / kTile, ni = along_m ? f / kTile : f % kTile;
-      const bool here = m0 + mi < p.m && n0 + ni < p.n;
-      e[u] = !here ? -1 : p.tall ? view_at(a.view, b, n0 + ni, m0 + mi) : view_at(a.view, b, m0 + mi, n0 + ni);
-      o[u] = tile[ni * W + mi];
+        for (int j = 0; j < 4; ++j) w[j] = muon_param(a, w[j], v[j]);
+        *(f32x4_t*)(a.p + e) = w;
+      } else if (a.bf16) {
+        bf16x4_t w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (__bf16)v[j];
+        *(bf16x4_t*)((__bf16*)a.out + e) = w;
+      } else {
+        *(f32x4_t*)((float*)a.out + e) = v;
+      }
+      continue;
     }
-    put<U>(a, e, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = along_m ? c0 + c + j : r0 + r, n = along_m ? r0 + r : c0 + c + j;
+      if (c0 + c + j < cn) put(a, p.tall ? view_at(a.view, b, n, m) : view_at(a.view, b, m, n), v[j]);
+    }
   }
 }
-constexpr int kPutLds = kTile * (kTile + 1) * 4;
+constexpr int kPutLds = kTile * kPutPitch * 4;
 
 // X' = a X + B X.  The product's rows are m, its columns n: an accumulator quad is 4
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
@@ -480,6 +517,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
               KB / Tile22::kStageBlocks, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   constexpr int kPitch = (kTile + 8) * 2;  // bytes of a row of the LDS tile
+  const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a, p);
   char* plane1 = lds + kTile * kPitch;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -500,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
         }
         if (last) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ((float*)lds)[c * (kTile + 1) + r + j] = v[j] * kInvS;
+          for (int j = 0; j < 4; ++j) ((float*)lds)[tile_at(along_m, gathered, r + j, c)] = v[j] * kInvS;
           continue;
         }
         const Planes4<2> f = to_planes4<2>(v);
@@ -553,6 +591,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
   ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0,
                  KB / ApplyTile::kStageBlocks, lds, acc);
   const float f = (float)rest[b] * kInvS / p.qscale;
+  const bool along_m = runs_along_m(a, p);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -560,8 +599,8 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int q = 0; q < 16; ++q)
-        ((float*)lds)[((wave & 1) * 64 + n * 32 + (lane & 31)) * (kTile + 1) + (wave >> 1) * 64 + m * 32 + acc_row(q, g)] =
-            acc[m][n][q] * f;
+        ((float*)lds)[tile_at(along_m, false, (wave >> 1) * 64 + m * 32 + acc_row(q, g),
+                              (wave & 1) * 64 + n * 32 + (lane & 31))] = acc[m][n][q] * f;
   __syncthreads();
   put_tile(a, p, (const float*)lds, b, tm * kTile, tn * kTile);
 }
@@ -574,11 +613,7 @@ __global__ __launch_bounds__(256) void k_ortho_scale(OrthoArgs a, const double* 
   const float f = (float)sqrt(norm_sum(part, b, red)) + a.eps;
   const int64_t total = (int64_t)a.rows * a.cols;
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256)
-  {
-    const int64_t at[1] = {b * a.view.sb + e};
-    const float o[1] = {entry(a, at[0]) / f};
-    put<1>(a, at, o);
-  }
+    put(a, b * a.view.sb + e, entry(a, b * a.view.sb + e) / f);
 }
 
 // The largest value of Q that singular values in [0, 1] give, by sampling.
