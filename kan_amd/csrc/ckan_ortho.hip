@@ -8,6 +8,7 @@
 // |A| stay below 1.5 and |b A + c A^2| below 7, far inside fp16's range, and two
 // planes keep 22 bits of entries down to 2^-15 of the largest.
 //
+// Matrices with a side of at most 64 are ckan_ortho_small.hip's.  Of the others,
 // fp32 matrices take the iteration as it is written, on two planes.  X is held
 // twice, as the operand with rows m and k = n (Xr, for A = X X^T) and as the one
 // with rows n and k = m (Xc, for the product with X).
@@ -19,7 +20,7 @@
 // those of small singular values by 3.4^2 a step (up to 1.5e-4 of the result for a
 // spectrum over four decades, 1e-5 for a gradient's), which bf16's 2e-3 hides and
 // fp32's 1e-6 would not.
-#include "ckan_mix.hpp"
+#include "ckan_ortho.hpp"
 #include "ckan_planes.hpp"
 
 namespace ckan {
@@ -55,11 +56,12 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   p.n32 = (int)round_up(p.n, 32);
   p.m128 = (int)round_up(p.m, kTile);
   p.n128 = (int)round_up(p.n, kTile);
-  // A = X X^T has few tiles and a long k: splits of k up to two blocks a CU (320 blocks
-  // of 8 x [512, 4608] took 54 us, 480 take 37), none shorter than 256 (16 k-blocks)
+  // A = X X^T has few tiles and a long k: enough splits of k to give every CU a block,
+  // none shorter than 256 (16 k-blocks).  Two blocks a CU (8 x [512, 4608]): the products
+  // 50 us instead of 54, the sum of the splits 12 instead of 9.
   const int T = p.m128 / kTile;
   const int64_t tiles = (int64_t)batch * T * (T + 1) / 2;
-  int64_t splits = 2 * kNumCUs / tiles;
+  int64_t splits = ceil_div(kNumCUs, tiles);
   const int kb = p.n32 / 16;
   if (splits > kb / 16) splits = kb / 16;
   if (splits < 1) splits = 1;
@@ -83,21 +85,6 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   for (int i = 0; i < (bf16 ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
   p.bytes = off;
   return p;
-}
-
-__device__ __forceinline__ int64_t view_at(const MatView& v, int b, int r, int c) {
-  const int q = v.inner == 1 ? c : c / v.inner;
-  return b * v.sb + r * v.sr + q * v.so + (v.inner == 1 ? 0 : (c - q * v.inner) * v.si);
-}
-
-// The matrix entry that enters the iteration: the input, or Muon's update
-// direction from the gradient and the (already updated) momentum.
-__device__ __forceinline__ float muon_dir(float g, float buf, const OrthoArgs& a) {
-  return a.nesterov ? fmaf(a.momentum, buf, (1.0f - a.momentum) * g) : buf;
-}
-__device__ __forceinline__ float entry(const OrthoArgs& a, int64_t at) {
-  if (!a.in) return muon_dir(a.g[at], a.buf[at], a);
-  return a.bf16 ? (float)((const __bf16*)a.in)[at] : ((const float*)a.in)[at];
 }
 
 // Sums of squares in 64 bits, kNormBlocks partials a matrix; Muon's momentum is
@@ -180,11 +167,6 @@ __device__ __forceinline__ double norm_sum(const double* part, int b, double* re
   return red[0];
 }
 
-// Whether memory runs along m: the columns of a tall matrix in row-major order, the
-// rows of a wide one in column-major order.
-__device__ __forceinline__ bool runs_along_m(const OrthoArgs& a, const OrthoPlan& p) {
-  return p.tall == (a.view.so == 1 || a.view.inner != 1);
-}
 // X0 in both operand forms: one block a 64 x 64 tile (m x n), through LDS.  In one
 // plane the scale is a power of two and what it leaves, a factor in [1, 2), goes to
 // rest[b]: the matrix is then X0 / rest exactly.
@@ -215,7 +197,7 @@ __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, co
     }
   } else {
     // memory runs along n for an ordinary matrix with rows m, along m for a transposed one
-    const bool along_m = runs_along_m(a, p);
+    const bool along_m = runs_along_m(a);
     for (int e = tid; e < 64 * 64; e += 256) {
       const int mi = along_m ? e & 63 : e >> 6, ni = along_m ? e >> 6 : e & 63;
       const int m = m0 + mi, n = n0 + ni;
@@ -405,19 +387,6 @@ __global__ __launch_bounds__(256 * kMmGroups) void k_ortho_mm(OrthoPlan p, MmJob
   }
 }
 
-// Muon's parameter from its old value and the update.
-__device__ __forceinline__ float muon_param(const OrthoArgs& a, float old, float o) {
-  return fmaf(-a.lr * a.scale, o, old * (1.0f - a.lr * a.decay));
-}
-__device__ __forceinline__ void put(const OrthoArgs& a, int64_t e, float o) {
-  if (!a.in)
-    a.p[e] = muon_param(a, a.p[e], o);
-  else if (a.bf16)
-    ((__bf16*)a.out)[e] = (__bf16)o;
-  else
-    ((float*)a.out)[e] = o;
-}
-
 // Where entry (m, n) of a 128 x 128 result tile is staged in LDS: the direction in
 // which it is stored is the contiguous one, except for a view with an inner
 // dimension, whose outer columns are gathered at an odd pitch.
@@ -460,7 +429,7 @@ __device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p,
     }
     return;
   }
-  const bool along_m = runs_along_m(a, p);
+  const bool along_m = runs_along_m(a);
   const int c0 = along_m ? m0 : n0, r0 = along_m ? n0 : m0, cn = along_m ? p.m : p.n, rn = along_m ? p.n : p.m;
   // stride of the slow direction; the fast one is 1 (or `inner` runs of a tall view)
   const int64_t slow = p.tall == along_m ? a.view.sr : a.view.so;
@@ -517,7 +486,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
               KB / Tile22::kStageBlocks, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   constexpr int kPitch = (kTile + 8) * 2;  // bytes of a row of the LDS tile
-  const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a, p);
+  const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
   char* plane1 = lds + kTile * kPitch;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -591,7 +560,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
   ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0,
                  KB / ApplyTile::kStageBlocks, lds, acc);
   const float f = (float)rest[b] * kInvS / p.qscale;
-  const bool along_m = runs_along_m(a, p);
+  const bool along_m = runs_along_m(a);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -634,10 +603,15 @@ float largest_q(const OrthoArgs& a) {
 }  // namespace
 
 size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16) {
+  if (ortho_small(rows, cols)) return ortho_small_workspace_bytes(batch, rows, cols);
   return make_ortho_plan(batch, rows, cols, bf16).bytes;
 }
 
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
+  if (ortho_small(a.rows, a.cols)) {
+    launch_ortho_small(a, ws, st);
+    return;
+  }
   OrthoPlan p = make_ortho_plan(a.batch, a.rows, a.cols, a.bf16 != 0);
   char* w = (char*)ws;
   double *norm = (double*)(w + p.norm_off), *rest = norm + (size_t)a.batch * kNormBlocks;
