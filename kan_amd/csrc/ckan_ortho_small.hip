@@ -75,7 +75,17 @@ __device__ __forceinline__ void each_entry(const OrthoArgs& a, int m, int n, int
   }
 }
 
-template <bool MUON>
+// What a kernel reads: the compiler batches a tile's loads only where their type is
+// no question at run time.
+enum SmallKind { kSmallF32, kSmallBf16, kSmallMuon };
+template <int KIND>
+__device__ __forceinline__ float small_entry(const OrthoArgs& a, int64_t e) {
+  if constexpr (KIND == kSmallMuon) return muon_dir(a.g[e], a.buf[e], a);
+  if constexpr (KIND == kSmallBf16) return (float)((const __bf16*)a.in)[e];
+  return ((const float*)a.in)[e];
+}
+
+template <int KIND>
 __global__ __launch_bounds__(256) void k_small_gram(OrthoArgs a, SmallPlan p, double* part) {
   __shared__ float tile[kM * kPitch];
   const int b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -85,25 +95,29 @@ __global__ __launch_bounds__(256) void k_small_gram(OrthoArgs a, SmallPlan p, do
     __syncthreads();
     each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) {
       float v;
-      if constexpr (MUON) {
+      if constexpr (KIND == kSmallMuon) {
         const float g = a.g[e], nb = fmaf(a.momentum, a.buf[e], (1.0f - a.momentum) * g);
         if (ok) a.buf[e] = nb;
         v = muon_dir(g, nb, a);
       } else {
-        v = entry(a, e);
+        v = small_entry<KIND>(a, e);
       }
       tile[mi * kPitch + ni] = ok ? v : 0.0f;
     });
     __syncthreads();
+    // the wave's tiles take turns, so that no instruction waits for the last one's sum
+    const float *x[3], *y[3];
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
-      if (wave + 4 * s >= kTiles) break;
       int tm, tn;
-      tile_of(wave + 4 * s, tm, tn);
-      const float *x = tile + (tm * 16 + (lane & 15)) * kPitch + (lane >> 4), *y = tile + (tn * 16 + (lane & 15)) * kPitch + (lane >> 4);
-#pragma unroll
-      for (int k = 0; k < 64; k += 4) acc[s] = mma((double)x[k], (double)y[k], acc[s]);
+      tile_of(wave + 4 * s < kTiles ? wave + 4 * s : wave, tm, tn);
+      x[s] = tile + (tm * 16 + (lane & 15)) * kPitch + (lane >> 4);
+      y[s] = tile + (tn * 16 + (lane & 15)) * kPitch + (lane >> 4);
     }
+#pragma unroll
+    for (int k = 0; k < 64; k += 4)
+#pragma unroll
+      for (int s = 0; s < 3; ++s) acc[s] = mma((double)x[s][k], (double)y[s][k], acc[s]);
   }
 #pragma unroll
   for (int s = 0; s < 3; ++s)
@@ -143,7 +157,7 @@ __global__ __launch_bounds__(64 * kTiles) void k_small_chain(OrthoArgs a, SmallP
   };
   f64x4_t v = {};
   const double* src = part + ((size_t)b * p.chunks * kTiles + t) * 256 + lane;
-#pragma unroll 4
+#pragma unroll 8
   for (int c = 0; c < p.chunks; ++c)
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += src[(size_t)c * kTiles * 256 + i * 64];
@@ -196,6 +210,7 @@ __global__ __launch_bounds__(64 * kTiles) void k_small_chain(OrthoArgs a, SmallP
 }
 
 // 64 columns of Q G a block, a wave 16 rows.
+template <int KIND>
 __global__ __launch_bounds__(256) void k_small_apply(OrthoArgs a, SmallPlan p, const double* q) {
   __shared__ float tile[kM * kPitch];
   __shared__ double Q[kM * kPitch];
@@ -205,7 +220,10 @@ __global__ __launch_bounds__(256) void k_small_apply(OrthoArgs a, SmallPlan p, c
     const int e = threadIdx.x + u * 256;
     Q[(e >> 6) * kPitch + (e & 63)] = q[(size_t)b * kM * kM + e];
   }
-  each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) { tile[mi * kPitch + ni] = ok ? entry(a, e) : 0.0f; });
+  each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) { 
+    const float v = small_entry<KIND>(a, e);
+    tile[mi * kPitch + ni] = ok ? v : 0.0f;
+  });
   __syncthreads();
   f64x4_t acc[4] = {};
   const int ks = (p.m + 3) / 4 * 4;
@@ -220,35 +238,44 @@ __global__ __launch_bounds__(256) void k_small_apply(OrthoArgs a, SmallPlan p, c
 #pragma unroll
     for (int v = 0; v < 4; ++v) tile[(wave * 16 + 4 * v + (lane >> 4)) * kPitch + j * 16 + (lane & 15)] = (float)acc[j][v];
   __syncthreads();
-  if (!a.in) {
-    each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) {
+  each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) {
+    const float o = tile[mi * kPitch + ni];
+    if constexpr (KIND == kSmallMuon) {
       const float old = a.p[e];
-      if (ok) a.p[e] = muon_param(a, old, tile[mi * kPitch + ni]);
-    });
-  } else {
-    each_entry(a, p.m, p.n, b, n0, [&](int mi, int ni, bool ok, int64_t e) {
-      if (ok) put(a, e, tile[mi * kPitch + ni]);
-    });
-  }
+      if (ok) a.p[e] = muon_param(a, old, o);
+    } else if constexpr (KIND == kSmallBf16) {
+      if (ok) ((__bf16*)a.out)[e] = (__bf16)o;
+    } else {
+      if (ok) ((float*)a.out)[e] = o;
+    }
+  });
 }
 
 }  // namespace
 
 size_t ortho_small_workspace_bytes(int batch, int rows, int cols) { return make_small_plan(batch, rows, cols).bytes; }
 
-void launch_ortho_small(const OrthoArgs& a, void* ws, hipStream_t st) {
-  const SmallPlan p = make_small_plan(a.batch, a.rows, a.cols);
-  double *part = (double*)((char*)ws + p.part_off), *q = (double*)((char*)ws + p.q_off);
-  const dim3 gram(p.chunks, a.batch), block(256);
-  if (a.in)
-    hipLaunchKernelGGL(k_small_gram<false>, gram, block, 0, st, a, p, part);
-  else
-    hipLaunchKernelGGL(k_small_gram<true>, gram, block, 0, st, a, p, part);
+namespace {
+template <int KIND>
+void launch_kind(const OrthoArgs& a, const SmallPlan& p, double* part, double* q, hipStream_t st) {
+  hipLaunchKernelGGL(k_small_gram<KIND>, dim3(p.chunks, a.batch), dim3(256), 0, st, a, p, part);
   constexpr int lds = 4 * kM * kPitch * (int)sizeof(double);
   static std::atomic<uint32_t> done;
   ensure_lds_limit((const void*)k_small_chain, lds, done);
   hipLaunchKernelGGL(k_small_chain, dim3(a.batch), dim3(64 * kTiles), lds, st, a, p, part, q);
-  hipLaunchKernelGGL(k_small_apply, dim3((unsigned)ceil_div(p.n, 64), a.batch), block, 0, st, a, p, q);
+  hipLaunchKernelGGL(k_small_apply<KIND>, dim3((unsigned)ceil_div(p.n, 64), a.batch), dim3(256), 0, st, a, p, q);
+}
+}  // namespace
+
+void launch_ortho_small(const OrthoArgs& a, void* ws, hipStream_t st) {
+  const SmallPlan p = make_small_plan(a.batch, a.rows, a.cols);
+  double *part = (double*)((char*)ws + p.part_off), *q = (double*)((char*)ws + p.q_off);
+  if (!a.in)
+    launch_kind<kSmallMuon>(a, p, part, q, st);
+  else if (a.bf16)
+    launch_kind<kSmallBf16>(a, p, part, q, st);
+  else
+    launch_kind<kSmallF32>(a, p, part, q, st);
 }
 
 }  // namespace ckan
