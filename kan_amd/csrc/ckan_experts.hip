@@ -850,6 +850,43 @@ __global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
   }
 }
 
+// dx += sum over j < nd of acc[.][j] U_{N+j}(x), the degrees N + 1 .. N + 4.  By Clenshaw's
+// recurrence in the run of four,
+//   sum_j g_j U_{N+j} = U_N B_0 - U_{N-1} B_1,   B_j = g_j + 2 x B_{j+1} - B_{j+2},
+// with U_N and U_{N-1} from products (U_{2n} = U_n^2 - U_{n-1}^2, U_{2n+1} = U_n (U_{n+1} -
+// U_{n-1})): straight code, so that the 32 elements of a lane hide one another's
+// latency; a loop over the degrees an element took 112 us of 398.
+template <int N>
+__device__ __forceinline__ void weigh_by_u(const f32x16_t (&acc)[2][4], int nd, const float (&x)[2][16], float (&dx)[2][16]) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      // volatile: what depends on x alone is made here, not kept in registers through
+      // the products of every run (240 of them, spilled)
+      float xv = x[m][q];
+      asm volatile("" : "+v"(xv));
+      const float y = xv + xv;
+      const float g1 = nd > 1 ? acc[m][1][q] : 0.0f, g2 = nd > 2 ? acc[m][2][q] : 0.0f, b3 = nd > 3 ? acc[m][3][q] : 0.0f;
+      const float b2 = fmaf(y, b3, g2), b1 = fmaf(y, b2, g1 - b3), b0 = fmaf(y, b1, acc[m][0][q] - b2);
+      if constexpr (N == 0) {
+        dx[m][q] += b0;
+      } else {
+        const float u2 = fmaf(y, y, -1.0f), u3 = fmaf(y, u2, -y), u4 = fmaf(y, u3, -u2);
+        float un = u4, um = u3;  // U_N, U_{N-1}
+        if constexpr (N == 8) {
+          un = fmaf(u4, u4, -u3 * u3);
+          um = u3 * (u4 - u2);
+        } else if constexpr (N == 12) {
+          const float u5 = fmaf(y, u4, -u3), u6 = fmaf(y, u5, -u4);
+          un = fmaf(u6, u6, -u5 * u5);
+          um = u5 * (u6 - u4);
+        }
+        dx[m][q] += fmaf(un, b0, -um * b1);
+      }
+    }
+}
+
 // dx of 128 rows x 64 inputs a block, waves of 64 rows x 32 inputs: four degrees a
 // pass over the outputs stand in four accumulator fragments; between passes only
 // their weighted sum is kept.
@@ -899,28 +936,19 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
       return cbase + ((size_t)ib * p.deg + d) * pitch;
     }, s0 * KS, nst, lds, acc);
     const int nd = p.deg - d0 < 4 ? p.deg - d0 : 4;
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const float x2 = x[m][q] + x[m][q];
-        float ua = 0.0f, ub = 1.0f;  // U_{-1}, U_0
-        for (int d = 0; d < d0; ++d) {
-          const float c = fmaf(x2, ub, -ua);
-          ua = ub;
-          ub = c;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          if (d < nd) s = fmaf(acc[m][d][q], ub, s);
-          const float c = fmaf(x2, ub, -ua);
-          ua = ub;
-          ub = c;
-        }
-        dx[m][q] = fmaf(s, 1.0f - x[m][q] * x[m][q], dx[m][q]);
-      }
+    if (d0 == 0)
+      weigh_by_u<0>(acc, nd, x, dx);
+    else if (d0 == 4)
+      weigh_by_u<4>(acc, nd, x, dx);
+    else if (d0 == 8)
+      weigh_by_u<8>(acc, nd, x, dx);
+    else
+      weigh_by_u<12>(acc, nd, x, dx);
   }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) dx[m][q] *= fmaf(-x[m][q], x[m][q], 1.0f);
   const float ic = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
   const float ig = 1.0f / ((const float*)(a.ws + p.gscale_off))[e];
   if (share.parts > 1) {
