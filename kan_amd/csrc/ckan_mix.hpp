@@ -5,15 +5,34 @@
 
 namespace ckan {
 
+// The largest value and the sum over a wave, uniform: within rows of 16 lanes and then
+// across them by data-parallel moves on the vector ALU.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_from(float fallback, float v) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(__float_as_int(fallback), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+// A lane whose move has no source keeps its value.  Two wait states lie between a
+// vector write and its read by a move across lanes.  In assembly: from fmaxf and the
+// builtin come five instructions a step.
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
-  return v;
+  asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf"
+      : "+v"(v));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
-  return v;
+  v += dpp_from<0x111, 0xf>(0.0f, v);
+  v += dpp_from<0x112, 0xf>(0.0f, v);
+  v += dpp_from<0x114, 0xf>(0.0f, v);
+  v += dpp_from<0x118, 0xf>(0.0f, v);
+  v += dpp_from<0x142, 0xa>(0.0f, v);
+  v += dpp_from<0x143, 0xc>(0.0f, v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // ---- routing (ckan_route.hip) -----------------------------------------------
@@ -33,6 +52,8 @@ struct RouteArgs {
   void* dlogits;       // [rows, E]
   int64_t rows, ld;
   int E, top_k, groups, top_groups;
+  int lanes_log2;      // lanes a group in the choice of groups
+  float inv_size;      // 1 / (experts a group): an expert's group is (e + 0.5) times it
   int softmax, renormalize, bf16;
   float scale;
 };

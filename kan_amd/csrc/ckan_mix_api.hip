@@ -61,6 +61,9 @@ int route_args(const ckan_route_desc* d, RouteArgs* a) {
   a->top_k = d->top_k;
   a->groups = d->groups;
   a->top_groups = d->top_groups;
+  // as many lanes a group as 64 lanes have for all of them, a power of two
+  while ((2 << a->lanes_log2) * d->groups <= 64) ++a->lanes_log2;
+  a->inv_size = (float)d->groups / (float)d->experts;
   a->softmax = d->score == CKAN_SCORE_SOFTMAX;
   a->renormalize = d->renormalize != 0;
   a->bf16 = d->dtype == CKAN_DTYPE_BF16;

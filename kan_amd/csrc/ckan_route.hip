@@ -52,8 +52,8 @@ __device__ __forceinline__ void row_logits(const T* row, int E, int lane, float 
 #pragma unroll
   for (int q = 0; q < J; ++q) {
     const int e = lane * J + q;
-    const float v = e < E ? (float)row[e] : -INFINITY;
-    l[q] = v > -INFINITY ? v : -INFINITY;  // NaN: not eligible
+    const float v = (float)row[e < E ? e : E - 1];
+    l[q] = e < E && v > -INFINITY ? v : -INFINITY;  // NaN: not eligible
   }
 }
 
@@ -69,12 +69,8 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void k_route(RouteArgs a) {
 #pragma unroll
   for (int q = 0; q < J; ++q) {
     const int e = lane * J + q;
-    float k = -INFINITY;
-    if (l[q] > -INFINITY) {
-      k = a.bias ? s[q] + a.bias[e] : s[q];
-      k = k > -INFINITY ? k : -INFINITY;  // a NaN bias: not eligible
-    }
-    key[q] = k;
+    const float k = a.bias ? s[q] + a.bias[e < a.E ? e : a.E - 1] : s[q];
+    key[q] = l[q] > -INFINITY && k > -INFINITY ? k : -INFINITY;  // nor with a NaN bias
   }
   if (a.groups > 1) {
     // lane (g, u) of LG lanes a group takes every LG-th key of group g for the
@@ -84,10 +80,8 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void k_route(RouteArgs a) {
 #pragma unroll
     for (int q = 0; q < J; ++q) keys[lane * J + q] = key[q];
     __builtin_amdgcn_wave_barrier();
-    const int G = a.groups, size = a.E / G;
-    int LG = 64;
-    while (LG * G > 64) LG >>= 1;
-    const int g = lane / LG, u = lane % LG;
+    const int G = a.groups, size = a.E / G, LG = 1 << a.lanes_log2;
+    const int g = lane >> a.lanes_log2, u = lane & (LG - 1);
     float b1 = -INFINITY, b2 = -INFINITY;
     if (g < G)
       for (int e = u; e < size; e += LG) {
@@ -103,7 +97,7 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void k_route(RouteArgs a) {
     const float value = b1 + (b2 > -INFINITY ? b2 : 0.0f);
     int ahead = 0;  // groups before this one in the order of the choice
     for (int h = 0; h < G; ++h) {
-      const float v = __shfl(value, h * LG);
+      const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(value), h * LG));
       ahead += v > value || (v == value && h < g);
     }
     if (g < G && u == 0) kept[g] = ahead < a.top_groups ? 1.0f : 0.0f;
@@ -111,38 +105,34 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void k_route(RouteArgs a) {
 #pragma unroll
     for (int q = 0; q < J; ++q) {
       const int e = lane * J + q;
-      if (e < a.E && kept[e / size] == 0.0f) key[q] = -INFINITY;
+      if (e < a.E && kept[(int)(((float)e + 0.5f) * a.inv_size)] == 0.0f) key[q] = -INFINITY;
     }
   }
   // top_k rounds: the largest key left, then its lowest index
   int mine = -1;      // lane j: the j-th chosen expert
   float chosen = 0.0f;
   for (int j = 0; j < a.top_k; ++j) {
-    float best = key[0];
+    float own = key[0];
 #pragma unroll
-    for (int q = 1; q < J; ++q) best = fmaxf(best, key[q]);
-    best = wave_max(best);
+    for (int q = 1; q < J; ++q) own = fmaxf(own, key[q]);
+    const float best = wave_max(own);
     if (!(best > -INFINITY)) break;  // uniform: no eligible expert is left
-    int at = J;
-    float score = 0.0f;
+    // the lowest lane that holds it, and its lowest register
+    const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(own == best)) - 1);
+    int at = J - 1;
+    float score = s[J - 1];
 #pragma unroll
-    for (int q = J - 1; q >= 0; --q)
-      if (key[q] == best) {
-        at = q;
-        score = s[q];
-      }
-    const int from = __ffsll((unsigned long long)__ballot(at < J)) - 1;
-    const int e = __shfl(lane * J + at, from);
-    score = __shfl(score, from);
-    if (lane == j) {
-      mine = e;
-      chosen = score;
+    for (int q = J - 2; q >= 0; --q) {
+      const bool here = key[q] == best;
+      at = here ? q : at;
+      score = here ? s[q] : score;
     }
-    if (lane == from) {
+    at = __builtin_amdgcn_readlane(at, from);
+    score = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(score), from));
+    mine = lane == j ? from * J + at : mine;
+    chosen = lane == j ? score : chosen;
 #pragma unroll
-      for (int q = 0; q < J; ++q)
-        if (q == at) key[q] = -INFINITY;
-    }
+    for (int q = 0; q < J; ++q) key[q] = lane == from && q == at ? -INFINITY : key[q];
   }
   float w = chosen;
   if (a.renormalize) w = chosen / (wave_sum(chosen) + kRouteEps);
