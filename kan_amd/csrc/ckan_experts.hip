@@ -19,6 +19,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "ckan_mix.hpp"
 #include "ckan_planes.hpp"
 
@@ -1018,9 +1020,10 @@ __global__ __launch_bounds__(256) void k_experts_tsort(ExpertsArgs a) {
 // values and g arrive by copies; each thread makes the basis values of 32 (row,
 // degree) pairs of one input into LDS for the next stage while the matrix
 // instructions work on this one.
-template <typename T, int NP, int DB>
-__global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
+template <typename T, int NP, int DB, bool HIGH>
+__global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
   extern __shared__ char lds[];
+  constexpr int d0 = HIGH ? 8 : 0;  // the degrees d0 + 1 .. d0 + DB
   constexpr int KS = 2, NI = 8 / DB, kA = 8 * KS * NP, kB = 4 * KS * NP, kT = 4 * NI;  // 1 KiB chunks of a stage
   constexpr int kBAt = 2 * kA * kPlaneBytes, kTAt = kBAt + 2 * kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
@@ -1047,7 +1050,8 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
   const int mq = DB == 8 ? tid >> 1 : tid;
   const int mi = mq & 31, mr = (mq >> 5) & 3, mib = mq >> 7, mh = DB == 8 ? tid & 1 : 0;
   constexpr int MR = DB == 8 ? 4 : 8;
-  auto make = [&](int s) {
+  typedef typename std::conditional<MR == 8, Planes8<NP>, Planes4<NP>>::type Made;
+  auto make = [&](int s, Made (&f)[DB]) {
     const float* src = (const float*)(lds + kTAt + (s & 1) * kT * kPlaneBytes) + ((mib * 4 + mr) * 32 + mi) * 8 + mh * 4;
     float tv[MR], ta[MR], tb[MR];
 #pragma unroll
@@ -1056,7 +1060,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
       ta[j] = 1.0f;
       tb[j] = tv[j];
     }
-    if (d0) {  // 8: T_8 and T_9 by products, T_{m+n} = 2 T_m T_n - T_{m-n}
+    if constexpr (HIGH) {  // T_8 and T_9 by products, T_{m+n} = 2 T_m T_n - T_{m-n}
 #pragma unroll
       for (int j = 0; j < MR; ++j) {
         const float x = tv[j], t2 = fmaf(x + x, x, -1.0f), t3 = fmaf(x + x, t2, -x), t4 = fmaf(t2 + t2, t2, -1.0f);
@@ -1064,19 +1068,12 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
         tb[j] = fmaf(t4 + t4, fmaf(t2 + t2, t3, -x), -x);
       }
     }
-    char* dst = lds + (s & 1) * kA * kPlaneBytes + (mi + 32 * (mr & 1)) * 16 + mh * 8;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
-      char* at = dst + ((((mib * DB + d) * KS + (mr >> 1)) * NP)) * kPlaneBytes;
-      if constexpr (MR == 8) {
-        const Planes8<NP> f = to_planes8<NP>(tb);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) *(f16x8_t*)(at + k * kPlaneBytes) = f.p[k];
-      } else {
-        const Planes4<NP> f = to_planes4<NP>(tb);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) *(f16x4_t*)(at + k * kPlaneBytes) = f.p[k];
-      }
+      if constexpr (MR == 8)
+        f[d] = to_planes8<NP>(tb);
+      else
+        f[d] = to_planes4<NP>(tb);
 #pragma unroll
       for (int j = 0; j < MR; ++j) {
         const float c = fmaf(tv[j] + tv[j], tb[j], -ta[j]);
@@ -1084,6 +1081,14 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
         tb[j] = c;
       }
     }
+  };
+  auto keep = [&](int s, const Made (&f)[DB]) {
+    char* dst = lds + (s & 1) * kA * kPlaneBytes + (mi + 32 * (mr & 1)) * 16 + mh * 8;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        *(typename Made::part*)(dst + (((mib * DB + d) * KS + (mr >> 1)) * NP + k) * kPlaneBytes) = f[d].p[k];
   };
   auto copy_g = [&](int s) {
 #pragma unroll
@@ -1111,7 +1116,9 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
     if (nst > 1) copy_t(1);
     wait_vm<0>();
     block_barrier();
-    make(0);
+    Made first[DB];
+    make(0, first);
+    keep(0, first);
   }
   for (int s = 0; s < nst; ++s) {
     wait_vm<0>();
@@ -1119,7 +1126,10 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
     block_barrier();
     if (s + 1 < nst) copy_g(s + 1);
     if (s + 2 < nst) copy_t(s + 2);  // over stage s, which was made from before the barrier
-    if (s + 1 < nst) make(s + 1);
+    // the next stage's basis values in registers while the matrix instructions run, to
+    // LDS behind them (past the last stage: of stale tanh values, not read)
+    Made next[DB];
+    make(s + 1, next);
     const char* buf = lds + (s & 1) * kA * kPlaneBytes;
     const char* bufb = lds + kBAt + (s & 1) * kB * kPlaneBytes;
 #pragma unroll
@@ -1135,6 +1145,13 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a, int d0) {
         for (int q = 0; q < NP; ++q) fb[n][q] = lds_frag(bufb + (((wo * 2 + n) * KS + k) * NP + q) * kPlaneBytes, lane);
       mfma_planes<NP, NP, 4, 2>(fa, fb, acc);
     }
+    // a matrix instruction, then vector ones in its shadow
+#pragma unroll
+    for (int i = 0; i < KS * 8 * (NP == 2 ? 3 : 1); ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, NP == 2 ? 5 : 7, 0);
+    }
+    keep(s + 1, next);
   }
   // The tile leaves through LDS, 8 inputs (of each row block) at a time, so that an
   // input's coefficients of 128 outputs are stored as they lie in memory.
@@ -1393,14 +1410,14 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
                      (const float*)(a.saved + p.z_off), a.y, p.O);
 }
 
-template <typename T, int NP, int DB>
-void launch_dc(const ExpertsArgs& a, int d0, hipStream_t st) {
+template <typename T, int NP, int DB, bool HIGH>
+void launch_dc(const ExpertsArgs& a, hipStream_t st) {
   constexpr int NI = 8 / DB, ring = 2 * ((8 + 4) * 2 * NP + 4 * NI) * kPlaneBytes;
   constexpr int tile = NI * 8 * 128 * (DB + 1) * 4, lds = ring > tile ? ring : tile;
   static std::atomic<uint32_t> done;
-  ensure_lds_limit((const void*)k_experts_dc<T, NP, DB>, lds, done);
+  ensure_lds_limit((const void*)k_experts_dc<T, NP, DB, HIGH>, lds, done);
   const int64_t blocks = a.p.E * xcd_grid(ceil_div(a.p.Ip / 32, NI) * ceil_div(a.p.O, 128));
-  hipLaunchKernelGGL((k_experts_dc<T, NP, DB>), dim3((unsigned)blocks), dim3(256), lds, st, a, d0);
+  hipLaunchKernelGGL((k_experts_dc<T, NP, DB, HIGH>), dim3((unsigned)blocks), dim3(256), lds, st, a);
 }
 
 template <typename T, int NP>
@@ -1423,9 +1440,14 @@ void backward_typed(const ExpertsArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(k_experts_gsum, dim3(p.E, (p.Op + 63) / 64), dim3(256), 0, st, a);
     hipLaunchKernelGGL(k_experts_tsort, dim3((unsigned)(p.R / 32), p.Ip / 32), dim3(256), 0, st, a);
     // runs of 8 degrees, and of 4 where no more are left
-    int d0 = 0;
-    for (; p.deg - d0 > 4; d0 += 8) launch_dc<T, NP, 8>(a, d0, st);
-    if (d0 < p.deg) launch_dc<T, NP, 4>(a, d0, st);
+    if (p.deg > 4)
+      launch_dc<T, NP, 8, false>(a, st);
+    else
+      launch_dc<T, NP, 4, false>(a, st);
+    if (p.deg > 12)
+      launch_dc<T, NP, 8, true>(a, st);
+    else if (p.deg > 8)
+      launch_dc<T, NP, 4, true>(a, st);
   }
 }
 

@@ -39,7 +39,7 @@ __device__ __forceinline__ float opaque(float v) {
 }
 
 // The 8 values of a lane in planes (round to nearest even each).
-template <int NP> struct Planes8 { f16x8_t p[NP]; };
+template <int NP> struct Planes8 { typedef f16x8_t part; f16x8_t p[NP]; };
 template <int NP>
 __device__ __forceinline__ Planes8<NP> to_planes8(const float* v) {
   Planes8<NP> f;
@@ -52,7 +52,7 @@ __device__ __forceinline__ Planes8<NP> to_planes8(const float* v) {
   }
   return f;
 }
-template <int NP> struct Planes4 { f16x4_t p[NP]; };
+template <int NP> struct Planes4 { typedef f16x4_t part; f16x4_t p[NP]; };
 template <int NP>
 __device__ __forceinline__ Planes4<NP> to_planes4(const float* v) {
   Planes4<NP> f;
