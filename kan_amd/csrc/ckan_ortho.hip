@@ -9,7 +9,8 @@
 // planes keep 22 bits of entries down to 2^-15 of the largest.
 //
 // Matrices with a side of at most 64 are ckan_ortho_small.hip's.  Of the others,
-// fp32 matrices take the iteration as it is written, on two planes.  X is held
+// fp32 matrices take the iteration on two planes, as it is written or, where they are
+// wide, two steps at a time (pairs() below).  X is held
 // twice, as the operand with rows m and k = n (Xr, for A = X X^T) and as the one
 // with rows n and k = m (Xc, for the product with X).
 //
@@ -43,6 +44,15 @@ struct OrthoPlan {
   size_t norm_off, xr_off, xc_off[2], part_off, mm_off[5], bytes;
   size_t xr_bytes, xc_bytes, a_bytes, part_elems;  // a matrix
 };
+
+// Two steps as one product with the long side:
+//   X'' = P_1 P_0 X,  P_s = a I + b A_s + c A_s^2,  A_1 = P_0 A_0 P_0,
+// five m x m products more and one pass over X and one X X^T less.  Errors of A_0 pass
+// through one step more, 1.3 to 1.9 times the iteration's error in simulations; where
+// the sums over n are long that is still below what plain fp32 products give (8 x
+// [512, 4608]: 1.6e-6 step by step, 3.4e-6 plain).  At n = 4 m the trade in
+// multiply-adds is 11 m^3 more for 12 m^3 less.
+bool pairs(int m, int n) { return n >= 4 * (int64_t)m && n >= 2048; }
 
 OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   OrthoPlan p{};
@@ -82,7 +92,7 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   p.xc_off[0] = take(p.xc_bytes * batch);
   p.xc_off[1] = bf16 ? 0 : take(p.xc_bytes * batch);
   p.part_off = take(p.part_elems * batch * p.splits * sizeof(float));
-  for (int i = 0; i < (bf16 ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
+  for (int i = 0; i < (bf16 || pairs(p.m, p.n) ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
   p.bytes = off;
   return p;
 }
@@ -467,11 +477,11 @@ __device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p,
 }
 constexpr int kPutLds = kTile * kPutPitch * 4;
 
-// X' = a X + B X.  The product's rows are m, its columns n: an accumulator quad is 4
+// X' = ax X + inv B X.  The product's rows are m, its columns n: an accumulator quad is 4
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
 // through LDS.  The last step writes the result instead (or Muon's parameters).
 __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan p, const char* B, const char* xc,
-                                                         char* xc_new, char* xr, int last) {
+                                                         char* xc_new, char* xr, float ax, float inv, int last) {
   extern __shared__ char lds[];
   const int TM = p.m128 / kTile, TN = p.n128 / kTile;
   int id = blockIdx.x;
@@ -503,7 +513,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
           const f16x4_t h = *(const f16x4_t*)(x + at), l = *(const f16x4_t*)(x + at + kPlaneBytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (k + j < p.m && col < p.n) v[j] = a.a * ((float)h[j] + (float)l[j]) + acc[m][n][q * 4 + j] * kInvS;
+            if (k + j < p.m && col < p.n) v[j] = ax * ((float)h[j] + (float)l[j]) + acc[m][n][q * 4 + j] * inv;
         }
         if (last) {
 #pragma unroll
@@ -600,6 +610,21 @@ float largest_q(const OrthoArgs& a) {
   return (float)most;
 }
 
+// The same of the product of two steps' P.
+float largest_pair(const OrthoArgs& a) {
+  double most = 0.0;
+  for (int i = 0; i <= 1024; ++i) {
+    double x = i / 1024.0, before = 1.0;
+    for (int s = 0; s < a.steps; ++s) {
+      const double f = a.a + a.b * x * x + a.c * x * x * x * x;
+      if (s) most = fmax(most, fabs(before * f));
+      before = f;
+      x *= f;
+    }
+  }
+  return (float)fmax(most, (double)a.a * a.a);
+}
+
 }  // namespace
 
 size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16) {
@@ -648,12 +673,33 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   };
   if (!p.bf16) {
     hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
-    for (int s = 0; s < a.steps; ++s) {
+    const bool two = pairs(p.m, p.n) && largest_pair(a) < 30.0f;  // its planes at 2^11 hold 32
+    constexpr float kS2 = 2048.0f;
+    char* x = xc[0];
+    char* xn = xc[1];
+    for (int s = 0; s < a.steps;) {
+      const int taken = two && s + 1 < a.steps ? 2 : 1;
       hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::kLdsBytes, st, p, xr, part);
       hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
-      products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f}, nullptr);
-      hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), block, kUpdateLds, st, a, p, mm[1], xc[s & 1], xc[(s + 1) & 1],
-                         xr, s == a.steps - 1);
+      if (taken == 1) {
+        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f}, nullptr);
+      } else {
+        const MmJob poly{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, a.a * kS, 0.0f};
+        products(poly, nullptr);                                                         // P_0
+        products(MmJob{mm[1], mm[0], mm[2], nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);  // P_0 A_0
+        products(MmJob{mm[2], mm[1], mm[0], nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);  // A_1
+        MmJob second = poly;
+        second.out = mm[3];
+        products(second, nullptr);  // P_1
+        // P_1 P_0 - a^2 I: X itself enters with a^2 in fp32
+        products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, 0.0f, -a.a * a.a * kS2, 0.0f}, nullptr);
+      }
+      s += taken;
+      hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), block, kUpdateLds, st, a, p, mm[taken == 1 ? 1 : 4], x, xn, xr,
+                         taken == 1 ? a.a : a.a * a.a, taken == 1 ? kInvS : 1.0f / kS2, s == a.steps);
+      char* o = x;
+      x = xn;
+      xn = o;
     }
     return;
   }
