@@ -495,9 +495,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   Tile22::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0,
               KB / Tile22::kStageBlocks, lds, acc);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
-  constexpr int kPitch = (kTile + 8) * 2;  // bytes of a row of the LDS tile
   const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
-  char* plane1 = lds + kTile * kPitch;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -526,10 +524,12 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
           *(f16x4_t*)d = f.p[0];
           *(f16x4_t*)(d + kPlaneBytes) = f.p[1];
         }
+        // both planes of an element in one LDS word: half the stores of two planes
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          *(_Float16*)(lds + (r + j) * kPitch + c * 2) = f.p[0][j];
-          *(_Float16*)(plane1 + (r + j) * kPitch + c * 2) = f.p[1][j];
+          const _Float16 h = f.p[0][j], l = f.p[1][j];  // a bit cast of a vector's element takes the first one
+          ((uint32_t*)lds)[(r + j) * kPutPitch + c] =
+              (uint32_t)__builtin_bit_cast(uint16_t, h) | (uint32_t)__builtin_bit_cast(uint16_t, l) << 16;
         }
       }
     }
@@ -546,13 +546,22 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
     const int row = tm * kTile + r, k = tn * kTile + k8 * 8;
     if (k >= p.n32) continue;
     char* d = xr + b * p.xr_bytes + ((size_t)(row >> 5) * KBr + (k >> 4)) * 2 * kPlaneBytes + ((row & 31) + 32 * (k8 & 1)) * 16;
-    *(f16x8_t*)d = *(const f16x8_t*)(lds + r * kPitch + k8 * 16);
-    *(f16x8_t*)(d + kPlaneBytes) = *(const f16x8_t*)(plane1 + r * kPitch + k8 * 16);
+    const u32x4_t* src = (const u32x4_t*)((const uint32_t*)lds + r * kPutPitch + k8 * 8);
+    const u32x4_t w0 = src[0], w1 = src[1];
+    u32x4_t h, l;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      h[j] = (w0[2 * j] & 0xffffu) | w0[2 * j + 1] << 16;
+      l[j] = w0[2 * j] >> 16 | (w0[2 * j + 1] & 0xffff0000u);
+      h[j + 2] = (w1[2 * j] & 0xffffu) | w1[2 * j + 1] << 16;
+      l[j + 2] = w1[2 * j] >> 16 | (w1[2 * j + 1] & 0xffff0000u);
+    }
+    *(u32x4_t*)d = h;
+    *(u32x4_t*)(d + kPlaneBytes) = l;
   }
 }
 
-constexpr int max3(int a, int b, int c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
-constexpr int kUpdateLds = max3(2 * kTile * (kTile + 8) * 2, Tile22::kLdsBytes, kPutLds);
+constexpr int kUpdateLds = Tile22::kLdsBytes > kPutLds ? Tile22::kLdsBytes : kPutLds;
 
 // The bf16 result Q X0: Q in two planes (scale qscale), X0 / rest in one.
 typedef NtTile<2, 1, 2, 2, 2, 2, 2, 3> ApplyTile;  // 72 KiB of LDS
