@@ -511,7 +511,11 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
 // 128 rows x 64 FN columns a block, four waves of 64 x 32 FN.  Each stage copies the
 // rows' tanh values of IN inputs (gathered by token) and KS k-blocks of Cf to LDS;
 // a wave makes its rows' basis values in registers, eight values of one or two
-// inputs a lane and k-block.
+// inputs a lane and k-block: a fragment of 12 vector instructions serves four
+// matrix ones.  16384 slots, 1024 -> 1024, degree 8, bf16: 311 us, 884 TFLOP/s, the
+// matrix pipe 45 % busy; without its copies 278, without the recurrence 301.
+// Shorter stages than these wait at their barriers, a 128-column tile makes the basis
+// twice as often.
 template <int NP, int P>
 __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   extern __shared__ char lds[];
@@ -891,7 +895,9 @@ __device__ __forceinline__ void weigh_by_u(const f32x16_t (&acc)[2][4], int nd, 
 
 // dx of 128 rows x 64 inputs a block, waves of 64 rows x 32 inputs: four degrees a
 // pass over the outputs stand in four accumulator fragments; between passes only
-// their weighted sum is kept.
+// their weighted sum is kept.  16384 slots, 1024 -> 1024, degree 8, bf16: 286 us, 962
+// TFLOP/s, the matrix pipe 48 % busy; bound by the copies (24 KiB for 2.1 MFLOP a
+// stage): with two or six buffers instead of three 418 and 413 where three took 398.
 template <int NP> using DxTile = NtTile<NP, NP, 2, 2, 2, 4, NP == 1 ? 2 : 1, 3>;  // 72 KiB of LDS
 
 template <int NP>
@@ -1019,7 +1025,9 @@ __global__ __launch_bounds__(256) void k_experts_tsort(ExpertsArgs a) {
 // blocks); waves of 4 row blocks x 64 outputs.  A stage is 32 rows.  The tanh
 // values and g arrive by copies; each thread makes the basis values of 32 (row,
 // degree) pairs of one input into LDS for the next stage while the matrix
-// instructions work on this one.
+// instructions work on this one.  16384 slots, 1024 -> 1024, degree 8, bf16: 324 us,
+// 848 TFLOP/s, the matrix pipe 41 % busy; without making the basis 275, without the
+// copies 346 of 353, without the last store 341.
 template <typename T, int NP, int DB, bool HIGH>
 __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
   extern __shared__ char lds[];
@@ -1268,7 +1276,10 @@ __device__ __forceinline__ void stream_unpack(const __bf16* row, int o, const ui
 // part[chunk, slot, o] = the slot's expert output over one chunk of inputs.  A block
 // takes one expert, 64 outputs (a lane each) and a chunk; it finds its expert's
 // slots itself, makes the basis values of up to 8 rows in LDS (read as
-// broadcasts), and its four waves stream the chunk's coefficients.
+// broadcasts), and its four waves stream the chunk's coefficients.  Bound by the
+// coefficients' stream: two experts of 2048 -> 2048, degree 8, bf16, for one row 30 us
+// (5.0 TB/s; a large copy reaches 5.15), 96 slots of 16 experts of 512 -> 512 in fp32
+// 34 us (4.5 TB/s).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_experts_stream(ExpertsArgs a) {
   constexpr int kDeg = D - 1, kW = (kDeg + 3) / 4 * 4, kU = 4;

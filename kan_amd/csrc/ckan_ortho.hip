@@ -333,7 +333,9 @@ struct MmJobs { MmJob j[2]; };
 
 // 64 x 64 tiles (128 x 128 ones leave most CUs without a block at these sizes): one
 // block a CU, so kMmGroups groups of four waves divide a stage's k-blocks to have
-// work while others wait.
+// work while others wait.  At m = 1024 a launch takes 14-17 us, 13 of them its copies
+// (16 KiB a k-block and CU): rings of 2 to 4 buffers, stages of 2 or 4 k-blocks, one
+// or three accumulators and one or two groups all measure within 1 us.
 constexpr int kMmGroups = 2;
 typedef NtTile<2, 2, 2, 2, 1, 1, 4, 2, 3, kMmGroups> MmTile;  // 64 KiB of LDS
 
@@ -480,6 +482,8 @@ constexpr int kPutLds = kTile * kPutPitch * 4;
 // X' = ax X + inv B X.  The product's rows are m, its columns n: an accumulator quad is 4
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
 // through LDS.  The last step writes the result instead (or Muon's parameters).
+// 8 x [512, 4608]: 100 us for 300 MB of X read and written and 58 GFLOP of plane
+// products, 1152 blocks in 512 places; without its copies 85, without its products 95.
 __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan p, const char* B, const char* xc,
                                                          char* xc_new, char* xr, float ax, float inv, int last) {
   extern __shared__ char lds[];
@@ -563,7 +567,8 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
 
 constexpr int kUpdateLds = Tile22::kLdsBytes > kPutLds ? Tile22::kLdsBytes : kPutLds;
 
-// The bf16 result Q X0: Q in two planes (scale qscale), X0 / rest in one.
+// The bf16 result Q X0: Q in two planes (scale qscale), X0 / rest in one.  1024 x 9216:
+// 58 us, 670 TFLOP/s on its two products.
 typedef NtTile<2, 1, 2, 2, 2, 2, 2, 3> ApplyTile;  // 72 KiB of LDS
 __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p, const char* Q, const char* xc,
                                                         const double* rest) {
