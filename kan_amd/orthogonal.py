@@ -47,12 +47,14 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     if g.numel() == 0:
         return torch.empty_like(g)
     x = g.reshape(-1, rows, cols)
-    if not (x.is_contiguous() or x.transpose(1, 2).is_contiguous()):
-        x = x.contiguous()
-    out = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+    if x.is_contiguous() or not x.transpose(1, 2).is_contiguous():
+        x, strides = x.contiguous(), (rows * cols, cols, 1)
+    else:
+        strides = (rows * cols, 1, rows)
+    # not x.stride(): a dimension of one may have any
+    out = torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
     a, b, c = (float(v) for v in coefficients)
-    desc = _lib.CkanOrthoDesc(x.stride(0), x.stride(1), x.stride(2), 0, x.shape[0], rows, cols, 1,
-                              int(steps), _DTYPES[g.dtype], a, b, c, float(eps))
+    desc = _lib.CkanOrthoDesc(*strides, 0, x.shape[0], rows, cols, 1, int(steps), _DTYPES[g.dtype], a, b, c, float(eps))
     with torch.cuda.device(x.device):
         ws, nbytes = _workspace(desc, x.device)
         _lib.check(_lib.load().ckan_orthogonalize(desc, x.data_ptr(), out.data_ptr(), ws.data_ptr(),

@@ -141,3 +141,10 @@ def test_muon_optimizer_trains_and_resumes():
     opt2.load_state_dict({"state": {k: {n: t.clone() for n, t in v.items()} for k, v in saved[1]["state"].items()},
                           "param_groups": saved[1]["param_groups"]})
     assert set(opt2.state[other.cheby_coeffs]) == {"momentum_buffer"}
+
+
+def test_strides_of_dimensions_of_one():
+    g = torch.randn(6, 8, 10, device="cuda")
+    for v in (g[::6, ::8, ::10], g[:, ::8, :], g[:, :, ::10], g[:1, :, ::10], g[2:3].transpose(1, 2)):
+        got = kan_amd.functional.orthogonalize(v)
+        assert got.shape == v.shape and torch.equal(got, kan_amd.functional.orthogonalize(v.clone(memory_format=torch.contiguous_format)))
