@@ -315,7 +315,8 @@ int ckan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int6
 /* ---- mixture of experts: routing -------------------------------------------- */
 /* Rows of logits choose top_k of `experts` experts each.
  *   s = softmax(l) or sigmoid(l);  key = s + bias (bias may be NULL).
- *   An expert with logit -inf or NaN (or a NaN key) is not eligible: s = 0.
+ *   An expert with logit -inf or NaN (or a NaN key) is not eligible: s = 0.  A logit
+ *   of +inf counts as the largest finite one.
  *   groups > 1: the experts are `groups` equal runs; a group's value is the sum of
  *   its two largest keys (a missing or ineligible second counts 0), and only the
  *   top_groups groups of largest value stay.
@@ -331,7 +332,7 @@ typedef enum ckan_score {
 } ckan_score;
 
 typedef struct ckan_route_desc {
-  int64_t rows;         /* >= 0                                           */
+  int64_t rows;         /* 0..2^26 - 1                                    */
   int64_t logits_ld;    /* elements from a row of logits to the next      */
   int32_t experts;      /* 1..512                                         */
   int32_t top_k;        /* 1..64, at most the experts of top_groups groups */
@@ -359,12 +360,14 @@ int ckan_route_backward(const ckan_route_desc* desc, const void* logits, const i
  * lies outside [0, experts) has no expert: it adds nothing and its weight's
  * gradient is 0.  A row may name an expert twice.
  * fp32 tensors are computed on two fp16 planes an operand (22 bits), bf16 ones on
- * one (11 bits); sums, tanh and the basis recurrence are in fp32.
+ * one (11 bits); sums, tanh and the basis recurrence are in fp32.  The planes are
+ * scaled by the largest coefficient of an expert (and the largest gradient of its
+ * rows): values down to 2^-13 of it keep 22 bits, smaller ones an error of 2^-35 of it.
  * `saved` (ckan_experts_saved_bytes) carries the sorted slots, tanh values, expert
  * outputs and packed coefficients from the forward to its backward; NULL where no
  * backward follows.  Buffers need 16-byte alignment. */
 typedef struct ckan_experts_desc {
-  int64_t rows;      /* >= 0; rows * top_k at most 2^29            */
+  int64_t rows;      /* >= 0; rows * top_k at most 2^26, rows * dims 2^33 */
   int32_t experts;   /* 1..512                                     */
   int32_t top_k;     /* 1..64                                      */
   int32_t in_dim;    /* 1..65536                                   */

@@ -31,8 +31,9 @@ int check_launch(const char* what) {
 int route_args(const ckan_route_desc* d, RouteArgs* a) {
   if (!d) return fail(CKAN_ERR_INVALID_ARG, "route desc is NULL");
   if (d->rows < 0) return fail(CKAN_ERR_INVALID_ARG, "rows must be >= 0 (got %lld)", (long long)d->rows);
-  if (d->rows > ((int64_t)1 << 31))
-    return fail(CKAN_ERR_UNSUPPORTED, "rows above 2^31 are not supported (got %lld)", (long long)d->rows);
+  // a wave a row: a launch holds fewer than 2^32 threads
+  if (d->rows >= ((int64_t)1 << 26))
+    return fail(CKAN_ERR_UNSUPPORTED, "2^26 rows or more are not supported (got %lld)", (long long)d->rows);
   if (d->experts < 1) return fail(CKAN_ERR_INVALID_ARG, "experts must be >= 1 (got %d)", d->experts);
   if (d->experts > kRouteMaxExperts)
     return fail(CKAN_ERR_UNSUPPORTED, "experts above %d are not supported (got %d)", kRouteMaxExperts, d->experts);
@@ -87,8 +88,11 @@ int experts_check(const ckan_experts_desc* d) {
     return fail(CKAN_ERR_UNSUPPORTED, "experts have degree 1 to %d (got %d)", kExpertsMaxDegree, d->degree);
   if (d->in_dim > 65536 || d->out_dim > 65536)
     return fail(CKAN_ERR_UNSUPPORTED, "in_dim and out_dim above 65536 are not supported (got %d, %d)", d->in_dim, d->out_dim);
-  if (d->rows > ((int64_t)1 << 29) / d->top_k)
-    return fail(CKAN_ERR_UNSUPPORTED, "rows * top_k above 2^29 is not supported");
+  // a launch holds fewer than 2^32 threads: 32 a slot, one for four values of a row
+  if (d->rows > ((int64_t)1 << 26) / d->top_k)
+    return fail(CKAN_ERR_UNSUPPORTED, "rows * top_k above 2^26 is not supported");
+  if (d->rows > ((int64_t)1 << 33) / (d->in_dim > d->out_dim ? d->in_dim : d->out_dim))
+    return fail(CKAN_ERR_UNSUPPORTED, "rows times in_dim or out_dim above 2^33 is not supported");
   return CKAN_OK;
 }
 

@@ -53,7 +53,9 @@ __device__ __forceinline__ void row_logits(const T* row, int E, int lane, float 
   for (int q = 0; q < J; ++q) {
     const int e = lane * J + q;
     const float v = (float)row[e < E ? e : E - 1];
-    l[q] = e < E && v > -INFINITY ? v : -INFINITY;  // NaN: not eligible
+    // NaN: not eligible; +inf as the largest finite value, so that the row's scores are
+    // the limit (all weight on it) and not NaN
+    l[q] = e < E && v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY;
   }
 }
 

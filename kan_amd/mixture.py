@@ -66,6 +66,12 @@ def _route_forward(logits, bias, desc):
     return w, idx
 
 
+def _once(name: str) -> None:
+    """Refuses a backward that is to be differentiated again: it would be a constant."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} is differentiable once (create_graph is not supported)")
+
+
 class RouteFunction(torch.autograd.Function):
     """The weights of ``route``, differentiable in the logits; the indices go by the
     side (``out``): an output more costs the autograd engine 4 us a step."""
@@ -74,13 +80,16 @@ class RouteFunction(torch.autograd.Function):
     def forward(ctx, logits: torch.Tensor, bias: Optional[torch.Tensor], desc, out: list):
         w, idx = _route_forward(logits, bias, desc)
         ctx.save_for_backward(logits)
-        ctx.desc, ctx.idx = desc, idx
+        ctx.desc, ctx.idx, ctx.idx_version = desc, idx, idx._version
         out.append(idx)
         return w
 
     @staticmethod
     def backward(ctx, dw: torch.Tensor):
+        _once("route")
         logits, = ctx.saved_tensors
+        if ctx.idx._version != ctx.idx_version:
+            raise RuntimeError("route's indices were modified in place before its backward; change a clone")
         if dw.dtype != torch.float32 or not dw.is_contiguous():
             dw = dw.to(torch.float32).contiguous()
         dl = torch.empty_like(logits, memory_format=torch.contiguous_format)
@@ -101,10 +110,11 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     with ``groups`` > 1 only the ``top_groups`` groups of consecutive experts stay
     whose two largest keys sum highest.  Equal keys go to the lowest index.  The
     weights are the chosen scores, over their sum with ``renormalize``, times
-    ``scale``.  An expert whose logit is -inf or NaN is never chosen; a row that
-    has fewer than ``top_k`` others fills up with index -1 and weight 0.
+    ``scale``.  An expert whose logit is -inf or NaN is never chosen (+inf counts as the
+    largest finite logit); a row that has fewer than ``top_k`` others fills up with index -1 and weight 0.
 
-    Differentiable in ``logits`` (through the weights, not through the choice)."""
+    Differentiable once in ``logits`` (through the weights, not through the choice);
+    the indices are not to be changed in place before the backward."""
     if score not in _SCORES:
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
     if logits.dim() != 2:
@@ -156,6 +166,7 @@ class ExpertsFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _once("kan_experts")
         saved, indices, weights = ctx.saved_tensors
         desc = ctx.desc
         xs, cs, dtype = ctx.shapes
@@ -188,10 +199,11 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
     bf16 (y [rows, out] likewise); ``indices`` [rows, top_k] int64 and ``weights`` [rows,
     top_k] (fp32 or bf16) as ``route`` returns them.  A slot whose index lies outside
     [0, experts) has no expert: a row of such slots gives zeros.  Degrees 1 to 16,
-    up to 512 experts.  fp32 results carry fp32 accuracy (operands of 22 bits), bf16
+    up to 512 experts.  fp32 results carry fp32 accuracy (operands of 22 bits, down to
+    2^-13 of the expert's largest coefficient, and an error of 2^-35 of that below), bf16
     ones are rounded once from fp32 sums of 11-bit basis values.
 
-    Differentiable in x, coeffs and weights; sums run in a fixed order, so a call
+    Differentiable once in x, coeffs and weights; sums run in a fixed order, so a call
     repeats bit for bit."""
     _require_device(x, coeffs, indices, weights)
     code = _dtype_code(x, "x")
@@ -222,8 +234,8 @@ class MixtureKANLayer(nn.Module):
 
     Parameters: ``gate`` [experts, input_dim] and ``cheby_coeffs`` [experts, input_dim,
     output_dim, degree+1], each expert initialised as the layer is.  ``compute``: 'fp32'
-    or 'bf16' (the experts' operands and outputs are bf16, the gate and the choice stay
-    fp32; the output is fp32, as a ChebyKANLayer's).
+    or 'bf16' (the experts' operands and outputs are bf16, the gate, the choice and the
+    weights stay fp32; the output is fp32, as a ChebyKANLayer's).
 
     With ``balance``, a per-expert bias steers the choice, not the weights:
     ``update_balance`` moves it towards experts that got fewer rows than the mean."""
@@ -263,7 +275,7 @@ class MixtureKANLayer(nn.Module):
         self._last_indices = indices if self.balance_bias is not None else None
         if self.compute == "fp32":
             return kan_experts(x, self.cheby_coeffs, indices, weights)
-        y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights.bfloat16())
+        y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights)
         return y.to(torch.float32)
 
     @torch.no_grad()

@@ -100,3 +100,11 @@ def test_oracle_gradients_against_differences():
             return (orc.kan_experts(v[0], v[1], idx, v[2]) * dy).sum()
 
         assert abs((f(1) - f(-1)) / 2e-6 - (grads[k] * u).sum()) < 1e-7
+
+
+@pytest.mark.parametrize("change", [dict(rows=1 << 26, top_k=2), dict(rows=1 << 24, top_k=1, in_dim=513),
+                                    dict(rows=1 << 24, top_k=1, out_dim=513)])
+def test_sizes_within_a_launch(change):
+    lib = _lib.load()
+    assert lib.ckan_experts_workspace_bytes(_desc(**change), 0, 1) == 0
+    assert b"above 2^" in lib.ckan_last_error()

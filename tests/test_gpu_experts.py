@@ -247,3 +247,12 @@ def test_one_expert_is_the_layer():
                                        torch.ones(200, 1, device="cuda"))
     want = layer(x)
     assert ((y - want).norm() / want.norm()).item() <= 2 * TOL[torch.float32]
+
+
+def test_second_derivative_is_refused():
+    x = torch.randn(5, 6, device="cuda", requires_grad=True)
+    c = torch.randn(3, 6, 4, 3, device="cuda")
+    idx = torch.tensor([[0, 2]] * 5, device="cuda")
+    y = kan_amd.functional.kan_experts(x, c, idx, torch.ones(5, 2, device="cuda"))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y.square().sum(), x, create_graph=True)

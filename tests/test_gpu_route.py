@@ -107,3 +107,33 @@ def test_strided_logits_other_stream_and_empty():
     w.sum().backward()
     same = kan_amd.functional.route(torch.zeros(1, 7, device="cuda").expand(6, 7), 3)
     assert same[1].tolist() == [[0, 1, 2]] * 6
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_infinite_logit_takes_its_limit(score):
+    l = _inputs(3, 70, torch.float32, 21)
+    l[0, 66] = float("inf")
+    l[1, 5] = float("inf")
+    l[1, 6] = -float("inf")
+    kw = dict(score=score, renormalize=False)
+    ld = l.cuda().requires_grad_()
+    w, idx = kan_amd.functional.route(ld, 3, **kw)
+    assert idx[0, 0] == 66 and idx[1, 0] == 5 and (w[:2, 0] == 1).all()
+    _check_choice(l.clamp(max=torch.finfo(torch.float32).max), idx, w.detach(), kw, 3)
+    got, = torch.autograd.grad(w.sum(), ld)
+    assert torch.isfinite(got).all()
+
+
+def test_indices_changed_before_the_backward_are_refused():
+    ld = _inputs(4, 9, torch.float32, 2).cuda().requires_grad_()
+    w, idx = kan_amd.functional.route(ld, 2)
+    idx[0, 0] = -1
+    with pytest.raises(RuntimeError, match="modified in place"):
+        w.sum().backward()
+
+
+def test_second_derivative_is_refused():
+    ld = _inputs(4, 9, torch.float32, 2).cuda().requires_grad_()
+    w, _ = kan_amd.functional.route(ld, 2)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(w.square().sum(), ld, create_graph=True)

@@ -73,3 +73,10 @@ def test_oracle_gradient_against_differences(score, renormalize):
         e = np.zeros_like(l)
         e[at] = h
         assert abs((f(l + e) - f(l - e)) / (2 * h) - got[at]) < 1e-8
+
+
+def test_route_rows_within_a_launch():
+    lib = _lib.load()
+    d = _desc(rows=1 << 26)
+    assert lib.ckan_route(d, 256, None, 256, 256, None) == _lib.CKAN_ERR_UNSUPPORTED
+    assert lib.ckan_route_backward(d, 256, 256, 256, 256, None) == _lib.CKAN_ERR_UNSUPPORTED
