@@ -384,6 +384,12 @@ __device__ __forceinline__ Share block_share(int block, int W) {
   }
   return s;
 }
+// The time of W tiles shared out so, in rounds of whole tiles.
+double share_rounds(int64_t W) {
+  const int64_t n = ceil_div(W, 8), rest = n % kXcdBlocks;
+  const int64_t parts = rest ? kXcdBlocks / rest : 1;
+  return (double)(n / kXcdBlocks) + (rest ? 1.0 / (parts < kMaxSplits ? parts : kMaxSplits) : 0.0);
+}
 int64_t share_grid(int64_t most) { return 8 * (ceil_div(most, 8) + kXcdBlocks); }
 
 // (tile, column block) of a product's block: 16 tiles go through one column block
@@ -400,13 +406,11 @@ __device__ __forceinline__ void tile_and_column(int v, int tiles, int cols, int&
 // The forward's stages: KS k-blocks, the IN inputs that they hold, and the ring of
 // LDS buffers.  One plane: short stages, three ahead (the copies of a stage take
 // longer than its products); two planes: a stage's products take three times as
-// long and one ahead is enough.  FN: column fragments a wave, so that two blocks'
-// rings share a CU.
+// long and one ahead is enough.
 template <int NP, int P> struct FwdStage {
   static constexpr int KS = P == 16 ? 4 : 2;
   static constexpr int IN = KS * 16 / P;
   static constexpr int NBUF = NP == 1 && P < 16 ? 4 : 2;
-  static constexpr int FN = NP == 2 && P == 16 ? 2 : 4;
 };
 
 // Cf: the forward's operand, rows o, k in stages of IN inputs: half g of a lane
@@ -514,13 +518,13 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
 // inputs a lane and k-block: a fragment of 12 vector instructions serves four
 // matrix ones.  16384 slots, 1024 -> 1024, degree 8, bf16: 311 us, 884 TFLOP/s, the
 // matrix pipe 45 % busy; without its copies 278, without the recurrence 301.
-// Shorter stages than these wait at their barriers, a 128-column tile makes the basis
-// twice as often.
-template <int NP, int P>
+// Shorter stages than these wait at their barriers.  FN = 2 (128 columns) where wide tiles
+// would be few.
+template <int NP, int P, int FN>
 __global__ __launch_bounds__(256, 2) void k_experts_fwd(ExpertsArgs a) {
   extern __shared__ char lds[];
   using FS = FwdStage<NP, P>;
-  constexpr int KS = FS::KS, IN = FS::IN, NBUF = FS::NBUF, FN = FS::FN;
+  constexpr int KS = FS::KS, IN = FS::IN, NBUF = FS::NBUF;
   constexpr int TB = IN * 4;  // bytes of a row's tanh values a stage
   constexpr int kT = 128 * TB, kB = 2 * FN * KS * NP;  // bytes, 1 KiB chunks
   constexpr int kStage = kT + kB * kPlaneBytes;
@@ -1396,6 +1400,17 @@ void stream_typed(const ExpertsArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_experts_stream_sum<T>), dim3((unsigned)ceil_div(p.T * p.O, 256)), block, 0, st, a);
 }
 
+template <int NP, int P, int FN>
+void launch_fwd(const ExpertsArgs& a, hipStream_t st) {
+  using FS = FwdStage<NP, P>;
+  constexpr int lds = FS::NBUF * (128 * FS::IN * 4 + 2 * FN * FS::KS * NP * kPlaneBytes);
+  static std::atomic<uint32_t> done;
+  ensure_lds_limit((const void*)k_experts_fwd<NP, P, FN>, lds, done);
+  const int64_t cols = ceil_div(a.p.O, 64 * FN);
+  hipLaunchKernelGGL((k_experts_fwd<NP, P, FN>), dim3((unsigned)share_grid(a.p.tiles * cols)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((k_experts_parts<false>), dim3(8 * kXcdBlocks, 8 * FN), dim3(256), 0, st, a, 64 * FN);
+}
+
 template <typename T, int NP, int P>
 void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
   const ExpertsPlan& p = a.p;
@@ -1410,13 +1425,16 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
     hipLaunchKernelGGL((k_experts_pack<T, NP, P, true>), pack_grid, dim3(256), pack_lds, st, a, keep);
   else
     hipLaunchKernelGGL((k_experts_pack<T, NP, P, false>), pack_grid, dim3(256), pack_lds, st, a, keep);
-  using FS = FwdStage<NP, P>;
-  constexpr int lds = FS::NBUF * (128 * FS::IN * 4 + 2 * FS::FN * FS::KS * NP * kPlaneBytes);
-  static std::atomic<uint32_t> done;
-  ensure_lds_limit((const void*)k_experts_fwd<NP, P>, lds, done);
-  const int cols = (p.O + 64 * FS::FN - 1) / (64 * FS::FN);
-  hipLaunchKernelGGL((k_experts_fwd<NP, P>), dim3((unsigned)share_grid((int64_t)p.tiles * cols)), dim3(256), lds, st, a);
-  hipLaunchKernelGGL((k_experts_parts<false>), dim3(8 * kXcdBlocks, 8 * FS::FN), dim3(256), 0, st, a, 64 * FS::FN);
+  // Tiles of 256 or of 128 columns: the narrow ones make the basis twice as often (some
+  // 10 % a tile), and of few tiles they leave fewer places empty.  In fp32, 16384 slots of
+  // 16 experts, 512 -> 512: 224 us narrow, 301 wide; 8 experts, 1024 -> 1024: 789 and
+  // 747; bf16, 8000 slots, 300 -> 500, degree 12: 104 and 60.  On two planes of 16
+  // degrees two blocks' rings of wide tiles would not share a CU.
+  const double narrow = 1.1 * share_rounds(p.tiles * ceil_div(p.O, 128)), wide = 2 * share_rounds(p.tiles * ceil_div(p.O, 256));
+  if ((NP == 2 && P == 16) || narrow < wide)
+    launch_fwd<NP, P, 2>(a, st);
+  else if constexpr (NP == 1 || P < 16)
+    launch_fwd<NP, P, 4>(a, st);
   hipLaunchKernelGGL((k_experts_gather<T, true>), dim3((unsigned)ceil_div(p.T * ((p.O + 3) / 4), 256)), dim3(256), 0, st, a,
                      (const float*)(a.saved + p.z_off), a.y, p.O);
 }
