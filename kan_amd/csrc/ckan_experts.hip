@@ -1032,12 +1032,20 @@ __global__ __launch_bounds__(256) void k_experts_tsort(ExpertsArgs a) {
 // instructions work on this one.  16384 slots, 1024 -> 1024, degree 8, bf16: 324 us,
 // 848 TFLOP/s, the matrix pipe 41 % busy; without making the basis 275, without the
 // copies 346 of 353, without the last store 341.
+//
+// On two planes the basis values have one LDS buffer and a barrier more, so that two
+// blocks share a CU: 16384 slots of 16 experts, 512 -> 512, degree 8, 241 us where one
+// block a CU with two buffers took 314; 8 experts, 1024 -> 1024, degree 4, 472 and 572.
+// With fewer blocks than CUs the barrier costs 2 %.
+template <int NP> struct DcRing { static constexpr int kA = NP == 1 ? 2 : 1; };
+
 template <typename T, int NP, int DB, bool HIGH>
 __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
   extern __shared__ char lds[];
   constexpr int d0 = HIGH ? 8 : 0;  // the degrees d0 + 1 .. d0 + DB
   constexpr int KS = 2, NI = 8 / DB, kA = 8 * KS * NP, kB = 4 * KS * NP, kT = 4 * NI;  // 1 KiB chunks of a stage
-  constexpr int kBAt = 2 * kA * kPlaneBytes, kTAt = kBAt + 2 * kB * kPlaneBytes;
+  constexpr int NA = DcRing<NP>::kA;
+  constexpr int kBAt = NA * kA * kPlaneBytes, kTAt = kBAt + 2 * kB * kPlaneBytes;
   const ExpertsPlan& p = a.p;
   const int nob = (p.O + 127) / 128, nib = p.Ip / 32, nbi = (nib + NI - 1) / NI;
   // Every XCD takes an eighth of each expert's blocks (whole columns of outputs, so
@@ -1095,7 +1103,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
     }
   };
   auto keep = [&](int s, const Made (&f)[DB]) {
-    char* dst = lds + (s & 1) * kA * kPlaneBytes + (mi + 32 * (mr & 1)) * 16 + mh * 8;
+    char* dst = lds + s % NA * kA * kPlaneBytes + (mi + 32 * (mr & 1)) * 16 + mh * 8;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1142,7 +1150,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
     // LDS behind them (past the last stage: of stale tanh values, not read)
     Made next[DB];
     make(s + 1, next);
-    const char* buf = lds + (s & 1) * kA * kPlaneBytes;
+    const char* buf = lds + s % NA * kA * kPlaneBytes;
     const char* bufb = lds + kBAt + (s & 1) * kB * kPlaneBytes;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -1162,6 +1170,10 @@ __global__ __launch_bounds__(256, 2) void k_experts_dc(ExpertsArgs a) {
     for (int i = 0; i < KS * 8 * (NP == 2 ? 3 : 1); ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x002, NP == 2 ? 5 : 7, 0);
+    }
+    if constexpr (NA == 1) {  // over this stage's values, once every wave has read them
+      wait_lds();
+      block_barrier();
     }
     keep(s + 1, next);
   }
@@ -1441,7 +1453,7 @@ void forward_typed(const ExpertsArgs& a, bool keep, hipStream_t st) {
 
 template <typename T, int NP, int DB, bool HIGH>
 void launch_dc(const ExpertsArgs& a, hipStream_t st) {
-  constexpr int NI = 8 / DB, ring = 2 * ((8 + 4) * 2 * NP + 4 * NI) * kPlaneBytes;
+  constexpr int NI = 8 / DB, ring = (DcRing<NP>::kA * 8 * 2 * NP + 2 * (4 * 2 * NP + 4 * NI)) * kPlaneBytes;
   constexpr int tile = NI * 8 * 128 * (DB + 1) * 4, lds = ring > tile ? ring : tile;
   static std::atomic<uint32_t> done;
   ensure_lds_limit((const void*)k_experts_dc<T, NP, DB, HIGH>, lds, done);
