@@ -64,7 +64,11 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.cb_off = take((size_t)E * p.Ip * deg * p.Op * 2 * p.NP);
   p.saved_bytes = off;
   off = 0;
-  p.bias_parts = (int)ceil_div(p.Ip, kPackInputs);
+  // inputs a block of the pack takes: 128, fewer where that leaves under four blocks a CU
+  // (6 experts, 500 -> 300, degree 5, fp32: 32 inputs 21 us, 128 35)
+  p.pack_inputs = 128;
+  while (p.pack_inputs > 32 && ceil_div(p.Ip, p.pack_inputs) * (p.Op / 32) * E < 4 * kNumCUs) p.pack_inputs /= 2;
+  p.bias_parts = (int)ceil_div(p.Ip, p.pack_inputs);
   p.hist_off = take((size_t)p.plan_blocks * E * 4);
   p.cmax_off = take((size_t)E * kMaxParts * 4);
   p.cf_off = take((size_t)E * p.Op * p.Ip * p.P * 2 * p.NP);
@@ -416,7 +420,7 @@ template <int NP, int P> struct FwdStage {
 // Cf: the forward's operand, rows o, k in stages of IN inputs: half g of a lane
 // pair holds inputs g IN/2.., P degrees each, eight values a k-block.  Cb: the dx
 // operand, rows i and k = o for each degree d, scaled by d.  And the sums over the
-// inputs of the T_0 coefficients.  A block takes 32 outputs and kPackInputs inputs of
+// inputs of the T_0 coefficients.  A block takes 32 outputs and p.pack_inputs inputs of
 // an expert, 16 inputs at a time through LDS, the next 16 inputs' loads in flight
 // meanwhile.
 template <typename T, int NP, int P, bool VEC>
@@ -425,7 +429,7 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
   __shared__ float red[4];
   using FS = FwdStage<NP, P>;
   constexpr int N = VEC ? Vec16<T>::N : 1;
-  constexpr int kLoads = 16 * 32 * 17 / N / 256 + 1;  // at degree 16
+  constexpr int kLoads = 16 * 32 * (P + 1) / N / 256 + 1;  // vectors a thread, at degree P
   const ExpertsPlan& p = a.p;
   const int e = blockIdx.z, ob = blockIdx.y, tid = threadIdx.x;
   const int D = p.D, W = 32 * D + 1;  // a row of the tile: 32 outputs, D coefficients each
@@ -438,27 +442,25 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
   char* cb = a.saved + p.cb_off + (size_t)e * p.Ip * p.deg * p.Op * 2 * NP;
   const int KBf = p.Ip * P / 16, KBo = p.Op / 16;
   const int o0 = ob * 32, no = p.O - o0 < 32 ? p.O - o0 : 32;
-  const int vrow = 32 * D / N, loads = (16 * vrow + 255) / 256;  // vectors of an input, of a thread
+  const int vrow = 32 * D / N;  // vectors of an input
   float bias = 0.0f;
-  const int i_end = (int)(blockIdx.x + 1) * kPackInputs < p.Ip ? (int)(blockIdx.x + 1) * kPackInputs : p.Ip;
+  const int i_end = (int)(blockIdx.x + 1) * p.pack_inputs < p.Ip ? (int)(blockIdx.x + 1) * p.pack_inputs : p.Ip;
   u32x4_t w[VEC ? kLoads : 1];
   auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      if (u >= loads) break;
       const int q = tid + u * 256, i = q / vrow, f = (q - i * vrow) * N;
       w[u] = u32x4_t{0, 0, 0, 0};
       if (i < 16 && i0 + i < p.I && f < no * D) w[u] = *(const u32x4_t*)(C + ((int64_t)(i0 + i) * p.O + o0) * D + f);
     }
   };
-  if constexpr (VEC) load(blockIdx.x * kPackInputs);
-  for (int i0 = blockIdx.x * kPackInputs; i0 < i_end; i0 += 16) {
+  if constexpr (VEC) load((int)blockIdx.x * p.pack_inputs);
+  for (int i0 = (int)blockIdx.x * p.pack_inputs; i0 < i_end; i0 += 16) {
     __syncthreads();
     if constexpr (VEC) {
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
-        if (u >= loads) break;
-        const int q = tid + u * 256, i = q / vrow, f = (q - i * vrow) * N;
+          const int q = tid + u * 256, i = q / vrow, f = (q - i * vrow) * N;
         if (i >= 16) continue;
         float v[N];
         widen(w[u], v, C);

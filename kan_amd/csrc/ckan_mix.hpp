@@ -89,7 +89,6 @@ constexpr int kExpertsMaxTopK = 64;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBlocks = 256;       // at most: a block's share of the slots grows past that
 constexpr int kMaxParts = 128;         // blocks an expert that look for its largest coefficient
-constexpr int kPackInputs = 128;       // inputs a block of the pack takes
 
 // Sizes and the layout of the buffers.  "Rows" are the kept slots sorted by expert,
 // each expert's run padded to a multiple of 32; "slots" are the T top_k entries of
@@ -112,6 +111,7 @@ struct ExpertsPlan {
   size_t hist_off, cmax_off, cf_off, bias_off, fpart_off, fwd_bytes;
   // backward workspace
   size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bpart_off, bwd_bytes;
+  int pack_inputs;     // inputs a block of the pack takes
   int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
   // the streaming forward (few slots): input chunks, inputs a chunk, partial sums
   bool stream;
