@@ -65,7 +65,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   p.saved_bytes = off;
   off = 0;
   // inputs a block of the pack takes: 128, fewer where that leaves under four blocks a CU
-  // (6 experts, 500 -> 300, degree 5, fp32: 32 inputs 21 us, 128 35)
+  // (6 experts, 500 -> 300, degree 5, fp32: 32 inputs 14 us, 128 20)
   p.pack_inputs = 128;
   while (p.pack_inputs > 32 && ceil_div(p.Ip, p.pack_inputs) * (p.Op / 32) * E < 4 * kNumCUs) p.pack_inputs /= 2;
   p.bias_parts = (int)ceil_div(p.Ip, p.pack_inputs);
