@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
   ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0,
                  KB / ApplyTile::kStageBlocks, lds, acc);
   const float f = (float)rest[b] * kInvS / p.qscale;
-  const bool along_m = runs_along_m(a);
+  const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -592,7 +592,7 @@ __global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int q = 0; q < 16; ++q)
-        ((float*)lds)[tile_at(along_m, false, (wave >> 1) * 64 + m * 32 + acc_row(q, g),
+        ((float*)lds)[tile_at(along_m, gathered, (wave >> 1) * 64 + m * 32 + acc_row(q, g),
                               (wave & 1) * 64 + n * 32 + (lane & 31))] = acc[m][n][q] * f;
   __syncthreads();
   put_tile(a, p, (const float*)lds, b, tm * kTile, tn * kTile);
