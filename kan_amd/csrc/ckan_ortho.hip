@@ -243,14 +243,24 @@ __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, co
   }
 }
 
-template <int NP> using GramTile = NtTile<NP, NP, 2, 2, 2, 2, 2, NP == 1 ? 4 : 2>;  // 128 x 128, 64 KiB of LDS
-typedef GramTile<2> Tile22;
+// 128 x 128, 64 KiB of LDS.  On two planes each of the three plane products has its own
+// sum: an entry then does not depend on which of its two rows is the tile's (h l and l h
+// change places).  With one sum it did, equal rows of X in different tiles got rows of A
+// that differed in a last bit, and what is no singular vector grew from there by
+// 3.4 a step: 200 x 1500, rows 0-99 twice, was 4e-3 off after 12 steps and 0.7 after 20.
+template <int NP> struct GramTile {
+  static constexpr int kSums = NP == 1 ? 1 : 3;
+  typedef NtTile<NP, NP, 2, 2, 2, 2, 2, NP == 1 ? 4 : 2, kSums> Tile;
+};
+typedef NtTile<2, 2, 2, 2, 2, 2, 2, 2> Tile22;
 
 // Partial sums of A = X X^T (scale kS^2): the tiles on and below the diagonal,
 // each stored with its mirror image, k split over blocks.
 template <int NP>
 __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* xr, float* part) {
   extern __shared__ char lds[];
+  typedef typename GramTile<NP>::Tile Tile;
+  constexpr int NC = GramTile<NP>::kSums;
   const int T = p.m128 / kTile, pairs = T * (T + 1) / 2;
   int id = blockIdx.x;
   const int split = id % p.splits;
@@ -263,8 +273,8 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
   const int kbs = KB - kb0 < p.kb_per_split ? KB - kb0 : p.kb_per_split;
   const size_t pitch = (size_t)KB * NP * kPlaneBytes;
   const char* x = xr + b * p.xr_bytes;
-  f32x16_t acc[2][2] = {};
-  GramTile<NP>::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / GramTile<NP>::kStageBlocks, lds, acc);
+  f32x16_t acc[NC * 2][2] = {};
+  Tile::run(RowBlocks{x + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, kb0, kbs / Tile::kStageBlocks, lds, acc);
   float* out = part + ((size_t)split * p.batch + b) * p.part_elems;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
@@ -277,7 +287,8 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
         f32x4_t v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[j] = acc[m][n][q * 4 + j];
+          const int r = q * 4 + j;
+          v[j] = NC == 1 ? acc[m][n][r] : (acc[m][n][r] + acc[NC / 3 * 2 + m][n][r]) + acc[NC / 3 * 4 + m][n][r];
           if (tm != tn) out[(size_t)(row + 8 * q + 4 * g + j) * p.m128 + col] = v[j];
         }
         *(f32x4_t*)(out + (size_t)col * p.m128 + row + 8 * q + 4 * g) = v;
@@ -660,8 +671,8 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   char* mm[5];
   for (int i = 0; i < 5; ++i) mm[i] = w + p.mm_off[i];
   static std::atomic<uint32_t> done[5];
-  ensure_lds_limit((const void*)k_ortho_gram<1>, GramTile<1>::kLdsBytes, done[0]);
-  ensure_lds_limit((const void*)k_ortho_gram<2>, GramTile<2>::kLdsBytes, done[1]);
+  ensure_lds_limit((const void*)k_ortho_gram<1>, GramTile<1>::Tile::kLdsBytes, done[0]);
+  ensure_lds_limit((const void*)k_ortho_gram<2>, GramTile<2>::Tile::kLdsBytes, done[1]);
   ensure_lds_limit((const void*)k_ortho_mm, MmTile::kLdsBytes, done[2]);
   ensure_lds_limit((const void*)k_ortho_update, kUpdateLds, done[3]);
   ensure_lds_limit((const void*)k_ortho_apply, kApplyLds, done[4]);
@@ -693,7 +704,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
     char* xn = xc[1];
     for (int s = 0; s < a.steps;) {
       const int taken = two && s + 1 < a.steps ? 2 : 1;
-      hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::kLdsBytes, st, p, xr, part);
+      hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::Tile::kLdsBytes, st, p, xr, part);
       hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
       if (taken == 1) {
         products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f}, nullptr);
@@ -722,7 +733,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   frexpf(largest_q(a), &x);
   p.qscale = ldexpf(1.0f, 14 - x > 12 ? 12 : 14 - x);
   hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
-  hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::kLdsBytes, st, p, xr, part);
+  hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::Tile::kLdsBytes, st, p, xr, part);
   hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
   char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
   for (int s = 0; s < a.steps; ++s) {
