@@ -46,7 +46,7 @@ struct OrthoPlan {
 };
 
 // Two steps as one product with the long side:
-//   X'' = P_1 P_0 X,  P_s = a I + b A_s + c A_s^2,  A_1 = P_0 A_0 P_0,
+//   X'' = P_1 P_0 X,  P_s = a I + B_s,  B_s = b A_s + c A_s^2,  A_1 = P_0 A_0 P_0,
 // five m x m products more and one pass over X and one X X^T less.  Errors of A_0 pass
 // through one step more, 1.3 to 1.9 times the iteration's error in simulations; where
 // the sums over n are long that is still below what plain fp32 products give (8 x
@@ -332,13 +332,13 @@ __device__ __forceinline__ size_t quad_at(int row, int k, int KB) {
   return ((size_t)(row >> 5) * KB + (k >> 4)) * NP * kPlaneBytes + ((row & 31) + 32 * ((k >> 3) & 1)) * 16 + (k & 4) * 2;
 }
 
-// One product of m x m matrices: out = alpha L R^T + beta R + gamma I in planes (out2
-// the same times `two`).  All of them are symmetric, polynomials in one matrix, so
+// One product of m x m matrices: out = alpha L R^T + beta R + delta L + gamma I in planes
+// (out2 the same times `two`).  All of them are symmetric, polynomials in one matrix, so
 // the product's rows are stored as the operand's k.
 struct MmJob {
   const char *l, *r;
   char *out, *out2;
-  float alpha, beta, gamma, two;
+  float alpha, beta, delta, gamma, two;
 };
 struct MmJobs { MmJob j[2]; };
 
@@ -393,6 +393,11 @@ __global__ __launch_bounds__(256 * kMmGroups) void k_ortho_mm(OrthoPlan p, MmJob
       const f16x4_t h = *(const f16x4_t*)(j.r + at), l = *(const f16x4_t*)(j.r + at + kPlaneBytes);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = fmaf(j.beta, (float)h[i] + (float)l[i], v[i]);
+    }
+    if (j.delta != 0.0f) {
+      const f16x4_t h = *(const f16x4_t*)(j.l + at), l = *(const f16x4_t*)(j.l + at + kPlaneBytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(j.delta, (float)h[i] + (float)l[i], v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -635,19 +640,19 @@ float largest_q(const OrthoArgs& a) {
   return (float)most;
 }
 
-// The same of the product of two steps' P.
+// The largest |P_1 P_0 - a^2| of two steps in a row.
 float largest_pair(const OrthoArgs& a) {
   double most = 0.0;
   for (int i = 0; i <= 1024; ++i) {
     double x = i / 1024.0, before = 1.0;
     for (int s = 0; s < a.steps; ++s) {
       const double f = a.a + a.b * x * x + a.c * x * x * x * x;
-      if (s) most = fmax(most, fabs(before * f));
+      if (s) most = fmax(most, fabs(before * f - (double)a.a * a.a));
       before = f;
       x *= f;
     }
   }
-  return (float)fmax(most, (double)a.a * a.a);
+  return (float)most;
 }
 
 }  // namespace
@@ -698,7 +703,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   };
   if (!p.bf16) {
     hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
-    const bool two = pairs(p.m, p.n) && largest_pair(a) < 30.0f;  // its planes at 2^11 hold 32
+    const bool two = pairs(p.m, p.n) && largest_pair(a) < 31.0f;  // its planes at 2^11 hold 31.98
     constexpr float kS2 = 2048.0f;
     char* x = xc[0];
     char* xn = xc[1];
@@ -707,17 +712,16 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
       hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::Tile::kLdsBytes, st, p, xr, part);
       hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
       if (taken == 1) {
-        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f}, nullptr);
+        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);
       } else {
-        const MmJob poly{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, a.a * kS, 0.0f};
-        products(poly, nullptr);                                                         // P_0
-        products(MmJob{mm[1], mm[0], mm[2], nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);  // P_0 A_0
-        products(MmJob{mm[2], mm[1], mm[0], nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);  // A_1
-        MmJob second = poly;
-        second.out = mm[3];
-        products(second, nullptr);  // P_1
-        // P_1 P_0 - a^2 I: X itself enters with a^2 in fp32
-        products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, 0.0f, -a.a * a.a * kS2, 0.0f}, nullptr);
+        // B_s = b A_s + c A_s^2 = P_s - a I: the identity stays out of the planes
+        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);  // B_0
+        products(MmJob{mm[1], mm[0], mm[2], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // P_0 A_0 = a A_0 + B_0 A_0
+        products(MmJob{mm[1], mm[2], mm[0], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // A_1 = P_0 (A_0 P_0)
+        products(MmJob{mm[0], mm[0], mm[3], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);  // B_1
+        // P_1 P_0 - a^2 I = B_1 B_0 + a (B_0 + B_1); X itself enters with a^2 in fp32
+        products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, a.a * kS2 * kInvS, a.a * kS2 * kInvS, 0.0f, 0.0f},
+                 nullptr);
       }
       s += taken;
       hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), block, kUpdateLds, st, a, p, mm[taken == 1 ? 1 : 4], x, xn, xr,
@@ -738,8 +742,8 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
   for (int s = 0; s < a.steps; ++s) {
     const bool last = s == a.steps - 1;
-    products(MmJob{A, A, P, s == 0 ? Q : nullptr, a.c * kInvS, a.b, a.a * kS, p.qscale * kInvS}, nullptr);
-    const MmJob pa{P, A, W, nullptr, kInvS, 0.0f, 0.0f, 0.0f}, qp{Q, P, Qn, nullptr, kInvS, 0.0f, 0.0f, 0.0f};
+    products(MmJob{A, A, P, s == 0 ? Q : nullptr, a.c * kInvS, a.b, 0.0f, a.a * kS, p.qscale * kInvS}, nullptr);
+    const MmJob pa{P, A, W, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, qp{Q, P, Qn, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f};
     if (s == 0) {
       if (!last) products(pa, nullptr);
     } else {
@@ -748,7 +752,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
       Q = Qn;
       Qn = q;
     }
-    if (!last) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f}, nullptr);
+    if (!last) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, nullptr);
   }
   hipLaunchKernelGGL(k_ortho_apply, dim3(a.batch * T * TN), block, kApplyLds, st, a, p, Q, xc[0], rest);
 }
