@@ -135,7 +135,7 @@ void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st);
 void launch_experts_stream(const ExpertsArgs& a, hipStream_t st);
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st);
 
-size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16);
+size_t ortho_workspace_bytes(const OrthoArgs& a);
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st);
 // Matrices whose smaller side is at most 64 (ckan_ortho_small.hip).
 inline bool ortho_small(int rows, int cols) { return (rows < cols ? rows : cols) <= 64; }

@@ -171,7 +171,7 @@ OrthoArgs ortho_args(const ckan_ortho_desc* d) {
 }
 
 int ortho_ws(const ckan_ortho_desc* d, void* ws, size_t ws_bytes) {
-  const size_t need = ortho_workspace_bytes(d->batch, d->rows, d->cols, d->dtype == CKAN_DTYPE_BF16);
+  const size_t need = ortho_workspace_bytes(ortho_args(d));
   if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", ws_bytes, need);
   if (!ws || !is_al16(ws)) return fail(CKAN_ERR_INVALID_ARG, "workspace is NULL or not 16-byte aligned");
   return CKAN_OK;
@@ -251,7 +251,7 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
 }
 
 size_t ckan_orthogonalize_workspace_bytes(const ckan_ortho_desc* desc) {
-  return ortho_check(desc) ? 0 : ortho_workspace_bytes(desc->batch, desc->rows, desc->cols, desc->dtype == CKAN_DTYPE_BF16);
+  return ortho_check(desc) ? 0 : ortho_workspace_bytes(ortho_args(desc));
 }
 
 int ckan_orthogonalize(const ckan_ortho_desc* desc, const void* in, void* out, void* ws, size_t ws_bytes,

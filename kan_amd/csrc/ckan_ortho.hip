@@ -14,13 +14,15 @@
 // twice, as the operand with rows m and k = n (Xr, for A = X X^T) and as the one
 // with rows n and k = m (Xc, for the product with X).
 //
-// bf16 matrices take it in the m x m domain.  Every factor is a polynomial in A_0:
-//   P_s = a I + b A_s + c A_s^2,   A_{s+1} = P_s A_s P_s,   Q = P_4 P_3 P_2 P_1 P_0,
-// and the result is Q X0: two products with the long side instead of fifteen, and X0,
-// scaled by a power of two, is exact in one plane.  Errors of A count more this way,
-// those of small singular values by 3.4^2 a step (up to 1.5e-4 of the result for a
-// spectrum over four decades, 1e-5 for a gradient's), which bf16's 2e-3 hides and
-// fp32's 1e-6 would not.
+// bf16 matrices begin in the m x m domain.  Every factor is a polynomial in A_0:
+//   P_s = a I + b A_s + c A_s^2,   A_{s+1} = P_s A_s P_s,   Q = P_{r-1} .. P_1 P_0,
+// and Q X0 are r steps in one: two products with the long side instead of 3 r, and X0,
+// scaled by a power of two, is exact in one plane.  But A is not made from X again
+// between them: what A_0 has as noise in the directions of small singular values grows by
+// a^2 = 11.9 a step (by a in the iteration itself), so only as many steps are taken this
+// way as keep it below bf16's own rounding (product_run() below: 3 of 5), and the rest
+// as fp32 matrices do.  All five in one product left a matrix of rank one 1.9e-2 off, more
+// of them anything.
 #include "ckan_ortho.hpp"
 #include "ckan_planes.hpp"
 
@@ -35,12 +37,12 @@ constexpr int kTile = 128;
 struct OrthoPlan {
   int batch, m, n;
   bool tall;           // rows > cols: m runs along the columns
-  bool bf16;
-  int np;              // planes of X
+  int run;             // steps at first in the m x m domain, of X0 in one plane
+  int np;              // planes that X's buffers have room for
   int mk, n32;         // k extents: m in whole stages of the m x m products, n in 32
   int m128, n128;      // row extents
   int splits, kb_per_split;
-  float qscale;        // bf16: the scale of Q's planes
+  float qscale;        // the scale of Q's planes
   size_t norm_off, xr_off, xc_off[2], part_off, mm_off[5], bytes;
   size_t xr_bytes, xc_bytes, a_bytes, part_elems;  // a matrix
 };
@@ -54,11 +56,44 @@ struct OrthoPlan {
 // multiply-adds is 11 m^3 more for 12 m^3 less.
 bool pairs(int m, int n) { return n >= 4 * (int64_t)m && n >= 2048; }
 
-OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
+// How many steps a bf16 matrix takes in the m x m domain: all of them, or the most (three
+// at least) that leave the result's error below 2^-9, half of a rounding to bf16 at its
+// largest.  A_0's noise is 2^-20 of it (rank one, 1024 x 4608: 1.8e-2 after five steps,
+// 2^-20 11.9^4); a step in the m x m domain takes an error of A by the slope of y p(y)^2,
+// each later one that of X by the slope of x p(x^2).  0: the iteration on two planes.
+int product_run(const OrthoArgs& a) {
+  constexpr int kSamples = 64;
+  if (!a.bf16) return 0;
+  double worst[101] = {};  // of a run of r steps
+  for (int i = 0; i <= kSamples; ++i) {
+    double x = (double)i / kSamples, in_a[101], in_x[101], prefix = 1.0, suffix = 1.0;
+    for (int s = 0; s < a.steps; ++s) {
+      const double y = x * x, p = a.a + a.b * y + a.c * y * y, slope = p + 2.0 * y * (a.b + 2.0 * a.c * y);
+      in_a[s] = fmax(fabs(p * slope), p * p);
+      in_x[s] = fmax(fabs(slope), fabs(p));
+      x *= p;
+    }
+    double after[101];
+    for (int s = a.steps; s >= 0; --s) {
+      after[s] = suffix;
+      if (s > 0) suffix = fmin(suffix * in_x[s - 1], 1e100);
+    }
+    for (int r = 1; r <= a.steps; ++r) {
+      if (r > 1) prefix = fmin(prefix * in_a[r - 2], 1e100);
+      worst[r] = fmax(worst[r], prefix * after[r]);
+    }
+  }
+  for (int r = a.steps; r > 0; r = r > 3 ? r - 1 : 0)
+    if (worst[r] <= 2048.0) return r;
+  return 0;
+}
+
+OrthoPlan make_ortho_plan(const OrthoArgs& a) {
+  const int batch = a.batch, rows = a.rows, cols = a.cols;
   OrthoPlan p{};
   p.batch = batch;
-  p.bf16 = bf16;
-  p.np = bf16 ? 1 : 2;
+  p.run = product_run(a);
+  p.np = p.run > 0 && p.run == a.steps ? 1 : 2;
   p.tall = rows > cols;
   p.m = p.tall ? cols : rows;
   p.n = p.tall ? rows : cols;
@@ -90,9 +125,9 @@ OrthoPlan make_ortho_plan(int batch, int rows, int cols, bool bf16) {
   p.norm_off = take((size_t)batch * (kNormBlocks + 1) * sizeof(double));
   p.xr_off = take(p.xr_bytes * batch);
   p.xc_off[0] = take(p.xc_bytes * batch);
-  p.xc_off[1] = bf16 ? 0 : take(p.xc_bytes * batch);
+  p.xc_off[1] = p.np == 1 ? 0 : take(p.xc_bytes * batch);
   p.part_off = take(p.part_elems * batch * p.splits * sizeof(float));
-  for (int i = 0; i < (bf16 || pairs(p.m, p.n) ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
+  for (int i = 0; i < (p.run > 0 || pairs(p.m, p.n) ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
   p.bytes = off;
   return p;
 }
@@ -252,7 +287,6 @@ template <int NP> struct GramTile {
   static constexpr int kSums = NP == 1 ? 1 : 3;
   typedef NtTile<NP, NP, 2, 2, 2, 2, 2, NP == 1 ? 4 : 2, kSums> Tile;
 };
-typedef NtTile<2, 2, 2, 2, 2, 2, 2, 2> Tile22;
 
 // Partial sums of A = X X^T (scale kS^2): the tiles on and below the diagonal,
 // each stored with its mirror image, k split over blocks.
@@ -296,14 +330,15 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
     }
 }
 
-// A in planes from the partial sums: a thread a row and 8 k.
+// A in planes from the partial sums: a thread a row and 8 k.  rest: X is X0 / rest of
+// one plane.
 __global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, const double* rest, char* A) {
   const int b = blockIdx.y;
   const int k8s = p.mk / 8;
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (q >= (int64_t)p.m128 * k8s) return;
   const int k8 = (int)(q % k8s), row = (int)(q / k8s);
-  const float f = p.bf16 ? (float)(rest[b] * rest[b]) * kInvS : kInvS;
+  const float f = rest ? (float)(rest[b] * rest[b]) * kInvS : kInvS;
   float v[8] = {};
   if (row < p.m) {
 #pragma unroll 4
@@ -498,22 +533,31 @@ constexpr int kPutLds = kTile * kPutPitch * 4;
 // X' = ax X + inv B X.  The product's rows are m, its columns n: an accumulator quad is 4
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
 // through LDS.  The last step writes the result instead (or Muon's parameters).
-// 8 x [512, 4608]: 100 us for 300 MB of X read and written and 58 GFLOP of plane
-// products, 1152 blocks in 512 places; without its copies 85, without its products 95.
+// On one plane (NB = 1) X is X0 / rest and B the whole factor Q of the run's steps.
+// 8 x [512, 4608]: 125 us for 300 MB of X read and written and 58 GFLOP of plane
+// products, 1152 blocks in 512 places; 1024 x 9216 on one plane, the result stored: 58 us,
+// 670 TFLOP/s on its two products.
+template <int NB> struct UpdateTile {
+  typedef NtTile<2, NB, 2, 2, 2, 2, 2, NB == 1 ? 3 : 2> Tile;  // 72 or 64 KiB of LDS
+  static constexpr int kLds = Tile::kLdsBytes > kPutLds ? Tile::kLdsBytes : kPutLds;
+};
+template <int NB>
 __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan p, const char* B, const char* xc,
-                                                         char* xc_new, char* xr, float ax, float inv, int last) {
+                                                         char* xc_new, char* xr, float ax, float inv, const double* rest,
+                                                         int last) {
   extern __shared__ char lds[];
+  typedef typename UpdateTile<NB>::Tile Tile;
   const int TM = p.m128 / kTile, TN = p.n128 / kTile;
   int id = blockIdx.x;
   const int tm = id % TM;
   id /= TM;
   const int tn = id % TN, b = id / TN;
   const int KB = p.mk / 16;
-  const size_t pitch = (size_t)KB * 2 * kPlaneBytes;
+  const size_t pb = (size_t)KB * 2 * kPlaneBytes, px = (size_t)KB * NB * kPlaneBytes;
   const char* x = xc + b * p.xc_bytes;
   f32x16_t acc[2][2] = {};
-  Tile22::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pitch, pitch}, RowBlocks{x + tn * 4 * pitch, pitch}, 0,
-              KB / Tile22::kStageBlocks, lds, acc);
+  Tile::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pb, pb}, RowBlocks{x + tn * 4 * px, px}, 0, KB / Tile::kStageBlocks, lds, acc);
+  if constexpr (NB == 1) inv *= (float)rest[b];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
 #pragma unroll
@@ -527,7 +571,11 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
         const int r = r0 + 8 * q + 4 * g, k = tm * kTile + r;
         float v[4] = {};
         const size_t at = quad_at<2>(col, k, KB);
-        if (k < p.mk) {
+        if constexpr (NB == 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (k + j < p.m && col < p.n) v[j] = acc[m][n][q * 4 + j] * inv;
+        } else if (k < p.mk) {
           const f16x4_t h = *(const f16x4_t*)(x + at), l = *(const f16x4_t*)(x + at + kPlaneBytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -581,40 +629,6 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   }
 }
 
-constexpr int kUpdateLds = Tile22::kLdsBytes > kPutLds ? Tile22::kLdsBytes : kPutLds;
-
-// The bf16 result Q X0: Q in two planes (scale qscale), X0 / rest in one.  1024 x 9216:
-// 58 us, 670 TFLOP/s on its two products.
-typedef NtTile<2, 1, 2, 2, 2, 2, 2, 3> ApplyTile;  // 72 KiB of LDS
-__global__ __launch_bounds__(256, 2) void k_ortho_apply(OrthoArgs a, OrthoPlan p, const char* Q, const char* xc,
-                                                        const double* rest) {
-  extern __shared__ char lds[];
-  const int TM = p.m128 / kTile, TN = p.n128 / kTile;
-  int id = blockIdx.x;
-  const int tm = id % TM;
-  id /= TM;
-  const int tn = id % TN, b = id / TN;
-  const int KB = p.mk / 16;
-  const size_t pq = (size_t)KB * 2 * kPlaneBytes, px = (size_t)KB * kPlaneBytes;
-  f32x16_t acc[2][2] = {};
-  ApplyTile::run(RowBlocks{Q + b * p.a_bytes + tm * 4 * pq, pq}, RowBlocks{xc + b * p.xc_bytes + tn * 4 * px, px}, 0,
-                 KB / ApplyTile::kStageBlocks, lds, acc);
-  const float f = (float)rest[b] * kInvS / p.qscale;
-  const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int q = 0; q < 16; ++q)
-        ((float*)lds)[tile_at(along_m, gathered, (wave >> 1) * 64 + m * 32 + acc_row(q, g),
-                              (wave & 1) * 64 + n * 32 + (lane & 31))] = acc[m][n][q] * f;
-  __syncthreads();
-  put_tile(a, p, (const float*)lds, b, tm * kTile, tn * kTile);
-}
-constexpr int kApplyLds = ApplyTile::kLdsBytes > kPutLds ? ApplyTile::kLdsBytes : kPutLds;
-
 // steps == 0: the normalised matrix itself.
 __global__ __launch_bounds__(256) void k_ortho_scale(OrthoArgs a, const double* part) {
   __shared__ double red[256];
@@ -625,12 +639,12 @@ __global__ __launch_bounds__(256) void k_ortho_scale(OrthoArgs a, const double* 
     put(a, b * a.view.sb + e, entry(a, b * a.view.sb + e) / f);
 }
 
-// The largest value of Q that singular values in [0, 1] give, by sampling.
-float largest_q(const OrthoArgs& a) {
+// The largest value of Q that singular values in [0, 1] give in a run of steps, by sampling.
+float largest_q(const OrthoArgs& a, int run) {
   double most = 0.0;
   for (int i = 0; i <= 1024; ++i) {
     double x = i / 1024.0, q = 1.0;
-    for (int s = 0; s < a.steps; ++s) {
+    for (int s = 0; s < run; ++s) {
       const double f = a.a + a.b * x * x + a.c * x * x * x * x;
       q *= f;
       x *= f;
@@ -657,9 +671,9 @@ float largest_pair(const OrthoArgs& a) {
 
 }  // namespace
 
-size_t ortho_workspace_bytes(int batch, int rows, int cols, bool bf16) {
-  if (ortho_small(rows, cols)) return ortho_small_workspace_bytes(batch, rows, cols);
-  return make_ortho_plan(batch, rows, cols, bf16).bytes;
+size_t ortho_workspace_bytes(const OrthoArgs& a) {
+  if (ortho_small(a.rows, a.cols)) return ortho_small_workspace_bytes(a.batch, a.rows, a.cols);
+  return make_ortho_plan(a).bytes;
 }
 
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
@@ -667,7 +681,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
     launch_ortho_small(a, ws, st);
     return;
   }
-  OrthoPlan p = make_ortho_plan(a.batch, a.rows, a.cols, a.bf16 != 0);
+  OrthoPlan p = make_ortho_plan(a);
   char* w = (char*)ws;
   double *norm = (double*)(w + p.norm_off), *rest = norm + (size_t)a.batch * kNormBlocks;
   char* xr = w + p.xr_off;
@@ -679,8 +693,8 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   ensure_lds_limit((const void*)k_ortho_gram<1>, GramTile<1>::Tile::kLdsBytes, done[0]);
   ensure_lds_limit((const void*)k_ortho_gram<2>, GramTile<2>::Tile::kLdsBytes, done[1]);
   ensure_lds_limit((const void*)k_ortho_mm, MmTile::kLdsBytes, done[2]);
-  ensure_lds_limit((const void*)k_ortho_update, kUpdateLds, done[3]);
-  ensure_lds_limit((const void*)k_ortho_apply, kApplyLds, done[4]);
+  ensure_lds_limit((const void*)k_ortho_update<1>, UpdateTile<1>::kLds, done[3]);
+  ensure_lds_limit((const void*)k_ortho_update<2>, UpdateTile<2>::kLds, done[4]);
   const dim3 norm_grid(kNormBlocks, a.batch);
   if (!a.in)
     hipLaunchKernelGGL(k_ortho_norm<kNormMuon>, norm_grid, dim3(256), 0, st, a, norm);
@@ -701,60 +715,65 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
     hipLaunchKernelGGL(k_ortho_mm, dim3(a.batch * T64 * T64, two ? 2 : 1), dim3(256 * kMmGroups), MmTile::kLdsBytes, st, p,
                        jobs);
   };
-  if (!p.bf16) {
-    hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
-    const bool two = pairs(p.m, p.n) && largest_pair(a) < 31.0f;  // its planes at 2^11 hold 31.98
-    constexpr float kS2 = 2048.0f;
-    char* x = xc[0];
-    char* xn = xc[1];
-    for (int s = 0; s < a.steps;) {
-      const int taken = two && s + 1 < a.steps ? 2 : 1;
-      hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::Tile::kLdsBytes, st, p, xr, part);
-      hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
-      if (taken == 1) {
-        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);
+  const dim3 update_grid(a.batch * T * TN);
+  char* x = xc[0];
+  char* xn = xc[1];
+  int s = p.run;
+  if (p.run == 0) {
+    hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, x);
+  } else {
+    int exponent;  // |Q| below 2^14 in its planes
+    frexpf(largest_q(a, p.run), &exponent);
+    p.qscale = ldexpf(1.0f, 14 - exponent > 12 ? 12 : 14 - exponent);
+    hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, xr, x);
+    hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::Tile::kLdsBytes, st, p, xr, part);
+    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
+    char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
+    for (int i = 0; i < p.run; ++i) {
+      const bool more = i + 1 < p.run;
+      products(MmJob{A, A, P, i == 0 ? Q : nullptr, a.c * kInvS, a.b, 0.0f, a.a * kS, p.qscale * kInvS}, nullptr);
+      const MmJob pa{P, A, W, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, qp{Q, P, Qn, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f};
+      if (i == 0) {
+        if (more) products(pa, nullptr);
       } else {
-        // B_s = b A_s + c A_s^2 = P_s - a I: the identity stays out of the planes
-        products(MmJob{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);  // B_0
-        products(MmJob{mm[1], mm[0], mm[2], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // P_0 A_0 = a A_0 + B_0 A_0
-        products(MmJob{mm[1], mm[2], mm[0], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // A_1 = P_0 (A_0 P_0)
-        products(MmJob{mm[0], mm[0], mm[3], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f}, nullptr);  // B_1
-        // P_1 P_0 - a^2 I = B_1 B_0 + a (B_0 + B_1); X itself enters with a^2 in fp32
-        products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, a.a * kS2 * kInvS, a.a * kS2 * kInvS, 0.0f, 0.0f},
-                 nullptr);
+        products(qp, more ? &pa : nullptr);
+        char* q = Q;
+        Q = Qn;
+        Qn = q;
       }
-      s += taken;
-      hipLaunchKernelGGL(k_ortho_update, dim3(a.batch * T * TN), block, kUpdateLds, st, a, p, mm[taken == 1 ? 1 : 4], x, xn, xr,
-                         taken == 1 ? a.a : a.a * a.a, taken == 1 ? kInvS : 1.0f / kS2, s == a.steps);
-      char* o = x;
-      x = xn;
-      xn = o;
+      if (more) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, nullptr);
     }
-    return;
+    hipLaunchKernelGGL(k_ortho_update<1>, update_grid, block, UpdateTile<1>::kLds, st, a, p, Q, x, xn, xr, 0.0f,
+                       1.0f / p.qscale, rest, s == a.steps);
+    x = xc[1];
+    xn = xc[0];
   }
-  // |Q| below 2^14 in its planes
-  int x;
-  frexpf(largest_q(a), &x);
-  p.qscale = ldexpf(1.0f, 14 - x > 12 ? 12 : 14 - x);
-  hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, xr, xc[0]);
-  hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::Tile::kLdsBytes, st, p, xr, part);
-  hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
-  char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
-  for (int s = 0; s < a.steps; ++s) {
-    const bool last = s == a.steps - 1;
-    products(MmJob{A, A, P, s == 0 ? Q : nullptr, a.c * kInvS, a.b, 0.0f, a.a * kS, p.qscale * kInvS}, nullptr);
-    const MmJob pa{P, A, W, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, qp{Q, P, Qn, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (s == 0) {
-      if (!last) products(pa, nullptr);
-    } else {
-      products(qp, last ? nullptr : &pa);
-      char* q = Q;
-      Q = Qn;
-      Qn = q;
+  const bool two = pairs(p.m, p.n) && largest_pair(a) < 31.0f;  // its planes at 2^11 hold 31.98
+  constexpr float kS2 = 2048.0f;
+  while (s < a.steps) {
+    const int taken = two && s + 1 < a.steps ? 2 : 1;
+    hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::Tile::kLdsBytes, st, p, xr, part);
+    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, nullptr, mm[0]);
+    // B_s = b A_s + c A_s^2 = P_s - a I: the identity stays out of the planes
+    const MmJob poly{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f};
+    products(poly, nullptr);  // B_0
+    if (taken == 2) {
+      products(MmJob{mm[1], mm[0], mm[2], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // P_0 A_0 = a A_0 + B_0 A_0
+      products(MmJob{mm[1], mm[2], mm[0], nullptr, kInvS, a.a, 0.0f, 0.0f, 0.0f}, nullptr);  // A_1 = P_0 (A_0 P_0)
+      MmJob second = poly;
+      second.out = mm[3];
+      products(second, nullptr);  // B_1
+      // P_1 P_0 - a^2 I = B_1 B_0 + a (B_0 + B_1); X itself enters with a^2 in fp32
+      products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, a.a * kS2 * kInvS, a.a * kS2 * kInvS, 0.0f, 0.0f},
+               nullptr);
     }
-    if (!last) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, nullptr);
+    s += taken;
+    hipLaunchKernelGGL(k_ortho_update<2>, update_grid, block, UpdateTile<2>::kLds, st, a, p, mm[taken == 1 ? 1 : 4], x, xn, xr,
+                       taken == 1 ? a.a : a.a * a.a, taken == 1 ? kInvS : 1.0f / kS2, rest, s == a.steps);
+    char* o = x;
+    x = xn;
+    xn = o;
   }
-  hipLaunchKernelGGL(k_ortho_apply, dim3(a.batch * T * TN), block, kApplyLds, st, a, p, Q, xc[0], rest);
 }
 
 }  // namespace ckan

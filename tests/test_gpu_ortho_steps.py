@@ -70,7 +70,7 @@ def _check(got, g, steps, extra=0.0, **kw):
     want = _definition(g.double().numpy(), steps, **kw)
     v = got.double().cpu().numpy()
     assert np.isfinite(v).all()
-    assert np.linalg.norm(v - want) <= (_bound(g.double().numpy(), steps) + extra) * np.linalg.norm(want)
+    assert np.linalg.norm(v - want) <= (_bound(g.double().numpy(), steps, **kw) + extra) * np.linalg.norm(want)
 
 
 def _equal_rows(got, kind, rows):
@@ -98,3 +98,49 @@ def test_two_steps_a_pass(rows, cols, kind, steps):
     if kind != "full":
         _equal_rows(got, kind, rows)
     _check(got, g, steps)
+
+
+BF16_EXTRA = 2.0 ** -8 + 2.0 ** -9
+
+
+@pytest.mark.parametrize("steps", [2, 3, 4, 5, 6, 7, 8, 10, 12, 20, 24, 30])
+@pytest.mark.parametrize("kind", ["full", "low rank", "rank one", "equal halves", "equal pairs", "four decades"])
+@pytest.mark.parametrize("rows,cols", [(130, 300), (200, 2100)])
+def test_bf16_steps(rows, cols, kind, steps):
+    g = _matrix(kind, rows, cols, rows + steps).bfloat16()
+    _check(kan_amd.functional.orthogonalize(g.cuda(), steps=steps), g, steps, BF16_EXTRA)
+
+
+@pytest.mark.parametrize("steps", [1, 5, 9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_batches_and_layouts_of_large_sides(dtype, steps):
+    """Several matrices of scales far apart, one of them zero, row-major, transposed and tall: the same bits."""
+    kinds = ["full", "rank one", "equal halves", "four decades"]
+    g = torch.stack([_matrix(k, 96, 200, 7) * 10.0 ** (2 * i - 3) for i, k in enumerate(kinds)] + [torch.zeros(96, 200)]).to(dtype)
+    base = kan_amd.functional.orthogonalize(g.cuda(), steps=steps)
+    for i in range(4):
+        _check(base[i], g[i], steps, BF16_EXTRA if dtype == torch.bfloat16 else 0.0)
+    assert (base[4] == 0).all()
+    turned = g.cuda().transpose(1, 2).contiguous()
+    assert torch.equal(kan_amd.functional.orthogonalize(turned.transpose(1, 2), steps=steps), base)
+    assert torch.equal(kan_amd.functional.orthogonalize(turned, steps=steps).transpose(1, 2), base)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steps", [9, 14])
+def test_other_coefficients(dtype, steps):
+    """The cubic iteration, whose m x m form holds for more steps, and two quintics of other slopes."""
+    for co in ((1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.3465, -1.0598, -0.2868)):
+        for kind in ("full", "rank one"):
+            g = _matrix(kind, 100, 260, steps).to(dtype)
+            got = kan_amd.functional.orthogonalize(g.cuda(), steps=steps, coefficients=co)
+            _check(got, g, steps, BF16_EXTRA if dtype == torch.bfloat16 else 0.0, coefficients=co)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_stays_in_its_matrix(dtype):
+    g = torch.stack([_matrix("full", 90, 300, s) for s in (1, 2)]).to(dtype)
+    alone = kan_amd.functional.orthogonalize(g[1:].cuda())
+    g[0, 4, 4] = float("nan")
+    both = kan_amd.functional.orthogonalize(g.cuda())
+    assert torch.isnan(both[0]).all() and torch.equal(both[1:], alone)
