@@ -139,7 +139,7 @@ size_t ortho_workspace_bytes(const OrthoArgs& a);
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st);
 // Matrices whose smaller side is at most 64 (ckan_ortho_small.hip).
 inline bool ortho_small(int rows, int cols) { return (rows < cols ? rows : cols) <= 64; }
-size_t ortho_small_workspace_bytes(int batch, int rows, int cols);
+size_t ortho_small_workspace_bytes(const OrthoArgs& a);
 void launch_ortho_small(const OrthoArgs& a, void* ws, hipStream_t st);
 
 }  // namespace ckan

@@ -672,7 +672,7 @@ float largest_pair(const OrthoArgs& a) {
 }  // namespace
 
 size_t ortho_workspace_bytes(const OrthoArgs& a) {
-  if (ortho_small(a.rows, a.cols)) return ortho_small_workspace_bytes(a.batch, a.rows, a.cols);
+  if (ortho_small(a.rows, a.cols)) return ortho_small_workspace_bytes(a);
   return make_ortho_plan(a).bytes;
 }
 

@@ -144,3 +144,37 @@ def test_nan_stays_in_its_matrix(dtype):
     g[0, 4, 4] = float("nan")
     both = kan_amd.functional.orthogonalize(g.cuda())
     assert torch.isnan(both[0]).all() and torch.equal(both[1:], alone)
+
+
+@pytest.mark.parametrize("steps", [0, 1, 7, 9, 10, 12, 18, 20, 30])
+@pytest.mark.parametrize("kind", ["full", "low rank", "equal halves", "equal pairs", "four decades"])
+@pytest.mark.parametrize("rows,cols", [(64, 512), (33, 900), (40, 41)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_small_side_steps(rows, cols, kind, steps, dtype):
+    """A side of at most 64; the iterate goes on in a run of its own from ten steps of the quintic on."""
+    g = _matrix(kind, rows, cols, rows + steps).to(dtype)
+    got = kan_amd.functional.orthogonalize(g.cuda(), steps=steps)
+    if kind.startswith("equal") and steps >= 10:
+        _equal_rows(got, kind, rows)
+    _check(got, g, steps, 1e-6 + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0))
+
+
+@pytest.mark.parametrize("steps", [5, 13])
+def test_small_side_batches_and_layouts(steps):
+    kinds = ["full", "equal halves", "four decades", "full"]
+    g = torch.stack([_matrix(k, 50, 130, 3) * 10.0 ** (3 * i - 4) for i, k in enumerate(kinds)] + [torch.zeros(50, 130)])
+    g[3, 2, 2] = float("nan")
+    base = kan_amd.functional.orthogonalize(g.cuda(), steps=steps)
+    for i in range(3):
+        _check(base[i], g[i], steps, 1e-6)
+    assert torch.isnan(base[3]).all() and (base[4] == 0).all()
+    turned = g.cuda().transpose(1, 2).contiguous()
+    for got in (kan_amd.functional.orthogonalize(turned.transpose(1, 2), steps=steps),
+                kan_amd.functional.orthogonalize(turned, steps=steps).transpose(1, 2)):
+        assert torch.equal(got.nan_to_num(0.5), base.nan_to_num(0.5))
+
+
+def test_small_side_other_coefficients():
+    for co, steps in (((1.5, -0.5, 0.0), 40), ((1.875, -1.25, 0.375), 25), ((2.3465, -1.0598, -0.2868), 16)):
+        g = _matrix("full", 48, 300, steps)
+        _check(kan_amd.functional.orthogonalize(g.cuda(), steps=steps, coefficients=co), g, steps, 1e-6, coefficients=co)
