@@ -360,9 +360,11 @@ int ckan_route_backward(const ckan_route_desc* desc, const void* logits, const i
  * lies outside [0, experts) has no expert: it adds nothing and its weight's
  * gradient is 0.  A row may name an expert twice.
  * fp32 tensors are computed on two fp16 planes an operand (22 bits), bf16 ones on
- * one (11 bits); sums, tanh and the basis recurrence are in fp32.  The planes are
- * scaled by the largest coefficient of an expert (and the largest gradient of its
- * rows): values down to 2^-13 of it keep 22 bits, smaller ones an error of 2^-35 of it.
+ * one (11 bits); sums, tanh and the basis recurrence are in fp32.  The planes are scaled
+ * by powers of two.  Coefficients by the largest of their expert: down to 2^-13 of it
+ * they keep 22 bits, smaller ones an error of 2^-35 of it.  Gradients w dy by the largest
+ * of their row for dx, and by the largest of the expert's rows for dcoeffs, where rows
+ * are summed (down to 2^-16 of it 22 bits, smaller ones an error of 2^-38 of it).
  * `saved` (ckan_experts_saved_bytes) carries the sorted slots, tanh values, expert
  * outputs and packed coefficients from the forward to its backward; NULL where no
  * backward follows.  Buffers need 16-byte alignment. */

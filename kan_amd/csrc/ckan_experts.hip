@@ -6,9 +6,9 @@
 // 32 rows, so one launch a product covers every expert and nothing is read back
 // by the host.  All three products run on fp16 planes (ckan_planes.hpp): one
 // plane for bf16 tensors (the basis values then carry 11 bits, more than a bf16
-// result), two for fp32.  fp16's range is met by one power-of-two scale an
-// expert for the coefficients and one for the upstream gradients; the basis
-// values lie in [-1, 1].
+// result), two for fp32.  fp16's range is met by powers of two: one an expert for the
+// coefficients; for the upstream gradients one a row in dx, where rows stay apart, and
+// one an expert in dC, where they are summed; the basis values lie in [-1, 1].
 //
 //   forward  z[row, o] = sum_k phi[row, k] Cf[o, k]: phi is made in registers from
 //            the row's tanh values, k = (input, degree 1..P); T_0 is a bias.
@@ -78,6 +78,7 @@ ExpertsPlan make_experts_plan(int64_t T, int E, int k, int I, int O, int deg, bo
   off = 0;
   p.gmax_off = take((size_t)(p.R / 32) * 4);
   p.gscale_off = take((size_t)E * 4);
+  p.rscale_off = take((size_t)p.R * 4);
   p.gr_off = take((size_t)p.R * p.Op * 2 * p.NP);
   p.gt_off = take((size_t)p.R * p.Op * 2 * p.NP);
   p.gsum_off = take((size_t)(p.R / 32) * p.Op * 4);
@@ -728,8 +729,8 @@ __global__ __launch_bounds__(256) void k_experts_gather(ExpertsArgs a, const flo
 
 // ---- backward -------------------------------------------------------------------
 
-// dweights of each slot, and the largest |w dy| of each block of 32 rows; 16 waves a
-// block, two rows each.
+// dweights of each slot, the inverse of the scale of each row's w dy, and the largest of each block of 32
+// rows; 16 waves a block, two rows each.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_experts_dweights(ExpertsArgs a) {
   __shared__ float most[16];
@@ -769,8 +770,9 @@ __global__ __launch_bounds__(1024) void k_experts_dweights(ExpertsArgs a) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (s[h] < 0) continue;
-    const float sum = wave_sum(dot[h]);
-    big = fmaxf(big, finite_abs(wave_max(m[h]) * load_weight(a, s[h])));
+    const float sum = wave_sum(dot[h]), most_g = finite_abs(wave_max(m[h]) * load_weight(a, s[h]));
+    if (lane == 0) ((float*)(a.ws + p.rscale_off))[rb * 32 + wave * 2 + h] = 1.0f / range_scale(most_g, 14);
+    big = fmaxf(big, most_g);
     if (lane == 0 && a.dweights) {
       if (p.wbf16)
         ((__bf16*)a.dweights)[s[h]] = (__bf16)sum;
@@ -800,7 +802,8 @@ __device__ __forceinline__ int row_expert(const int* off, int E, int r) {
 }
 
 // g = w dy (scaled) of 32 rows x 64 outputs in both operand forms: rows = slots and
-// k = o for dx, rows = o and k = slots for dC; and the rows' sum for each output.
+// k = o for dx (scaled by the row), rows = o and k = slots for dC (by the expert); and
+// the rows' sum for each output.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
   __shared__ float tile[32][65], red[4];
@@ -839,8 +842,9 @@ __global__ __launch_bounds__(256) void k_experts_gpack(ExpertsArgs a) {
   {  // rows = slots: 32 rows x 8 groups of 8 outputs
     const int r = tid & 31, k8 = tid >> 5, o = o0 + k8 * 8;
     if (o < p.Op) {
+      const float own = slot[rb * 32 + r] >= 0 ? 1.0f / ((const float*)(a.ws + p.rscale_off))[rb * 32 + r] : 1.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = scale * tile[r][k8 * 8 + j];
+      for (int j = 0; j < 8; ++j) v[j] = own * tile[r][k8 * 8 + j];
       const Planes8<NP> f = to_planes8<NP>(v);
       char* d = a.ws + p.gr_off + (((size_t)rb * KBo + (o >> 4)) * NP) * kPlaneBytes + (r + 32 * (k8 & 1)) * 16;
 #pragma unroll
@@ -964,14 +968,20 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) dx[m][q] *= fmaf(-x[m][q], x[m][q], 1.0f);
   const float ic = 1.0f / ((const float*)(a.saved + p.scale_off))[e];
-  const float ig = 1.0f / ((const float*)(a.ws + p.gscale_off))[e];
+  // the rows' scales undone; pad rows, and rows past the expert's, have any: they are not used
+  const float* rinv = (const float*)(a.ws + p.rscale_off) + row0 + (wave >> 1) * 64;
+  asm volatile("" ::: "memory");  // read here, not held in registers through the products
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) dx[m][q] = dx[m][q] * ic * rinv[m * 32 + acc_row(q, g)];
   if (share.parts > 1) {
     float* part = (float*)(a.ws + p.bpart_off) + ((size_t)(blockIdx.x & 7) * kXcdBlocks + share.place) * 128 * 64;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int q = 0; q < 16; ++q)
-        part[((wave >> 1) * 64 + m * 32 + acc_row(q, g)) * 64 + (wave & 1) * 32 + (lane & 31)] = dx[m][q] * ic * ig;
+        part[((wave >> 1) * 64 + m * 32 + acc_row(q, g)) * 64 + (wave & 1) * 32 + (lane & 31)] = dx[m][q];
     return;
   }
   if (i >= p.I) return;
@@ -981,7 +991,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_dx(ExpertsArgs a) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
       const int r = row0 + (wave >> 1) * 64 + m * 32 + acc_row(q, g);
-      if (r < end) out[(size_t)r * p.I + i] = dx[m][q] * ic * ig;
+      if (r < end) out[(size_t)r * p.I + i] = dx[m][q];
     }
 }
 

@@ -110,7 +110,7 @@ struct ExpertsPlan {
   // forward workspace
   size_t hist_off, cmax_off, cf_off, bias_off, fpart_off, fwd_bytes;
   // backward workspace
-  size_t gmax_off, gscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bpart_off, bwd_bytes;
+  size_t gmax_off, gscale_off, rscale_off, gr_off, gt_off, gsum_off, gtot_off, ts_off, dxs_off, bpart_off, bwd_bytes;
   int pack_inputs;     // inputs a block of the pack takes
   int bias_parts;      // input chunks of the pack's sums of T_0 coefficients
   // the streaming forward (few slots): input chunks, inputs a chunk, partial sums

@@ -199,9 +199,11 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
     bf16 (y [rows, out] likewise); ``indices`` [rows, top_k] int64 and ``weights`` [rows,
     top_k] (fp32 or bf16) as ``route`` returns them.  A slot whose index lies outside
     [0, experts) has no expert: a row of such slots gives zeros.  Degrees 1 to 16,
-    up to 512 experts.  fp32 results carry fp32 accuracy (operands of 22 bits, down to
-    2^-13 of the expert's largest coefficient, and an error of 2^-35 of that below), bf16
-    ones are rounded once from fp32 sums of 11-bit basis values.
+    up to 512 experts.  fp32 results carry fp32 accuracy: operands of 22 bits, coefficients
+    down to 2^-13 of their expert's largest (an error of 2^-35 of that below), gradients of
+    any size for x; for the coefficients' gradient those down to 2^-16 of the largest among
+    the expert's rows (an error of 2^-38 of that below).  bf16 results are rounded once from
+    fp32 sums of 11-bit basis values.
 
     Differentiable once in x, coeffs and weights; sums run in a fixed order, so a call
     repeats bit for bit."""
