@@ -13,7 +13,8 @@ import ctypes
 import os
 import threading
 
-import torch  # noqa: F401  (must be loaded before the HIP library)
+import torch  # must be loaded before the HIP library
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libckan_gfx950.so")
 
@@ -294,6 +295,16 @@ def stream_ptr(device: torch.device) -> int:
 
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raises where a tensor carries a forward-mode tangent: the library has no such
+    derivative, and a call that takes no autograd node would drop it."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative; use reverse mode")
 
 
 def profile_enable(on: bool) -> None:

@@ -410,6 +410,7 @@ def chebykan(x: torch.Tensor, coeffs: torch.Tensor, compute: str = "fp32") -> to
     fp64 coefficients select the fp64 path (``compute`` does not apply there)."""
     if coeffs.dtype == torch.float64:
         return ChebyKANFunction64.apply(x, coeffs)
+    _lib.refuse_tangents("chebykan", x, coeffs)
     if not _needs_graph(x, coeffs):  # inference: no autograd node, no tanh cache kept
         return _layer_forward(x, coeffs, compute, None, None, keep_t=False)[0]
     return ChebyKANFunction.apply(x, coeffs, compute, None)
@@ -424,6 +425,7 @@ def family_kan(x: torch.Tensor, coeffs: torch.Tensor, spec, compute: str = "fp32
             raise RuntimeError("kan_amd: a Hermite layer with a finite domain (an affine input map) "
                                "runs in float32 or bfloat16; its fp64 path takes the tanh map only")
         return ChebyKANFunction64.apply(x, coeffs, spec)
+    _lib.refuse_tangents("family_kan", x, coeffs)
     if not _needs_graph(x, coeffs):
         return _layer_forward(x, coeffs, compute, spec, affine, keep_t=False)[0]
     return ChebyKANFunction.apply(x, coeffs, compute, spec, affine)
@@ -515,6 +517,7 @@ def derivatives(x: torch.Tensor, coeffs: torch.Tensor, spec, order: int = 1,
 def jacobian(x: torch.Tensor, coeffs: torch.Tensor, spec, affine=None) -> torch.Tensor:
     """[B, out, in]: d y[b, o] / d x[b, i] (fp32; not differentiable); ``affine``
     as in derivatives."""
+    _lib.refuse_tangents("jacobian", x, coeffs)
     c = _f32_coeffs(coeffs.detach())
     _require_device(x)
     in_dim, out_dim, _ = c.shape

@@ -119,6 +119,7 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
     if logits.dim() != 2:
         raise RuntimeError(f"logits must be [rows, experts], got {tuple(logits.shape)}")
+    _lib.refuse_tangents("route", logits)
     _require_device(logits, bias)
     code = _dtype_code(logits, "logits")
     experts = logits.shape[1]
@@ -207,6 +208,7 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
 
     Differentiable once in x, coeffs and weights; sums run in a fixed order, so a call
     repeats bit for bit."""
+    _lib.refuse_tangents("kan_experts", x, coeffs, weights)
     _require_device(x, coeffs, indices, weights)
     code = _dtype_code(x, "x")
     if coeffs.dtype != x.dtype:

@@ -37,6 +37,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     fp32 products; the result has g's dtype.  Not differentiable."""
     if g.dim() < 2:
         raise RuntimeError(f"g must be [..., rows, cols], got {tuple(g.shape)}")
+    _lib.refuse_tangents("orthogonalize", g)
     if not g.is_cuda:
         raise RuntimeError("kan_amd's orthogonalisation runs only on a ROCm device (MI355X); "
                            f"got a tensor on {g.device}")
