@@ -315,8 +315,9 @@ int ckan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int6
 /* ---- mixture of experts: routing -------------------------------------------- */
 /* Rows of logits choose top_k of `experts` experts each.
  *   s = softmax(l) or sigmoid(l);  key = s + bias (bias may be NULL).
- *   An expert with logit -inf or NaN (or a NaN key) is not eligible: s = 0.  A logit
- *   of +inf counts as the largest finite one.
+ *   An expert with logit -inf or NaN is not eligible: s = 0.  A logit of +inf counts as
+ *   the largest finite one.  One with a key of NaN or -inf (by its bias) is never chosen
+ *   either, but its score stays what it is and counts in a softmax's sum.
  *   groups > 1: the experts are `groups` equal runs; a group's value is the sum of
  *   its two largest keys (a missing or ineligible second counts 0), and only the
  *   top_groups groups of largest value stay.

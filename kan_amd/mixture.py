@@ -110,8 +110,9 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     with ``groups`` > 1 only the ``top_groups`` groups of consecutive experts stay
     whose two largest keys sum highest.  Equal keys go to the lowest index.  The
     weights are the chosen scores, over their sum with ``renormalize``, times
-    ``scale``.  An expert whose logit is -inf or NaN is never chosen (+inf counts as the
-    largest finite logit); a row that has fewer than ``top_k`` others fills up with index -1 and weight 0.
+    ``scale``.  An expert whose logit is -inf or NaN is never chosen and scores 0 (+inf
+    counts as the largest finite logit), one whose bias is -inf or NaN is never chosen and
+    keeps its score; a row that has fewer than ``top_k`` others fills up with index -1 and weight 0.
 
     Differentiable once in ``logits`` (through the weights, not through the choice);
     the indices are not to be changed in place before the backward."""
