@@ -272,9 +272,15 @@ class MixtureKANLayer(nn.Module):
         self.register_buffer("balance_bias", torch.zeros(experts) if balance else None)
         self._last_indices: Optional[torch.Tensor] = None
 
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        if not torch.is_autocast_enabled(x.device.type):
+            return x @ self.gate.t()
+        with torch.autocast(x.device.type, enabled=False):  # the choice is fp32's there too
+            return x @ self.gate.t()
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = x.reshape(-1, self.input_dim).to(torch.float32)
-        weights, indices = route(x @ self.gate.t(), self.top_k, score=self.score, bias=self.balance_bias,
+        weights, indices = route(self._logits(x), self.top_k, score=self.score, bias=self.balance_bias,
                                  groups=self.groups, top_groups=self.top_groups, renormalize=self.renormalize,
                                  scale=self.scale)
         self._last_indices = indices if self.balance_bias is not None else None
