@@ -403,7 +403,8 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
  * Element (r, col) of matrix i lies at i batch_stride + r row_stride +
  * (col / inner) outer_stride + (col % inner) inner_stride elements; inner divides
  * cols, and the strides have to make each matrix dense: row-major, column-major or, with
- * inner > 1, [cols / inner, rows, inner].  An ordinary matrix has inner = 1 and its column stride in outer_stride.  A
+ * inner > 1, [cols / inner, rows, inner].  The matrices of a batch must not overlap.  An
+ * ordinary matrix has inner = 1 and its column stride in outer_stride.  A
  * ChebyKAN layer's coefficients [in, out, D] as [out, in D], the matrix by which
  * the basis values act on the outputs, have inner = D, row_stride = D,
  * outer_stride = out D, inner_stride = 1.  Replaces nothing in the reference, whose

@@ -137,6 +137,9 @@ int ortho_check(const ckan_ortho_desc* d) {
     return fail(CKAN_ERR_INVALID_ARG, "inner must divide cols %d (got %d)", d->cols, d->inner);
   if (d->batch_stride < 0 || d->row_stride < 0 || d->outer_stride < 0 || d->inner_stride < 0)
     return fail(CKAN_ERR_INVALID_ARG, "strides must be >= 0");
+  if (d->batch > 1 && d->batch_stride < (int64_t)d->rows * d->cols)
+    return fail(CKAN_ERR_INVALID_ARG, "batch_stride %lld is below a matrix's %lld elements", (long long)d->batch_stride,
+                (long long)d->rows * d->cols);
   const bool rows_first = d->inner == 1 && d->outer_stride == 1 && d->row_stride == d->cols;
   const bool cols_first = d->inner == 1 && d->row_stride == 1 && d->outer_stride == d->rows;
   const bool coeffs = d->inner > 1 && d->inner_stride == 1 && d->row_stride == d->inner &&
