@@ -176,10 +176,14 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void k_route_backward(RouteArgs
   __builtin_amdgcn_wave_barrier();
   float ds, r = 0.0f;
   if (a.renormalize) {
-    const float total = wave_sum(sj) + kRouteEps;
-    const float mean = wave_sum(dw * sj) / total;
-    ds = a.scale * (dw - mean) / total;
-    r = a.scale * mean * (kRouteEps / total);  // sum s ds, of which total leaves this
+    // ds_j = scale (dw_j - mean) / total, mean = sum w_j dw_j.  From the differences to the
+    // first slot's dw: what all dw of a row share leaves no rounding, and one slot alone,
+    // whose weight is 1, gets 0.  short_of_one = 1 - sum w_j, of which that share is left.
+    const float own = wave_sum(sj), total = own + kRouteEps, short_of_one = total > own ? kRouteEps / total : 0.0f;
+    const float base = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(dw)));
+    const float diff = e >= 0 ? dw - base : 0.0f, mean = wave_sum(diff * sj) / total;
+    ds = a.scale * ((diff - mean) + base * short_of_one) / total;
+    r = a.scale * (mean + base * (1.0f - short_of_one)) * short_of_one;  // sum s ds
   } else {
     ds = a.scale * dw;
     r = wave_sum(sj * ds);
