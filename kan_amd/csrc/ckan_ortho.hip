@@ -49,12 +49,14 @@ struct OrthoPlan {
 
 // Two steps as one product with the long side:
 //   X'' = P_1 P_0 X,  P_s = a I + B_s,  B_s = b A_s + c A_s^2,  A_1 = P_0 A_0 P_0,
-// five m x m products more and one pass over X and one X X^T less.  Errors of A_0 pass
-// through one step more, 1.3 to 1.9 times the iteration's error in simulations; where
-// the sums over n are long that is still below what plain fp32 products give (8 x
-// [512, 4608]: 1.6e-6 step by step, 3.4e-6 plain).  At n = 4 m the trade in
-// multiply-adds is 11 m^3 more for 12 m^3 less.
-bool pairs(int m, int n) { return n >= 4 * (int64_t)m && n >= 2048; }
+// five m x m products more and one pass over X and one X X^T less.  At n = 4 m the trade
+// in multiply-adds is 11 m^3 more for 12 m^3 less: 8 x [512, 4608] 776 us against 997,
+// [256, 2304] 192 against 209.  The errors are 1.2 to 3 times the iteration's (the result is
+// a difference of a^2 X and the rest), 2.1-2.8e-6 of a random matrix whatever its size,
+// where plain fp32 products' grow with their sums: 1.3-1.7e-6 with m = 80 to 192, 2.1e-6
+// with 256, 4.4e-6 with 512.  So fp32 matrices take it from m = 256 on; results in bf16 do
+// not see it.
+bool pairs(int m, int n, bool bf16) { return n >= 4 * (int64_t)m && n >= 2048 && (bf16 || m >= 256); }
 
 // How many steps a bf16 matrix takes in the m x m domain: all of them, or the most (three
 // at least) that leave the result's error below 2^-9, half of a rounding to bf16 at its
@@ -127,7 +129,7 @@ OrthoPlan make_ortho_plan(const OrthoArgs& a) {
   p.xc_off[0] = take(p.xc_bytes * batch);
   p.xc_off[1] = p.np == 1 ? 0 : take(p.xc_bytes * batch);
   p.part_off = take(p.part_elems * batch * p.splits * sizeof(float));
-  for (int i = 0; i < (p.run > 0 || pairs(p.m, p.n) ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
+  for (int i = 0; i < (p.run > 0 || pairs(p.m, p.n, a.bf16 != 0) ? 5 : 2); ++i) p.mm_off[i] = take(p.a_bytes * batch);
   p.bytes = off;
   return p;
 }
@@ -748,7 +750,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
     x = xc[1];
     xn = xc[0];
   }
-  const bool two = pairs(p.m, p.n) && largest_pair(a) < 31.0f;  // its planes at 2^11 hold 31.98
+  const bool two = pairs(p.m, p.n, a.bf16 != 0) && largest_pair(a) < 31.0f;  // its planes at 2^11 hold 31.98
   constexpr float kS2 = 2048.0f;
   while (s < a.steps) {
     const int taken = two && s + 1 < a.steps ? 2 : 1;

@@ -90,9 +90,9 @@ def test_equal_rows_stay_equal(rows, cols, kind, steps):
 
 @pytest.mark.parametrize("steps", [5, 12, 19, 30])
 @pytest.mark.parametrize("kind", ["equal halves", "equal pairs", "full"])
-@pytest.mark.parametrize("rows,cols", [(200, 2048), (510, 2300)])
+@pytest.mark.parametrize("rows,cols", [(200, 2048), (300, 2100), (510, 2300)])
 def test_two_steps_a_pass(rows, cols, kind, steps):
-    """The form of wide matrices, at least four times and 2048 columns."""
+    """The form of wide matrices, from 256 x 2048 and four times as long as high on, and one of the other side."""
     g = _matrix(kind, rows, cols, rows + steps)
     got = kan_amd.functional.orthogonalize(g.cuda(), steps=steps)
     if kind != "full":
@@ -178,3 +178,18 @@ def test_small_side_other_coefficients():
     for co, steps in (((1.5, -0.5, 0.0), 40), ((1.875, -1.25, 0.375), 25), ((2.3465, -1.0598, -0.2868), 16)):
         g = _matrix("full", 48, 300, steps)
         _check(kan_amd.functional.orthogonalize(g.cuda(), steps=steps, coefficients=co), g, steps, 1e-6, coefficients=co)
+
+
+@pytest.mark.parametrize("rows,cols", [(80, 2100), (96, 2592), (160, 4032), (192, 2135), (256, 2304), (300, 2500), (512, 4608),
+                                       (130, 140), (700, 900)])
+def test_no_less_exact_than_plain_products(rows, cols):
+    """fp32: at most half as much again as the error of torch's fp32 products, or 1e-6."""
+    g = _matrix("full", rows, cols, rows).cuda()
+    x = g / (g.norm() + 1e-7)
+    for _ in range(5):
+        gram = x @ x.t().contiguous()
+        x = NS[0] * x + (NS[1] * gram + NS[2] * gram @ gram) @ x
+    want = torch.from_numpy(_definition(g.double().cpu().numpy(), 5)).cuda()
+    plain = ((x.double() - want).norm() / want.norm()).item()
+    got = kan_amd.functional.orthogonalize(g)
+    assert ((got.double() - want).norm() / want.norm()).item() <= max(1e-6, 1.5 * plain)
