@@ -6,7 +6,9 @@
 //
 // The products run on fp16 planes (ckan_planes.hpp), X and A scaled by 2^12: |X| and
 // |A| stay below 1.5 and |b A + c A^2| below 7, far inside fp16's range, and two
-// planes keep 22 bits of entries down to 2^-15 of the largest.
+// planes keep 22 bits of entries down to 2^-15 of the largest.  A matrix whose norm is
+// far below eps enters with |X0| far below 1: it is lifted by a power of two of its own, which
+// its steps use up again as X grows (lift_at below).
 //
 // Matrices with a side of at most 64 are ckan_ortho_small.hip's.  Of the others,
 // fp32 matrices take the iteration on two planes, as it is written or, where they are
@@ -23,6 +25,8 @@
 // way as keep it below bf16's own rounding (product_run() below: 3 of 5), and the rest
 // as fp32 matrices do.  All five in one product left a matrix of rank one 1.9e-2 off, more
 // of them anything.
+#include <math.h>
+
 #include "ckan_ortho.hpp"
 #include "ckan_planes.hpp"
 
@@ -124,7 +128,7 @@ OrthoPlan make_ortho_plan(const OrthoArgs& a) {
     off = align256(off + n);
     return at;
   };
-  p.norm_off = take((size_t)batch * (kNormBlocks + 1) * sizeof(double));
+  p.norm_off = take((size_t)batch * (kNormBlocks + 2) * sizeof(double));
   p.xr_off = take(p.xr_bytes * batch);
   p.xc_off[0] = take(p.xc_bytes * batch);
   p.xc_off[1] = p.np == 1 ? 0 : take(p.xc_bytes * batch);
@@ -214,22 +218,39 @@ __device__ __forceinline__ double norm_sum(const double* part, int b, double* re
   return red[0];
 }
 
+// The lift of X after some steps: the matrix's own, less what the steps may have grown X
+// by (`used`, at most 1), and none below 1.
+__device__ __forceinline__ float lift_at(const double* lift, int b, float used) { return fmaxf((float)lift[b] * used, 1.0f); }
+
 // X0 in both operand forms: one block a 64 x 64 tile (m x n), through LDS.  In one
-// plane the scale is a power of two and what it leaves, a factor in [1, 2), goes to
-// rest[b]: the matrix is then X0 / rest exactly.
+// plane the scale is a power of two and what it leaves goes to rest[b]: the matrix is then
+// X0 / rest exactly.
 template <int NP>
 __global__ __launch_bounds__(256) void k_ortho_pack(OrthoArgs a, OrthoPlan p, const double* part, double* rest,
-                                                    char* xr, char* xc) {
+                                                    double* lift, char* xr, char* xc) {
   __shared__ float tile[64][65];
   __shared__ double red[256];
   const int b = blockIdx.z, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tid = threadIdx.x;
-  float f = kS / ((float)sqrt(norm_sum(part, b, red)) + a.eps);
+  const float norm = (float)sqrt(norm_sum(part, b, red));
+  float f = kS / (norm + a.eps);
+  // the largest power of two that leaves |X0| below 1, and f below 2^120
+  int up = 0, top = 0;
+  if (norm > 0.0f && norm < a.eps) {
+    frexpf(fminf((norm + a.eps) / norm, 0x1p100f), &up);
+    frexpf(f, &top);
+    up = up - 1 < 120 - top ? up - 1 : 120 - top;
+    up = up > 0 ? up : 0;
+  }
+  const float own = ldexpf(1.0f, up);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) lift[b] = (double)own;
   if constexpr (NP == 1) {
     int x;
-    frexpf(f, &x);
+    frexpf(f * own, &x);
     const float two = ldexpf(1.0f, x - 1);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) rest[b] = (double)(f / two);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) rest[b] = (double)f / (double)two;
     f = two;
+  } else {
+    f *= own;
   }
   if (a.view.inner != 1 && !p.tall) {
     // memory runs along (row, inner column): 64 rows of each outer column in the tile
@@ -333,14 +354,16 @@ __global__ __launch_bounds__(256, 2) void k_ortho_gram(OrthoPlan p, const char* 
 }
 
 // A in planes from the partial sums: a thread a row and 8 k.  rest: X is X0 / rest of
-// one plane.
-__global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, const double* rest, char* A) {
+// one plane; else X is lifted.
+__global__ __launch_bounds__(256) void k_ortho_gram_sum(OrthoPlan p, const float* part, const double* rest, const double* lift,
+                                                        float used, char* A) {
   const int b = blockIdx.y;
   const int k8s = p.mk / 8;
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (q >= (int64_t)p.m128 * k8s) return;
   const int k8 = (int)(q % k8s), row = (int)(q / k8s);
-  const float f = rest ? (float)(rest[b] * rest[b]) * kInvS : kInvS;
+  const double u = rest ? rest[b] : 1.0 / (double)lift_at(lift, b, used);
+  const float f = (float)(u * u) * kInvS;
   float v[8] = {};
   if (row < p.m) {
 #pragma unroll 4
@@ -546,7 +569,7 @@ template <int NB> struct UpdateTile {
 template <int NB>
 __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan p, const char* B, const char* xc,
                                                          char* xc_new, char* xr, float ax, float inv, const double* rest,
-                                                         int last) {
+                                                         const double* lift, float before, float after, int last) {
   extern __shared__ char lds[];
   typedef typename UpdateTile<NB>::Tile Tile;
   const int TM = p.m128 / kTile, TN = p.n128 / kTile;
@@ -559,7 +582,15 @@ __global__ __launch_bounds__(256, 2) void k_ortho_update(OrthoArgs a, OrthoPlan 
   const char* x = xc + b * p.xc_bytes;
   f32x16_t acc[2][2] = {};
   Tile::run(RowBlocks{B + b * p.a_bytes + tm * 4 * pb, pb}, RowBlocks{x + tn * 4 * px, px}, 0, KB / Tile::kStageBlocks, lds, acc);
-  if constexpr (NB == 1) inv *= (float)rest[b];
+  // from the lift before to the one after, or to the result
+  const float to = last ? 1.0f : lift_at(lift, b, after);
+  if constexpr (NB == 1) {
+    inv *= (float)(rest[b] * (double)to);
+  } else {
+    const float by = to / lift_at(lift, b, before);
+    ax *= by;
+    inv *= by;
+  }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 5;
   const bool gathered = a.view.inner != 1 && !p.tall, along_m = runs_along_m(a);
 #pragma unroll
@@ -656,6 +687,22 @@ float largest_q(const OrthoArgs& a, int run) {
   return (float)most;
 }
 
+// 2^-k with 2^k at least what a step multiplies X by.
+float step_use(const OrthoArgs& a) {
+  double most = 1.0;
+  for (int i = 0; i <= 1024; ++i) {
+    double x = i / 1024.0;
+    for (int s = 0; s < a.steps; ++s) {
+      const double f = a.a + a.b * x * x + a.c * x * x * x * x;
+      most = fmax(most, fabs(f));
+      x *= f;
+    }
+  }
+  int e;
+  frexp(most, &e);
+  return ldexpf(1.0f, -e);
+}
+
 // The largest |P_1 P_0 - a^2| of two steps in a row.
 float largest_pair(const OrthoArgs& a) {
   double most = 0.0;
@@ -685,7 +732,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   }
   OrthoPlan p = make_ortho_plan(a);
   char* w = (char*)ws;
-  double *norm = (double*)(w + p.norm_off), *rest = norm + (size_t)a.batch * kNormBlocks;
+  double *norm = (double*)(w + p.norm_off), *rest = norm + (size_t)a.batch * kNormBlocks, *lift = rest + a.batch;
   char* xr = w + p.xr_off;
   char* xc[2] = {w + p.xc_off[0], w + p.xc_off[1]};
   float* part = (float*)(w + p.part_off);
@@ -720,16 +767,21 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   const dim3 update_grid(a.batch * T * TN);
   char* x = xc[0];
   char* xn = xc[1];
+  const float use = step_use(a);
+  auto used = [&](int steps) {  // all of it where the power leaves fp32
+    const int e = ilogbf(use) * steps;
+    return e > -126 ? ldexpf(1.0f, e) : 0.0f;
+  };
   int s = p.run;
   if (p.run == 0) {
-    hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, xr, x);
+    hipLaunchKernelGGL(k_ortho_pack<2>, pack_grid, block, 0, st, a, p, norm, rest, lift, xr, x);
   } else {
     int exponent;  // |Q| below 2^14 in its planes
     frexpf(largest_q(a, p.run), &exponent);
     p.qscale = ldexpf(1.0f, 14 - exponent > 12 ? 12 : 14 - exponent);
-    hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, xr, x);
+    hipLaunchKernelGGL(k_ortho_pack<1>, pack_grid, block, 0, st, a, p, norm, rest, lift, xr, x);
     hipLaunchKernelGGL(k_ortho_gram<1>, gram_grid, block, GramTile<1>::Tile::kLdsBytes, st, p, xr, part);
-    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, mm[0]);
+    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, rest, lift, 1.0f, mm[0]);
     char *A = mm[0], *P = mm[1], *W = mm[2], *Q = mm[3], *Qn = mm[4];
     for (int i = 0; i < p.run; ++i) {
       const bool more = i + 1 < p.run;
@@ -746,7 +798,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
       if (more) products(MmJob{W, P, A, nullptr, kInvS, 0.0f, 0.0f, 0.0f, 0.0f}, nullptr);
     }
     hipLaunchKernelGGL(k_ortho_update<1>, update_grid, block, UpdateTile<1>::kLds, st, a, p, Q, x, xn, xr, 0.0f,
-                       1.0f / p.qscale, rest, s == a.steps);
+                       1.0f / p.qscale, rest, lift, 1.0f, used(s), s == a.steps);
     x = xc[1];
     xn = xc[0];
   }
@@ -755,7 +807,7 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
   while (s < a.steps) {
     const int taken = two && s + 1 < a.steps ? 2 : 1;
     hipLaunchKernelGGL(k_ortho_gram<2>, gram_grid, block, GramTile<2>::Tile::kLdsBytes, st, p, xr, part);
-    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, nullptr, mm[0]);
+    hipLaunchKernelGGL(k_ortho_gram_sum, sum_grid, block, 0, st, p, part, nullptr, lift, used(s), mm[0]);
     // B_s = b A_s + c A_s^2 = P_s - a I: the identity stays out of the planes
     const MmJob poly{mm[0], mm[0], mm[1], nullptr, a.c * kInvS, a.b, 0.0f, 0.0f, 0.0f};
     products(poly, nullptr);  // B_0
@@ -769,9 +821,10 @@ void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st) {
       products(MmJob{mm[3], mm[1], mm[4], nullptr, kS2 * kInvS * kInvS, a.a * kS2 * kInvS, a.a * kS2 * kInvS, 0.0f, 0.0f},
                nullptr);
     }
+    const int from = s;
     s += taken;
     hipLaunchKernelGGL(k_ortho_update<2>, update_grid, block, UpdateTile<2>::kLds, st, a, p, mm[taken == 1 ? 1 : 4], x, xn, xr,
-                       taken == 1 ? a.a : a.a * a.a, taken == 1 ? kInvS : 1.0f / kS2, rest, s == a.steps);
+                       taken == 1 ? a.a : a.a * a.a, taken == 1 ? kInvS : 1.0f / kS2, rest, lift, used(from), used(s), s == a.steps);
     char* o = x;
     x = xn;
     xn = o;

@@ -193,3 +193,21 @@ def test_no_less_exact_than_plain_products(rows, cols):
     plain = ((x.double() - want).norm() / want.norm()).item()
     got = kan_amd.functional.orthogonalize(g)
     assert ((got.double() - want).norm() / want.norm()).item() <= max(1e-6, 1.5 * plain)
+
+
+@pytest.mark.parametrize("steps", [1, 3, 5, 8, 12])
+@pytest.mark.parametrize("rows,cols", [(70, 150), (300, 2500), (140, 130), (64, 200)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_far_below_eps(rows, cols, dtype, steps):
+    """X0 is far below 1 then, and so is the result; its error is held to its own size."""
+    g = torch.stack([_matrix("full", rows, cols, i) for i in range(5)])
+    g = (g / g.norm(dim=(1, 2), keepdim=True) * torch.tensor([1.0, 1e-8, 1e-11, 1e-15, 1e-22]).view(-1, 1, 1)).to(dtype)
+    got = kan_amd.functional.orthogonalize(g.cuda(), steps=steps)
+    for i in range(5):
+        _check(got[i], g[i], steps, 1e-6 + (BF16_EXTRA if dtype == torch.bfloat16 else 0.0))
+
+
+def test_a_large_eps():
+    g = _matrix("full", 100, 300, 3) * 1e-3
+    for eps in (1.0, 1e3):
+        _check(kan_amd.functional.orthogonalize(g.cuda(), eps=eps), g, 5, 1e-6, eps=eps)
