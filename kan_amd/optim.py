@@ -107,7 +107,7 @@ class Muon(torch.optim.Optimizer):
 
     Takes [rows, cols] weights, ChebyKAN coefficients [in, out, degree+1] (each as
     the matrix [out, in (degree+1)]) and experts' [E, in, out, degree+1]; anything
-    else raises ValueError at construction: give biases and gains to another
+    else raises ValueError when it is added: give biases and gains to another
     optimizer."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
@@ -119,9 +119,15 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"Invalid momentum: {momentum}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps, coefficients=coefficients, eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        try:
+            for p in self.param_groups[-1]["params"]:
                 matrix_shape(p.shape)
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     @torch.no_grad()
     def step(self, closure=None):
