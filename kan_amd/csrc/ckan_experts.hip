@@ -301,7 +301,7 @@ __device__ __forceinline__ float range_scale(float m, int e) {
 }
 __device__ __forceinline__ float finite_abs(float v) {
   const float m = fabsf(v);
-  return m <= FLT_MAX ? m : 0.0f;  // infinities and NaN pass through the planes as they are
+  return m <= FLT_MAX ? m : 0.0f;  // infinities and NaN set no scale; on two planes both come out as NaN (inf - inf)
 }
 __device__ __forceinline__ float block_max_256(float v, float* red) {
 #pragma unroll
@@ -519,8 +519,9 @@ __global__ __launch_bounds__(256) void k_experts_pack(ExpertsArgs a, bool backwa
 // rows' tanh values of IN inputs (gathered by token) and KS k-blocks of Cf to LDS;
 // a wave makes its rows' basis values in registers, eight values of one or two
 // inputs a lane and k-block: a fragment of 12 vector instructions serves four
-// matrix ones.  16384 slots, 1024 -> 1024, degree 8, bf16: 311 us, 884 TFLOP/s, the
-// matrix pipe 45 % busy; without its copies 278, without the recurrence 301.
+// matrix ones.  16384 slots, 1024 -> 1024, degree 8, bf16: 340 us within a step
+// (808 TFLOP/s), 317 at best, the matrix pipe 45 % busy; of 311 in an early trial without
+// its copies 278, without the recurrence 301.
 // Shorter stages than these wait at their barriers.  FN = 2 (128 columns) where wide tiles
 // would be few.
 template <int NP, int P, int FN>
@@ -879,7 +880,7 @@ __device__ __forceinline__ void weigh_by_u(const f32x16_t (&acc)[2][4], int nd, 
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
       // volatile: what depends on x alone is made here, not kept in registers through
-      // the products of every run (240 of them, spilled)
+      // the products of every run (240 registers more than there are)
       float xv = x[m][q];
       asm volatile("" : "+v"(xv));
       const float y = xv + xv;
@@ -905,9 +906,11 @@ __device__ __forceinline__ void weigh_by_u(const f32x16_t (&acc)[2][4], int nd, 
 
 // dx of 128 rows x 64 inputs a block, waves of 64 rows x 32 inputs: four degrees a
 // pass over the outputs stand in four accumulator fragments; between passes only
-// their weighted sum is kept.  16384 slots, 1024 -> 1024, degree 8, bf16: 286 us, 962
-// TFLOP/s, the matrix pipe 48 % busy; bound by the copies (24 KiB for 2.1 MFLOP a
-// stage): with two or six buffers instead of three 418 and 413 where three took 398.
+// their weighted sum is kept.  16384 slots, 1024 -> 1024, degree 8, bf16: 315 us
+// within a step (873 TFLOP/s), 293 at best, the matrix pipe 44 % busy; bound by the copies
+// (24 KiB for 2.1 MFLOP a stage): with two or six buffers instead of three 418 and 413
+// where three took 398.  All 256 registers are taken (the accumulators 128, the tanh
+// values and sums 64) and 12 more live in scratch on one plane, 18 on two.
 template <int NP> using DxTile = NtTile<NP, NP, 2, 2, 2, 4, NP == 1 ? 2 : 1, 3>;  // 72 KiB of LDS
 
 template <int NP>
@@ -1041,9 +1044,10 @@ __global__ __launch_bounds__(256) void k_experts_tsort(ExpertsArgs a) {
 // blocks); waves of 4 row blocks x 64 outputs.  A stage is 32 rows.  The tanh
 // values and g arrive by copies; each thread makes the basis values of 32 (row,
 // degree) pairs of one input into LDS for the next stage while the matrix
-// instructions work on this one.  16384 slots, 1024 -> 1024, degree 8, bf16: 324 us,
-// 848 TFLOP/s, the matrix pipe 41 % busy; without making the basis 275, without the
-// copies 346 of 353, without the last store 341.
+// instructions work on this one.  16384 slots, 1024 -> 1024, degree 8, bf16: 362 us
+// within a step (759 TFLOP/s), 330 at best, the matrix pipe 42 % busy; of 324 in one trial
+// without making the basis 275, of 353 in another without the copies 346, without the
+// last store 341.
 //
 // On two planes the basis values have one LDS buffer and a barrier more, so that two
 // blocks share a CU: 16384 slots of 16 experts, 512 -> 512, degree 8, 241 us where one

@@ -67,6 +67,7 @@ bool pairs(int m, int n, bool bf16) { return n >= 4 * (int64_t)m && n >= 2048 &&
 // largest.  A_0's noise is 2^-20 of it (rank one, 1024 x 4608: 1.8e-2 after five steps,
 // 2^-20 11.9^4); a step in the m x m domain takes an error of A by the slope of y p(y)^2,
 // each later one that of X by the slope of x p(x^2).  0: the iteration on two planes.
+// 1024 x 9216, five steps: three of them this way 498 us, none 693, all 356 (and wrong).
 int product_run(const OrthoArgs& a) {
   constexpr int kSamples = 64;
   if (!a.bf16) return 0;
@@ -485,7 +486,7 @@ __device__ __forceinline__ int tile_at(bool along_m, bool gathered, int m, int n
 
 // The staged tile to where it belongs.  Four elements a thread and step along the
 // contiguous direction, in one access where the addresses allow; one element at a
-// time cost the apply launch 40 of its 77 us.
+// time cost the bf16 result's launch 40 of its 77 us.
 __device__ __forceinline__ void put_tile(const OrthoArgs& a, const OrthoPlan& p, const float* tile, int b, int m0, int n0) {
   if (a.view.inner != 1 && !p.tall) {
     constexpr int U = 8;
@@ -559,9 +560,9 @@ constexpr int kPutLds = kTile * kPutPitch * 4;
 // consecutive k of Xc, where the old X is read and the new one stored; Xr goes
 // through LDS.  The last step writes the result instead (or Muon's parameters).
 // On one plane (NB = 1) X is X0 / rest and B the whole factor Q of the run's steps.
-// 8 x [512, 4608]: 125 us for 300 MB of X read and written and 58 GFLOP of plane
-// products, 1152 blocks in 512 places; 1024 x 9216 on one plane, the result stored: 58 us,
-// 670 TFLOP/s on its two products.
+// 8 x [512, 4608]: 128 us for 300 MB of X read and written and 58 GFLOP of plane
+// products, 1152 blocks in 512 places, the matrix pipe 19 % busy; 1024 x 9216 on one
+// plane: 63 us, 620 TFLOP/s on its two products.
 template <int NB> struct UpdateTile {
   typedef NtTile<2, NB, 2, 2, 2, 2, 2, NB == 1 ? 3 : 2> Tile;  // 72 or 64 KiB of LDS
   static constexpr int kLds = Tile::kLdsBytes > kPutLds ? Tile::kLdsBytes : kPutLds;

@@ -240,7 +240,9 @@ class MixtureKANLayer(nn.Module):
     Parameters: ``gate`` [experts, input_dim] and ``cheby_coeffs`` [experts, input_dim,
     output_dim, degree+1], each expert initialised as the layer is.  ``compute``: 'fp32'
     or 'bf16' (the experts' operands and outputs are bf16, the gate, the choice and the
-    weights stay fp32; the output is fp32, as a ChebyKANLayer's).
+    weights stay fp32; the output is fp32, as a ChebyKANLayer's).  'bf16' casts the
+    coefficients of all experts in every forward: to serve single rows in bf16, call
+    ``kan_experts`` on coefficients cast once.
 
     With ``balance``, a per-expert bias steers the choice, not the weights:
     ``update_balance`` moves it towards experts that got fewer rows than the mean."""
