@@ -20,7 +20,7 @@
 //   P_s = a I + b A_s + c A_s^2,   A_{s+1} = P_s A_s P_s,   Q = P_{r-1} .. P_1 P_0,
 // and Q X0 are r steps in one: two products with the long side instead of 3 r, and X0,
 // scaled by a power of two, is exact in one plane.  But A is not made from X again
-// between them: what A_0 has as noise in the directions of small singular values grows by
+// between them: what A has as noise in the directions of small singular values grows by
 // a^2 = 11.9 a step (by a in the iteration itself), so only as many steps are taken this
 // way as keep it below bf16's own rounding (product_run() below: 3 of 5), and the rest
 // as fp32 matrices do.  All five in one product left a matrix of rank one 1.9e-2 off, more
@@ -64,10 +64,12 @@ bool pairs(int m, int n, bool bf16) { return n >= 4 * (int64_t)m && n >= 2048 &&
 
 // How many steps a bf16 matrix takes in the m x m domain: all of them, or the most (three
 // at least) that leave the result's error below 2^-9, half of a rounding to bf16 at its
-// largest.  A_0's noise is 2^-20 of it (rank one, 1024 x 4608: 1.8e-2 after five steps,
-// 2^-20 11.9^4); a step in the m x m domain takes an error of A by the slope of y p(y)^2,
-// each later one that of X by the slope of x p(x^2).  0: the iteration on two planes.
-// 1024 x 9216, five steps: three of them this way 498 us, none 693, all 356 (and wrong).
+// largest.  The noise is 2^-20 of A, from the fp32 sums of X X^T and of a A and
+// b A^2 + c A^3, which cancel in A_1 (rank one, 1024 x 4608: 1.8e-2 after five steps,
+// 2^-20 11.9^4; shorter sums, or the product of the low planes too, change nothing).  A
+// step in the m x m domain takes an error of A by the slope of y p(y)^2, each later one
+// that of X by the slope of x p(x^2).  0: the iteration on two planes.  1024 x 9216, five
+// steps: three of them this way 498 us, none 693, all 356 (and wrong).
 int product_run(const OrthoArgs& a) {
   constexpr int kSamples = 64;
   if (!a.bf16) return 0;
