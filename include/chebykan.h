@@ -395,8 +395,8 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
 /* Newton-Schulz orthogonalisation of a batch of matrices G [rows, cols]:
  *   X = G / (|G|_F + eps), then `steps` times
  *   X = a X + (b A + c A^2) X with A = X X^T (X^T X for rows > cols).
- * Products run on two fp16 planes an operand (22 bits) with fp32 sums; the
- * norm is summed in fp64.  bf16 matrices take as many steps in powers of X X^T as keep
+ * Products run on two fp16 planes an operand (22 bits) with fp32 sums, those of a side of
+ * at most 64 in fp64; the norm is summed in fp64.  bf16 matrices take as many steps in powers of X X^T as keep
  * the error that this adds below 2^-9, their own rounding.  |b A + c A^2| and |a + b A + c A^2|
  * have to stay below 15 for singular values in [0, 1] over all steps (checked on
  * the host).
