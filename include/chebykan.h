@@ -391,6 +391,115 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
                           const void* dy, void* dx, void* dcoeffs, void* dweights, void* ws, size_t ws_bytes,
                           void* stream);
 
+/* ---- a whole mixture layer for few rows ---------------------------------------------- */
+/* logits = x gate^T, ckan_route's choice and weights on them, and ckan_experts_forward's
+ * sum, without a backward, for as few rows as the experts' coefficients are streamed for
+ * (ckan_mixture_few: at most 1024 slots, 16 an expert on average).  The logits are summed in 64 bits and rounded
+ * once to fp32, so that the choice does not hang on an order of sums.  x [rows, in] and y
+ * have x_dtype, gate [experts, in] and coeffs [experts, in, out, degree + 1] a dtype each;
+ * bias fp32 [experts] or NULL; weights fp32 and indices [rows, top_k] are outputs.  Buffers need
+ * 16-byte alignment. */
+typedef struct ckan_mixture_desc {
+  int64_t rows;
+  int32_t experts, top_k, in_dim, out_dim, degree;      /* as ckan_experts_desc's */
+  int32_t score, groups, top_groups, renormalize;       /* as ckan_route_desc's   */
+  int32_t x_dtype, gate_dtype, coeff_dtype;
+  float scale;
+} ckan_mixture_desc;
+int ckan_mixture_few(const ckan_mixture_desc* desc);  /* 1: ckan_mixture_forward takes it */
+size_t ckan_mixture_workspace_bytes(const ckan_mixture_desc* desc);
+int ckan_mixture_forward(const ckan_mixture_desc* desc, const void* x, const void* gate, const void* coeffs,
+                         const float* bias, void* y, float* weights, int64_t* indices, void* ws, size_t ws_bytes,
+                         void* stream);
+
+/* ---- norms around a residual block ------------------------------------------------ */
+/*   u = drop(post(y)),  out = x + scale gate u,  h = next(out)
+ * over rows of `dim` values, post and next being (v - mean) r w + b with
+ * r = 1 / sqrt(mean((v - mean)^2) + eps), mean taken as 0 in the RMS form.  A NULL
+ * post_weight or next_weight leaves that norm (and h) out, a NULL gate is 1, a NULL y
+ * leaves only h = next(x).  gate is [dim] or, with gate_rows, [rows, dim].
+ * x, out, dout and dx have x_dtype, y, h, dh and dy have y_dtype; parameters, row gates
+ * and their gradients have a dtype each.  Rows are contiguous, `*_ld` elements apart (out, h and
+ * the gradients dense).  Arithmetic in fp32, results rounded once; h comes from out
+ * before its rounding.
+ * Dropout (dropout > 0) as ckan_dropout's, on rows and columns of y. */
+typedef enum ckan_norm {
+  CKAN_NORM_RMS = 0,
+  CKAN_NORM_LAYER = 1
+} ckan_norm;
+
+typedef struct ckan_residual_desc {
+  int64_t rows;        /* 0..2^32 - 1                                        */
+  int64_t x_ld, y_ld, gate_ld, dout_ld, dh_ld;
+  int32_t dim;         /* 1..2^20                                            */
+  int32_t x_dtype, y_dtype;
+  int32_t gate_dtype, post_weight_dtype, post_bias_dtype, next_weight_dtype, next_bias_dtype;
+  int32_t norm;        /* ckan_norm                                          */
+  int32_t gate_rows;   /* 0 or 1                                             */
+  float eps, scale;
+  double dropout;      /* 0..1                                               */
+  uint64_t dropout_seed, dropout_offset;
+} ckan_residual_desc;
+
+typedef struct ckan_residual_buffers {
+  const void *x, *y, *gate, *post_weight, *post_bias, *next_weight, *next_bias;
+  const int64_t* dropout_state;  /* as ckan_dropout's                         */
+  void *out, *h;                 /* written by the forward                     */
+  void* stats;                   /* written by a forward that a backward follows (else NULL), read by it */
+  const void *dout, *dh;         /* gradients of out and h; NULL is zero       */
+  void *dx, *dy, *dgate, *dpost_weight, *dpost_bias, *dnext_weight, *dnext_bias;  /* NULL: not wanted */
+} ckan_residual_buffers;
+
+size_t ckan_residual_stats_bytes(const ckan_residual_desc* desc);
+size_t ckan_residual_workspace_bytes(const ckan_residual_desc* desc);
+int ckan_residual_forward(const ckan_residual_desc* desc, const ckan_residual_buffers* buffers, void* stream);
+/* Needs the forward's inputs and stats as they were; sums over rows run in a fixed order. */
+int ckan_residual_backward(const ckan_residual_desc* desc, const ckan_residual_buffers* buffers, void* ws,
+                           size_t ws_bytes, void* stream);
+
+/* ---- dropout -------------------------------------------------------------------------- */
+/* y[r, c] = keep(r, c) x[r, c] / (1 - p).  The 32-bit number of an element is made of two
+ * 16-bit halves, the high one from Philox 4x32-10 on the counter (c / 8, r, call) under the
+ * seed, half c % 8 of its four words; the low one likewise from the counter with its top
+ * bit set; the element is kept where the number reaches round(p 2^32).  (seed, call): the
+ * given ones, or with `state` (int64[2] on the device) state[0] and state[1] + offset; calls
+ * count modulo 2^63.  `used` (int64[2], or NULL) receives them: a gradient is the same call
+ * on dy with `used` as its state. */
+typedef struct ckan_dropout_desc {
+  int64_t rows;      /* 0..2^32 - 1                        */
+  int64_t dim;       /* 1..2^34; contiguous within a row   */
+  int64_t x_ld;      /* elements from a row to the next    */
+  double p;          /* 0..1                               */
+  uint64_t seed, offset;
+  int32_t dtype;     /* ckan_dtype of x and y              */
+} ckan_dropout_desc;
+int ckan_dropout(const ckan_dropout_desc* desc, const int64_t* state, const void* x, void* y, int64_t* used,
+                 void* stream);
+
+/* ---- log probabilities -------------------------------------------------------------- */
+/* Of rows of logits [rows, classes]: logp[r] = log softmax(logits[r])[targets[r]] (0 where the
+ * target lies outside [0, classes): such a row has none), entropy[r], and with top > 0
+ * the top likeliest classes' log probabilities and indices [rows, top], equal logits by the lower
+ * index.  A logit of -inf has no probability and is not among the likeliest (index -1,
+ * log probability -inf fill up); a row of nothing else has logp -inf, entropy 0 and no gradient.
+ * NaN or +inf in a row gives NaN.  Sums in fp32, the largest logit's share apart, so that rows
+ * that are sure of one class keep their relative precision. */
+typedef struct ckan_log_probs_desc {
+  int64_t rows;      /* 0..2^31 - 1                        */
+  int64_t logits_ld; /* elements from a row to the next    */
+  int32_t classes;   /* 1..2^30                            */
+  int32_t top;       /* 0..64, at most classes             */
+  int32_t dtype;     /* ckan_dtype of logits and dlogits   */
+} ckan_log_probs_desc;
+size_t ckan_log_probs_workspace_bytes(const ckan_log_probs_desc* desc);
+/* stats: fp32 [rows, 3], or NULL where no backward follows. */
+int ckan_log_probs(const ckan_log_probs_desc* desc, const void* logits, const int64_t* targets, float* logp,
+                   float* entropy, float* top_logp, int64_t* top_indices, float* stats, void* ws, size_t ws_bytes,
+                   void* stream);
+/* dlogits (dense rows) from the gradients of logp and entropy (fp32 [rows]; NULL is zero). */
+int ckan_log_probs_backward(const ckan_log_probs_desc* desc, const void* logits, const int64_t* targets,
+                            const float* stats, const float* dlogp, const float* dentropy, void* dlogits, void* stream);
+
 /* ---- orthogonalised updates ---------------------------------------------------- */
 /* Newton-Schulz orthogonalisation of a batch of matrices G [rows, cols]:
  *   X = G / (|G|_F + eps), then `steps` times

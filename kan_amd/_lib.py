@@ -247,6 +247,94 @@ SIGNATURES.update({
                                       _vp, _sz, _vp]),
 })
 
+
+
+class CkanMixtureDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64)] + [(name, ctypes.c_int32) for name in (
+        "experts", "top_k", "in_dim", "out_dim", "degree", "score", "groups", "top_groups", "renormalize", "x_dtype",
+        "gate_dtype", "coeff_dtype")] + [("scale", ctypes.c_float)]
+
+
+_pmixture = ctypes.POINTER(CkanMixtureDesc)
+SIGNATURES.update({
+    "ckan_mixture_few": (ctypes.c_int, [_pmixture]),
+    "ckan_mixture_workspace_bytes": (_sz, [_pmixture]),
+    "ckan_mixture_forward": (ctypes.c_int, [_pmixture, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+})
+
+CKAN_NORM_RMS = 0
+CKAN_NORM_LAYER = 1
+
+
+class CkanResidualDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("y_ld", ctypes.c_int64),
+        ("gate_ld", ctypes.c_int64),
+        ("dout_ld", ctypes.c_int64),
+        ("dh_ld", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("gate_dtype", ctypes.c_int32),
+        ("post_weight_dtype", ctypes.c_int32),
+        ("post_bias_dtype", ctypes.c_int32),
+        ("next_weight_dtype", ctypes.c_int32),
+        ("next_bias_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("gate_rows", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("scale", ctypes.c_float),
+        ("dropout", ctypes.c_double),
+        ("dropout_seed", ctypes.c_uint64),
+        ("dropout_offset", ctypes.c_uint64),
+    ]
+
+
+class CkanResidualBuffers(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "x", "y", "gate", "post_weight", "post_bias", "next_weight", "next_bias", "dropout_state", "out", "h", "stats",
+        "dout", "dh", "dx", "dy", "dgate", "dpost_weight", "dpost_bias", "dnext_weight", "dnext_bias")]
+
+
+class CkanDropoutDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("p", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("offset", ctypes.c_uint64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class CkanLogProbsDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("logits_ld", ctypes.c_int64),
+        ("classes", ctypes.c_int32),
+        ("top", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+_presidual = ctypes.POINTER(CkanResidualDesc)
+_pbuffers = ctypes.POINTER(CkanResidualBuffers)
+_pdropout = ctypes.POINTER(CkanDropoutDesc)
+_plogp = ctypes.POINTER(CkanLogProbsDesc)
+SIGNATURES.update({
+    "ckan_residual_stats_bytes": (_sz, [_presidual]),
+    "ckan_residual_workspace_bytes": (_sz, [_presidual]),
+    "ckan_residual_forward": (ctypes.c_int, [_presidual, _pbuffers, _vp]),
+    "ckan_residual_backward": (ctypes.c_int, [_presidual, _pbuffers, _vp, _sz, _vp]),
+    "ckan_dropout": (ctypes.c_int, [_pdropout, _vp, _vp, _vp, _vp, _vp]),
+    "ckan_log_probs_workspace_bytes": (_sz, [_plogp]),
+    "ckan_log_probs": (ctypes.c_int, [_plogp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ckan_log_probs_backward": (ctypes.c_int, [_plogp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+})
+
 _lib = None
 _lock = threading.Lock()
 

@@ -1,0 +1,325 @@
+"""What stands around the layers of a deep KAN, over the C-ABI: the norms, gate, dropout and
+sum of a residual block, dropout by itself, and the log probabilities at a network's end.
+
+Device memory and streams come from torch; all compute is the HIP library's.
+Tensors on the CPU are rejected: there is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from .mixture import _on, _once, _stream
+
+_NORMS = {"rms": _lib.CKAN_NORM_RMS, "layer": _lib.CKAN_NORM_LAYER}
+_DTYPES = {torch.float32: _lib.CKAN_DTYPE_F32, torch.bfloat16: _lib.CKAN_DTYPE_BF16}
+
+
+def _check(name: str, device: torch.device, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"kan_amd's block operators run only on a ROCm device (MI355X); {name} is on {t.device}")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, another tensor on {device}: one device is needed")
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _rows(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """t as [rows, dim], its rows contiguous; a copy only where no view has that form."""
+    t = t.reshape(-1, dim)
+    return t if (t.stride(1) == 1 or dim == 1) and t.stride(0) >= 0 else t.contiguous()
+
+
+def _pitch(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.stride(0)
+
+
+def _drop_state(p: float, state, call: int, device: torch.device):
+    """(device tensor or None, seed, offset) of a dropout's ``state`` and ``call``."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"the dropout probability must lie in [0, 1], got {p}")
+    if not 0 <= call < 1 << 63:
+        raise ValueError(f"the dropout call must lie in [0, 2^63), got {call}")
+    if p == 0.0:
+        return None, 0, 0
+    if isinstance(state, torch.Tensor):
+        if state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous() or state.device != device:
+            raise RuntimeError(f"the dropout state must be a contiguous int64 tensor of (seed, offset) on {device}, got "
+                               f"{state.dtype} {tuple(state.shape)} on {state.device}")
+        return state, 0, call
+    if isinstance(state, int):
+        return None, state & (1 << 64) - 1, call
+    raise ValueError("dropout needs its state: an int seed, or an int64 tensor of (seed, offset) on the device")
+
+
+# ---- norms around a residual block ---------------------------------------------
+
+class ResidualFunction(torch.autograd.Function):
+    """``residual_norm`` and ``row_norm`` with their gradients; outputs (out, h), absent
+    ones None."""
+
+    @staticmethod
+    def forward(ctx, x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state, h_dtype):
+        out, h, stats = _residual_forward(x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state,
+                                          h_dtype, keep=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, y, gate, post_weight, post_bias, next_weight, next_bias, stats)
+        ctx.desc, ctx.h_dtype = desc, h_dtype
+        return out, h
+
+    @staticmethod
+    def backward(ctx, dout, dh):
+        _once("residual_norm")
+        need = ctx.needs_input_grad
+        if not any(need[:7]) or (dout is None and dh is None):
+            return (None,) * 10
+        *inputs, stats = ctx.saved_tensors
+        x = inputs[0]
+        desc = _lib.CkanResidualDesc.from_buffer_copy(ctx.desc)
+        if dout is not None:
+            dout = _rows(dout.to(x.dtype), desc.dim)
+            desc.dout_ld = _pitch(dout)
+        if dh is not None:
+            dh = _rows(dh.to(ctx.h_dtype), desc.dim)
+            desc.dh_ld = _pitch(dh)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip(inputs, need)]
+        if desc.rows == 0:
+            return (*(None if g is None else g.zero_() for g in grads), None, None, None)
+        lib = _lib.load()
+        nbytes = lib.ckan_residual_workspace_bytes(desc)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        buffers = _lib.CkanResidualBuffers(*(_lib.ptr(t) for t in inputs), 0, 0, 0, stats.data_ptr(), _lib.ptr(dout),
+                                           _lib.ptr(dh), *(_lib.ptr(g) for g in grads))
+        # the engine runs a node on its device and stream
+        _lib.check(lib.ckan_residual_backward(desc, buffers, ws.data_ptr(), nbytes, _stream(x.device)))
+        return (*grads, None, None, None)
+
+
+def _residual_forward(x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state, h_dtype, keep):
+    """(out, h, stats); the tensors are [rows, dim] and [dim]."""
+    lib, dev = _lib.load(), x.device
+    shape = (desc.rows, desc.dim)
+    out = torch.empty(shape, dtype=x.dtype, device=dev) if y is not None else None
+    h = torch.empty(shape, dtype=h_dtype, device=dev) if next_weight is not None else None
+    stats = torch.empty(desc.rows * 4 + 4, dtype=torch.float32, device=dev) if keep else None
+    buffers = _lib.CkanResidualBuffers(x.data_ptr(), *(_lib.ptr(t) for t in (
+        y, gate, post_weight, post_bias, next_weight, next_bias, state, out, h, stats)))
+    with _on(dev):
+        _lib.check(lib.ckan_residual_forward(desc, buffers, _stream(dev)))
+    return out, h, stats
+
+
+def _residual(x, y, gate, post_weight, post_bias, next_weight, next_bias, norm, eps, scale, dropout, state, call,
+              h_dtype):
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"x must be [..., dim] with dim >= 1, got {tuple(x.shape)}")
+    dim, shape = x.shape[-1], x.shape
+    params = {"post_weight": post_weight, "post_bias": post_bias, "next_weight": next_weight, "next_bias": next_bias}
+    _lib.refuse_tangents("residual_norm", x, y, gate, *params.values())
+    for name, t in (("x", x), ("y", y), ("gate", gate), *params.items()):
+        if t is not None:
+            _check(name, x.device, t)
+    for name, t in params.items():
+        if t is not None and tuple(t.shape) != (dim,):
+            raise RuntimeError(f"{name} must be [{dim}], got {tuple(t.shape)}")
+    if (post_bias is not None and post_weight is None) or (next_bias is not None and next_weight is None):
+        raise RuntimeError("a norm's bias needs its weight")
+    if h_dtype not in _DTYPES:
+        raise RuntimeError(f"a norm's result is float32 or bfloat16, not {h_dtype}")
+    gate_rows = False
+    if gate is not None:
+        gate_rows = gate.dim() > 1 and gate.shape == shape
+        if not gate_rows and tuple(gate.shape) != (dim,):
+            raise RuntimeError(f"gate must be [{dim}] or {tuple(shape)}, got {tuple(gate.shape)}")
+    if y is not None and y.shape != shape:
+        raise RuntimeError(f"y must be of x's shape {tuple(shape)}, got {tuple(y.shape)}")
+    drop_state, seed, offset = _drop_state(dropout, state, call, x.device)
+    x = _rows(x, dim)
+    y = None if y is None else _rows(y, dim)
+    if gate is not None:
+        gate = _rows(gate, dim) if gate_rows else gate.contiguous()
+    post_weight, post_bias, next_weight, next_bias = (None if t is None else t.contiguous() for t in params.values())
+    codes = [0 if t is None else _DTYPES[t.dtype] for t in (gate, post_weight, post_bias, next_weight, next_bias)]
+    desc = _lib.CkanResidualDesc(x.shape[0], x.stride(0), _pitch(y), gate.stride(0) if gate_rows else 0, 0, 0, dim,
+                                 _DTYPES[x.dtype], _DTYPES[h_dtype if y is None else y.dtype], *codes, _NORMS[norm],
+                                 int(gate_rows), float(eps), float(scale), float(dropout), seed, offset)
+    tensors = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        out, h = ResidualFunction.apply(*tensors, desc, drop_state, h_dtype)
+    else:
+        out, h, _ = _residual_forward(*tensors, desc, drop_state, h_dtype, keep=False)
+    return None if out is None else out.view(shape), None if h is None else h.view(shape)
+
+
+def row_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, norm: str = "rms",
+             eps: float = 1e-6, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The norm before a block: each row of x [..., dim] as (v - mean) / sqrt(mean((v -
+    mean)^2) + eps) * weight + bias, with mean 0 for norm='rms' ('layer' takes it out).
+
+    x, weight and bias [dim] are fp32 or bf16 each; the result has ``dtype``, x's by
+    default.  fp32 arithmetic, rounded once.  Differentiable once in x, weight and bias."""
+    return _residual(x, None, None, None, None, weight, bias, norm, eps, 1.0, 0.0, None, 0, dtype or x.dtype)[1]
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", eps: float = 1e-6,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, scale: float = 1.0, dropout: float = 0.0,
+                  dropout_state: Union[int, torch.Tensor, None] = None, dropout_call: int = 0,
+                  next_weight: Optional[torch.Tensor] = None, next_bias: Optional[torch.Tensor] = None
+                  ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """What follows a block: out = x + scale * gate * drop(post(y)), and with ``next_weight``
+    also h = next(out), the norm before the block that comes after: (out, h).
+
+    ``x`` [..., dim] is the residual stream, ``y`` of its shape the block's result; each is fp32 or
+    bf16.  ``post`` and ``next`` are ``row_norm``'s norms with their own weights [dim] and
+    biases, absent without a weight.  ``gate`` is [dim] or of x's shape, 1 without one.
+    ``dropout`` draws ``functional.dropout``'s mask for y's shape from ``dropout_state`` and
+    ``dropout_call``.  out has x's dtype, h has y's and comes from out before its rounding;
+    arithmetic is in fp32.
+
+    Differentiable once in x, y, gate, weights and biases; sums run in a fixed order, so
+    a call repeats bit for bit."""
+    out, h = _residual(x, y, gate, post_weight, post_bias, next_weight, next_bias, norm, eps, scale, dropout,
+                       dropout_state, dropout_call, y.dtype)
+    return out if next_weight is None else (out, h)
+
+
+# ---- dropout -----------------------------------------------------------------------
+
+def _dropout_launch(x, p, state, seed, offset, keep):
+    """(y, used) of x [rows, dim]."""
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    used = torch.empty(2, dtype=torch.int64, device=dev) if keep else None
+    desc = _lib.CkanDropoutDesc(x.shape[0], max(x.shape[1], 1), x.stride(0), p, seed, offset, _DTYPES[x.dtype])
+    with _on(dev):
+        _lib.check(_lib.load().ckan_dropout(desc, _lib.ptr(state), x.data_ptr(), y.data_ptr(), _lib.ptr(used),
+                                            _stream(dev)))
+    return y, used
+
+
+class DropoutFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, state, seed, offset):
+        y, used = _dropout_launch(x, p, state, seed, offset, keep=True)
+        ctx.p, ctx.used, ctx.dtype = p, used, x.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _once("dropout")
+        dx, _ = _dropout_launch(_rows(dy.to(ctx.dtype), dy.shape[-1]), ctx.p, ctx.used, 0, 0, keep=False)
+        return dx, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, state: Union[int, torch.Tensor], call: int = 0) -> torch.Tensor:
+    """x [..., dim] (fp32 or bf16) with each element kept with probability 1 - p and divided by it, else 0.
+
+    The mask is a function of the seed, the call's number, the row and the column, by a
+    counter-based generator (Philox 4x32-10), and never stored.  ``state`` is the seed, or a
+    device tensor int64[2] of (seed, offset), to whose offset ``call`` is added: a captured graph that
+    adds to the tensor between its calls draws new masks at every replay.  Equal state and
+    call give equal masks.  Differentiable once in x, with the state as the forward read it."""
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., dim], got a scalar")
+    _lib.refuse_tangents("dropout", x)
+    _check("x", x.device, x)
+    state, seed, offset = _drop_state(float(p), state, int(call), x.device)
+    if x.numel() == 0:
+        return x.clone()
+    rows = _rows(x, x.shape[-1])
+    if torch.is_grad_enabled() and rows.requires_grad:
+        return DropoutFunction.apply(rows, float(p), state, seed, offset).view(x.shape)
+    return _dropout_launch(rows, float(p), state, seed, offset, keep=False)[0].view(x.shape)
+
+
+# ---- log probabilities ----------------------------------------------------------------
+
+class LogProbs(NamedTuple):
+    """What ``log_probs`` returns; the last two are None without ``top``."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    top_logp: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+def _log_probs_forward(logits, targets, desc, keep):
+    lib, dev, rows = _lib.load(), logits.device, desc.rows
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_logp = torch.empty(rows, desc.top, dtype=torch.float32, device=dev) if desc.top else None
+    top_idx = torch.empty(rows, desc.top, dtype=torch.int64, device=dev) if desc.top else None
+    stats = torch.empty(rows, 3, dtype=torch.float32, device=dev) if keep else None
+    nbytes = lib.ckan_log_probs_workspace_bytes(desc)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev):
+        _lib.check(lib.ckan_log_probs(desc, logits.data_ptr(), targets.data_ptr(), logp.data_ptr(), entropy.data_ptr(),
+                                      _lib.ptr(top_logp), _lib.ptr(top_idx), _lib.ptr(stats), _lib.ptr(ws), nbytes,
+                                      _stream(dev)))
+    return logp, entropy, top_logp, top_idx, stats
+
+
+class LogProbsFunction(torch.autograd.Function):
+    """logp and entropy, differentiable in the logits; the likeliest classes go by the side."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, desc, out: list):
+        logp, entropy, top_logp, top_idx, stats = _log_probs_forward(logits, targets, desc, keep=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.desc = desc
+        out += [top_logp, top_idx]
+        return logp, entropy
+
+    @staticmethod
+    def backward(ctx, dlogp, dentropy):
+        _once("log_probs")
+        if dlogp is None and dentropy is None:
+            return None, None, None, None
+        logits, targets, stats = ctx.saved_tensors
+        dlogp, dentropy = (None if g is None else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))
+        dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _lib.check(_lib.load().ckan_log_probs_backward(ctx.desc, logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
+                                                       _lib.ptr(dlogp), _lib.ptr(dentropy), dl.data_ptr(),
+                                                       _stream(dl.device)))
+        return dl, None, None, None
+
+
+def log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> LogProbs:
+    """Log probabilities of given classes under softmax(logits): (logp, entropy, top_logp,
+    top_indices), the first two fp32 of ``targets``' shape, the last two [..., top] or None.
+
+    ``logits`` [..., classes] fp32 or bf16, ``targets`` [...] int64.  A target outside [0,
+    classes) is none: logp 0, no gradient.  ``entropy`` is the row's, in nats.  ``top`` (up to 64)
+    asks for the likeliest classes in falling order, equal logits by the lower index.  A class
+    whose logit is -inf has no probability and is not listed (index -1 and -inf fill up); a
+    row of such classes only has logp -inf, entropy 0 and no gradient.  NaN or +inf makes a row's
+    numbers NaN.
+
+    -logp.mean() is the cross entropy.  Differentiable once in the logits through logp and
+    entropy."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError(f"logits must be [..., classes], got {tuple(logits.shape)}")
+    if targets.shape != logits.shape[:-1]:
+        raise RuntimeError(f"targets must be {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
+    if targets.dtype != torch.int64:
+        raise RuntimeError(f"targets must be int64, got {targets.dtype}")
+    _lib.refuse_tangents("log_probs", logits)
+    _check("logits", logits.device, logits)
+    if targets.device != logits.device:
+        raise RuntimeError(f"targets are on {targets.device}, logits on {logits.device}: one device is needed")
+    shape, classes = targets.shape, logits.shape[-1]
+    logits, targets = _rows(logits, classes), targets.reshape(-1).contiguous()
+    desc = _lib.CkanLogProbsDesc(logits.shape[0], logits.stride(0), classes, int(top), _DTYPES[logits.dtype])
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out: list = []
+        got = (*LogProbsFunction.apply(logits, targets, desc, out), *out)
+    else:
+        got = _log_probs_forward(logits, targets, desc, keep=False)[:4]
+    if len(shape) == 1:
+        return LogProbs(*got)
+    return LogProbs(*(None if t is None else t.view(shape + t.shape[1:]) for t in got))

@@ -1,0 +1,199 @@
+// Launch interface of the residual-block, dropout, log-probability and few-row
+// mixture kernels, and the device helpers that they share.
+#pragma once
+
+#include <float.h>
+
+#include "ckan_kernels.hpp"
+
+namespace ckan {
+
+// ---- rows in chunks of eight values -------------------------------------------
+// A row of any length and alignment is read in chunks of eight consecutive values:
+// whole chunks by unaligned vector accesses (16 bytes of bf16, 32 of fp32; the
+// target's memory mode allows them at any element), a row's last, partial one by
+// elements, so that nothing past a row's end is touched.
+constexpr int kChunk = 8;
+
+struct __attribute__((packed)) RawBf16 { u32x4_t v; };
+struct __attribute__((packed)) RawF32 { u32x4_t v[2]; };
+template <typename T> struct RawOf;
+template <> struct RawOf<__bf16> { typedef RawBf16 type; };
+template <> struct RawOf<float> { typedef RawF32 type; };
+
+__device__ __forceinline__ void unpack8(const RawBf16& r, float (&f)[kChunk]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(r.v[i] << 16);
+    f[2 * i + 1] = __uint_as_float(r.v[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const RawF32& r, float (&f)[kChunk]) {
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) f[i] = __uint_as_float(r.v[i >> 2][i & 3]);
+}
+
+// `left` values of the row remain from p on (at least one); those past it read as 0.
+template <typename T>
+__device__ __forceinline__ typename RawOf<T>::type load_raw8(const T* p, int64_t left) {
+  typename RawOf<T>::type r;
+  if (left >= kChunk) {
+    r = *(const typename RawOf<T>::type*)p;
+  } else {
+    union { typename RawOf<T>::type raw; T e[kChunk]; } u;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) u.e[i] = i < left ? p[i] : (T)0.0f;
+    r = u.raw;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, float (&f)[kChunk]) {
+  unpack8(load_raw8(p, left), f);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t left, const float (&f)[kChunk]) {
+  union { typename RawOf<T>::type raw; T e[kChunk]; } u;
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) u.e[i] = (T)f[i];
+  if (left >= kChunk) {
+    *(typename RawOf<T>::type*)p = u.raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (i < left) p[i] = u.e[i];
+  }
+}
+
+// A tensor whose type is known at run time (parameters, row gates).
+struct AnyPtr {
+  const void* p;
+  int bf16;
+};
+__device__ __forceinline__ void load8(const AnyPtr& a, int64_t at, int64_t left, float (&f)[kChunk]) {
+  if (a.bf16)
+    load8((const __bf16*)a.p + at, left, f);
+  else
+    load8((const float*)a.p + at, left, f);
+}
+
+// ---- dropout's generator ---------------------------------------------------------
+// Philox 4x32 with ten rounds (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as
+// easy as 1, 2, 3", 2011), keyed by the seed, on the counter (column / 8, row, call):
+// four words are 16 bits for each of a chunk's eight values.  An element is kept where
+// its 32-bit number reaches p 2^32.  Its high half decides all but one case in 2^16: only
+// where that half equals the threshold's is the stream of the low halves (the counter's
+// top bit) drawn, so the mask has the resolution of 32 bits for little more than the
+// cost of 16.
+struct DropArgs {
+  const int64_t* state;  // (seed, offset) on the device, or NULL: (seed, offset) below
+  uint64_t seed, offset; // offset is added to the state's
+  uint32_t high, low;    // round(p 2^32) = high 2^16 + low; high 2^16: nothing is kept
+  float scale;           // 1 / (1 - p)
+  int on;
+};
+
+__device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
+    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    c[1] = (uint32_t)b;
+    c[3] = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+}
+
+// Seed and call of a launch: uniform, read once a thread.
+struct DropKey {
+  uint32_t k0, k1, call0, call1;
+};
+__device__ __forceinline__ DropKey drop_key(const DropArgs& d) {
+  uint64_t seed = d.seed, call = d.offset;
+  if (d.state) {
+    seed = (uint64_t)d.state[0];
+    call += (uint64_t)d.state[1];
+  }
+  return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)call, (uint32_t)(call >> 32) & 0x7fffffffu};
+}
+
+// Bit i: element i of the chunk is kept.
+__device__ __forceinline__ uint32_t drop_keep(const DropArgs& d, const DropKey& k, uint32_t row, uint32_t chunk) {
+  uint32_t c[4] = {chunk, row, k.call0, k.call1};
+  philox(c, k.k0, k.k1);
+  uint32_t keep = 0, tie = 0;
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) {
+    const uint32_t r = i & 1 ? c[i >> 1] >> 16 : c[i >> 1] & 0xffffu;
+    keep |= r >= d.high ? 1u << i : 0u;
+    tie |= r == d.high ? 1u << i : 0u;
+  }
+  if (d.low && tie) {  // the low halves decide
+    uint32_t e[4] = {chunk, row, k.call0, k.call1 | 0x80000000u};
+    philox(e, k.k0, k.k1);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      const uint32_t r = i & 1 ? e[i >> 1] >> 16 : e[i >> 1] & 0xffffu;
+      if (r < d.low) keep &= ~(tie & (1u << i));
+    }
+  }
+  return keep;
+}
+
+constexpr int64_t kDropMaxRows = (int64_t)1 << 32, kDropMaxDim = (int64_t)1 << 34;
+
+struct DropoutArgs {
+  const void* x;
+  void* y;
+  int64_t rows, dim, ld;
+  int bf16;
+  DropArgs drop;
+  int64_t* used;  // (seed, offset) as this launch read them, or NULL
+};
+void launch_dropout(const DropoutArgs& a, hipStream_t st);
+
+// ---- norms around a residual block (ckan_residual.hip) -----------------------------
+// out = x + scale gate drop(post(y)) and h = next(out); post and next are norms of the
+// rows.  Without y: h = next(x).
+struct ResidualArgs {
+  int64_t rows, x_ld, y_ld, gate_ld, dout_ld, dh_ld;
+  int dim;
+  int x_bf16, y_bf16;  // the stream's type (x, out, dout, dx), the branch's (y, h, dh, dy)
+  int layer;           // norms with the mean taken out
+  int gate_rows;       // gate is [rows, dim] (else [dim])
+  float eps, scale;
+  DropArgs drop;
+  const void *x, *y;
+  AnyPtr gate, post_w, post_b, next_w, next_b;  // p NULL: absent
+  void *out, *h;
+  float* stats;        // [rows, 4]: post's mean and factor, next's mean and factor; then (seed, offset)
+  const void *dout, *dh;
+  void *dx, *dy, *dgate, *dpost_w, *dpost_b, *dnext_w, *dnext_b;  // NULL: not wanted
+  float* ws;
+};
+constexpr int kResMaxDim = 1 << 20;
+size_t residual_workspace_bytes(const ResidualArgs& a);
+void launch_residual_forward(const ResidualArgs& a, hipStream_t st);
+void launch_residual_backward(const ResidualArgs& a, hipStream_t st);
+
+// ---- log probabilities (ckan_logprobs.hip) ------------------------------------------
+constexpr int kLogpMaxTop = 64;
+struct LogpArgs {
+  const void* logits;  // [rows, classes], row pitch ld
+  const int64_t* targets;
+  int64_t rows, ld;
+  int classes, top, bf16;
+  float *logp, *entropy, *top_logp;
+  int64_t* top_idx;
+  float* stats;        // [rows, 3]: shift, log of the sum, entropy; NULL where no backward follows
+  const float *dlogp, *dentropy;  // NULL: zero
+  void* dlogits;
+  char* ws;
+};
+size_t logprobs_workspace_bytes(const LogpArgs& a);
+void launch_logprobs(const LogpArgs& a, hipStream_t st);
+void launch_logprobs_backward(const LogpArgs& a, hipStream_t st);
+
+}  // namespace ckan

@@ -108,6 +108,26 @@ size_t experts_fwd_ws(const ExpertsPlan& p, bool without_saved) {
   return p.fwd_bytes + (without_saved ? p.cb_off : 0);
 }
 
+ckan_experts_desc mixture_experts(const ckan_mixture_desc* d) {
+  return ckan_experts_desc{d->rows, d->experts, d->top_k, d->in_dim, d->out_dim, d->degree, d->coeff_dtype, CKAN_DTYPE_F32};
+}
+
+int mixture_args(const ckan_mixture_desc* d, FewArgs* a) {
+  if (!d) return fail(CKAN_ERR_INVALID_ARG, "mixture desc is NULL");
+  for (const int t : {d->x_dtype, d->gate_dtype, d->coeff_dtype})
+    if (t != CKAN_DTYPE_F32 && t != CKAN_DTYPE_BF16) return fail(CKAN_ERR_INVALID_ARG, "unknown dtype %d", t);
+  const ckan_experts_desc e = mixture_experts(d);
+  if (const int rc = experts_check(&e)) return rc;
+  const ckan_route_desc r = {d->rows, d->experts, d->experts, d->top_k, d->score, d->groups, d->top_groups, d->renormalize,
+                             CKAN_DTYPE_F32, d->scale};
+  *a = FewArgs{};
+  if (const int rc = route_args(&r, &a->route)) return rc;
+  a->x_bf16 = d->x_dtype == CKAN_DTYPE_BF16;
+  a->gate_bf16 = d->gate_dtype == CKAN_DTYPE_BF16;
+  if (d->rows) a->p = experts_plan(&e);
+  return CKAN_OK;
+}
+
 // The largest |b s^2 + c s^4| and |a + b s^2 + c s^4|, the iteration's matrices, that
 // singular values in [0, 1] can reach over all steps, by sampling the interval.
 double ortho_reach(const ckan_ortho_desc* d) {
@@ -214,7 +234,7 @@ int ckan_experts_forward(const ckan_experts_desc* desc, const void* x, const voi
   a.y = y;
   if (!saved && a.p.stream) {
     a.ws = (char*)ws;
-    launch_experts_stream(a, reinterpret_cast<hipStream_t>(stream));
+    launch_experts_stream(a, a.p.bf16, reinterpret_cast<hipStream_t>(stream));
     return check_launch("experts_forward");
   }
   a.saved = saved ? (char*)saved : (char*)ws;
@@ -292,6 +312,41 @@ int ckan_muon_step(const ckan_ortho_desc* desc, float* p, const float* g, float*
   a.nesterov = nesterov != 0;
   launch_ortho(a, ws, reinterpret_cast<hipStream_t>(stream));
   return check_launch("muon_step");
+}
+
+int ckan_mixture_few(const ckan_mixture_desc* desc) {
+  FewArgs a;
+  return mixture_args(desc, &a) == CKAN_OK && desc->rows > 0 && a.p.stream;
+}
+
+size_t ckan_mixture_workspace_bytes(const ckan_mixture_desc* desc) {
+  FewArgs a;
+  return mixture_args(desc, &a) || desc->rows == 0 || !a.p.stream ? 0 : few_workspace_bytes(a);
+}
+
+int ckan_mixture_forward(const ckan_mixture_desc* desc, const void* x, const void* gate, const void* coeffs,
+                         const float* bias, void* y, float* weights, int64_t* indices, void* ws, size_t ws_bytes,
+                         void* stream) {
+  FewArgs a;
+  if (const int rc = mixture_args(desc, &a)) return rc;
+  if (desc->rows == 0) return CKAN_OK;
+  if (!a.p.stream) return fail(CKAN_ERR_UNSUPPORTED, "mixture_forward: too many rows for its form, use the parts' entry points");
+  if (!x || !gate || !coeffs || !y || !weights || !indices) return fail(CKAN_ERR_INVALID_ARG, "mixture_forward: NULL pointer");
+  const size_t need = few_workspace_bytes(a);
+  if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "mixture workspace too small: %zu < %zu bytes", ws_bytes, need);
+  if (!ws || !is_al16(ws)) return fail(CKAN_ERR_INVALID_ARG, "mixture_forward: workspace is NULL or not 16-byte aligned");
+  if (!is_al16(x) || !is_al16(gate) || !is_al16(coeffs) || !is_al16(y))
+    return fail(CKAN_ERR_INVALID_ARG, "mixture_forward: x, gate, coeffs and y must be 16-byte aligned");
+  a.x = x;
+  a.gate = gate;
+  a.coeffs = coeffs;
+  a.y = y;
+  a.ws = (char*)ws;
+  a.route.bias = bias;
+  a.route.weights = weights;
+  a.route.indices = indices;
+  launch_few(a, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("mixture_forward");
 }
 
 int ckan_route(const ckan_route_desc* desc, const void* logits, const float* bias, float* weights,

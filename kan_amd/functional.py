@@ -535,5 +535,6 @@ def jacobian(x: torch.Tensor, coeffs: torch.Tensor, spec, affine=None) -> torch.
 
 
 # public operators of this namespace that live in modules of their own
-from .mixture import kan_experts, route  # noqa: E402
+from .mixture import kan_experts, kan_mixture, route  # noqa: E402
 from .orthogonal import orthogonalize  # noqa: E402
+from .block import LogProbs, dropout, log_probs, residual_norm, row_norm  # noqa: E402

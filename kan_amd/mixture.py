@@ -232,6 +232,65 @@ def kan_experts(x: torch.Tensor, coeffs: torch.Tensor, indices: torch.Tensor,
     return _experts_forward(x, coeffs, indices, weights, desc, keep=False)[0]
 
 
+def _gate_logits(x: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
+    """x gate^T in fp32, inside autocast too: the choice hangs on it."""
+    if not torch.is_autocast_enabled(x.device.type):
+        return x @ gate.t()
+    with torch.autocast(x.device.type, enabled=False):
+        return x @ gate.t()
+
+
+def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k: int, *, score: str = "softmax",
+                bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+                scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A whole mixture layer: (y, weights, indices) with ``route``'s choice among the experts by
+    the logits x gate^T and y[t] = sum_j weights[t, j] f_e(x[t]) as ``kan_experts``'.
+
+    ``x`` [rows, in], ``gate`` [experts, in] and ``coeffs`` [experts, in, out, degree+1] are fp32 or
+    bf16 each; y [rows, out] has x's dtype, weights and indices are ``route``'s.  Few rows without a
+    gradient (up to 1024 slots, 16 an expert on average) take a form of their own: the gate's sums in 64
+    bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
+    product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (on x in the coefficients'
+    dtype), differentiable as they are in x, gate and coeffs."""
+    if score not in _SCORES:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+    _lib.refuse_tangents("kan_mixture", x, gate, coeffs)
+    _require_device(x, gate, coeffs, bias)
+    codes = [_dtype_code(t, name) for t, name in ((x, "x"), (gate, "gate"), (coeffs, "coeffs"))]
+    if coeffs.dim() != 4:
+        raise RuntimeError(f"coeffs must be [experts, in, out, degree+1], got {tuple(coeffs.shape)}")
+    experts, in_dim, out_dim, dd = coeffs.shape
+    if x.dim() != 2 or x.shape[1] != in_dim:
+        raise RuntimeError(f"x must be [rows, {in_dim}], got {tuple(x.shape)}")
+    if tuple(gate.shape) != (experts, in_dim):
+        raise RuntimeError(f"gate must be [{experts}, {in_dim}], got {tuple(gate.shape)}")
+    if bias is not None and tuple(bias.shape) != (experts,):
+        raise RuntimeError(f"bias must be [{experts}], got {tuple(bias.shape)}")
+    rows, lib = x.shape[0], _lib.load()
+    desc = _lib.CkanMixtureDesc(rows, experts, int(top_k), in_dim, out_dim, dd - 1, _SCORES[score], int(groups),
+                                int(top_groups), int(bool(renormalize)), *codes, float(scale))
+    trains = torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or coeffs.requires_grad)
+    if trains or not lib.ckan_mixture_few(desc):
+        weights, indices = route(_gate_logits(x.to(torch.float32), gate.to(torch.float32)), top_k, score=score, bias=bias,
+                                 groups=groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
+        return kan_experts(x.to(coeffs.dtype), coeffs, indices, weights).to(x.dtype), weights, indices
+    dev = x.device
+    x, gate, coeffs = _aligned(x), _aligned(gate), _aligned(coeffs)
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    y = torch.empty(rows, out_dim, dtype=x.dtype, device=dev)
+    weights = torch.empty(rows, desc.top_k, dtype=torch.float32, device=dev)
+    indices = torch.empty(rows, desc.top_k, dtype=torch.int64, device=dev)
+    nbytes = lib.ckan_mixture_workspace_bytes(desc)
+    # from torch's allocator on the current stream: reused by it in stream order
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(lib.ckan_mixture_forward(desc, x.data_ptr(), gate.data_ptr(), coeffs.data_ptr(), _lib.ptr(bias),
+                                            y.data_ptr(), weights.data_ptr(), indices.data_ptr(), ws.data_ptr(), nbytes,
+                                            _stream(dev)))
+    return y, weights, indices
+
+
 class MixtureKANLayer(nn.Module):
     """A mixture of ChebyKAN layers: each row goes to ``top_k`` of ``experts`` layers of
     ``ChebyKANLayer(input_dim, output_dim, degree)`` (kan/layers/chebykan.py:21-51), chosen
@@ -240,9 +299,10 @@ class MixtureKANLayer(nn.Module):
     Parameters: ``gate`` [experts, input_dim] and ``cheby_coeffs`` [experts, input_dim,
     output_dim, degree+1], each expert initialised as the layer is.  ``compute``: 'fp32'
     or 'bf16' (the experts' operands and outputs are bf16, the gate, the choice and the
-    weights stay fp32; the output is fp32, as a ChebyKANLayer's).  'bf16' casts the
-    coefficients of all experts in every forward: to serve single rows in bf16, call
-    ``kan_experts`` on coefficients cast once.
+    weights stay fp32; the output is fp32, as a ChebyKANLayer's).  Few rows without a
+    gradient go through ``kan_mixture`` on the fp32 parameters in either mode; otherwise 'bf16' casts the
+    coefficients of all experts in every forward.  To serve rows from bf16 coefficients, call
+    ``kan_mixture`` on coefficients cast once.
 
     With ``balance``, a per-expert bias steers the choice, not the weights:
     ``update_balance`` moves it towards experts that got fewer rows than the mean."""
@@ -274,22 +334,25 @@ class MixtureKANLayer(nn.Module):
         self.register_buffer("balance_bias", torch.zeros(experts) if balance else None)
         self._last_indices: Optional[torch.Tensor] = None
 
-    def _logits(self, x: torch.Tensor) -> torch.Tensor:
-        if not torch.is_autocast_enabled(x.device.type):
-            return x @ self.gate.t()
-        with torch.autocast(x.device.type, enabled=False):  # the choice is fp32's there too
-            return x @ self.gate.t()
-
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = x.reshape(-1, self.input_dim).to(torch.float32)
-        weights, indices = route(self._logits(x), self.top_k, score=self.score, bias=self.balance_bias,
-                                 groups=self.groups, top_groups=self.top_groups, renormalize=self.renormalize,
-                                 scale=self.scale)
+        how = dict(score=self.score, bias=self.balance_bias, groups=self.groups, top_groups=self.top_groups,
+                   renormalize=self.renormalize, scale=self.scale)
+        if self.compute == "fp32" or self._few(x):
+            y, _, indices = kan_mixture(x, self.gate, self.cheby_coeffs, self.top_k, **how)
+        else:
+            weights, indices = route(_gate_logits(x, self.gate), self.top_k, **how)
+            y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights).to(torch.float32)
         self._last_indices = indices if self.balance_bias is not None else None
-        if self.compute == "fp32":
-            return kan_experts(x, self.cheby_coeffs, indices, weights)
-        y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights)
-        return y.to(torch.float32)
+        return y
+
+    def _few(self, x: torch.Tensor) -> bool:
+        """Whether ``kan_mixture`` would take its own form for x."""
+        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+            return False
+        desc = _lib.CkanMixtureDesc(x.shape[0], self.experts, self.top_k, self.input_dim, self.output_dim, self.degree,
+                                    _SCORES[self.score], self.groups, self.top_groups, 1, 0, 0, 0, self.scale)
+        return bool(_lib.load().ckan_mixture_few(desc))
 
     @torch.no_grad()
     def update_balance(self, speed: float = 1e-3) -> None:
