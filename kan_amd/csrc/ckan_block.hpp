@@ -65,6 +65,41 @@ __device__ __forceinline__ void store8(T* p, int64_t left, const float (&f)[kChu
   }
 }
 
+// The same where `room` values from p on may be read, at least `left` of them the row's:
+// a row's partial chunk in one access, its surplus left to zero_past.
+template <typename T>
+__device__ __forceinline__ typename RawOf<T>::type load_room8(const T* p, int left, int64_t room) {
+  if (left > 0 && room >= kChunk) return *(const typename RawOf<T>::type*)p;
+  return load_raw8(p, (int64_t)left);
+}
+__device__ __forceinline__ void zero_past(int left, float (&f)[kChunk]) {
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) f[i] = i < left ? f[i] : 0.0f;
+}
+
+// The sum over a group of L lanes (8, 16, 32 or 64, aligned), in each of them: butterflies
+// on the vector ALU, so every lane has the same bits.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = dpp_add<0xb1>(v);   // lanes 1, 0, 3, 2
+  v = dpp_add<0x4e>(v);   // lanes 2, 3, 0, 1
+  v = dpp_add<0x141>(v);  // the mirror of 8
+  if constexpr (L >= 16) v = dpp_add<0x140>(v);  // the mirror of 16
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
 // A tensor whose type is known at run time (parameters, row gates).
 struct AnyPtr {
   const void* p;

@@ -285,9 +285,10 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_sums(ResidualArgs 
   for (int k = 0; k < kSums; ++k) store8(p + (int64_t)k * a.dim, left, s[k]);
 }
 
-// The partial sums of one column of one parameter, in order.
-__global__ __launch_bounds__(256) void k_residual_sums(ResidualArgs a, const float* part, int slabs) {
-  __shared__ float red[4][64];
+// The parts of one parameter's sums: 64 columns a block, a wave every 16th part, each in
+// order, then the waves in order.
+__global__ __launch_bounds__(1024) void k_residual_sums(ResidualArgs a, const float* part, int parts) {
+  __shared__ float red[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = blockIdx.y;
   void* outs[kSums] = {a.dpost_w, a.dpost_b, a.gate_rows ? nullptr : a.dgate, a.dnext_w, a.dnext_b};
   const int types[kSums] = {a.post_w.bf16, a.post_b.bf16, a.gate.bf16, a.next_w.bf16, a.next_b.bf16};
@@ -295,20 +296,433 @@ __global__ __launch_bounds__(256) void k_residual_sums(ResidualArgs a, const flo
   if (!out) return;
   const int64_t col = (int64_t)blockIdx.x * 64 + lane;
   float v = 0.0f;
-  if (col < a.dim)
-    for (int s = wave; s < slabs; s += 4) v += part[((int64_t)s * kSums + k) * a.dim + col];
+  if (col < a.dim) {
+#pragma unroll 8
+    for (int s = wave; s < parts; s += 16) v += part[((int64_t)s * kSums + k) * a.dim + col];
+  }
   red[wave][lane] = v;
   __syncthreads();
   if (wave || col >= a.dim) return;
-  v = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) v += red[w][lane];
   if (types[k])
     ((__bf16*)out)[col] = (__bf16)v;
   else
     ((float*)out)[col] = v;
 }
 
-bool wants_sums(const ResidualArgs& a) {
-  return a.dpost_w || a.dpost_b || a.dnext_w || a.dnext_b || (a.dgate && !a.gate_rows);
+// ---- up to kTeamMaxDim values: a row in the registers of a team of lanes --------------
+//
+// A team of LANES lanes holds a row, N chunks a lane; a block holds several teams and its
+// rows stride over the batch, so that the parameters, and in the backward the sums over
+// rows, stay in registers. Every value of a row is read once, the next row's while this one is
+// worked on.
+template <int LANES, int N, int BLOCK>
+struct Team {
+  static constexpr int kTeams = BLOCK / LANES;
+  static constexpr int kWaves = LANES > 64 ? LANES / 64 : 1;
+  int team, lane, turn;
+  float* red;  // [2][BLOCK / 64][2]
+  __device__ Team(float* lds) : team(threadIdx.x / LANES), lane(threadIdx.x % LANES), turn(0), red(lds) {}
+  // Sums over the team, in every lane; all teams of the block call it together. Two
+  // buffers in turn: a wave writes one again only after the barrier of the sum between, which its
+  // readers reach when they have read it.
+  template <int K>
+  __device__ __forceinline__ void sum(float (&v)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lanes_sum<(LANES < 64 ? LANES : 64)>(v[k]);
+    if constexpr (LANES > 64) {
+      float* r = red + turn * (BLOCK / 64) * 2;
+      turn ^= 1;
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) r[wave * 2 + k] = v[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) t += r[(team * kWaves + w) * 2 + k];
+        v[k] = t;
+      }
+    }
+  }
+};
+
+// A row's values of one tensor as they were read.
+template <typename T, int N>
+struct RowRaw {
+  typename RawOf<T>::type v[N];
+  template <int LANES>
+  __device__ __forceinline__ void load(const T* base, int64_t row, int64_t ld, const ResidualArgs& a, int lane) {
+    const T* p = base + row * ld;
+    const int64_t spare = (a.rows - 1 - row) * ld;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
+      v[n] = load_room8(p + at, left, left + spare);
+    }
+  }
+};
+// The same of a tensor whose type is known at run time.
+template <int N>
+struct RowAny {
+  u32x4_t v[N][2];
+  template <int LANES>
+  __device__ __forceinline__ void load(const AnyPtr& t, int64_t row, int64_t ld, const ResidualArgs& a, int lane) {
+    const int64_t spare = (a.rows - 1 - row) * ld;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
+      if (t.bf16) {
+        v[n][0] = load_room8((const __bf16*)t.p + row * ld + at, left, left + spare).v;
+      } else {
+        const RawF32 r = load_room8((const float*)t.p + row * ld + at, left, left + spare);
+        v[n][0] = r.v[0];
+        v[n][1] = r.v[1];
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(int n, int bf16, float (&f)[kChunk]) const {
+    if (bf16) {
+      unpack8(RawBf16{v[n][0]}, f);
+    } else {
+      RawF32 r;
+      r.v[0] = v[n][0];
+      r.v[1] = v[n][1];
+      unpack8(r, f);
+    }
+  }
+};
+
+// What stays in registers from row to row: the parameters, 0 past the row's end. The
+// gate times scale; 1 or 0 stand for absent ones.
+template <int N>
+struct RowParams {
+  float pw[N][kChunk], pb[N][kChunk], gate[N][kChunk];
+  template <int LANES>
+  __device__ __forceinline__ void load(const ResidualArgs& a, int lane) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        pw[n][i] = pb[n][i] = 0.0f;
+        gate[n][i] = a.scale;
+      }
+      if (left <= 0) continue;
+      if (a.post_w.p) load8(a.post_w, at, left, pw[n]);
+      if (a.post_b.p) load8(a.post_b, at, left, pb[n]);
+      if (a.gate.p && !a.gate_rows) {
+        load8(a.gate, at, left, gate[n]);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
+      }
+    }
+  }
+};
+
+// u (after dropout), y^ in y's place, and out's value in x's.
+template <int N, int LANES>
+__device__ __forceinline__ void row_values(const ResidualArgs& a, const DropKey& key, int64_t row, int lane, float m1, float r1,
+                                           const float (&gate)[N][kChunk], const RowParams<N>& par, float (&x)[N][kChunk],
+                                           float (&y)[N][kChunk], float (&u)[N][kChunk], uint32_t (&keep)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) u[n][i] = y[n][i];
+    if (a.post_w.p) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        y[n][i] = (y[n][i] - m1) * r1;
+        u[n][i] = fmaf(y[n][i], par.pw[n][i], par.pb[n][i]);
+      }
+    }
+    keep[n] = 0xff;
+    if (a.drop.on) {
+      keep[n] = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)(n * LANES + lane));
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) u[n][i] = keep[n] >> i & 1 ? u[n][i] * a.drop.scale : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf(gate[n][i], u[n][i], x[n][i]);
+  }
+}
+
+// The mean (layer norms) and 1 / root mean square of a row's values, which are 0 past its end.
+template <int N, int LANES, typename TEAM>
+__device__ __forceinline__ void row_stats(TEAM& team, const ResidualArgs& a, const float (&v)[N][kChunk], float inv,
+                                          float& mean, float& r) {
+  float s[1] = {0.0f};
+  mean = 0.0f;
+  if (a.layer) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) s[0] += v[n][i];
+    team.sum(s);
+    mean = s[0] * inv;
+    s[0] = 0.0f;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int left = a.dim - (n * LANES + team.lane) * kChunk;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      const float d = i < left ? v[n][i] - mean : 0.0f;
+      s[0] = fmaf(d, d, s[0]);
+    }
+  }
+  team.sum(s);
+  r = 1.0f / sqrtf(fmaf(s[0], inv, a.eps));
+}
+
+template <typename TX, typename TY, int LANES, int N, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_residual_rows(ResidualArgs a) {
+  __shared__ float red[2 * BLOCK / 64 * 2];
+  Team<LANES, N, BLOCK> team(red);
+  const int lane = team.lane;
+  const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
+  if (a.stats && a.drop.on && blockIdx.x == 0 && threadIdx.x == 0) {
+    int64_t* used = (int64_t*)(a.stats + a.rows * kStats);
+    used[0] = a.drop.state ? a.drop.state[0] : (int64_t)a.drop.seed;
+    used[1] = (int64_t)(((uint64_t)key.call1 << 32) | key.call0);
+  }
+  const float inv = 1.0f / (float)a.dim;
+  RowParams<N> par;
+  par.template load<LANES>(a, lane);
+  float nw[N][kChunk] = {}, nb[N][kChunk] = {};
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
+    if (a.next_w.p && left > 0) load8(a.next_w, at, left, nw[n]);
+    if (a.next_b.p && left > 0) load8(a.next_b, at, left, nb[n]);
+  }
+  const int64_t step = (int64_t)gridDim.x * team.kTeams;
+  int64_t row = (int64_t)blockIdx.x * team.kTeams + team.team;
+  RowRaw<TX, N> xr;
+  RowRaw<TY, N> yr;
+  RowAny<N> gr;
+  const auto fetch = [&](int64_t r) {
+    if (r >= a.rows) return;
+    xr.template load<LANES>((const TX*)a.x, r, a.x_ld, a, lane);
+    if (a.y) yr.template load<LANES>((const TY*)a.y, r, a.y_ld, a, lane);
+    if (a.gate_rows) gr.template load<LANES>(a.gate, r, a.gate_ld, a, lane);
+  };
+  fetch(row);
+  // every team of the block takes as many turns as its first: the sums' barriers are the block's
+  for (int64_t first = (int64_t)blockIdx.x * team.kTeams; first < a.rows; first += step, row += step) {
+    const bool active = row < a.rows;
+    float x[N][kChunk], y[N][kChunk], u[N][kChunk], gate[N][kChunk];
+    uint32_t keep[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      unpack8(xr.v[n], x[n]);
+      if (a.y) unpack8(yr.v[n], y[n]);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) gate[n][i] = par.gate[n][i];
+      if (a.gate_rows) {
+        gr.unpack(n, a.gate.bf16, gate[n]);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
+      }
+      if (a.dim & (kChunk - 1)) {
+        const int left = a.dim - (n * LANES + lane) * kChunk;
+        zero_past(left, x[n]);
+        zero_past(left, y[n]);
+        zero_past(left, gate[n]);
+      }
+    }
+    fetch(row + step);
+    float m1 = 0.0f, r1 = 0.0f, m2 = 0.0f, r2 = 0.0f;
+    if (a.y) {
+      if (a.post_w.p) row_stats<N, LANES>(team, a, y, inv, m1, r1);
+      row_values<N, LANES>(a, key, row, lane, m1, r1, gate, par, x, y, u, keep);
+      if (active)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int at = (n * LANES + lane) * kChunk;
+          if (at < a.dim) store8((TX*)a.out + row * a.dim + at, a.dim - at, x[n]);
+        }
+    }
+    if (a.next_w.p) {
+      row_stats<N, LANES>(team, a, x, inv, m2, r2);
+      if (active)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int at = (n * LANES + lane) * kChunk;
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf((x[n][i] - m2) * r2, nw[n][i], nb[n][i]);
+          if (at < a.dim) store8((TY*)a.h + row * a.dim + at, a.dim - at, x[n]);
+        }
+    }
+    if (a.stats && active && lane == 0) *(f32x4_t*)(a.stats + row * kStats) = f32x4_t{m1, r1, m2, r2};
+  }
+}
+
+template <typename TX, typename TY, int LANES, int N, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a, int sums) {
+  __shared__ float red[2 * BLOCK / 64 * 2];
+  __shared__ __align__(16) float tile[BLOCK * kChunk];
+  Team<LANES, N, BLOCK> team(red);
+  const int lane = team.lane;
+  const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
+  const float inv = 1.0f / (float)a.dim;
+  RowParams<N> par;
+  par.template load<LANES>(a, lane);
+  float nw[N][kChunk] = {};
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
+    if (a.next_w.p && left > 0) load8(a.next_w, at, left, nw[n]);
+  }
+  float acc[kSums][N][kChunk] = {};
+  const int64_t step = (int64_t)gridDim.x * team.kTeams;
+  int64_t row = (int64_t)blockIdx.x * team.kTeams + team.team;
+  RowRaw<TX, N> xr, dor;
+  RowRaw<TY, N> yr, dhr;
+  RowAny<N> gr;
+  f32x4_t st;
+  const bool next = a.next_w.p && a.dh, post = a.post_w.p;
+  const auto fetch = [&](int64_t r) {
+    if (r >= a.rows) return;
+    st = *(const f32x4_t*)(a.stats + r * kStats);
+    xr.template load<LANES>((const TX*)a.x, r, a.x_ld, a, lane);
+    if (a.y) yr.template load<LANES>((const TY*)a.y, r, a.y_ld, a, lane);
+    if (a.gate_rows) gr.template load<LANES>(a.gate, r, a.gate_ld, a, lane);
+    if (a.dout) dor.template load<LANES>((const TX*)a.dout, r, a.dout_ld, a, lane);
+    if (a.dh) dhr.template load<LANES>((const TY*)a.dh, r, a.dh_ld, a, lane);
+  };
+  fetch(row);
+  for (int64_t first = (int64_t)blockIdx.x * team.kTeams; first < a.rows; first += step, row += step) {
+    const bool active = row < a.rows;
+    float x[N][kChunk], y[N][kChunk], u[N][kChunk] = {}, gate[N][kChunk], dx[N][kChunk], dh[N][kChunk];
+    uint32_t keep[N];
+    const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      unpack8(xr.v[n], x[n]);
+      if (a.y) unpack8(yr.v[n], y[n]);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) gate[n][i] = par.gate[n][i], dx[n][i] = dh[n][i] = 0.0f;
+      if (a.gate_rows) {
+        gr.unpack(n, a.gate.bf16, gate[n]);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
+      }
+      if (a.dout) unpack8(dor.v[n], dx[n]);
+      if (a.dh) unpack8(dhr.v[n], dh[n]);
+      if (a.dim & (kChunk - 1)) {
+        const int left = a.dim - (n * LANES + lane) * kChunk;
+        zero_past(left, x[n]);
+        zero_past(left, y[n]);
+        zero_past(left, gate[n]);
+        zero_past(left, dx[n]);
+        zero_past(left, dh[n]);
+      }
+    }
+    fetch(row + step);
+    if (a.y) row_values<N, LANES>(a, key, row, lane, m1, r1, gate, par, x, y, u, keep);
+    if (next) {
+      // x becomes o^
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          x[n][i] = (x[n][i] - m2) * r2;
+          if (active) {
+            acc[3][n][i] = fmaf(dh[n][i], x[n][i], acc[3][n][i]);
+            acc[4][n][i] += dh[n][i];
+          }
+          const float g = dh[n][i] * nw[n][i];
+          s[0] = fmaf(g, x[n][i], s[0]);
+          s[1] += g;
+        }
+      team.sum(s);
+      const float go = s[0] * inv, gm = a.layer ? s[1] * inv : 0.0f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) dx[n][i] = fmaf(r2, fmaf(dh[n][i], nw[n][i], -fmaf(x[n][i], go, gm)), dx[n][i]);
+    }
+    if (a.dx && active)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int at = (n * LANES + lane) * kChunk;
+        if (at < a.dim) store8((TX*)a.dx + row * a.dim + at, a.dim - at, dx[n]);
+      }
+    if (!a.y) continue;
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) u[n][i] *= a.scale * dx[n][i];
+      if (a.gate_rows && a.dgate) {
+        const int at = (n * LANES + lane) * kChunk;
+        if (active && at < a.dim) {
+          if (a.gate.bf16)
+            store8((__bf16*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
+          else
+            store8((float*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        float e = gate[n][i] * dx[n][i];
+        if (a.drop.on) e = keep[n] >> i & 1 ? e * a.drop.scale : 0.0f;
+        if (active) {
+          acc[0][n][i] = fmaf(e, y[n][i], acc[0][n][i]);
+          acc[1][n][i] += e;
+          acc[2][n][i] += u[n][i];
+        }
+        if (post) {
+          e *= par.pw[n][i];
+          s[0] = fmaf(e, y[n][i], s[0]);
+          s[1] += e;
+        }
+        dx[n][i] = e;
+      }
+    }
+    if (!a.dy) continue;
+    if (post) {
+      team.sum(s);
+      const float ey = s[0] * inv, em = a.layer ? s[1] * inv : 0.0f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) dx[n][i] = r1 * (dx[n][i] - fmaf(y[n][i], ey, em));
+    }
+    if (active)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int at = (n * LANES + lane) * kChunk;
+        if (at < a.dim) store8((TY*)a.dy + row * a.dim + at, a.dim - at, dx[n]);
+      }
+  }
+  if (!sums) return;
+  // the teams' sums, in order, to this block's part
+  float* part = a.ws + (int64_t)blockIdx.x * kSums * a.dim;
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+    if (!(sums >> k & 1)) continue;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) tile[(team.team * LANES + lane) * kChunk + i] = acc[k][n][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < LANES * kChunk; c += BLOCK) {
+        float v = 0.0f;
+#pragma unroll
+        for (int t = 0; t < team.kTeams; ++t) v += tile[t * LANES * kChunk + c];
+        const int col = n * LANES * kChunk + c;
+        if (col < a.dim) part[(int64_t)k * a.dim + col] = v;
+      }
+    }
+  }
 }
 
 int any_slabs(const ResidualArgs& a) {
@@ -319,28 +733,76 @@ int any_slabs(const ResidualArgs& a) {
   return (int)slabs;
 }
 
+// The parameters' sums that are wanted, as bits.
+int sum_bits(const ResidualArgs& a) {
+  return (a.dpost_w ? 1 : 0) | (a.dpost_b ? 2 : 0) | (a.dgate && !a.gate_rows ? 4 : 0) | (a.dnext_w ? 8 : 0) | (a.dnext_b ? 16 : 0);
+}
+
+constexpr int kTeamMaxDim = 8192;
+
+// Blocks of a launch of teams: as many as the chip holds at once, fewer where rows run out.
+int64_t team_blocks(const ResidualArgs& a, int teams, int per_cu) {
+  const int64_t all = ceil_div(a.rows, teams), most = (int64_t)per_cu * kNumCUs;
+  return all < most ? all : most;
+}
+
+// Calls f<LANES, N, BLOCK>() with the team for a width.
+#define CKAN_TEAM(dim, F)                          \
+  do {                                             \
+    if ((dim) <= 64) { F(8, 1, 512) }              \
+    else if ((dim) <= 128) { F(16, 1, 512) }       \
+    else if ((dim) <= 256) { F(32, 1, 512) }       \
+    else if ((dim) <= 512) { F(64, 1, 512) }       \
+    else if ((dim) <= 1024) { F(128, 1, 512) }     \
+    else if ((dim) <= 2048) { F(256, 1, 512) }     \
+    else if ((dim) <= 4096) { F(512, 1, 512) }     \
+    else { F(1024, 1, 1024) }                      \
+  } while (0)
+
 template <typename TX, typename TY>
 void forward_typed(const ResidualArgs& a, hipStream_t st) {
+  if (a.dim <= kTeamMaxDim) {
+#define CKAN_FORWARD(L, NN, B)                                                                               \
+  hipLaunchKernelGGL((k_residual_rows<TX, TY, L, NN, B>), dim3((unsigned)team_blocks(a, B / L, 2048 / B)), dim3(B), 0, st, a); \
+  return;
+    CKAN_TEAM(a.dim, CKAN_FORWARD);
+#undef CKAN_FORWARD
+  }
   const int64_t blocks = a.rows < 8 * kNumCUs ? a.rows : 8 * kNumCUs;
   hipLaunchKernelGGL((k_residual_any<TX, TY>), dim3((unsigned)blocks), dim3(kAnyThreads), 0, st, a);
 }
 
+constexpr int kPartBlocks = 2;  // blocks a CU of the backward: each leaves a part of every sum
+
 template <typename TX, typename TY>
 void backward_typed(const ResidualArgs& a, hipStream_t st) {
+  const int sums = sum_bits(a);
+  const dim3 sum_grid((unsigned)ceil_div(a.dim, 64), kSums);
+  if (a.dim <= kTeamMaxDim) {
+    int64_t blocks = 0;
+#define CKAN_BACKWARD(L, NN, B)                                                                                          \
+  blocks = team_blocks(a, B / L, kPartBlocks * 512 / B);                                                                  \
+  hipLaunchKernelGGL((k_residual_rows_backward<TX, TY, L, NN, B>), dim3((unsigned)blocks), dim3(B), 0, st, a, sums);
+    CKAN_TEAM(a.dim, CKAN_BACKWARD);
+#undef CKAN_BACKWARD
+    if (sums) hipLaunchKernelGGL(k_residual_sums, sum_grid, dim3(1024), 0, st, a, a.ws, (int)blocks);
+    return;
+  }
   const int64_t blocks = a.rows < 8 * kNumCUs ? a.rows : 8 * kNumCUs;
   hipLaunchKernelGGL((k_residual_any_dx<TX, TY>), dim3((unsigned)blocks), dim3(kAnyThreads), 0, st, a);
-  if (!wants_sums(a)) return;
+  if (!sums) return;
   const int slabs = any_slabs(a);
   float* part = a.ws + round_up(a.rows * 2, 4);
   hipLaunchKernelGGL((k_residual_any_sums<TX, TY>), dim3((unsigned)ceil_div(a.dim, kChunk * kAnyThreads), (unsigned)slabs),
                      dim3(kAnyThreads), 0, st, a, part);
-  hipLaunchKernelGGL(k_residual_sums, dim3((unsigned)ceil_div(a.dim, 64), kSums), dim3(256), 0, st, a, part, slabs);
+  hipLaunchKernelGGL(k_residual_sums, sum_grid, dim3(1024), 0, st, a, part, slabs);
 }
 
 }  // namespace
 
 size_t residual_workspace_bytes(const ResidualArgs& a) {
-  return align256((round_up(a.rows * 2, 4) + (wants_sums(a) ? (int64_t)any_slabs(a) * kSums * a.dim : 0)) * sizeof(float));
+  const int64_t parts = a.dim <= kTeamMaxDim ? kPartBlocks * kNumCUs : any_slabs(a);
+  return align256(((a.dim <= kTeamMaxDim ? 0 : round_up(a.rows * 2, 4)) + parts * kSums * a.dim) * sizeof(float));
 }
 
 void launch_residual_forward(const ResidualArgs& a, hipStream_t st) {
