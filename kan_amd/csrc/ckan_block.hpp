@@ -226,6 +226,8 @@ struct LogpArgs {
   const float *dlogp, *dentropy;  // NULL: zero
   void* dlogits;
   char* ws;
+  int parts, part_len; // a long row's parts (set by the launch)
+  size_t keys_off;
 };
 size_t logprobs_workspace_bytes(const LogpArgs& a);
 void launch_logprobs(const LogpArgs& a, hipStream_t st);

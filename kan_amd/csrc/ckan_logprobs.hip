@@ -120,47 +120,345 @@ __device__ __forceinline__ void write_top(const LogpArgs& a, int64_t row, int j,
 }
 
 constexpr int kThreads = 256;
+constexpr int kTeamMaxClasses = 2048;
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_logprobs_any(LogpArgs a) {
-  __shared__ RowSum sums[kThreads / 64];
-  __shared__ uint64_t best[kThreads / 64];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-  const T* l = (const T*)a.logits + row * a.ld;
-  RowSum r = empty_sum();
-  for (int64_t c = (int64_t)tid * kChunk; c < a.classes; c += kThreads * kChunk) {
-    float v[kChunk];
-    load8(l + c, a.classes - c, v);
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i] = c + i < a.classes ? v[i] : -INFINITY;
-    add_logits(r, v);
+// ---- up to kTeamMaxClasses: a row in the registers of a team of lanes ----------------
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+// The largest over a group of L lanes, in each of them (as lanes_sum).
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+  v = dpp_max<0xb1>(v);
+  v = dpp_max<0x4e>(v);
+  v = dpp_max<0x141>(v);
+  if constexpr (L >= 16) v = dpp_max<0x140>(v);
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
   }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
+}
+
+// One team a row: LANES lanes hold N chunks each. Lane j of the team holds columns j N 8 on, so
+// that the lowest column among equal logits is the lowest lane's lowest. The likeliest classes come
+// in `top` rounds of the team's largest.
+template <typename T, int LANES, int N>
+__global__ __launch_bounds__(kThreads) void k_logprobs_team(LogpArgs a) {
+  const int lane = threadIdx.x % LANES, in_wave = threadIdx.x & 63;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / LANES);
+  // all teams of a wave take the same turns: lanes of rows past the end work on the last row
+  for (int64_t first = (int64_t)blockIdx.x * (kThreads / LANES); first < a.rows; first += step) {
+    const int64_t mine = first + threadIdx.x / LANES, row = mine < a.rows ? mine : a.rows - 1;
+    const T* l = (const T*)a.logits + row * a.ld;
+    float v[N * kChunk];
+    const int64_t spare = (a.rows - 1 - row) * a.ld;
+    typename RawOf<T>::type raw[N];
 #pragma unroll
-  for (int w = 1; w < 64; w <<= 1)
-    r = merged(r, RowSum{__shfl_xor(r.m, w), __shfl_xor(r.n, w), __shfl_xor(r.s, w), __shfl_xor(r.a, w)});
-  if (lane == 0) sums[wave] = r;
+    for (int n = 0; n < N; ++n) {
+      const int at = (lane * N + n) * kChunk, left = a.classes - at;
+      raw[n] = load_room8(l + at, left, left + spare);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int left = a.classes - (lane * N + n) * kChunk;
+      float f[kChunk];
+      unpack8(raw[n], f);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) v[n * kChunk + i] = i < left ? f[i] : -INFINITY;
+    }
+    RowSum r = empty_sum();
+#pragma unroll
+    for (int i = 0; i < N * kChunk; ++i) r.m = fmaxf(r.m, v[i]);
+    r.m = lanes_max<LANES>(r.m);
+#pragma unroll
+    for (int i = 0; i < N * kChunk; ++i) {
+      const float d = v[i] - r.m, e = exp_of(d);
+      const bool top = v[i] == r.m;
+      r.n += top ? 1.0f : 0.0f;
+      r.s += top ? 0.0f : e;
+      r.a = fmaf(e, fmaxf(d, kFar), r.a);
+    }
+    r.n = lanes_sum<LANES>(r.n);
+    r.s = lanes_sum<LANES>(r.s);
+    r.a = lanes_sum<LANES>(r.a);
+    const RowResult q = row_result(r);
+    const bool write = mine < a.rows;
+    if (lane == 0 && write) write_row(a, row, q);
+    for (int j = 0; j < a.top; ++j) {
+      float own = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < N * kChunk; ++i) own = fmaxf(own, v[i]);
+      const float best = lanes_max<LANES>(own);
+      const unsigned long long has = __ballot(own == best && best > -INFINITY) >> (in_wave & ~(LANES - 1));
+      const unsigned long long team = LANES == 64 ? has : has & ((1ull << (LANES & 63)) - 1);
+      const int from = team ? __ffsll(team) - 1 : -1;
+      if (lane == from) {
+        int at = N * kChunk - 1;
+#pragma unroll
+        for (int i = N * kChunk - 2; i >= 0; --i) at = v[i] == best ? i : at;
+#pragma unroll
+        for (int i = 0; i < N * kChunk; ++i) v[i] = i == at ? -INFINITY : v[i];
+        if (write) {
+          a.top_logp[row * a.top + j] = (best - q.m) - q.logs;
+          a.top_idx[row * a.top + j] = (int64_t)lane * N * kChunk + at;
+        }
+      } else if (from < 0 && lane == 0 && write) {
+        write_top(a, row, j, 0, q);
+      }
+    }
+  }
+}
+
+// ---- longer rows: a block a row, or a part of one ------------------------------------
+constexpr int kMaxParts = 32;
+constexpr int kPartMin = 4096;        // logits a part is worth
+constexpr int kCandidates = 1024;
+constexpr int kWaves = kThreads / 64;
+
+// Lanes whose condition holds count up in thread order: the thread's place, and the total.
+__device__ __forceinline__ int block_place(bool mine, int* counts, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long has = __ballot(mine);
+  if (lane == 0) counts[wave] = __popcll(has);
   __syncthreads();
-  r = sums[0];
-  for (int w = 1; w < kThreads / 64; ++w) r = merged(r, sums[w]);
-  const RowResult q = row_result(r);
-  if (tid == 0) write_row(a, row, q);
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? counts[w] : 0;
+    total += counts[w];
+  }
+  __syncthreads();
+  return before + __popcll(has & ((1ull << lane) - 1));
+}
+
+struct TopShared {
+  float most[kThreads];
+  int list[kThreads], counts[kWaves];
+  int found, bound;
+  float threshold;
+  uint64_t keys[kCandidates];
+  uint64_t best[kWaves];
+};
+
+// The `top` largest keys of a block's logits [c0, c1) of a row, each handed to out(j, key) once (key
+// 0 where there is none). `most` is the thread's largest logit (-inf: none) and `seen` the
+// column of the chunk that first held it; chunk i of thread t lies at begin + (i kThreads + t) 8,
+// and a thread may hold columns outside of them (`edge` on, `edges` of them: thread t has
+// edge + t).
+//
+// At least `top` threads have a largest of at least the top-th largest among the threads' largest, so
+// the logits from this threshold on hold the answer, and hardly more than it: those of the few
+// threads that reach it are read again, by the whole block. Of logits equal to the
+// threshold only columns up to a bound count, that of the first `top` threads that hold it, so that rows of equal
+// logits give few candidates too. The candidates' ranks among each other are their places. Where
+// they are too many after all, `top` rounds over the row find the answer.
+template <typename T, typename F>
+__device__ __forceinline__ void block_top(const T* l, int top, int begin, int chunks, int edge0, int edges0, int edge1, int edges1,
+                                          int c0, int c1, float most, int seen, TopShared& sh, const F& out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  sh.most[tid] = most;
+  if (tid == 0) {
+    sh.found = 0;
+    sh.bound = -1;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    float v[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v[w] = sh.most[w * 64 + lane];
+    float best = INFINITY;
+    for (int j = 0; j < top && best > -INFINITY; ++j) {
+      float own = v[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) own = fmaxf(own, v[w]);
+      best = wave_max(own);
+      if (lane == __ffsll((unsigned long long)__ballot(own == best)) - 1) {
+        bool gone = false;  // one of them
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const bool here = !gone && v[w] == best;
+          v[w] = here ? -INFINITY : v[w];
+          gone = gone || here;
+        }
+      }
+    }
+    if (lane == 0) sh.threshold = best;
+  }
+  __syncthreads();
+  const float threshold = sh.threshold;  // -inf: fewer than `top` threads hold any
+  int total, reach;
+  const int order = block_place(most == threshold && most > -INFINITY, sh.counts, total);
+  if (most == threshold && most > -INFINITY && order < top) atomicMax(&sh.bound, seen + kChunk - 1);
+  const int place = block_place(most >= threshold && most > -INFINITY, sh.counts, reach);
+  if (most >= threshold && most > -INFINITY) sh.list[place] = tid;
+  __syncthreads();
+  const int bound = total >= top ? sh.bound : c1;
+  const auto offer = [&](float v, int c) {
+    if ((v > threshold || (v == threshold && c <= bound)) && v > -INFINITY) {
+      const int at = atomicAdd(&sh.found, 1);
+      if (at < kCandidates) sh.keys[at] = top_key(v, c);
+    }
+  };
+  const int turns = (chunks + kThreads - 1) / kThreads;
+  for (int p = tid; p < reach * turns; p += kThreads) {
+    const int i = p / reach, t = sh.list[p - i * reach], q = i * kThreads + t;
+    if (q >= chunks) continue;
+    float f[kChunk];
+    load8(l + begin + q * kChunk, (int64_t)kChunk, f);
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) offer(f[e], begin + q * kChunk + e);
+  }
+  if (tid < edges0) offer((float)l[edge0 + tid], edge0 + tid);
+  if (tid < edges1) offer((float)l[edge1 + tid], edge1 + tid);
+  __syncthreads();
+  const int found = sh.found;
+  if (found <= kCandidates) {
+    for (int i = tid; i < found; i += kThreads) {
+      const uint64_t key = sh.keys[i];
+      int rank = 0;
+      for (int o = 0; o < found; ++o) rank += sh.keys[o] > key;
+      if (rank < top) out(rank, key);
+    }
+    for (int j = found + tid; j < top; j += kThreads) out(j, 0);
+    __syncthreads();
+    return;
+  }
   uint64_t last = ~0ull;
-  for (int j = 0; j < a.top; ++j) {
+  for (int j = 0; j < top; ++j) {
     uint64_t mine = 0;
-    for (int c = tid; c < a.classes; c += kThreads) {
+    for (int c = c0 + tid; c < c1; c += kThreads) {
       const uint64_t k = top_key((float)l[c], c);
       mine = k < last && k > mine ? k : mine;
     }
     mine = wave_max64(mine);
     __syncthreads();
-    if (lane == 0) best[wave] = mine;
+    if (lane == 0) sh.best[wave] = mine;
     __syncthreads();
-    last = best[0];
-    for (int w = 1; w < kThreads / 64; ++w) last = best[w] > last ? best[w] : last;
-    if (tid == 0) write_top(a, row, j, last, q);
+    last = sh.best[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) last = sh.best[w] > last ? sh.best[w] : last;
+    if (tid == 0) out(j, last);
   }
   __syncthreads();
+}
+
+__device__ __forceinline__ RowSum block_sums(RowSum r, RowSum* sums) {
+  const float m = wave_max(r.m);
+  raise(r, m);
+  r = {m, lanes_sum<64>(r.n), lanes_sum<64>(r.s), lanes_sum<64>(r.a)};
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = r;
+  __syncthreads();
+  r = sums[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) r = merged(r, sums[w]);
+  return r;
+}
+
+// The parts of a row: their sums and largest keys, for k_logprobs_join.
+__device__ __forceinline__ RowSum* part_sums(const LogpArgs& a, int64_t row) { return (RowSum*)a.ws + row * a.parts; }
+__device__ __forceinline__ uint64_t* part_keys(const LogpArgs& a, int64_t row) {
+  return (uint64_t*)(a.ws + a.keys_off) + row * a.parts * a.top;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_logprobs_block(LogpArgs a) {
+  __shared__ RowSum sums[kWaves];
+  __shared__ TopShared sh;
+  const int tid = threadIdx.x, part = blockIdx.y;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* l = (const T*)a.logits + row * a.ld;
+    const int c0 = part * a.part_len, c1 = a.classes - c0 < a.part_len ? a.classes : c0 + a.part_len;
+    // chunks at 16-byte addresses (unaligned ones cost up to half of the bandwidth); what lies before
+    // and after them goes one by one to the first threads
+    const int off = (int)(((uintptr_t)(l + c0) & 15) / sizeof(T)), per16 = 16 / (int)sizeof(T);
+    int head = off ? per16 - off : 0;
+    if (head > c1 - c0) head = c1 - c0;
+    const int begin = c0 + head, chunks = (c1 - begin) / kChunk, tail = begin + chunks * kChunk;
+    RowSum r = empty_sum();
+    float edge = -INFINITY, edge2 = -INFINITY;
+    if (tid < head) edge = (float)l[c0 + tid];
+    if (tid < c1 - tail) edge2 = (float)l[tail + tid];
+    int seen = 0;
+    const T* p = l + begin;
+#pragma unroll 2
+    for (int q = tid; q < chunks; q += kThreads) {
+      float v[kChunk];
+      unpack8(*(const typename RawOf<T>::type*)__builtin_assume_aligned(p + (int64_t)q * kChunk, 16), v);
+      const float before = r.n > 0.0f ? r.m : -INFINITY;  // the lowest finite value is a largest too
+      add_logits(r, v);
+      seen = r.n > 0.0f && r.m > before ? begin + q * kChunk : seen;
+    }
+    const float most = r.n > 0.0f ? r.m : -INFINITY;
+    {
+      const float v[2] = {edge, edge2};
+      add_logits(r, v);
+    }
+    r = block_sums(r, sums);
+    if (a.parts > 1) {
+      if (tid == 0) part_sums(a, row)[part] = r;
+      if (a.top) {
+        uint64_t* keys = part_keys(a, row) + part * a.top;
+        block_top(l, a.top, begin, chunks, c0, head, tail, c1 - tail, c0, c1, most, seen, sh,
+                  [&](int j, uint64_t key) { keys[j] = key; });
+      }
+    } else {
+      const RowResult q = row_result(r);
+      if (tid == 0) write_row(a, row, q);
+      if (a.top)
+        block_top(l, a.top, begin, chunks, c0, head, tail, c1 - tail, c0, c1, most, seen, sh,
+                  [&](int j, uint64_t key) { write_top(a, row, j, key, q); });
+    }
+    __syncthreads();
+  }
+}
+
+// A row's result from its parts. Their keys lie in falling order; with c = ceil(top /
+// parts), every part has c keys from the least of the parts' c-th on, top in all, and one part has top keys from
+// its last on: keys below either are not among the likeliest.
+__global__ __launch_bounds__(kThreads) void k_logprobs_join(LogpArgs a) {
+  __shared__ uint64_t keys[kMaxParts * kLogpMaxTop], floors[kMaxParts][2];
+  __shared__ int found;
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    RowSum r = part_sums(a, row)[0];
+    for (int p = 1; p < a.parts; ++p) r = merged(r, part_sums(a, row)[p]);
+    const RowResult q = row_result(r);
+    if (tid == 0) write_row(a, row, q);
+    if (!a.top) continue;
+    const uint64_t* from = part_keys(a, row);
+    const int c = (a.top + a.parts - 1) / a.parts;
+    if (tid < a.parts) {
+      floors[tid][0] = from[tid * a.top + a.top - 1];
+      floors[tid][1] = from[tid * a.top + c - 1];
+    }
+    if (tid == 0) found = 0;
+    __syncthreads();
+    uint64_t most = 1, least = ~0ull;  // 1: keys of 0 are none
+    for (int p = 0; p < a.parts; ++p) {
+      most = floors[p][0] > most ? floors[p][0] : most;
+      least = floors[p][1] < least ? floors[p][1] : least;
+    }
+    const uint64_t floor = least > most ? least : most;
+    for (int i = tid; i < a.parts * a.top; i += kThreads) {
+      const uint64_t k = from[i];
+      if (k >= floor) keys[atomicAdd(&found, 1)] = k;
+    }
+    __syncthreads();
+    for (int i = tid; i < found; i += kThreads) {
+      const uint64_t key = keys[i];
+      int rank = 0;
+      for (int o = 0; o < found; ++o) rank += keys[o] > key;
+      if (rank < a.top) write_top(a, row, rank, key, q);
+    }
+    for (int j = found + tid; j < a.top; j += kThreads) write_top(a, row, j, 0, q);
+    __syncthreads();
   }
 }
 
@@ -192,16 +490,56 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_backward(LogpArgs a) {
   }
 }
 
+
+// Parts of a row: one where rows fill the chip, else as many as leave kPartMin logits each
+// or two blocks a CU.
+void logprobs_plan(LogpArgs& a) {
+  a.parts = 1;
+  if (a.classes > kTeamMaxClasses && a.rows < 2 * kNumCUs) {
+    int64_t parts = ceil_div(a.classes, kPartMin);
+    if (parts > ceil_div(2 * kNumCUs, a.rows)) parts = ceil_div(2 * kNumCUs, a.rows);
+    a.parts = (int)(parts < kMaxParts ? parts : kMaxParts);
+  }
+  // whole chunks, so that parts begin at one alignment
+  a.part_len = (int)round_up(ceil_div(a.classes, a.parts), kChunk);
+  a.parts = (int)ceil_div(a.classes, a.part_len);
+  a.keys_off = align256((size_t)a.rows * a.parts * sizeof(RowSum));
+}
+
+template <typename T>
+void forward_typed(const LogpArgs& a, hipStream_t st) {
+  if (a.classes <= kTeamMaxClasses) {
+#define CKAN_LOGP_TEAM(L, NN)                                                                                       \
+  if (a.classes <= L * NN * kChunk) {                                                                               \
+    const int64_t blocks = ceil_div(a.rows, kThreads / L);                                                          \
+    hipLaunchKernelGGL((k_logprobs_team<T, L, NN>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),         \
+                       dim3(kThreads), 0, st, a);                                                                   \
+    return;                                                                                                         \
+  }
+    CKAN_LOGP_TEAM(8, 1) CKAN_LOGP_TEAM(16, 1) CKAN_LOGP_TEAM(32, 1) CKAN_LOGP_TEAM(64, 1) CKAN_LOGP_TEAM(64, 2)
+    CKAN_LOGP_TEAM(64, 4)
+#undef CKAN_LOGP_TEAM
+  }
+  const unsigned rows = (unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20);
+  hipLaunchKernelGGL((k_logprobs_block<T>), dim3(rows, (unsigned)a.parts), dim3(kThreads), 0, st, a);
+  if (a.parts > 1) hipLaunchKernelGGL(k_logprobs_join, dim3(rows), dim3(kThreads), 0, st, a);
+}
+
 }  // namespace
 
-size_t logprobs_workspace_bytes(const LogpArgs&) { return 0; }
+size_t logprobs_workspace_bytes(const LogpArgs& a) {
+  LogpArgs b = a;
+  logprobs_plan(b);
+  return b.parts > 1 ? align256(b.keys_off + (size_t)b.rows * b.parts * b.top * sizeof(uint64_t)) : 0;
+}
 
-void launch_logprobs(const LogpArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.rows < 65536 ? a.rows : 65536));
+void launch_logprobs(const LogpArgs& args, hipStream_t st) {
+  LogpArgs a = args;
+  logprobs_plan(a);
   if (a.bf16)
-    hipLaunchKernelGGL((k_logprobs_any<__bf16>), grid, dim3(kThreads), 0, st, a);
+    forward_typed<__bf16>(a, st);
   else
-    hipLaunchKernelGGL((k_logprobs_any<float>), grid, dim3(kThreads), 0, st, a);
+    forward_typed<float>(a, st);
 }
 
 void launch_logprobs_backward(const LogpArgs& a, hipStream_t st) {
