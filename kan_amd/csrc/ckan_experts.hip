@@ -1312,7 +1312,7 @@ __device__ __forceinline__ void stream_unpack(const __bf16* row, int o, const ui
 // coefficients' stream: two experts of 2048 -> 2048, degree 8, bf16, for one row 30 us
 // (5.0 TB/s; a large copy reaches 5.15), 96 slots of 16 experts of 512 -> 512 in fp32
 // 34 us (4.5 TB/s).
-template <typename T, typename TX, int D>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void k_experts_stream(ExpertsArgs a) {
   constexpr int kDeg = D - 1, kW = (kDeg + 3) / 4 * 4, kU = 4;
   constexpr int kN = sizeof(T) == 4 ? StreamRow<D>::kF32 : StreamRow<D>::kBf16;
@@ -1347,7 +1347,7 @@ __global__ __launch_bounds__(256) void k_experts_stream(ExpertsArgs a) {
     const int nr = n - r0 < kStreamRows ? n - r0 : kStreamRows;
     for (int q = tid; q < ni * nr; q += 256) {
       const int r = q / ni, i = q - r * ni;
-      const float t = tanhf((float)((const TX*)a.x)[(int64_t)(slots[r0 + r] / p.k) * p.I + i0 + i]);
+      const float t = tanhf((float)((const T*)a.x)[(int64_t)(slots[r0 + r] / p.k) * p.I + i0 + i]);
       float* b = basis + (i * kStreamRows + r) * kW;
       float ta = 1.0f, tb = t;
 #pragma unroll
@@ -1412,20 +1412,20 @@ __global__ __launch_bounds__(256) void k_experts_stream_sum(ExpertsArgs a) {
   ((T*)a.y)[q] = (T)v;
 }
 
-template <typename T, typename TX>
+template <typename T>
 void stream_typed(const ExpertsArgs& a, hipStream_t st) {
   const ExpertsPlan& p = a.p;
   const dim3 grid((unsigned)(p.chunks * ((p.O + 63) / 64) * p.E)), block(256);
   switch (p.D) {
 #define CKAN_STREAM_CASE(N) \
-  case N: hipLaunchKernelGGL((k_experts_stream<T, TX, N>), grid, block, 0, st, a); break;
+  case N: hipLaunchKernelGGL((k_experts_stream<T, N>), grid, block, 0, st, a); break;
     CKAN_STREAM_CASE(2) CKAN_STREAM_CASE(3) CKAN_STREAM_CASE(4) CKAN_STREAM_CASE(5) CKAN_STREAM_CASE(6)
     CKAN_STREAM_CASE(7) CKAN_STREAM_CASE(8) CKAN_STREAM_CASE(9) CKAN_STREAM_CASE(10) CKAN_STREAM_CASE(11)
     CKAN_STREAM_CASE(12) CKAN_STREAM_CASE(13) CKAN_STREAM_CASE(14) CKAN_STREAM_CASE(15) CKAN_STREAM_CASE(16)
     CKAN_STREAM_CASE(17)
 #undef CKAN_STREAM_CASE
   }
-  hipLaunchKernelGGL((k_experts_stream_sum<TX>), dim3((unsigned)ceil_div(p.T * p.O, 256)), block, 0, st, a);
+  hipLaunchKernelGGL((k_experts_stream_sum<T>), dim3((unsigned)ceil_div(p.T * p.O, 256)), block, 0, st, a);
 }
 
 template <int NP, int P, int FN>
@@ -1522,11 +1522,11 @@ void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st) {
   }
 }
 
-void launch_experts_stream(const ExpertsArgs& a, bool x_bf16, hipStream_t st) {
+void launch_experts_stream(const ExpertsArgs& a, hipStream_t st) {
   if (a.p.bf16)
-    x_bf16 ? stream_typed<__bf16, __bf16>(a, st) : stream_typed<__bf16, float>(a, st);
+    stream_typed<__bf16>(a, st);
   else
-    x_bf16 ? stream_typed<float, __bf16>(a, st) : stream_typed<float, float>(a, st);
+    stream_typed<float>(a, st);
 }
 
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st) {

@@ -131,23 +131,26 @@ struct ExpertsArgs {
   char *saved, *ws;
 };
 void launch_experts_forward(const ExpertsArgs& a, bool keep, hipStream_t st);
-// The forward without a backward of few slots (p.stream); x and y may have another type
-// than the coefficients.
-void launch_experts_stream(const ExpertsArgs& a, bool x_bf16, hipStream_t st);
+// The forward without a backward of few slots (p.stream).
+void launch_experts_stream(const ExpertsArgs& a, hipStream_t st);
 void launch_experts_backward(const ExpertsArgs& a, hipStream_t st);
 
 // ---- a mixture layer for few rows (ckan_few.hip) ---------------------------------
 // Gate, choice, experts and their sum without a backward.
 struct FewArgs {
-  RouteArgs route;     // rows, experts, choice; logits in the workspace
-  ExpertsPlan p;
+  RouteArgs route;     // rows, experts, choice; the outputs' weights and indices
+  int I, O, D, S;      // S: slots, rows top_k
   const void *x, *gate, *coeffs;
-  int x_bf16, gate_bf16;
+  int x_bf16, gate_bf16, coeff_bf16;
   void* y;
   char* ws;
+  // the launch's plan (few_plan)
+  bool few;            // whether this form takes the call
+  bool apart;          // logits by a launch of their own
+  int active, chunks, chunk_inputs;
+  size_t part_off, ws_bytes;
 };
-inline size_t few_logits_bytes(const FewArgs& a) { return align256((size_t)a.route.rows * a.route.E * sizeof(float)); }
-inline size_t few_workspace_bytes(const FewArgs& a) { return few_logits_bytes(a) + a.p.stream_bytes; }
+void few_plan(FewArgs* a);
 void launch_few(const FewArgs& a, hipStream_t st);
 
 size_t ortho_workspace_bytes(const OrthoArgs& a);

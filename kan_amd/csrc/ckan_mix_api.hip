@@ -124,7 +124,11 @@ int mixture_args(const ckan_mixture_desc* d, FewArgs* a) {
   if (const int rc = route_args(&r, &a->route)) return rc;
   a->x_bf16 = d->x_dtype == CKAN_DTYPE_BF16;
   a->gate_bf16 = d->gate_dtype == CKAN_DTYPE_BF16;
-  if (d->rows) a->p = experts_plan(&e);
+  a->coeff_bf16 = d->coeff_dtype == CKAN_DTYPE_BF16;
+  a->I = d->in_dim;
+  a->O = d->out_dim;
+  a->D = d->degree + 1;
+  few_plan(a);
   return CKAN_OK;
 }
 
@@ -234,7 +238,7 @@ int ckan_experts_forward(const ckan_experts_desc* desc, const void* x, const voi
   a.y = y;
   if (!saved && a.p.stream) {
     a.ws = (char*)ws;
-    launch_experts_stream(a, a.p.bf16, reinterpret_cast<hipStream_t>(stream));
+    launch_experts_stream(a, reinterpret_cast<hipStream_t>(stream));
     return check_launch("experts_forward");
   }
   a.saved = saved ? (char*)saved : (char*)ws;
@@ -316,12 +320,12 @@ int ckan_muon_step(const ckan_ortho_desc* desc, float* p, const float* g, float*
 
 int ckan_mixture_few(const ckan_mixture_desc* desc) {
   FewArgs a;
-  return mixture_args(desc, &a) == CKAN_OK && desc->rows > 0 && a.p.stream;
+  return mixture_args(desc, &a) == CKAN_OK && a.few;
 }
 
 size_t ckan_mixture_workspace_bytes(const ckan_mixture_desc* desc) {
   FewArgs a;
-  return mixture_args(desc, &a) || desc->rows == 0 || !a.p.stream ? 0 : few_workspace_bytes(a);
+  return mixture_args(desc, &a) || !a.few ? 0 : a.ws_bytes;
 }
 
 int ckan_mixture_forward(const ckan_mixture_desc* desc, const void* x, const void* gate, const void* coeffs,
@@ -330,9 +334,9 @@ int ckan_mixture_forward(const ckan_mixture_desc* desc, const void* x, const voi
   FewArgs a;
   if (const int rc = mixture_args(desc, &a)) return rc;
   if (desc->rows == 0) return CKAN_OK;
-  if (!a.p.stream) return fail(CKAN_ERR_UNSUPPORTED, "mixture_forward: too many rows for its form, use the parts' entry points");
+  if (!a.few) return fail(CKAN_ERR_UNSUPPORTED, "mixture_forward: too many rows for its form, use the parts' entry points");
   if (!x || !gate || !coeffs || !y || !weights || !indices) return fail(CKAN_ERR_INVALID_ARG, "mixture_forward: NULL pointer");
-  const size_t need = few_workspace_bytes(a);
+  const size_t need = a.ws_bytes;
   if (ws_bytes < need) return fail(CKAN_ERR_WORKSPACE, "mixture workspace too small: %zu < %zu bytes", ws_bytes, need);
   if (!ws || !is_al16(ws)) return fail(CKAN_ERR_INVALID_ARG, "mixture_forward: workspace is NULL or not 16-byte aligned");
   if (!is_al16(x) || !is_al16(gate) || !is_al16(coeffs) || !is_al16(y))
