@@ -430,7 +430,7 @@ typedef enum ckan_norm {
 
 typedef struct ckan_residual_desc {
   int64_t rows;        /* 0..2^32 - 1                                        */
-  int64_t x_ld, y_ld, gate_ld, dout_ld, dh_ld;
+  int64_t x_ld, y_ld, gate_ld;
   int32_t dim;         /* 1..2^20                                            */
   int32_t x_dtype, y_dtype;
   int32_t gate_dtype, post_weight_dtype, post_bias_dtype, next_weight_dtype, next_bias_dtype;
@@ -438,7 +438,6 @@ typedef struct ckan_residual_desc {
   int32_t gate_rows;   /* 0 or 1                                             */
   float eps, scale;
   double dropout;      /* 0..1                                               */
-  uint64_t dropout_seed, dropout_offset;
 } ckan_residual_desc;
 
 typedef struct ckan_residual_buffers {
@@ -448,6 +447,8 @@ typedef struct ckan_residual_buffers {
   void* stats;                   /* written by a forward that a backward follows (else NULL), read by it */
   const void *dout, *dh;         /* gradients of out and h; NULL is zero       */
   void *dx, *dy, *dgate, *dpost_weight, *dpost_bias, *dnext_weight, *dnext_bias;  /* NULL: not wanted */
+  int64_t dout_ld, dh_ld;
+  uint64_t dropout_seed, dropout_offset;  /* as ckan_dropout_desc's; a backward takes the forward's from stats */
 } ckan_residual_buffers;
 
 size_t ckan_residual_stats_bytes(const ckan_residual_desc* desc);

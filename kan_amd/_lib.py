@@ -272,8 +272,6 @@ class CkanResidualDesc(ctypes.Structure):
         ("x_ld", ctypes.c_int64),
         ("y_ld", ctypes.c_int64),
         ("gate_ld", ctypes.c_int64),
-        ("dout_ld", ctypes.c_int64),
-        ("dh_ld", ctypes.c_int64),
         ("dim", ctypes.c_int32),
         ("x_dtype", ctypes.c_int32),
         ("y_dtype", ctypes.c_int32),
@@ -287,15 +285,15 @@ class CkanResidualDesc(ctypes.Structure):
         ("eps", ctypes.c_float),
         ("scale", ctypes.c_float),
         ("dropout", ctypes.c_double),
-        ("dropout_seed", ctypes.c_uint64),
-        ("dropout_offset", ctypes.c_uint64),
     ]
 
 
 class CkanResidualBuffers(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in (
         "x", "y", "gate", "post_weight", "post_bias", "next_weight", "next_bias", "dropout_state", "out", "h", "stats",
-        "dout", "dh", "dx", "dy", "dgate", "dpost_weight", "dpost_bias", "dnext_weight", "dnext_bias")]
+        "dout", "dh", "dx", "dy", "dgate", "dpost_weight", "dpost_bias", "dnext_weight", "dnext_bias")] + [
+        ("dout_ld", ctypes.c_int64), ("dh_ld", ctypes.c_int64), ("dropout_seed", ctypes.c_uint64),
+        ("dropout_offset", ctypes.c_uint64)]
 
 
 class CkanDropoutDesc(ctypes.Structure):

@@ -18,22 +18,29 @@ _DTYPES = {torch.float32: _lib.CKAN_DTYPE_F32, torch.bfloat16: _lib.CKAN_DTYPE_B
 
 
 def _check(name: str, device: torch.device, t: torch.Tensor) -> None:
+    if t.is_cuda and t.device == device and t.dtype in _DTYPES:
+        return
     if not t.is_cuda:
         raise RuntimeError(f"kan_amd's block operators run only on a ROCm device (MI355X); {name} is on {t.device}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, another tensor on {device}: one device is needed")
-    if t.dtype not in _DTYPES:
-        raise RuntimeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    raise RuntimeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
 
 
 def _rows(t: torch.Tensor, dim: int) -> torch.Tensor:
-    """t as [rows, dim], its rows contiguous; a copy only where no view has that form."""
-    t = t.reshape(-1, dim)
+    """t as [rows, dim], its rows contiguous; itself where it has that form (a view would cost
+    a node of the graph), a copy only where no view has it."""
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
     return t if (t.stride(1) == 1 or dim == 1) and t.stride(0) >= 0 else t.contiguous()
 
 
 def _pitch(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.stride(0)
+
+
+def _shaped(t: Optional[torch.Tensor], shape) -> Optional[torch.Tensor]:
+    return t if t is None or len(shape) == 2 else t.view(shape)
 
 
 def _drop_state(p: float, state, call: int, device: torch.device):
@@ -61,54 +68,82 @@ class ResidualFunction(torch.autograd.Function):
     ones None."""
 
     @staticmethod
-    def forward(ctx, x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state, h_dtype):
-        out, h, stats = _residual_forward(x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state,
-                                          h_dtype, keep=True)
+    def forward(ctx, x, y, gate, post_weight, post_bias, next_weight, next_bias, call):
+        tensors = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
+        out, h, stats = _residual_forward(tensors, call, keep=True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, y, gate, post_weight, post_bias, next_weight, next_bias, stats)
-        ctx.desc, ctx.h_dtype = desc, h_dtype
+        ctx.save_for_backward(*tensors, stats)
+        ctx.desc, ctx.h_dtype = call.desc, call.h_dtype
         return out, h
 
     @staticmethod
     def backward(ctx, dout, dh):
         _once("residual_norm")
         need = ctx.needs_input_grad
-        if not any(need[:7]) or (dout is None and dh is None):
-            return (None,) * 10
-        *inputs, stats = ctx.saved_tensors
-        x = inputs[0]
-        desc = _lib.CkanResidualDesc.from_buffer_copy(ctx.desc)
+        if dout is None and dh is None:
+            return (None,) * 8
+        x, y, gate, post_weight, post_bias, next_weight, next_bias, stats = ctx.saved_tensors
+        desc, dev = ctx.desc, x.device
         if dout is not None:
-            dout = _rows(dout.to(x.dtype), desc.dim)
-            desc.dout_ld = _pitch(dout)
+            dout = _rows(dout if dout.dtype == x.dtype else dout.to(x.dtype), desc.dim)
         if dh is not None:
-            dh = _rows(dh.to(ctx.h_dtype), desc.dim)
-            desc.dh_ld = _pitch(dh)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip(inputs, need)]
+            dh = _rows(dh if dh.dtype == ctx.h_dtype else dh.to(ctx.h_dtype), desc.dim)
+        inputs = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip(inputs, need)]
         if desc.rows == 0:
-            return (*(None if g is None else g.zero_() for g in grads), None, None, None)
+            return (*(None if g is None else g.zero_() for g in grads), None)
         lib = _lib.load()
         nbytes = lib.ckan_residual_workspace_bytes(desc)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        buffers = _lib.CkanResidualBuffers(*(_lib.ptr(t) for t in inputs), 0, 0, 0, stats.data_ptr(), _lib.ptr(dout),
-                                           _lib.ptr(dh), *(_lib.ptr(g) for g in grads))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ptr = _lib.ptr
+        buffers = _lib.CkanResidualBuffers(
+            x.data_ptr(), ptr(y), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(next_weight), ptr(next_bias), 0, 0, 0,
+            stats.data_ptr(), ptr(dout), ptr(dh), *map(ptr, grads), _pitch(dout), _pitch(dh))
         # the engine runs a node on its device and stream
-        _lib.check(lib.ckan_residual_backward(desc, buffers, ws.data_ptr(), nbytes, _stream(x.device)))
-        return (*grads, None, None, None)
+        _lib.check(lib.ckan_residual_backward(desc, buffers, ws.data_ptr(), nbytes, _stream(dev)))
+        return (*grads, None)
 
 
-def _residual_forward(x, y, gate, post_weight, post_bias, next_weight, next_bias, desc, state, h_dtype, keep):
+class _ResidualCall(NamedTuple):
+    """What a call takes besides its tensors."""
+    desc: "_lib.CkanResidualDesc"
+    state: Optional[torch.Tensor]
+    seed: int
+    offset: int
+    h_dtype: torch.dtype
+
+
+def _residual_forward(tensors, call, keep):
     """(out, h, stats); the tensors are [rows, dim] and [dim]."""
-    lib, dev = _lib.load(), x.device
-    shape = (desc.rows, desc.dim)
-    out = torch.empty(shape, dtype=x.dtype, device=dev) if y is not None else None
-    h = torch.empty(shape, dtype=h_dtype, device=dev) if next_weight is not None else None
-    stats = torch.empty(desc.rows * 4 + 4, dtype=torch.float32, device=dev) if keep else None
-    buffers = _lib.CkanResidualBuffers(x.data_ptr(), *(_lib.ptr(t) for t in (
-        y, gate, post_weight, post_bias, next_weight, next_bias, state, out, h, stats)))
+    x, y, gate, post_weight, post_bias, next_weight, next_bias = tensors
+    desc, dev, ptr = call.desc, x.device, _lib.ptr
+    rows, dim = desc.rows, desc.dim
+    out = torch.empty(rows, dim, dtype=x.dtype, device=dev) if y is not None else None
+    h = torch.empty(rows, dim, dtype=call.h_dtype, device=dev) if next_weight is not None else None
+    stats = torch.empty(rows * 4 + 4, dtype=torch.float32, device=dev) if keep else None
+    buffers = _lib.CkanResidualBuffers(
+        x.data_ptr(), ptr(y), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(next_weight), ptr(next_bias),
+        ptr(call.state), ptr(out), ptr(h), ptr(stats), dropout_seed=call.seed, dropout_offset=call.offset)
     with _on(dev):
-        _lib.check(lib.ckan_residual_forward(desc, buffers, _stream(dev)))
+        _lib.check(_lib.load().ckan_residual_forward(desc, buffers, _stream(dev)))
     return out, h, stats
+
+
+# Descriptors by their fields: a structure of this size costs microseconds to build.
+_residual_descs = {}
+
+
+def _residual_desc(*fields) -> "_lib.CkanResidualDesc":
+    desc = _residual_descs.get(fields)
+    if desc is None:
+        if len(_residual_descs) > 4096:
+            _residual_descs.clear()
+        desc = _residual_descs[fields] = _lib.CkanResidualDesc(*fields)
+    return desc
+
+
+def _code(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else _DTYPES[t.dtype]
 
 
 def _residual(x, y, gate, post_weight, post_bias, next_weight, next_bias, norm, eps, scale, dropout, state, call,
@@ -117,42 +152,49 @@ def _residual(x, y, gate, post_weight, post_bias, next_weight, next_bias, norm, 
         raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"x must be [..., dim] with dim >= 1, got {tuple(x.shape)}")
-    dim, shape = x.shape[-1], x.shape
-    params = {"post_weight": post_weight, "post_bias": post_bias, "next_weight": next_weight, "next_bias": next_bias}
-    _lib.refuse_tangents("residual_norm", x, y, gate, *params.values())
-    for name, t in (("x", x), ("y", y), ("gate", gate), *params.items()):
+    shape, dev = x.shape, x.device
+    dim = shape[-1]
+    _lib.refuse_tangents("residual_norm", x, y, gate, post_weight, post_bias, next_weight, next_bias)
+    _check("x", dev, x)
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("next_weight", next_weight),
+                    ("next_bias", next_bias)):
         if t is not None:
-            _check(name, x.device, t)
-    for name, t in params.items():
-        if t is not None and tuple(t.shape) != (dim,):
-            raise RuntimeError(f"{name} must be [{dim}], got {tuple(t.shape)}")
+            _check(name, dev, t)
+            if t.dim() != 1 or t.shape[0] != dim:
+                raise RuntimeError(f"{name} must be [{dim}], got {tuple(t.shape)}")
     if (post_bias is not None and post_weight is None) or (next_bias is not None and next_weight is None):
         raise RuntimeError("a norm's bias needs its weight")
     if h_dtype not in _DTYPES:
         raise RuntimeError(f"a norm's result is float32 or bfloat16, not {h_dtype}")
     gate_rows = False
     if gate is not None:
+        _check("gate", dev, gate)
         gate_rows = gate.dim() > 1 and gate.shape == shape
         if not gate_rows and tuple(gate.shape) != (dim,):
             raise RuntimeError(f"gate must be [{dim}] or {tuple(shape)}, got {tuple(gate.shape)}")
-    if y is not None and y.shape != shape:
-        raise RuntimeError(f"y must be of x's shape {tuple(shape)}, got {tuple(y.shape)}")
-    drop_state, seed, offset = _drop_state(dropout, state, call, x.device)
+    if y is not None:
+        _check("y", dev, y)
+        if y.shape != shape:
+            raise RuntimeError(f"y must be of x's shape {tuple(shape)}, got {tuple(y.shape)}")
+    drop_state, seed, offset = _drop_state(dropout, state, call, dev)
     x = _rows(x, dim)
-    y = None if y is None else _rows(y, dim)
+    if y is not None:
+        y = _rows(y, dim)
     if gate is not None:
         gate = _rows(gate, dim) if gate_rows else gate.contiguous()
-    post_weight, post_bias, next_weight, next_bias = (None if t is None else t.contiguous() for t in params.values())
-    codes = [0 if t is None else _DTYPES[t.dtype] for t in (gate, post_weight, post_bias, next_weight, next_bias)]
-    desc = _lib.CkanResidualDesc(x.shape[0], x.stride(0), _pitch(y), gate.stride(0) if gate_rows else 0, 0, 0, dim,
-                                 _DTYPES[x.dtype], _DTYPES[h_dtype if y is None else y.dtype], *codes, _NORMS[norm],
-                                 int(gate_rows), float(eps), float(scale), float(dropout), seed, offset)
+    post_weight, post_bias, next_weight, next_bias = (
+        t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, post_bias, next_weight, next_bias))
+    desc = _residual_desc(x.shape[0], x.stride(0), _pitch(y), gate.stride(0) if gate_rows else 0, dim, _DTYPES[x.dtype],
+                          _DTYPES[h_dtype if y is None else y.dtype], _code(gate), _code(post_weight), _code(post_bias),
+                          _code(next_weight), _code(next_bias), _NORMS[norm], int(gate_rows), float(eps), float(scale),
+                          float(dropout))
     tensors = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
+    how = _ResidualCall(desc, drop_state, seed, offset, h_dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        out, h = ResidualFunction.apply(*tensors, desc, drop_state, h_dtype)
+        out, h = ResidualFunction.apply(*tensors, how)
     else:
-        out, h, _ = _residual_forward(*tensors, desc, drop_state, h_dtype, keep=False)
-    return None if out is None else out.view(shape), None if h is None else h.view(shape)
+        out, h, _ = _residual_forward(tensors, how, keep=False)
+    return _shaped(out, shape), _shaped(h, shape)
 
 
 def row_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, norm: str = "rms",
@@ -212,7 +254,8 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _once("dropout")
-        dx, _ = _dropout_launch(_rows(dy.to(ctx.dtype), dy.shape[-1]), ctx.p, ctx.used, 0, 0, keep=False)
+        dy = _rows(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), dy.shape[-1])
+        dx, _ = _dropout_launch(dy, ctx.p, ctx.used, 0, 0, keep=False)
         return dx, None, None, None, None
 
 
@@ -233,8 +276,8 @@ def dropout(x: torch.Tensor, p: float, state: Union[int, torch.Tensor], call: in
         return x.clone()
     rows = _rows(x, x.shape[-1])
     if torch.is_grad_enabled() and rows.requires_grad:
-        return DropoutFunction.apply(rows, float(p), state, seed, offset).view(x.shape)
-    return _dropout_launch(rows, float(p), state, seed, offset, keep=False)[0].view(x.shape)
+        return _shaped(DropoutFunction.apply(rows, float(p), state, seed, offset), x.shape)
+    return _shaped(_dropout_launch(rows, float(p), state, seed, offset, keep=False)[0], x.shape)
 
 
 # ---- log probabilities ----------------------------------------------------------------
@@ -281,7 +324,8 @@ class LogProbsFunction(torch.autograd.Function):
         if dlogp is None and dentropy is None:
             return None, None, None, None
         logits, targets, stats = ctx.saved_tensors
-        dlogp, dentropy = (None if g is None else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))
+        dlogp, dentropy = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
+                           else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))
         dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _lib.check(_lib.load().ckan_log_probs_backward(ctx.desc, logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
                                                        _lib.ptr(dlogp), _lib.ptr(dentropy), dl.data_ptr(),
@@ -313,7 +357,9 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> L
     if targets.device != logits.device:
         raise RuntimeError(f"targets are on {targets.device}, logits on {logits.device}: one device is needed")
     shape, classes = targets.shape, logits.shape[-1]
-    logits, targets = _rows(logits, classes), targets.reshape(-1).contiguous()
+    logits = _rows(logits, classes)
+    if len(shape) != 1 or not targets.is_contiguous():
+        targets = targets.reshape(-1).contiguous()
     desc = _lib.CkanLogProbsDesc(logits.shape[0], logits.stride(0), classes, int(top), _DTYPES[logits.dtype])
     if torch.is_grad_enabled() and logits.requires_grad:
         out: list = []

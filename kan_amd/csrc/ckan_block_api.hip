@@ -55,7 +55,7 @@ int residual_check(const ckan_residual_desc* d) {
   if (d->gate_rows != 0 && d->gate_rows != 1) return fail(CKAN_ERR_INVALID_ARG, "gate_rows must be 0 or 1");
   if (!(d->eps >= 0.0f) || !isfinite(d->eps) || !isfinite(d->scale))
     return fail(CKAN_ERR_INVALID_ARG, "eps and scale must be finite, eps >= 0");
-  for (const int64_t ld : {d->x_ld, d->y_ld, d->gate_ld, d->dout_ld, d->dh_ld})
+  for (const int64_t ld : {d->x_ld, d->y_ld, d->gate_ld})
     if (ld < 0) return fail(CKAN_ERR_INVALID_ARG, "row pitches must be >= 0");
   return CKAN_OK;
 }
@@ -64,9 +64,10 @@ int residual_args(const ckan_residual_desc* d, const ckan_residual_buffers* b, b
   if (const int rc = residual_check(d)) return rc;
   if (!b) return fail(CKAN_ERR_INVALID_ARG, "residual buffers are NULL");
   *a = ResidualArgs{};
-  if (const int rc = drop_args(d->dropout, d->dropout_seed, d->dropout_offset, b->dropout_state, &a->drop)) return rc;
+  if (const int rc = drop_args(d->dropout, b->dropout_seed, b->dropout_offset, b->dropout_state, &a->drop)) return rc;
   if (d->rows == 0) return CKAN_OK;
   if (!b->x) return fail(CKAN_ERR_INVALID_ARG, "residual: x is NULL");
+  if (backward && (b->dout_ld < 0 || b->dh_ld < 0)) return fail(CKAN_ERR_INVALID_ARG, "row pitches must be >= 0");
   if (!b->y && (b->gate || b->post_weight || b->dout || d->dropout > 0.0))
     return fail(CKAN_ERR_INVALID_ARG, "residual: without y there is no gate, post norm, dropout or out");
   if (!b->y && !b->next_weight) return fail(CKAN_ERR_INVALID_ARG, "residual: neither y nor next_weight");
@@ -97,8 +98,8 @@ int residual_args(const ckan_residual_desc* d, const ckan_residual_buffers* b, b
   a->x_ld = d->x_ld;
   a->y_ld = d->y_ld;
   a->gate_ld = d->gate_ld;
-  a->dout_ld = d->dout_ld;
-  a->dh_ld = d->dh_ld;
+  a->dout_ld = b->dout_ld;
+  a->dh_ld = b->dh_ld;
   a->dim = d->dim;
   a->x_bf16 = d->x_dtype == CKAN_DTYPE_BF16;
   a->y_bf16 = d->y_dtype == CKAN_DTYPE_BF16;

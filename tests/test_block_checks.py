@@ -19,7 +19,7 @@ def _struct(cls, base, change):
     return cls(**d)
 
 
-RESIDUAL = dict(rows=4, x_ld=8, y_ld=8, gate_ld=8, dout_ld=8, dh_ld=8, dim=8, eps=1e-6, scale=1.0)
+RESIDUAL = dict(rows=4, x_ld=8, y_ld=8, gate_ld=8, dim=8, eps=1e-6, scale=1.0)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -28,7 +28,7 @@ RESIDUAL = dict(rows=4, x_ld=8, y_ld=8, gate_ld=8, dout_ld=8, dh_ld=8, dim=8, ep
     (dict(gate_dtype=9), INVALID), (dict(next_bias_dtype=3), INVALID), (dict(norm=2), INVALID),
     (dict(gate_rows=2), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID),
     (dict(scale=float("inf")), INVALID), (dict(dropout=1.5), INVALID), (dict(dropout=float("nan")), INVALID),
-    (dict(x_ld=-8), INVALID), (dict(dh_ld=-1), INVALID),
+    (dict(x_ld=-8), INVALID), (dict(gate_ld=-1), INVALID),
 ])
 def test_residual_desc_refused(change, code):
     lib = _lib.load()
@@ -56,7 +56,7 @@ def test_residual_forward_buffers_refused(buffers):
 
 @pytest.mark.parametrize("buffers", [
     dict(), dict(dh=256), dict(dy=256, y=None), dict(dgate=256), dict(dpost_weight=256), dict(dpost_bias=256),
-    dict(dnext_weight=256), dict(dnext_bias=256), dict(dx=257),
+    dict(dnext_weight=256), dict(dnext_bias=256), dict(dx=257), dict(dx=256, dout_ld=-1), dict(dx=256, dh_ld=-8),
 ])
 def test_residual_backward_buffers_refused(buffers):
     lib = _lib.load()
