@@ -65,16 +65,32 @@ __device__ __forceinline__ void store8(T* p, int64_t left, const float (&f)[kChu
   }
 }
 
-// The same where `room` values from p on may be read, at least `left` of them the row's:
-// a row's partial chunk in one access, its surplus left to zero_past.
+// The same without elementwise reads, for rows of at least eight values: a row's partial chunk in one
+// access too, reaching past the row's end where `spare` values follow it, and beginning `back` values
+// early where they do not. settle8 puts its values right.
+__device__ __forceinline__ int back_of(int left, int64_t spare) {
+  return left < kChunk && left + spare < kChunk ? (int)(kChunk - left - spare) : 0;
+}
 template <typename T>
-__device__ __forceinline__ typename RawOf<T>::type load_room8(const T* p, int left, int64_t room) {
-  if (left > 0 && room >= kChunk) return *(const typename RawOf<T>::type*)p;
-  return load_raw8(p, (int64_t)left);
+__device__ __forceinline__ typename RawOf<T>::type load_near8(const T* row, int at, int left, int64_t spare) {
+  typename RawOf<T>::type r = {};
+  if (left > 0) r = *(const typename RawOf<T>::type*)(row + at - back_of(left, spare));
+  return r;
 }
 __device__ __forceinline__ void zero_past(int left, float (&f)[kChunk]) {
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) f[i] = i < left ? f[i] : 0.0f;
+}
+
+__device__ __forceinline__ void settle8(int left, int64_t spare, float (&f)[kChunk]) {
+  const int back = left > 0 ? back_of(left, spare) : 0;
+  if (__any(back)) {  // the tensor's last row
+#pragma unroll
+    for (int w = 4; w; w >>= 1)
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) f[i] = back & w ? (i + w < kChunk ? f[i + w < kChunk ? i + w : i] : 0.0f) : f[i];
+  }
+  zero_past(left, f);
 }
 
 // The sum over a group of L lanes (8, 16, 32 or 64, aligned), in each of them: butterflies

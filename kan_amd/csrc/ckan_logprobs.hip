@@ -162,13 +162,14 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_team(LogpArgs a) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int at = (lane * N + n) * kChunk, left = a.classes - at;
-      raw[n] = load_room8(l + at, left, left + spare);
+      raw[n] = a.classes >= kChunk ? load_near8(l, at, left, spare) : load_raw8(l + at, (int64_t)left);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int left = a.classes - (lane * N + n) * kChunk;
       float f[kChunk];
       unpack8(raw[n], f);
+      if (a.classes >= kChunk && (a.classes & (kChunk - 1))) settle8(left, spare, f);
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) v[n * kChunk + i] = i < left ? f[i] : -INFINITY;
     }

@@ -12,6 +12,8 @@
 //
 // out is made again from x and y, unrounded, so that no gradient sees its rounding: the
 // same bytes as reading out.  Sums over a row and over rows are in fp32, in a fixed order.
+#include <type_traits>
+
 #include "ckan_block.hpp"
 
 namespace ckan {
@@ -315,8 +317,8 @@ __global__ __launch_bounds__(1024) void k_residual_sums(ResidualArgs a, const fl
 // ---- up to kTeamMaxDim values: a row in the registers of a team of lanes --------------
 //
 // A team of LANES lanes holds a row, N chunks a lane; a block holds several teams and its
-// rows stride over the batch, so that the parameters, and in the backward the sums over
-// rows, stay in registers. Every value of a row is read once, the next row's while this one is
+// rows stride over the batch, so that the parameters stay in LDS, and in the backward the sums over
+// rows in registers. Every value of a row is read once, the next row's while this one is
 // worked on.
 template <int LANES, int N, int BLOCK>
 struct Team {
@@ -324,7 +326,9 @@ struct Team {
   static constexpr int kWaves = LANES > 64 ? LANES / 64 : 1;
   int team, lane, turn;
   float* red;  // [2][BLOCK / 64][2]
-  __device__ Team(float* lds) : team(threadIdx.x / LANES), lane(threadIdx.x % LANES), turn(0), red(lds) {}
+  __device__ Team(float* lds) : team(threadIdx.x / LANES), lane(threadIdx.x % LANES), turn(0), red(lds) {
+    if constexpr (LANES >= 64) team = __builtin_amdgcn_readfirstlane(team);  // rows are a wave's: scalar
+  }
   // Sums over the team, in every lane; all teams of the block call it together. Two
   // buffers in turn: a wave writes one again only after the barrier of the sum between, which its
   // readers reach when they have read it.
@@ -358,11 +362,10 @@ struct RowRaw {
   template <int LANES>
   __device__ __forceinline__ void load(const T* base, int64_t row, int64_t ld, const ResidualArgs& a, int lane) {
     const T* p = base + row * ld;
-    const int64_t spare = (a.rows - 1 - row) * ld;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
-      v[n] = load_room8(p + at, left, left + spare);
+      const int at = (n * LANES + lane) * kChunk;
+      v[n] = load_near8(p, at, a.dim - at, (a.rows - 1 - row) * ld);
     }
   }
 };
@@ -377,9 +380,9 @@ struct RowAny {
     for (int n = 0; n < N; ++n) {
       const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
       if (t.bf16) {
-        v[n][0] = load_room8((const __bf16*)t.p + row * ld + at, left, left + spare).v;
+        v[n][0] = load_near8((const __bf16*)t.p + row * ld, at, left, spare).v;
       } else {
-        const RawF32 r = load_room8((const float*)t.p + row * ld + at, left, left + spare);
+        const RawF32 r = load_near8((const float*)t.p + row * ld, at, left, spare);
         v[n][0] = r.v[0];
         v[n][1] = r.v[1];
       }
@@ -397,58 +400,102 @@ struct RowAny {
   }
 };
 
-// What stays in registers from row to row: the parameters, 0 past the row's end. The
-// gate times scale; 1 or 0 stand for absent ones.
-template <int N>
-struct RowParams {
-  float pw[N][kChunk], pb[N][kChunk], gate[N][kChunk];
-  template <int LANES>
-  __device__ __forceinline__ void load(const ResidualArgs& a, int lane) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        pw[n][i] = pb[n][i] = 0.0f;
-        gate[n][i] = a.scale;
+// The parameters as every row of a block reads them: in LDS, a lane's eight values of a chunk as two
+// reads of 16 bytes at neighbouring lanes' neighbouring addresses; 0 past the row's end. In registers
+// they would take the room of one to two waves a SIMD.
+enum Param { kPostW, kPostB, kGate, kNextW, kNextB, kParams };
+template <int LANES, int N>
+struct ParamTable {
+  float* lds;
+  int lane;
+  static constexpr int kFloats = LANES * N * kChunk;
+  __device__ __forceinline__ static AnyPtr source(const ResidualArgs& a, int k) {
+    switch (k) {
+      case kPostW: return a.post_w;
+      case kPostB: return a.post_b;
+      case kGate: return AnyPtr{a.gate_rows ? nullptr : a.gate.p, a.gate.bf16};
+      case kNextW: return a.next_w;
+      default: return a.next_b;
+    }
+  }
+  // Every thread of the block calls it, and a barrier follows.
+  __device__ __forceinline__ void fill(const ResidualArgs& a, int params) {
+    int slot = 0;
+    for (int k = 0; k < params; ++k) {
+      const AnyPtr src = source(a, k);
+      if (!src.p) continue;
+      for (int c = threadIdx.x; c < LANES * N; c += blockDim.x) {
+        const int64_t left = a.dim - (int64_t)c * kChunk;
+        float f[kChunk];
+        if (left > 0)
+          load8(src, (int64_t)c * kChunk, left, f);
+        else
+          zero_past(0, f);
+        f32x4_t* to = (f32x4_t*)(lds + slot * kFloats + c / LANES * LANES * kChunk) + c % LANES;
+        to[0] = f32x4_t{f[0], f[1], f[2], f[3]};
+        to[LANES] = f32x4_t{f[4], f[5], f[6], f[7]};
       }
-      if (left <= 0) continue;
-      if (a.post_w.p) load8(a.post_w, at, left, pw[n]);
-      if (a.post_b.p) load8(a.post_b, at, left, pb[n]);
-      if (a.gate.p && !a.gate_rows) {
-        load8(a.gate, at, left, gate[n]);
+      ++slot;
+    }
+  }
+  // Where parameter k lies, once it is known to be there.
+  __device__ __forceinline__ const float* at(const ResidualArgs& a, int k) const {
+    int slot = 0;
+    for (int q = 0; q < k; ++q) slot += source(a, q).p != nullptr;
+    return lds + slot * kFloats;
+  }
+  __device__ __forceinline__ void get(const float* p, int n, float (&f)[kChunk]) const {
+    const f32x4_t* from = (const f32x4_t*)(p + n * LANES * kChunk) + lane;
+    const f32x4_t lo = from[0], hi = from[LANES];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
-      }
+    for (int i = 0; i < 4; ++i) {
+      f[i] = lo[i];
+      f[4 + i] = hi[i];
     }
   }
 };
 
-// u (after dropout), y^ in y's place, and out's value in x's.
-template <int N, int LANES>
-__device__ __forceinline__ void row_values(const ResidualArgs& a, const DropKey& key, int64_t row, int lane, float m1, float r1,
-                                           const float (&gate)[N][kChunk], const RowParams<N>& par, float (&x)[N][kChunk],
-                                           float (&y)[N][kChunk], float (&u)[N][kChunk], uint32_t (&keep)[N]) {
+// The gate of a row's chunk, times scale.
+template <int LANES, int N>
+__device__ __forceinline__ void gate_values(const ResidualArgs& a, const ParamTable<LANES, N>& par, const float* pg, const RowAny<N>& rows,
+                                            int64_t row, int n, float (&g)[kChunk]) {
+  if (a.gate_rows) {
+    rows.unpack(n, a.gate.bf16, g);
+    if (a.dim & (kChunk - 1)) settle8(a.dim - (n * LANES + par.lane) * kChunk, (a.rows - 1 - row) * a.gate_ld, g);
+  } else if (a.gate.p) {
+    par.get(pg, n, g);
+  } else {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) u[n][i] = y[n][i];
-    if (a.post_w.p) {
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        y[n][i] = (y[n][i] - m1) * r1;
-        u[n][i] = fmaf(y[n][i], par.pw[n][i], par.pb[n][i]);
-      }
-    }
-    keep[n] = 0xff;
-    if (a.drop.on) {
-      keep[n] = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)(n * LANES + lane));
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) u[n][i] = keep[n] >> i & 1 ? u[n][i] * a.drop.scale : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf(gate[n][i], u[n][i], x[n][i]);
+    for (int i = 0; i < kChunk; ++i) g[i] = 1.0f;
   }
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) g[i] *= a.scale;
+}
+
+// u (after dropout), y^ in y's place; the mask of the chunk.
+template <int LANES, int N>
+__device__ __forceinline__ uint32_t branch_values(const ResidualArgs& a, const DropKey& key, const ParamTable<LANES, N>& par,
+                                                  const float* pw, const float* pb, int64_t row, int n, float m1, float r1,
+                                                  float (&y)[kChunk], float (&u)[kChunk]) {
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) u[i] = y[i];
+  if (a.post_w.p) {
+    float w[kChunk], b[kChunk] = {};
+    par.get(pw, n, w);
+    if (a.post_b.p) par.get(pb, n, b);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      y[i] = (y[i] - m1) * r1;
+      u[i] = fmaf(y[i], w[i], b[i]);
+    }
+  }
+  uint32_t keep = 0xff;
+  if (a.drop.on) {
+    keep = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)(n * LANES + par.lane));
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) u[i] = keep >> i & 1 ? u[i] * a.drop.scale : 0.0f;
+  }
+  return keep;
 }
 
 // The mean (layer norms) and 1 / root mean square of a row's values, which are 0 past its end.
@@ -480,7 +527,8 @@ __device__ __forceinline__ void row_stats(TEAM& team, const ResidualArgs& a, con
 }
 
 template <typename TX, typename TY, int LANES, int N, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void k_residual_rows(ResidualArgs a) {
+__global__ __launch_bounds__(BLOCK, 4) void k_residual_rows(ResidualArgs a) {
+  extern __shared__ __align__(16) float lds[];
   __shared__ float red[2 * BLOCK / 64 * 2];
   Team<LANES, N, BLOCK> team(red);
   const int lane = team.lane;
@@ -491,15 +539,6 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows(ResidualArgs a) {
     used[1] = (int64_t)(((uint64_t)key.call1 << 32) | key.call0);
   }
   const float inv = 1.0f / (float)a.dim;
-  RowParams<N> par;
-  par.template load<LANES>(a, lane);
-  float nw[N][kChunk] = {}, nb[N][kChunk] = {};
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
-    if (a.next_w.p && left > 0) load8(a.next_w, at, left, nw[n]);
-    if (a.next_b.p && left > 0) load8(a.next_b, at, left, nb[n]);
-  }
   const int64_t step = (int64_t)gridDim.x * team.kTeams;
   int64_t row = (int64_t)blockIdx.x * team.kTeams + team.team;
   RowRaw<TX, N> xr;
@@ -512,73 +551,71 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows(ResidualArgs a) {
     if (a.gate_rows) gr.template load<LANES>(a.gate, r, a.gate_ld, a, lane);
   };
   fetch(row);
+  ParamTable<LANES, N> par{lds, lane};
+  par.fill(a, kParams);
+  __syncthreads();
+  const float *pw = par.at(a, kPostW), *pb = par.at(a, kPostB), *pg = par.at(a, kGate), *nw = par.at(a, kNextW),
+              *nb = par.at(a, kNextB);
   // every team of the block takes as many turns as its first: the sums' barriers are the block's
   for (int64_t first = (int64_t)blockIdx.x * team.kTeams; first < a.rows; first += step, row += step) {
     const bool active = row < a.rows;
-    float x[N][kChunk], y[N][kChunk], u[N][kChunk], gate[N][kChunk];
-    uint32_t keep[N];
+    float x[N][kChunk], y[N][kChunk];
+    RowAny<N> gate = gr;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       unpack8(xr.v[n], x[n]);
       if (a.y) unpack8(yr.v[n], y[n]);
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) gate[n][i] = par.gate[n][i];
-      if (a.gate_rows) {
-        gr.unpack(n, a.gate.bf16, gate[n]);
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
-      }
       if (a.dim & (kChunk - 1)) {
         const int left = a.dim - (n * LANES + lane) * kChunk;
-        zero_past(left, x[n]);
-        zero_past(left, y[n]);
-        zero_past(left, gate[n]);
+        const int64_t after = a.rows - 1 - row;
+        settle8(left, after * a.x_ld, x[n]);
+        if (a.y) settle8(left, after * a.y_ld, y[n]);
       }
     }
     fetch(row + step);
     float m1 = 0.0f, r1 = 0.0f, m2 = 0.0f, r2 = 0.0f;
     if (a.y) {
       if (a.post_w.p) row_stats<N, LANES>(team, a, y, inv, m1, r1);
-      row_values<N, LANES>(a, key, row, lane, m1, r1, gate, par, x, y, u, keep);
-      if (active)
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const int at = (n * LANES + lane) * kChunk;
-          if (at < a.dim) store8((TX*)a.out + row * a.dim + at, a.dim - at, x[n]);
-        }
+      for (int n = 0; n < N; ++n) {
+        float u[kChunk], g[kChunk];
+        branch_values(a, key, par, pw, pb, row, n, m1, r1, y[n], u);
+        gate_values(a, par, pg, gate, row, n, g);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf(g[i], u[i], x[n][i]);
+        const int at = (n * LANES + lane) * kChunk;
+        if (active && at < a.dim) store8((TX*)a.out + row * a.dim + at, a.dim - at, x[n]);
+      }
     }
     if (a.next_w.p) {
       row_stats<N, LANES>(team, a, x, inv, m2, r2);
-      if (active)
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const int at = (n * LANES + lane) * kChunk;
+      for (int n = 0; n < N; ++n) {
+        float w[kChunk], b[kChunk] = {};
+        par.get(nw, n, w);
+        if (a.next_b.p) par.get(nb, n, b);
 #pragma unroll
-          for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf((x[n][i] - m2) * r2, nw[n][i], nb[n][i]);
-          if (at < a.dim) store8((TY*)a.h + row * a.dim + at, a.dim - at, x[n]);
-        }
+        for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf((x[n][i] - m2) * r2, w[i], b[i]);
+        const int at = (n * LANES + lane) * kChunk;
+        if (active && at < a.dim) store8((TY*)a.h + row * a.dim + at, a.dim - at, x[n]);
+      }
     }
     if (a.stats && active && lane == 0) *(f32x4_t*)(a.stats + row * kStats) = f32x4_t{m1, r1, m2, r2};
   }
 }
 
+// Waves a SIMD that the backward's registers leave room for.
+__host__ __device__ constexpr int backward_waves(int lanes) { return lanes < 64 ? 2 : lanes == 1024 ? 4 : 3; }
+
+// Its sums over rows a block leaves as a part of each, [block, 5, dim].
 template <typename TX, typename TY, int LANES, int N, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a, int sums) {
+__global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_backward(ResidualArgs a, int sums) {
+  extern __shared__ __align__(16) float lds[];
   __shared__ float red[2 * BLOCK / 64 * 2];
-  __shared__ __align__(16) float tile[BLOCK * kChunk];
   Team<LANES, N, BLOCK> team(red);
   const int lane = team.lane;
   const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
   const float inv = 1.0f / (float)a.dim;
-  RowParams<N> par;
-  par.template load<LANES>(a, lane);
-  float nw[N][kChunk] = {};
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
-    if (a.next_w.p && left > 0) load8(a.next_w, at, left, nw[n]);
-  }
-  float acc[kSums][N][kChunk] = {};
   const int64_t step = (int64_t)gridDim.x * team.kTeams;
   int64_t row = (int64_t)blockIdx.x * team.kTeams + team.team;
   RowRaw<TX, N> xr, dor;
@@ -595,10 +632,17 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
     if (a.dout) dor.template load<LANES>((const TX*)a.dout, r, a.dout_ld, a, lane);
     if (a.dh) dhr.template load<LANES>((const TY*)a.dh, r, a.dh_ld, a, lane);
   };
-  fetch(row);
+  ParamTable<LANES, N> par{lds, lane};
+  par.fill(a, kNextB);  // next's bias has no part in it
+  __syncthreads();
+  const float *pw = par.at(a, kPostW), *pb = par.at(a, kPostB), *pg = par.at(a, kGate), *nw = par.at(a, kNextW);
+  float acc[kSums][N][kChunk] = {};
   for (int64_t first = (int64_t)blockIdx.x * team.kTeams; first < a.rows; first += step, row += step) {
     const bool active = row < a.rows;
-    float x[N][kChunk], y[N][kChunk], u[N][kChunk] = {}, gate[N][kChunk], dx[N][kChunk], dh[N][kChunk];
+    fetch(row);
+    float x[N][kChunk], y[N][kChunk], u[N][kChunk] = {}, dx[N][kChunk];
+    RowRaw<TY, N> dh = dhr;
+    RowAny<N> gate = gr;
     uint32_t keep[N];
     const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
 #pragma unroll
@@ -606,47 +650,52 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
       unpack8(xr.v[n], x[n]);
       if (a.y) unpack8(yr.v[n], y[n]);
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) gate[n][i] = par.gate[n][i], dx[n][i] = dh[n][i] = 0.0f;
-      if (a.gate_rows) {
-        gr.unpack(n, a.gate.bf16, gate[n]);
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) gate[n][i] *= a.scale;
-      }
+      for (int i = 0; i < kChunk; ++i) dx[n][i] = 0.0f;
       if (a.dout) unpack8(dor.v[n], dx[n]);
-      if (a.dh) unpack8(dhr.v[n], dh[n]);
       if (a.dim & (kChunk - 1)) {
         const int left = a.dim - (n * LANES + lane) * kChunk;
-        zero_past(left, x[n]);
-        zero_past(left, y[n]);
-        zero_past(left, gate[n]);
-        zero_past(left, dx[n]);
-        zero_past(left, dh[n]);
+        const int64_t after = a.rows - 1 - row;
+        settle8(left, after * a.x_ld, x[n]);
+        if (a.y) settle8(left, after * a.y_ld, y[n]);
+        if (a.dout) settle8(left, after * a.dout_ld, dx[n]);
       }
     }
-    fetch(row + step);
-    if (a.y) row_values<N, LANES>(a, key, row, lane, m1, r1, gate, par, x, y, u, keep);
-    if (next) {
-      // x becomes o^
-      float s[2] = {0.0f, 0.0f};
+    if (a.y)
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n) {
+        float g[kChunk];
+        keep[n] = branch_values(a, key, par, pw, pb, row, n, m1, r1, y[n], u[n]);
+        gate_values(a, par, pg, gate, row, n, g);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) x[n][i] = fmaf(g[i], u[n][i], x[n][i]);
+      }
+    if (next) {
+      // x becomes o^; g = dh w
+      float s[2] = {0.0f, 0.0f}, g[N][kChunk];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        float d[kChunk];
+        unpack8(dh.v[n], d);
+        if (a.dim & (kChunk - 1)) settle8(a.dim - (n * LANES + lane) * kChunk, (a.rows - 1 - row) * a.dh_ld, d);
+        par.get(nw, n, g[n]);
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
           x[n][i] = (x[n][i] - m2) * r2;
           if (active) {
-            acc[3][n][i] = fmaf(dh[n][i], x[n][i], acc[3][n][i]);
-            acc[4][n][i] += dh[n][i];
+            acc[3][n][i] = fmaf(d[i], x[n][i], acc[3][n][i]);
+            acc[4][n][i] += d[i];
           }
-          const float g = dh[n][i] * nw[n][i];
-          s[0] = fmaf(g, x[n][i], s[0]);
-          s[1] += g;
+          g[n][i] *= d[i];
+          s[0] = fmaf(g[n][i], x[n][i], s[0]);
+          s[1] += g[n][i];
         }
+      }
       team.sum(s);
       const float go = s[0] * inv, gm = a.layer ? s[1] * inv : 0.0f;
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) dx[n][i] = fmaf(r2, fmaf(dh[n][i], nw[n][i], -fmaf(x[n][i], go, gm)), dx[n][i]);
+        for (int i = 0; i < kChunk; ++i) dx[n][i] = fmaf(r2, g[n][i] - fmaf(x[n][i], go, gm), dx[n][i]);
     }
     if (a.dx && active)
 #pragma unroll
@@ -669,9 +718,12 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
             store8((float*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
         }
       }
+      float g[kChunk], w[kChunk];
+      gate_values(a, par, pg, gate, row, n, g);
+      if (post) par.get(pw, n, w);
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
-        float e = gate[n][i] * dx[n][i];
+        float e = g[i] * dx[n][i];
         if (a.drop.on) e = keep[n] >> i & 1 ? e * a.drop.scale : 0.0f;
         if (active) {
           acc[0][n][i] = fmaf(e, y[n][i], acc[0][n][i]);
@@ -679,7 +731,7 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
           acc[2][n][i] += u[n][i];
         }
         if (post) {
-          e *= par.pw[n][i];
+          e *= w[i];
           s[0] = fmaf(e, y[n][i], s[0]);
           s[1] += e;
         }
@@ -712,12 +764,12 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
     for (int n = 0; n < N; ++n) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) tile[(team.team * LANES + lane) * kChunk + i] = acc[k][n][i];
+      for (int i = 0; i < kChunk; ++i) lds[(team.team * LANES + lane) * kChunk + i] = acc[k][n][i];
       __syncthreads();
       for (int c = threadIdx.x; c < LANES * kChunk; c += BLOCK) {
         float v = 0.0f;
 #pragma unroll
-        for (int t = 0; t < team.kTeams; ++t) v += tile[t * LANES * kChunk + c];
+        for (int t = 0; t < team.kTeams; ++t) v += lds[t * LANES * kChunk + c];
         const int col = n * LANES * kChunk + c;
         if (col < a.dim) part[(int64_t)k * a.dim + col] = v;
       }
@@ -725,6 +777,7 @@ __global__ __launch_bounds__(BLOCK) void k_residual_rows_backward(ResidualArgs a
   }
 }
 
+// Row slabs of the sums at any width.
 int any_slabs(const ResidualArgs& a) {
   const int64_t wide = ceil_div(a.dim, kChunk * kAnyThreads);
   int64_t slabs = ceil_div(4 * kNumCUs, wide);
@@ -739,31 +792,66 @@ int sum_bits(const ResidualArgs& a) {
 }
 
 constexpr int kTeamMaxDim = 8192;
+constexpr int kLdsBytes = 160 * 1024 - 512;  // less the sums' words
 
-// Blocks of a launch of teams: as many as the chip holds at once, fewer where rows run out.
-int64_t team_blocks(const ResidualArgs& a, int teams, int per_cu) {
+// The parameters that a launch holds in LDS (the backward all but next's bias).
+int held(const ResidualArgs& a, bool backward) {
+  return (a.post_w.p ? 1 : 0) + (a.post_b.p ? 1 : 0) + (a.gate.p && !a.gate_rows ? 1 : 0) + (a.next_w.p ? 1 : 0) +
+         (a.next_b.p && !backward ? 1 : 0);
+}
+// LDS bytes of a launch of teams; the backward's hold its blocks' sums at the end.
+int team_lds(const ResidualArgs& a, bool backward, int lanes, int n, int block) {
+  const int params = held(a, backward) * lanes * n * kChunk * 4, tile = backward ? block * kChunk * 4 : 0;
+  return params > tile ? params : tile;
+}
+
+// Blocks of a launch of teams: as many as the chip holds at once (their waves by registers,
+// `waves` a SIMD, and their LDS), fewer where rows run out.
+int64_t team_blocks(const ResidualArgs& a, int teams, int block, int waves, int lds) {
+  int per_cu = waves * 256 / block;
+  while (per_cu > 1 && per_cu * (lds + 512) > kLdsBytes) --per_cu;
+  if (per_cu < 1) per_cu = 1;
   const int64_t all = ceil_div(a.rows, teams), most = (int64_t)per_cu * kNumCUs;
   return all < most ? all : most;
 }
+constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
 
-// Calls f<LANES, N, BLOCK>() with the team for a width.
-#define CKAN_TEAM(dim, F)                          \
-  do {                                             \
-    if ((dim) <= 64) { F(8, 1, 512) }              \
-    else if ((dim) <= 128) { F(16, 1, 512) }       \
-    else if ((dim) <= 256) { F(32, 1, 512) }       \
-    else if ((dim) <= 512) { F(64, 1, 512) }       \
-    else if ((dim) <= 1024) { F(128, 1, 512) }     \
-    else if ((dim) <= 2048) { F(256, 1, 512) }     \
-    else if ((dim) <= 4096) { F(512, 1, 512) }     \
-    else { F(1024, 1, 1024) }                      \
+// The team of a width.
+#define CKAN_TEAM(dim, F)                       \
+  do {                                          \
+    if ((dim) <= 64) { F(8, 1, 256) }           \
+    else if ((dim) <= 128) { F(16, 1, 256) }    \
+    else if ((dim) <= 256) { F(32, 1, 256) }    \
+    else if ((dim) <= 512) { F(64, 1, 256) }    \
+    else if ((dim) <= 1024) { F(128, 1, 256) }  \
+    else if ((dim) <= 2048) { F(256, 1, 256) }  \
+    else if ((dim) <= 4096) { F(512, 1, 512) }  \
+    else { F(1024, 1, 1024) }                   \
   } while (0)
+
+template <typename K>
+void launch_team(K kernel, const ResidualArgs& a, int64_t blocks, int block, int lds, hipStream_t st, std::atomic<uint32_t>& done,
+                 int sums = -1) {
+  ensure_lds_limit((const void*)kernel, kLdsBytes, done);
+  if constexpr (std::is_invocable_v<K, ResidualArgs, int>)
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(block), lds, st, a, sums);
+  else
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(block), lds, st, a);
+}
+
+// Whether the teams' form takes a call: its width, and the parameters' room.
+bool by_teams(const ResidualArgs& a, bool backward) {
+  if (a.dim > kTeamMaxDim || a.dim < kChunk) return false;
+  return a.dim <= 4096 || team_lds(a, backward, 1024, 1, 1024) <= kLdsBytes;
+}
 
 template <typename TX, typename TY>
 void forward_typed(const ResidualArgs& a, hipStream_t st) {
-  if (a.dim <= kTeamMaxDim) {
-#define CKAN_FORWARD(L, NN, B)                                                                               \
-  hipLaunchKernelGGL((k_residual_rows<TX, TY, L, NN, B>), dim3((unsigned)team_blocks(a, B / L, 2048 / B)), dim3(B), 0, st, a); \
+  if (by_teams(a, false)) {
+#define CKAN_FORWARD(L, NN, B)                                                                           \
+  static std::atomic<uint32_t> done;                                                                     \
+  const int lds = team_lds(a, false, L, NN, B);                                                          \
+  launch_team(k_residual_rows<TX, TY, L, NN, B>, a, team_blocks(a, B / L, B, 4, lds), B, lds, st, done); \
   return;
     CKAN_TEAM(a.dim, CKAN_FORWARD);
 #undef CKAN_FORWARD
@@ -772,17 +860,17 @@ void forward_typed(const ResidualArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_residual_any<TX, TY>), dim3((unsigned)blocks), dim3(kAnyThreads), 0, st, a);
 }
 
-constexpr int kPartBlocks = 2;  // blocks a CU of the backward: each leaves a part of every sum
-
 template <typename TX, typename TY>
 void backward_typed(const ResidualArgs& a, hipStream_t st) {
   const int sums = sum_bits(a);
   const dim3 sum_grid((unsigned)ceil_div(a.dim, 64), kSums);
-  if (a.dim <= kTeamMaxDim) {
+  if (by_teams(a, true)) {
     int64_t blocks = 0;
-#define CKAN_BACKWARD(L, NN, B)                                                                                          \
-  blocks = team_blocks(a, B / L, kPartBlocks * 512 / B);                                                                  \
-  hipLaunchKernelGGL((k_residual_rows_backward<TX, TY, L, NN, B>), dim3((unsigned)blocks), dim3(B), 0, st, a, sums);
+#define CKAN_BACKWARD(L, NN, B)                                                                          \
+  static std::atomic<uint32_t> done;                                                                     \
+  const int lds = team_lds(a, true, L, NN, B);                                                           \
+  blocks = team_blocks(a, B / L, B, backward_waves(L), lds);                                             \
+  launch_team(k_residual_rows_backward<TX, TY, L, NN, B>, a, blocks, B, lds, st, done, sums);
     CKAN_TEAM(a.dim, CKAN_BACKWARD);
 #undef CKAN_BACKWARD
     if (sums) hipLaunchKernelGGL(k_residual_sums, sum_grid, dim3(1024), 0, st, a, a.ws, (int)blocks);
@@ -801,8 +889,13 @@ void backward_typed(const ResidualArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t residual_workspace_bytes(const ResidualArgs& a) {
-  const int64_t parts = a.dim <= kTeamMaxDim ? kPartBlocks * kNumCUs : any_slabs(a);
-  return align256(((a.dim <= kTeamMaxDim ? 0 : round_up(a.rows * 2, 4)) + parts * kSums * a.dim) * sizeof(float));
+  // either form's: which one runs hangs on the parameters too
+  int64_t parts = any_slabs(a);
+  if (a.dim <= kTeamMaxDim) {
+    const int64_t most = (int64_t)kPartBlocks * kNumCUs, blocks = a.rows < most ? a.rows : most;
+    if (blocks > parts) parts = blocks;
+  }
+  return align256((round_up(a.rows * 2, 4) + parts * kSums * a.dim) * sizeof(float));
 }
 
 void launch_residual_forward(const ResidualArgs& a, hipStream_t st) {
