@@ -71,10 +71,12 @@ __device__ __forceinline__ void store8(T* p, int64_t left, const float (&f)[kChu
 __device__ __forceinline__ int back_of(int left, int64_t spare) {
   return left < kChunk && left + spare < kChunk ? (int)(kChunk - left - spare) : 0;
 }
+// `tail`, uniform: rows have a partial chunk.
 template <typename T>
-__device__ __forceinline__ typename RawOf<T>::type load_near8(const T* row, int at, int left, int64_t spare) {
+__device__ __forceinline__ typename RawOf<T>::type load_near8(const T* row, int at, int left, int64_t spare, bool tail) {
   typename RawOf<T>::type r = {};
-  if (left > 0) r = *(const typename RawOf<T>::type*)(row + at - back_of(left, spare));
+  if (tail) at -= back_of(left, spare);
+  if (left > 0) r = *(const typename RawOf<T>::type*)(row + at);
   return r;
 }
 __device__ __forceinline__ void zero_past(int left, float (&f)[kChunk]) {

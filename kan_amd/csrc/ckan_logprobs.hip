@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_team(LogpArgs a) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int at = (lane * N + n) * kChunk, left = a.classes - at;
-      raw[n] = a.classes >= kChunk ? load_near8(l, at, left, spare) : load_raw8(l + at, (int64_t)left);
+      raw[n] = a.classes >= kChunk ? load_near8(l, at, left, spare, a.classes & (kChunk - 1)) : load_raw8(l + at, (int64_t)left);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {

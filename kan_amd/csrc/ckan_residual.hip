@@ -365,7 +365,7 @@ struct RowRaw {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int at = (n * LANES + lane) * kChunk;
-      v[n] = load_near8(p, at, a.dim - at, (a.rows - 1 - row) * ld);
+      v[n] = load_near8(p, at, a.dim - at, (a.rows - 1 - row) * ld, a.dim & (kChunk - 1));
     }
   }
 };
@@ -380,9 +380,9 @@ struct RowAny {
     for (int n = 0; n < N; ++n) {
       const int at = (n * LANES + lane) * kChunk, left = a.dim - at;
       if (t.bf16) {
-        v[n][0] = load_near8((const __bf16*)t.p + row * ld, at, left, spare).v;
+        v[n][0] = load_near8((const __bf16*)t.p + row * ld, at, left, spare, a.dim & (kChunk - 1)).v;
       } else {
-        const RawF32 r = load_near8((const float*)t.p + row * ld, at, left, spare);
+        const RawF32 r = load_near8((const float*)t.p + row * ld, at, left, spare, a.dim & (kChunk - 1));
         v[n][0] = r.v[0];
         v[n][1] = r.v[1];
       }
@@ -624,7 +624,15 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
   f32x4_t st;
   const bool next = a.next_w.p && a.dh, post = a.post_w.p;
   const auto fetch = [&](int64_t r) {
-    if (r >= a.rows) return;
+    if (r >= a.rows) {  // zeros, which add nothing to the sums
+      st = f32x4_t{};
+      xr = RowRaw<TX, N>{};
+      yr = RowRaw<TY, N>{};
+      gr = RowAny<N>{};
+      dor = RowRaw<TX, N>{};
+      dhr = RowRaw<TY, N>{};
+      return;
+    }
     st = *(const f32x4_t*)(a.stats + r * kStats);
     xr.template load<LANES>((const TX*)a.x, r, a.x_ld, a, lane);
     if (a.y) yr.template load<LANES>((const TY*)a.y, r, a.y_ld, a, lane);
@@ -681,14 +689,16 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
           x[n][i] = (x[n][i] - m2) * r2;
-          if (active) {
-            acc[3][n][i] = fmaf(d[i], x[n][i], acc[3][n][i]);
-            acc[4][n][i] += d[i];
-          }
+          acc[3][n][i] = fmaf(d[i], x[n][i], acc[3][n][i]);
           g[n][i] *= d[i];
           s[0] = fmaf(g[n][i], x[n][i], s[0]);
-          s[1] += g[n][i];
         }
+        if (sums & 16)
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) acc[4][n][i] += d[i];
+        if (a.layer)
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) s[1] += g[n][i];
       }
       team.sum(s);
       const float go = s[0] * inv, gm = a.layer ? s[1] * inv : 0.0f;
@@ -707,35 +717,44 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
+      if (a.gate.p) {
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) u[n][i] *= a.scale * dx[n][i];
-      if (a.gate_rows && a.dgate) {
-        const int at = (n * LANES + lane) * kChunk;
-        if (active && at < a.dim) {
-          if (a.gate.bf16)
-            store8((__bf16*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
-          else
-            store8((float*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
+        for (int i = 0; i < kChunk; ++i) u[n][i] *= a.scale * dx[n][i];
+        if (!a.gate_rows) {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) acc[2][n][i] += u[n][i];
+        } else if (a.dgate) {
+          const int at = (n * LANES + lane) * kChunk;
+          if (active && at < a.dim) {
+            if (a.gate.bf16)
+              store8((__bf16*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
+            else
+              store8((float*)a.dgate + row * a.dim + at, a.dim - at, u[n]);
+          }
         }
       }
-      float g[kChunk], w[kChunk];
+      float g[kChunk];
       gate_values(a, par, pg, gate, row, n, g);
-      if (post) par.get(pw, n, w);
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        float e = g[i] * dx[n][i];
-        if (a.drop.on) e = keep[n] >> i & 1 ? e * a.drop.scale : 0.0f;
-        if (active) {
-          acc[0][n][i] = fmaf(e, y[n][i], acc[0][n][i]);
-          acc[1][n][i] += e;
-          acc[2][n][i] += u[n][i];
+      for (int i = 0; i < kChunk; ++i) dx[n][i] *= g[i];
+      if (a.drop.on)
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) dx[n][i] = keep[n] >> i & 1 ? dx[n][i] * a.drop.scale : 0.0f;
+      if (post) {
+        float w[kChunk];
+        par.get(pw, n, w);
+        if (sums & 2)
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) acc[1][n][i] += dx[n][i];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          acc[0][n][i] = fmaf(dx[n][i], y[n][i], acc[0][n][i]);
+          dx[n][i] *= w[i];
+          s[0] = fmaf(dx[n][i], y[n][i], s[0]);
         }
-        if (post) {
-          e *= w[i];
-          s[0] = fmaf(e, y[n][i], s[0]);
-          s[1] += e;
-        }
-        dx[n][i] = e;
+        if (a.layer)
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) s[1] += dx[n][i];
       }
     }
     if (!a.dy) continue;
