@@ -610,6 +610,8 @@ __host__ __device__ constexpr int backward_waves(int lanes) { return lanes < 64 
 // Its sums over rows a block leaves as a part of each, [block, 5, dim].
 template <typename TX, typename TY, int LANES, int N, int BLOCK>
 __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_backward(ResidualArgs a, int sums) {
+  // the next row's values on their way, where the registers have room for them
+  constexpr bool kAhead = LANES < 64 || (LANES < 1024 && sizeof(TX) + sizeof(TY) == 4);
   extern __shared__ __align__(16) float lds[];
   __shared__ float red[2 * BLOCK / 64 * 2];
   Team<LANES, N, BLOCK> team(red);
@@ -640,6 +642,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
     if (a.dout) dor.template load<LANES>((const TX*)a.dout, r, a.dout_ld, a, lane);
     if (a.dh) dhr.template load<LANES>((const TY*)a.dh, r, a.dh_ld, a, lane);
   };
+  if (kAhead) fetch(row);
   ParamTable<LANES, N> par{lds, lane};
   par.fill(a, kNextB);  // next's bias has no part in it
   __syncthreads();
@@ -647,7 +650,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
   float acc[kSums][N][kChunk] = {};
   for (int64_t first = (int64_t)blockIdx.x * team.kTeams; first < a.rows; first += step, row += step) {
     const bool active = row < a.rows;
-    fetch(row);
+    if (!kAhead) fetch(row);
     float x[N][kChunk], y[N][kChunk], u[N][kChunk] = {}, dx[N][kChunk];
     RowRaw<TY, N> dh = dhr;
     RowAny<N> gate = gr;
@@ -668,6 +671,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
         if (a.dout) settle8(left, after * a.dout_ld, dx[n]);
       }
     }
+    if (kAhead) fetch(row + step);
     if (a.y)
 #pragma unroll
       for (int n = 0; n < N; ++n) {
