@@ -1,14 +1,16 @@
 """What stands around the layers of a deep KAN, over the C-ABI: the norms, gate, dropout and
-sum of a residual block, dropout by itself, and the log probabilities at a network's end.
+sum of a residual block, the stack of such blocks, dropout by itself, and the log
+probabilities at a network's end.
 
 Device memory and streams come from torch; all compute is the HIP library's.
 Tensors on the CPU are rejected: there is no CPU path.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import Iterable, NamedTuple, Optional, Tuple, Union
 
 import torch
+import torch.nn as nn
 
 from . import _lib
 from .mixture import _on, _once, _stream
@@ -369,3 +371,71 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> L
     if len(shape) == 1:
         return LogProbs(*got)
     return LogProbs(*(None if t is None else t.view(shape + t.shape[1:]) for t in got))
+
+
+# ---- a stack of residual blocks ----------------------------------------------------------
+
+class ResidualKAN(nn.Module):
+    """KAN layers of one width as a stack of residual blocks:
+
+        h = norm_0(x);  for each layer i:  x = x + scale gate_i drop(post_i(layer_i(h))),  h = norm_{i+1}(x)
+
+    ``layers`` map [rows, dim] to [rows, dim] (ChebyKANLayer, MixtureKANLayer, ...); their tanh saturates
+    where a deep stack's values grow, which the norms before them keep in place.  ``row_norm`` opens the
+    stack, one ``residual_norm`` closes each block together with the next one's norm.  ``norm``: 'rms', or
+    'layer' with biases; ``post``: a norm after each layer too; ``gate``: the initial value of a
+    learned gate [dim] a block, None for none.  The last norm's h is the result with
+    ``final_norm``, else x.
+
+    ``dropout`` is drawn in training mode from the buffer ``dropout_state`` (seed, offset): a forward uses one
+    call a layer and moves the offset on, on the device, so that replays of a captured step draw anew."""
+
+    def __init__(self, layers: Iterable[nn.Module], dim: int, *, norm: str = "rms", post: bool = True,
+                 gate: Optional[float] = 0.1, scale: float = 1.0, dropout: float = 0.0, eps: float = 1e-6,
+                 final_norm: bool = True):
+        super().__init__()
+        if norm not in _NORMS:
+            raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"the dropout probability must lie in [0, 1], got {dropout}")
+        self.layers = nn.ModuleList(layers)
+        for i, layer in enumerate(self.layers):
+            width = getattr(layer, "input_dim", dim), getattr(layer, "output_dim", dim)
+            if width != (dim, dim):
+                raise ValueError(f"layer {i} maps {width[0]} to {width[1]} values, the stack has {dim}")
+        self.dim, self.norm, self.scale, self.dropout, self.eps = dim, norm, scale, dropout, eps
+        n = len(self.layers)
+        norms = n + 1 if final_norm else n
+
+        def vectors(count, value):
+            return nn.ParameterList([nn.Parameter(torch.full((dim,), float(value))) for _ in range(count)])
+
+        self.pre_weight = vectors(norms, 1)
+        self.pre_bias = vectors(norms if norm == "layer" else 0, 0)
+        self.post_weight = vectors(n if post else 0, 1)
+        self.post_bias = vectors(n if post and norm == "layer" else 0, 0)
+        self.gate = vectors(0 if gate is None else n, gate or 0)
+        self.register_buffer("dropout_state", torch.tensor([int(torch.randint(0, 2 ** 62, ())), 0]))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        def at(vectors, i):
+            return vectors[i] if i < len(vectors) else None
+
+        x = x.reshape(-1, self.dim)
+        n, drop = len(self.layers), self.dropout if self.training else 0.0
+        if not len(self.pre_weight):
+            return x
+        h = row_norm(x, self.pre_weight[0], at(self.pre_bias, 0), norm=self.norm, eps=self.eps)
+        for i, layer in enumerate(self.layers):
+            got = residual_norm(x, layer(h), norm=self.norm, eps=self.eps, post_weight=at(self.post_weight, i),
+                                post_bias=at(self.post_bias, i), gate=at(self.gate, i), scale=self.scale, dropout=drop,
+                                dropout_state=self.dropout_state if drop else None, dropout_call=i,
+                                next_weight=at(self.pre_weight, i + 1), next_bias=at(self.pre_bias, i + 1))
+            x, h = got if isinstance(got, tuple) else (got, got)
+        if drop:
+            with torch.no_grad():
+                self.dropout_state[1:].add_(n)
+        return h
+
+    def extra_repr(self) -> str:
+        return f"dim={self.dim}, norm={self.norm}, scale={self.scale}, dropout={self.dropout}"
