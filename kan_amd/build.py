@@ -26,7 +26,7 @@ ARCH = "gfx950"
 SOURCES = ["ckan_api.hip", "ckan_aux.hip", "ckan_gemm.hip", "ckan_exec.hip", "ckan_family.hip",
            "ckan_general.hip", "ckan_mix_api.hip", "ckan_route.hip", "ckan_ortho.hip", "ckan_ortho_small.hip",
            "ckan_experts.hip", "ckan_block_api.hip", "ckan_residual.hip", "ckan_dropout.hip", "ckan_logprobs.hip",
-           "ckan_few.hip"]
+           "ckan_few.hip", "ckan_few_bf16.hip"]
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

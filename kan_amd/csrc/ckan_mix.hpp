@@ -147,11 +147,13 @@ struct FewArgs {
   // the launch's plan (few_plan)
   bool few;            // whether this form takes the call
   bool apart;          // logits by a launch of their own
+  bool gated;          // the choice made by the products' launch
   int active, chunks, chunk_inputs;
   size_t part_off, ws_bytes;
 };
 void few_plan(FewArgs* a);
 void launch_few(const FewArgs& a, hipStream_t st);
+void launch_few_bf16(const FewArgs& a, hipStream_t st);  // the products on bf16 coefficients (ckan_few_bf16.hip)
 
 size_t ortho_workspace_bytes(const OrthoArgs& a);
 void launch_ortho(const OrthoArgs& a, void* ws, hipStream_t st);
