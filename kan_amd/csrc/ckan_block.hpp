@@ -141,17 +141,21 @@ __device__ __forceinline__ void load8(const AnyPtr& a, int64_t at, int64_t left,
 struct DropArgs {
   const int64_t* state;  // (seed, offset) on the device, or NULL: (seed, offset) below
   uint64_t seed, offset; // offset is added to the state's
-  uint32_t high, low;    // round(p 2^32) = high 2^16 + low; high 2^16: nothing is kept
+  uint32_t high, low;    // round(p 2^32) = high 2^16 + low
+  uint32_t cut;          // what kept() compares with: high, at least 1
   float scale;           // 1 / (1 - p)
-  int on;
+  int on, none;          // none: p 2^32 rounds to 2^32, nothing is kept
 };
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
 __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
-    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
-    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    c[0] = xor3((uint32_t)(b >> 32), c[1], k0);
+    c[2] = xor3((uint32_t)(a >> 32), c[3], k1);
     c[1] = (uint32_t)b;
     c[3] = (uint32_t)a;
     k0 += 0x9E3779B9u;
@@ -172,27 +176,41 @@ __device__ __forceinline__ DropKey drop_key(const DropArgs& d) {
   return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)call, (uint32_t)(call >> 32) & 0x7fffffffu};
 }
 
-// Bit i: element i of the chunk is kept.
-__device__ __forceinline__ uint32_t drop_keep(const DropArgs& d, const DropKey& k, uint32_t row, uint32_t chunk) {
+// A chunk's eight numbers, 16 bits each, settled such that an element is kept where its
+// number reaches DropArgs::cut: 0 where the low halves decided against it.
+struct DropWords {
+  uint32_t w[kChunk / 2];
+  __device__ __forceinline__ bool kept(int i, const DropArgs& d) const {
+    return (i & 1 ? w[i >> 1] : w[i >> 1] << 16) >= d.cut << 16;
+  }
+};
+__device__ __forceinline__ DropWords drop_words(const DropArgs& d, const DropKey& k, uint32_t row, uint32_t chunk) {
+  DropWords r;
   uint32_t c[4] = {chunk, row, k.call0, k.call1};
   philox(c, k.k0, k.k1);
-  uint32_t keep = 0, tie = 0;
+  // halves that equal the threshold's: those that are 0 in x. (x - 0x10001) & ~x & 0x80008000 marks
+  // the words that have one (and with them perhaps another half)
+  uint32_t any = 0;
+  const uint32_t twice = d.high << 16 | d.high;
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    const uint32_t r = i & 1 ? c[i >> 1] >> 16 : c[i >> 1] & 0xffffu;
-    keep |= r >= d.high ? 1u << i : 0u;
-    tie |= r == d.high ? 1u << i : 0u;
+  for (int i = 0; i < 4; ++i) {
+    r.w[i] = c[i];
+    const uint32_t x = c[i] ^ twice;
+    any |= (x - 0x10001u) & ~x & 0x80008000u;
   }
-  if (d.low && tie) {  // the low halves decide
+  if (d.high == 0 || d.none)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = d.none ? 0u : 0xffffffffu;
+  if (d.low && any && !d.none) {  // the low halves decide
     uint32_t e[4] = {chunk, row, k.call0, k.call1 | 0x80000000u};
     philox(e, k.k0, k.k1);
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      const uint32_t r = i & 1 ? e[i >> 1] >> 16 : e[i >> 1] & 0xffffu;
-      if (r < d.low) keep &= ~(tie & (1u << i));
+    for (int i = 0; i < 4; ++i) {
+      if ((c[i] & 0xffffu) == d.high && (e[i] & 0xffffu) < d.low) r.w[i] &= 0xffff0000u;
+      if (c[i] >> 16 == d.high && e[i] >> 16 < d.low) r.w[i] &= 0xffffu;
     }
   }
-  return keep;
+  return r;
 }
 
 constexpr int64_t kDropMaxRows = (int64_t)1 << 32, kDropMaxDim = (int64_t)1 << 34;

@@ -37,8 +37,9 @@ int drop_args(double p, uint64_t seed, uint64_t offset, const int64_t* state, Dr
   if (!(p >= 0.0 && p <= 1.0)) return fail(CKAN_ERR_INVALID_ARG, "the dropout probability must lie in [0, 1] (got %g)", p);
   if ((uintptr_t)state & 7) return fail(CKAN_ERR_INVALID_ARG, "the dropout state must be 8-byte aligned");
   const uint64_t threshold = (uint64_t)nearbyint(p * 4294967296.0);
-  *d = DropArgs{state, seed, offset, (uint32_t)(threshold >> 16), (uint32_t)(threshold & 0xffff),
-                p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f, p > 0.0};
+  const uint32_t high = (uint32_t)(threshold >> 16);
+  *d = DropArgs{state, seed, offset, high, (uint32_t)(threshold & 0xffff), high && !(high >> 16) ? high : 1,
+                p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f, p > 0.0, (int)(high >> 16)};
   return CKAN_OK;
 }
 

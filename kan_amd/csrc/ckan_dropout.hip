@@ -22,9 +22,9 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     for (int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += (int64_t)gridDim.x * blockDim.x) {
       float v[kChunk];
       load8(x + c * kChunk, a.dim - c * kChunk, v);
-      const uint32_t keep = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)c);
+      const DropWords keep = drop_words(a.drop, key, (uint32_t)row, (uint32_t)c);
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) v[i] = keep >> i & 1 ? v[i] * a.drop.scale : 0.0f;
+      for (int i = 0; i < kChunk; ++i) v[i] = keep.kept(i, a.drop) ? v[i] * a.drop.scale : 0.0f;
       store8(y + c * kChunk, a.dim - c * kChunk, v);
     }
   }

@@ -40,12 +40,12 @@ struct RowStats {
 
 // One chunk of a row: u (after dropout), y^ and out's unrounded value.
 template <typename TX, typename TY>
-__device__ __forceinline__ uint32_t chunk_values(const ResidualArgs& a, const DropKey& key, int64_t row, int c,
+__device__ __forceinline__ DropWords chunk_values(const ResidualArgs& a, const DropKey& key, int64_t row, int c,
                                                  const RowStats& st, float (&yh)[kChunk], float (&u)[kChunk],
                                                  float (&gate)[kChunk], float (&o)[kChunk]) {
   const int64_t at = (int64_t)c * kChunk, left = a.dim - at;
   load8((const TX*)a.x + row * a.x_ld + at, left, o);
-  uint32_t keep = 0xff;
+  DropWords keep = {};
   if (!a.y) return keep;
   load8((const TY*)a.y + row * a.y_ld + at, left, yh);
 #pragma unroll
@@ -61,9 +61,9 @@ __device__ __forceinline__ uint32_t chunk_values(const ResidualArgs& a, const Dr
     }
   }
   if (a.drop.on) {
-    keep = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)c);
+    keep = drop_words(a.drop, key, (uint32_t)row, (uint32_t)c);
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) u[i] = keep >> i & 1 ? u[i] * a.drop.scale : 0.0f;
+    for (int i = 0; i < kChunk; ++i) u[i] = keep.kept(i, a.drop) ? u[i] * a.drop.scale : 0.0f;
   }
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) gate[i] = 1.0f;
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_dx(ResidualArgs a)
       float ey = 0.0f, e = 0.0f;
       for (int c = tid; c < chunks; c += kAnyThreads) {
         const int64_t at = (int64_t)c * kChunk, left = a.dim - at;
-        const uint32_t keep = chunk_values<TX, TY>(a, key, row, c, st, yh, u, gate, o);
+        const DropWords keep = chunk_values<TX, TY>(a, key, row, c, st, yh, u, gate, o);
         chunk_dx<TX, TY>(a, row, c, st, mean, o, oh, dh, dx);
         if (pass && a.dx) store8((TX*)a.dx + row * a.dim + at, left, dx);
         if (!a.y) continue;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_dx(ResidualArgs a)
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
           float v = gate[i] * dx[i];
-          if (a.drop.on) v = keep >> i & 1 ? v * a.drop.scale : 0.0f;
+          if (a.drop.on) v = keep.kept(i, a.drop) ? v * a.drop.scale : 0.0f;
           if (post) {
             v *= w[i];
             ey = fmaf(v, yh[i], ey);
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_sums(ResidualArgs 
     mean.go = a.ws[row * 2];
     mean.g = a.ws[row * 2 + 1];
     float yh[kChunk], u[kChunk], gate[kChunk], o[kChunk], oh[kChunk], dh[kChunk], dx[kChunk];
-    const uint32_t keep = chunk_values<TX, TY>(a, key, row, c, st, yh, u, gate, o);
+    const DropWords keep = chunk_values<TX, TY>(a, key, row, c, st, yh, u, gate, o);
     chunk_dx<TX, TY>(a, row, c, st, mean, o, oh, dh, dx);
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) {
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_sums(ResidualArgs 
       if (!a.y) continue;
       s[2][i] = fmaf(a.scale * dx[i], u[i], s[2][i]);
       float v = gate[i] * dx[i];
-      if (a.drop.on) v = keep >> i & 1 ? v * a.drop.scale : 0.0f;
+      if (a.drop.on) v = keep.kept(i, a.drop) ? v * a.drop.scale : 0.0f;
       s[0][i] = fmaf(v, yh[i], s[0][i]);
       s[1][i] += v;
     }
@@ -474,7 +474,7 @@ __device__ __forceinline__ void gate_values(const ResidualArgs& a, const ParamTa
 
 // u (after dropout), y^ in y's place; the mask of the chunk.
 template <int LANES, int N>
-__device__ __forceinline__ uint32_t branch_values(const ResidualArgs& a, const DropKey& key, const ParamTable<LANES, N>& par,
+__device__ __forceinline__ DropWords branch_values(const ResidualArgs& a, const DropKey& key, const ParamTable<LANES, N>& par,
                                                   const float* pw, const float* pb, int64_t row, int n, float m1, float r1,
                                                   float (&y)[kChunk], float (&u)[kChunk]) {
 #pragma unroll
@@ -489,11 +489,11 @@ __device__ __forceinline__ uint32_t branch_values(const ResidualArgs& a, const D
       u[i] = fmaf(y[i], w[i], b[i]);
     }
   }
-  uint32_t keep = 0xff;
+  DropWords keep = {};
   if (a.drop.on) {
-    keep = drop_keep(a.drop, key, (uint32_t)row, (uint32_t)(n * LANES + par.lane));
+    keep = drop_words(a.drop, key, (uint32_t)row, (uint32_t)(n * LANES + par.lane));
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) u[i] = keep >> i & 1 ? u[i] * a.drop.scale : 0.0f;
+    for (int i = 0; i < kChunk; ++i) u[i] = keep.kept(i, a.drop) ? u[i] * a.drop.scale : 0.0f;
   }
   return keep;
 }
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
     float x[N][kChunk], y[N][kChunk], u[N][kChunk] = {}, dx[N][kChunk];
     RowRaw<TY, N> dh = dhr;
     RowAny<N> gate = gr;
-    uint32_t keep[N];
+    DropWords keep[N];
     const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -743,7 +743,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_
       for (int i = 0; i < kChunk; ++i) dx[n][i] *= g[i];
       if (a.drop.on)
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) dx[n][i] = keep[n] >> i & 1 ? dx[n][i] * a.drop.scale : 0.0f;
+        for (int i = 0; i < kChunk; ++i) dx[n][i] = keep[n].kept(i, a.drop) ? dx[n][i] * a.drop.scale : 0.0f;
       if (post) {
         float w[kChunk];
         par.get(pw, n, w);
