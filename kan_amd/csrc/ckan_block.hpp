@@ -75,7 +75,7 @@ __device__ __forceinline__ int back_of(int left, int64_t spare) {
 template <typename T>
 __device__ __forceinline__ typename RawOf<T>::type load_near8(const T* row, int at, int left, int64_t spare, bool tail) {
   typename RawOf<T>::type r = {};
-  if (tail) at -= back_of(left, spare);
+  if (tail && spare < kChunk - 1) at -= back_of(left, spare);
   if (left > 0) r = *(const typename RawOf<T>::type*)(row + at);
   return r;
 }
@@ -85,8 +85,8 @@ __device__ __forceinline__ void zero_past(int left, float (&f)[kChunk]) {
 }
 
 __device__ __forceinline__ void settle8(int left, int64_t spare, float (&f)[kChunk]) {
-  const int back = left > 0 ? back_of(left, spare) : 0;
-  if (__any(back)) {  // the tensor's last row
+  if (spare < kChunk - 1) {  // the tensor's last row
+    const int back = left > 0 ? back_of(left, spare) : 0;
 #pragma unroll
     for (int w = 4; w; w >>= 1)
 #pragma unroll

@@ -605,13 +605,13 @@ __global__ __launch_bounds__(BLOCK, 4) void k_residual_rows(ResidualArgs a) {
 }
 
 // Waves a SIMD that the backward's registers leave room for.
-__host__ __device__ constexpr int backward_waves(int lanes) { return lanes < 64 ? 2 : lanes == 1024 ? 4 : 3; }
+__host__ __device__ constexpr int backward_waves(int lanes, int n) { return lanes < 64 || n > 1 ? 2 : 3; }
 
 // Its sums over rows a block leaves as a part of each, [block, 5, dim].
 template <typename TX, typename TY, int LANES, int N, int BLOCK>
-__global__ __launch_bounds__(BLOCK, backward_waves(LANES)) void k_residual_rows_backward(ResidualArgs a, int sums) {
+__global__ __launch_bounds__(BLOCK, backward_waves(LANES, N)) void k_residual_rows_backward(ResidualArgs a, int sums) {
   // the next row's values on their way, where the registers have room for them
-  constexpr bool kAhead = LANES < 64 || (LANES < 1024 && sizeof(TX) + sizeof(TY) == 4);
+  constexpr bool kAhead = LANES < 64 || (N == 1 && sizeof(TX) + sizeof(TY) == 4);
   extern __shared__ __align__(16) float lds[];
   __shared__ float red[2 * BLOCK / 64 * 2];
   Team<LANES, N, BLOCK> team(red);
@@ -839,8 +839,10 @@ int64_t team_blocks(const ResidualArgs& a, int teams, int block, int waves, int 
 }
 constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
 
-// The team of a width.
-#define CKAN_TEAM(dim, F)                       \
+// The team of a width, WIDE that of the widest rows: in the backward half as many lanes, whose 256
+// registers hold two chunks and their sums (4096 x 8192 212 us in fp32 and 142 in bf16; 1024 lanes
+// of 128 registers 291 and 175).
+#define CKAN_TEAM(dim, F, WIDE)                 \
   do {                                          \
     if ((dim) <= 64) { F(8, 1, 256) }           \
     else if ((dim) <= 128) { F(16, 1, 256) }    \
@@ -849,7 +851,7 @@ constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
     else if ((dim) <= 1024) { F(128, 1, 256) }  \
     else if ((dim) <= 2048) { F(256, 1, 256) }  \
     else if ((dim) <= 4096) { F(512, 1, 512) }  \
-    else { F(1024, 1, 1024) }                   \
+    else { WIDE }                               \
   } while (0)
 
 template <typename K>
@@ -876,7 +878,7 @@ void forward_typed(const ResidualArgs& a, hipStream_t st) {
   const int lds = team_lds(a, false, L, NN, B);                                                          \
   launch_team(k_residual_rows<TX, TY, L, NN, B>, a, team_blocks(a, B / L, B, 4, lds), B, lds, st, done); \
   return;
-    CKAN_TEAM(a.dim, CKAN_FORWARD);
+    CKAN_TEAM(a.dim, CKAN_FORWARD, CKAN_FORWARD(1024, 1, 1024));
 #undef CKAN_FORWARD
   }
   const int64_t blocks = a.rows < 8 * kNumCUs ? a.rows : 8 * kNumCUs;
@@ -892,9 +894,9 @@ void backward_typed(const ResidualArgs& a, hipStream_t st) {
 #define CKAN_BACKWARD(L, NN, B)                                                                          \
   static std::atomic<uint32_t> done;                                                                     \
   const int lds = team_lds(a, true, L, NN, B);                                                           \
-  blocks = team_blocks(a, B / L, B, backward_waves(L), lds);                                             \
+  blocks = team_blocks(a, B / L, B, backward_waves(L, NN), lds);                                             \
   launch_team(k_residual_rows_backward<TX, TY, L, NN, B>, a, blocks, B, lds, st, done, sums);
-    CKAN_TEAM(a.dim, CKAN_BACKWARD);
+    CKAN_TEAM(a.dim, CKAN_BACKWARD, CKAN_BACKWARD(512, 2, 512));
 #undef CKAN_BACKWARD
     if (sums) hipLaunchKernelGGL(k_residual_sums, sum_grid, dim3(1024), 0, st, a, a.ws, (int)blocks);
     return;
