@@ -404,11 +404,16 @@ struct RowAny {
 // reads of 16 bytes at neighbouring lanes' neighbouring addresses; 0 past the row's end. In registers
 // they would take the room of one to two waves a SIMD.
 enum Param { kPostW, kPostB, kGate, kNextW, kNextB, kParams };
-template <int LANES, int N>
+//
+// A parameter takes two runs of 16 bytes a chunk: a chunk for every lane of the team, or, PACKED, the
+// row's chunks and one of zeros for the lanes past it, which lets five parameters of up to 6500 values
+// fit (and costs the backward registers that it does not have).
+template <int LANES, int N, bool PACKED>
 struct ParamTable {
   float* lds;
-  int lane;
-  static constexpr int kFloats = LANES * N * kChunk;
+  int lane, chunks;
+  __device__ ParamTable(float* at, int l, int dim)
+      : lds(at), lane(l), chunks(PACKED ? (dim + kChunk - 1) / kChunk + 1 : LANES * N) {}
   __device__ __forceinline__ static AnyPtr source(const ResidualArgs& a, int k) {
     switch (k) {
       case kPostW: return a.post_w;
@@ -424,16 +429,13 @@ struct ParamTable {
     for (int k = 0; k < params; ++k) {
       const AnyPtr src = source(a, k);
       if (!src.p) continue;
-      for (int c = threadIdx.x; c < LANES * N; c += blockDim.x) {
-        const int64_t left = a.dim - (int64_t)c * kChunk;
-        float f[kChunk];
-        if (left > 0)
-          load8(src, (int64_t)c * kChunk, left, f);
-        else
-          zero_past(0, f);
-        f32x4_t* to = (f32x4_t*)(lds + slot * kFloats + c / LANES * LANES * kChunk) + c % LANES;
+      for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+        float f[kChunk] = {};
+        if (c * kChunk < a.dim) load8(src, (int64_t)c * kChunk, a.dim - (int64_t)c * kChunk, f);
+        f32x4_t* to = PACKED ? (f32x4_t*)lds + slot * 2 * chunks + c
+                             : (f32x4_t*)(lds + slot * LANES * N * kChunk + c / LANES * LANES * kChunk) + c % LANES;
         to[0] = f32x4_t{f[0], f[1], f[2], f[3]};
-        to[LANES] = f32x4_t{f[4], f[5], f[6], f[7]};
+        to[PACKED ? chunks : LANES] = f32x4_t{f[4], f[5], f[6], f[7]};
       }
       ++slot;
     }
@@ -442,11 +444,19 @@ struct ParamTable {
   __device__ __forceinline__ const float* at(const ResidualArgs& a, int k) const {
     int slot = 0;
     for (int q = 0; q < k; ++q) slot += source(a, q).p != nullptr;
-    return lds + slot * kFloats;
+    return lds + slot * (PACKED ? chunks : LANES * N) * kChunk;
   }
   __device__ __forceinline__ void get(const float* p, int n, float (&f)[kChunk]) const {
-    const f32x4_t* from = (const f32x4_t*)(p + n * LANES * kChunk) + lane;
-    const f32x4_t lo = from[0], hi = from[LANES];
+    f32x4_t lo, hi;
+    if constexpr (PACKED) {
+      const int own = n * LANES + lane, c = own < chunks ? own : chunks - 1;
+      lo = ((const f32x4_t*)p)[c];
+      hi = ((const f32x4_t*)p)[chunks + c];
+    } else {
+      const f32x4_t* from = (const f32x4_t*)(p + n * LANES * kChunk) + lane;
+      lo = from[0];
+      hi = from[LANES];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[i] = lo[i];
@@ -456,8 +466,8 @@ struct ParamTable {
 };
 
 // The gate of a row's chunk, times scale.
-template <int LANES, int N>
-__device__ __forceinline__ void gate_values(const ResidualArgs& a, const ParamTable<LANES, N>& par, const float* pg, const RowAny<N>& rows,
+template <int LANES, int N, bool PACKED>
+__device__ __forceinline__ void gate_values(const ResidualArgs& a, const ParamTable<LANES, N, PACKED>& par, const float* pg, const RowAny<N>& rows,
                                             int64_t row, int n, float (&g)[kChunk]) {
   if (a.gate_rows) {
     rows.unpack(n, a.gate.bf16, g);
@@ -473,8 +483,8 @@ __device__ __forceinline__ void gate_values(const ResidualArgs& a, const ParamTa
 }
 
 // u (after dropout), y^ in y's place; the mask of the chunk.
-template <int LANES, int N>
-__device__ __forceinline__ DropWords branch_values(const ResidualArgs& a, const DropKey& key, const ParamTable<LANES, N>& par,
+template <int LANES, int N, bool PACKED>
+__device__ __forceinline__ DropWords branch_values(const ResidualArgs& a, const DropKey& key, const ParamTable<LANES, N, PACKED>& par,
                                                   const float* pw, const float* pb, int64_t row, int n, float m1, float r1,
                                                   float (&y)[kChunk], float (&u)[kChunk]) {
 #pragma unroll
@@ -551,7 +561,7 @@ __global__ __launch_bounds__(BLOCK, 4) void k_residual_rows(ResidualArgs a) {
     if (a.gate_rows) gr.template load<LANES>(a.gate, r, a.gate_ld, a, lane);
   };
   fetch(row);
-  ParamTable<LANES, N> par{lds, lane};
+  ParamTable<LANES, N, (LANES == 1024)> par(lds, lane, a.dim);
   par.fill(a, kParams);
   __syncthreads();
   const float *pw = par.at(a, kPostW), *pb = par.at(a, kPostB), *pg = par.at(a, kGate), *nw = par.at(a, kNextW),
@@ -643,7 +653,7 @@ __global__ __launch_bounds__(BLOCK, backward_waves(LANES, N)) void k_residual_ro
     if (a.dh) dhr.template load<LANES>((const TY*)a.dh, r, a.dh_ld, a, lane);
   };
   if (kAhead) fetch(row);
-  ParamTable<LANES, N> par{lds, lane};
+  ParamTable<LANES, N, false> par(lds, lane, a.dim);
   par.fill(a, kNextB);  // next's bias has no part in it
   __syncthreads();
   const float *pw = par.at(a, kPostW), *pb = par.at(a, kPostB), *pg = par.at(a, kGate), *nw = par.at(a, kNextW);
@@ -824,7 +834,8 @@ int held(const ResidualArgs& a, bool backward) {
 }
 // LDS bytes of a launch of teams; the backward's hold its blocks' sums at the end.
 int team_lds(const ResidualArgs& a, bool backward, int lanes, int n, int block) {
-  const int params = held(a, backward) * lanes * n * kChunk * 4, tile = backward ? block * kChunk * 4 : 0;
+  const int chunks = !backward && lanes == 1024 ? (int)ceil_div(a.dim, kChunk) + 1 : lanes * n;
+  const int params = held(a, backward) * chunks * kChunk * 4, tile = backward ? block * kChunk * 4 : 0;
   return params > tile ? params : tile;
 }
 
