@@ -239,12 +239,24 @@ __device__ __forceinline__ int block_place(bool mine, int* counts, int& total) {
   return before + __popcll(has & ((1ull << lane) - 1));
 }
 
+// How many of n keys in LDS are larger than key; they lie at 16 bytes, a key of 0 behind an odd count.
+__device__ __forceinline__ int rank_among(const uint64_t* keys, int n, uint64_t key) {
+  int rank = 0;
+#pragma unroll 4
+  for (int o = 0; o < n; o += 2) {
+    const u32x4_t two = *(const u32x4_t*)(keys + o);
+    rank += ((uint64_t)two[1] << 32 | two[0]) > key;
+    rank += ((uint64_t)two[3] << 32 | two[2]) > key;
+  }
+  return rank;
+}
+
 struct TopShared {
   float most[kThreads];
   int list[kThreads], counts[kWaves];
   int found, bound;
   float threshold;
-  uint64_t keys[kCandidates];
+  __align__(16) uint64_t keys[kCandidates + 2];
   uint64_t best[kWaves];
 };
 
@@ -321,10 +333,13 @@ __device__ __forceinline__ void block_top(const T* l, int top, int begin, int ch
   __syncthreads();
   const int found = sh.found;
   if (found <= kCandidates) {
+    if (found & 1) {
+      if (tid == 0) sh.keys[found] = 0;
+      __syncthreads();
+    }
     for (int i = tid; i < found; i += kThreads) {
       const uint64_t key = sh.keys[i];
-      int rank = 0;
-      for (int o = 0; o < found; ++o) rank += sh.keys[o] > key;
+      const int rank = rank_among(sh.keys, found, key);
       if (rank < top) out(rank, key);
     }
     for (int j = found + tid; j < top; j += kThreads) out(j, 0);
@@ -420,45 +435,52 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_block(LogpArgs a) {
   }
 }
 
-// A row's result from its parts. Their keys lie in falling order; with c = ceil(top /
-// parts), every part has c keys from the least of the parts' c-th on, top in all, and one part has top keys from
-// its last on: keys below either are not among the likeliest.
+// A row's result from its parts. Their keys lie in falling order; with c = ceil(top / parts)
+// and n = ceil(top / c), n parts have c keys each from the n-th largest of the parts' c-th keys
+// on, top in all: keys below it are not among the likeliest.
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogpArgs a) {
-  __shared__ uint64_t keys[kMaxParts * kLogpMaxTop], floors[kMaxParts][2];
+  __shared__ __align__(16) uint64_t keys[kMaxParts * kLogpMaxTop + 2], cth[kMaxParts];
+  __shared__ RowSum sums;
+  __shared__ uint64_t floor;
   __shared__ int found;
   const int tid = threadIdx.x;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    RowSum r = part_sums(a, row)[0];
-    for (int p = 1; p < a.parts; ++p) r = merged(r, part_sums(a, row)[p]);
-    const RowResult q = row_result(r);
-    if (tid == 0) write_row(a, row, q);
-    if (!a.top) continue;
     const uint64_t* from = part_keys(a, row);
-    const int c = (a.top + a.parts - 1) / a.parts;
-    if (tid < a.parts) {
-      floors[tid][0] = from[tid * a.top + a.top - 1];
-      floors[tid][1] = from[tid * a.top + c - 1];
-    }
-    if (tid == 0) found = 0;
-    __syncthreads();
-    uint64_t most = 1, least = ~0ull;  // 1: keys of 0 are none
-    for (int p = 0; p < a.parts; ++p) {
-      most = floors[p][0] > most ? floors[p][0] : most;
-      least = floors[p][1] < least ? floors[p][1] : least;
-    }
-    const uint64_t floor = least > most ? least : most;
-    for (int i = tid; i < a.parts * a.top; i += kThreads) {
-      const uint64_t k = from[i];
-      if (k >= floor) keys[atomicAdd(&found, 1)] = k;
+    const int c = a.top ? (a.top + a.parts - 1) / a.parts : 1, n = (a.top + c - 1) / c;
+    uint64_t mine = 0;
+    if (tid < 64) {
+      RowSum r = tid < a.parts ? part_sums(a, row)[tid] : empty_sum();
+      if (a.top && tid < kMaxParts) cth[tid] = mine = tid < a.parts ? from[tid * a.top + c - 1] : 0;
+      const float m = wave_max(r.m);
+      raise(r, m);
+      r = {m, lanes_sum<64>(r.n), lanes_sum<64>(r.s), lanes_sum<64>(r.a)};
+      if (tid == 0) {
+        sums = r;
+        found = 0;
+        floor = 1;  // keys of 0 are none
+      }
     }
     __syncthreads();
-    for (int i = tid; i < found; i += kThreads) {
-      const uint64_t key = keys[i];
-      int rank = 0;
-      for (int o = 0; o < found; ++o) rank += keys[o] > key;
-      if (rank < a.top) write_top(a, row, rank, key, q);
+    const RowResult q = row_result(sums);
+    if (tid == 0) write_row(a, row, q);
+    if (a.top) {
+      if (mine && rank_among(cth, kMaxParts, mine) == n - 1) floor = mine;
+      __syncthreads();
+      for (int i = tid; i < a.parts * a.top; i += kThreads) {
+        const uint64_t k = from[i];
+        if (k >= floor) keys[atomicAdd(&found, 1)] = k;
+      }
+      __syncthreads();
+      const int count = found;
+      if (tid == 0) keys[count] = 0;
+      __syncthreads();
+      for (int i = tid; i < count; i += kThreads) {
+        const uint64_t key = keys[i];
+        const int rank = rank_among(keys, count, key);
+        if (rank < a.top) write_top(a, row, rank, key, q);
+      }
+      for (int j = count + tid; j < a.top; j += kThreads) write_top(a, row, j, 0, q);
     }
-    for (int j = found + tid; j < a.top; j += kThreads) write_top(a, row, j, 0, q);
     __syncthreads();
   }
 }

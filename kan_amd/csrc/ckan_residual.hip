@@ -299,7 +299,7 @@ __global__ __launch_bounds__(1024) void k_residual_sums(ResidualArgs a, const fl
   const int64_t col = (int64_t)blockIdx.x * 64 + lane;
   float v = 0.0f;
   if (col < a.dim) {
-#pragma unroll 8
+#pragma unroll 16
     for (int s = wave; s < parts; s += 16) v += part[((int64_t)s * kSums + k) * a.dim + col];
   }
   red[wave][lane] = v;
