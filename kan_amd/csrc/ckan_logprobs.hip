@@ -191,27 +191,46 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_team(LogpArgs a) {
     const RowResult q = row_result(r);
     const bool write = mine < a.rows;
     if (lane == 0 && write) write_row(a, row, q);
-    for (int j = 0; j < a.top; ++j) {
-      float own = -INFINITY;
+    if (!a.top) continue;
+    float largest[N];  // of each chunk
 #pragma unroll
-      for (int i = 0; i < N * kChunk; ++i) own = fmaxf(own, v[i]);
+    for (int n = 0; n < N; ++n) {
+      largest[n] = v[n * kChunk];
+#pragma unroll
+      for (int i = 1; i < kChunk; ++i) largest[n] = fmaxf(largest[n], v[n * kChunk + i]);
+    }
+    for (int j = 0; j < a.top; ++j) {
+      float own = largest[0];
+#pragma unroll
+      for (int n = 1; n < N; ++n) own = fmaxf(own, largest[n]);
       const float best = lanes_max<LANES>(own);
       const unsigned long long has = __ballot(own == best && best > -INFINITY) >> (in_wave & ~(LANES - 1));
       const unsigned long long team = LANES == 64 ? has : has & ((1ull << (LANES & 63)) - 1);
       const int from = team ? __ffsll(team) - 1 : -1;
-      if (lane == from) {
-        int at = N * kChunk - 1;
+      // the lane's first chunk that holds it, a scalar where a wave has one row
+      int chunk = N - 1;
 #pragma unroll
-        for (int i = N * kChunk - 2; i >= 0; --i) at = v[i] == best ? i : at;
+      for (int n = N - 2; n >= 0; --n) chunk = largest[n] == best ? n : chunk;
+      if constexpr (N > 1) chunk = __builtin_amdgcn_readlane(chunk, from < 0 ? 0 : __builtin_amdgcn_readfirstlane(from));
 #pragma unroll
-        for (int i = 0; i < N * kChunk; ++i) v[i] = i == at ? -INFINITY : v[i];
+      for (int n = 0; n < N; ++n) {
+        if (n != chunk || lane != from) continue;
+        float* w = v + n * kChunk;
+        int at = kChunk - 1;
+#pragma unroll
+        for (int i = kChunk - 2; i >= 0; --i) at = w[i] == best ? i : at;
+        largest[n] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          w[i] = i == at ? -INFINITY : w[i];
+          largest[n] = fmaxf(largest[n], w[i]);
+        }
         if (write) {
           a.top_logp[row * a.top + j] = (best - q.m) - q.logs;
-          a.top_idx[row * a.top + j] = (int64_t)lane * N * kChunk + at;
+          a.top_idx[row * a.top + j] = ((int64_t)lane * N + n) * kChunk + at;
         }
-      } else if (from < 0 && lane == 0 && write) {
-        write_top(a, row, j, 0, q);
       }
+      if (from < 0 && lane == 0 && write) write_top(a, row, j, 0, q);
     }
   }
 }
@@ -384,7 +403,7 @@ __device__ __forceinline__ uint64_t* part_keys(const LogpArgs& a, int64_t row) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_logprobs_block(LogpArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 1) void k_logprobs_block(LogpArgs a) {
   __shared__ RowSum sums[kWaves];
   __shared__ TopShared sh;
   const int tid = threadIdx.x, part = blockIdx.y;
@@ -397,21 +416,51 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_block(LogpArgs a) {
     int head = off ? per16 - off : 0;
     if (head > c1 - c0) head = c1 - c0;
     const int begin = c0 + head, chunks = (c1 - begin) / kChunk, tail = begin + chunks * kChunk;
+    // r.m is the wave's: a chunk of the wave with nothing as large, all but a few, needs no comparison
+    // with it and no rescaling (4000 rows of 50001 classes in bf16: 98 -> 84 us)
     RowSum r = empty_sum();
     float edge = -INFINITY, edge2 = -INFINITY;
     if (tid < head) edge = (float)l[c0 + tid];
     if (tid < c1 - tail) edge2 = (float)l[tail + tid];
     int seen = 0;
+    float most = -INFINITY;
     const T* p = l + begin;
-#pragma unroll 2
-    for (int q = tid; q < chunks; q += kThreads) {
+    constexpr int kAhead = 2;  // chunks on their way
+    typename RawOf<T>::type raw[kAhead];
+    const auto fetch = [&](int q, typename RawOf<T>::type& to) {
+      if (q < chunks) to = *(const typename RawOf<T>::type*)__builtin_assume_aligned(p + (int64_t)q * kChunk, 16);
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) fetch(u * kThreads + tid, raw[u]);
+    for (int q0 = 0; q0 < chunks; q0 += kAhead * kThreads)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int q = q0 + u * kThreads + tid;
+      if (q0 + u * kThreads >= chunks) break;
       float v[kChunk];
-      unpack8(*(const typename RawOf<T>::type*)__builtin_assume_aligned(p + (int64_t)q * kChunk, 16), v);
-      const float before = r.n > 0.0f ? r.m : -INFINITY;  // the lowest finite value is a largest too
-      add_logits(r, v);
-      seen = r.n > 0.0f && r.m > before ? begin + q * kChunk : seen;
+      unpack8(raw[u], v);
+      if (q >= chunks) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] = -INFINITY;
+      }
+      fetch(q + kAhead * kThreads, raw[u]);
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < kChunk; ++i) top = fmaxf(top, v[i]);
+      if (__any(top >= r.m)) {
+        raise(r, wave_max(fmaxf(top, r.m)));
+        add_logits(r, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          const float d = v[i] - r.m, e = exp_of(d);
+          r.s += e;
+          r.a = fmaf(e, fmaxf(d, kFar), r.a);
+        }
+      }
+      seen = top > most ? begin + q * kChunk : seen;
+      most = fmaxf(most, top);
     }
-    const float most = r.n > 0.0f ? r.m : -INFINITY;
     {
       const float v[2] = {edge, edge2};
       add_logits(r, v);
