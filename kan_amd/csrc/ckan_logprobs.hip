@@ -120,7 +120,7 @@ __device__ __forceinline__ void write_top(const LogpArgs& a, int64_t row, int j,
 }
 
 constexpr int kThreads = 256;
-constexpr int kTeamMaxClasses = 2048;
+constexpr int kTeamMaxClasses = 4096;
 
 // ---- up to kTeamMaxClasses: a row in the registers of a team of lanes ----------------
 template <int CTRL>
@@ -589,7 +589,7 @@ void forward_typed(const LogpArgs& a, hipStream_t st) {
     return;                                                                                                         \
   }
     CKAN_LOGP_TEAM(8, 1) CKAN_LOGP_TEAM(16, 1) CKAN_LOGP_TEAM(32, 1) CKAN_LOGP_TEAM(64, 1) CKAN_LOGP_TEAM(64, 2)
-    CKAN_LOGP_TEAM(64, 4)
+    CKAN_LOGP_TEAM(64, 4) CKAN_LOGP_TEAM(64, 8)
 #undef CKAN_LOGP_TEAM
   }
   const unsigned rows = (unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20);
