@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .mixture import _on, _once, _stream
+from .mixture import _on, _once, _pitched, _stream
 
 _NORMS = {"rms": _lib.CKAN_NORM_RMS, "layer": _lib.CKAN_NORM_LAYER}
 _DTYPES = {torch.float32: _lib.CKAN_DTYPE_F32, torch.bfloat16: _lib.CKAN_DTYPE_BF16}
@@ -90,6 +90,10 @@ class ResidualFunction(torch.autograd.Function):
             dout = _rows(dout if dout.dtype == x.dtype else dout.to(x.dtype), desc.dim)
         if dh is not None:
             dh = _rows(dh if dh.dtype == ctx.h_dtype else dh.to(ctx.h_dtype), desc.dim)
+        x, y = _rows(x, desc.dim), y if y is None else _rows(y, desc.dim)
+        if desc.gate_rows:
+            gate = _rows(gate, desc.dim)
+        desc = _pitched(desc, x_ld=x.stride(0), y_ld=_pitch(y), gate_ld=gate.stride(0) if desc.gate_rows else 0)
         inputs = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip(inputs, need)]
         if desc.rows == 0:
@@ -156,6 +160,8 @@ def _residual(x, y, gate, post_weight, post_bias, next_weight, next_bias, norm, 
         raise RuntimeError(f"x must be [..., dim] with dim >= 1, got {tuple(x.shape)}")
     shape, dev = x.shape, x.device
     dim = shape[-1]
+    if dim > 1 << 20:  # the descriptor's 32 bits would take a larger one for another
+        raise RuntimeError(f"dim above 2^20 is not supported, got {dim}")
     _lib.refuse_tangents("residual_norm", x, y, gate, post_weight, post_bias, next_weight, next_bias)
     _check("x", dev, x)
     for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("next_weight", next_weight),
@@ -326,10 +332,12 @@ class LogProbsFunction(torch.autograd.Function):
         if dlogp is None and dentropy is None:
             return None, None, None, None
         logits, targets, stats = ctx.saved_tensors
+        logits = _rows(logits, ctx.desc.classes)
+        desc = _pitched(ctx.desc, logits_ld=logits.stride(0))
         dlogp, dentropy = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
                            else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))
         dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _lib.check(_lib.load().ckan_log_probs_backward(ctx.desc, logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
+        _lib.check(_lib.load().ckan_log_probs_backward(desc, logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
                                                        _lib.ptr(dlogp), _lib.ptr(dentropy), dl.data_ptr(),
                                                        _stream(dl.device)))
         return dl, None, None, None
@@ -354,11 +362,13 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> L
         raise RuntimeError(f"targets must be {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
     if targets.dtype != torch.int64:
         raise RuntimeError(f"targets must be int64, got {targets.dtype}")
+    shape, classes = targets.shape, logits.shape[-1]
+    if classes > 1 << 30 or not 0 <= top <= 64:  # the descriptor's 32 bits would take others for these
+        raise RuntimeError(f"log_probs takes up to 2^30 classes and top from 0 to 64, got {classes} and {top}")
     _lib.refuse_tangents("log_probs", logits)
     _check("logits", logits.device, logits)
     if targets.device != logits.device:
         raise RuntimeError(f"targets are on {targets.device}, logits on {logits.device}: one device is needed")
-    shape, classes = targets.shape, logits.shape[-1]
     logits = _rows(logits, classes)
     if len(shape) != 1 or not targets.is_contiguous():
         targets = targets.reshape(-1).contiguous()

@@ -72,6 +72,25 @@ def _once(name: str) -> None:
         raise RuntimeError(f"{name} is differentiable once (create_graph is not supported)")
 
 
+def _pitched(desc, **pitches):
+    """desc with these row pitches: a hook on saved tensors may have returned them in another layout
+    than they were saved in."""
+    if all(getattr(desc, name) == pitch for name, pitch in pitches.items()):
+        return desc
+    desc = type(desc).from_buffer_copy(desc)
+    for name, pitch in pitches.items():
+        setattr(desc, name, pitch)
+    return desc
+
+
+def _logit_rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """logits with contiguous rows, and their pitch."""
+    experts = logits.shape[1]
+    if logits.stride(1) != 1 or logits.stride(0) < experts:
+        logits = logits.contiguous()
+    return logits, max(logits.stride(0), experts)
+
+
 class RouteFunction(torch.autograd.Function):
     """The weights of ``route``, differentiable in the logits; the indices go by the
     side (``out``): an output more costs the autograd engine 4 us a step."""
@@ -92,9 +111,10 @@ class RouteFunction(torch.autograd.Function):
             raise RuntimeError("route's indices were modified in place before its backward; change a clone")
         if dw.dtype != torch.float32 or not dw.is_contiguous():
             dw = dw.to(torch.float32).contiguous()
-        dl = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        logits, ld = _logit_rows(logits)
         # the engine runs a node on its device and stream
-        _lib.check(_lib.load().ckan_route_backward(ctx.desc, logits.data_ptr(), ctx.idx.data_ptr(), dw.data_ptr(),
+        _lib.check(_lib.load().ckan_route_backward(_pitched(ctx.desc, logits_ld=ld), logits.data_ptr(), ctx.idx.data_ptr(), dw.data_ptr(),
                                                    dl.data_ptr(), _stream(dl.device)))
         return dl, None, None, None
 
@@ -128,9 +148,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
         if tuple(bias.shape) != (experts,):
             raise RuntimeError(f"bias must be [{experts}], got {tuple(bias.shape)}")
         bias = bias.detach().to(torch.float32).contiguous()
-    if logits.stride(1) != 1 or logits.stride(0) < experts:
-        logits = logits.contiguous()
-    desc = _lib.CkanRouteDesc(logits.shape[0], max(logits.stride(0), experts), experts, int(top_k),
+    logits, ld = _logit_rows(logits)
+    desc = _lib.CkanRouteDesc(logits.shape[0], ld, experts, int(top_k),
                               _SCORES[score], int(groups), int(top_groups), int(bool(renormalize)),
                               code, float(scale))
     if torch.is_grad_enabled() and logits.requires_grad:
@@ -266,6 +285,10 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
         raise RuntimeError(f"gate must be [{experts}, {in_dim}], got {tuple(gate.shape)}")
     if bias is not None and tuple(bias.shape) != (experts,):
         raise RuntimeError(f"bias must be [{experts}], got {tuple(bias.shape)}")
+    for name, v in (("in_dim", in_dim), ("out_dim", out_dim), ("degree", dd - 1), ("top_k", top_k), ("groups", groups),
+                    ("top_groups", top_groups)):
+        if not -1 <= v < 1 << 31:  # the descriptor's 32 bits would take another number for it
+            raise RuntimeError(f"{name} is out of range: {v}")
     rows, lib = x.shape[0], _lib.load()
     desc = _lib.CkanMixtureDesc(rows, experts, int(top_k), in_dim, out_dim, dd - 1, _SCORES[score], int(groups),
                                 int(top_groups), int(bool(renormalize)), *codes, float(scale))

@@ -158,6 +158,15 @@ def test_python_refusals(call, error, match):
         call()
 
 
+def test_sizes_past_the_descriptors_32_bits_are_refused():
+    meta = dict(device="meta")
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        f.row_norm(torch.zeros(1, 2 ** 32 + 8, **meta), W)
+    for classes, top in ((2 ** 32 + 8, 0), (100, 2 ** 32 + 1), (100, -1)):
+        with pytest.raises(RuntimeError, match="2\\^30 classes"):
+            f.log_probs(torch.zeros(1, classes, **meta), torch.zeros(1, dtype=torch.int64, **meta), top=top)
+
+
 @pytest.mark.parametrize("call", [
     lambda d: f.row_norm(d, W), lambda d: f.residual_norm(X, d), lambda d: f.residual_norm(d, X),
     lambda d: f.dropout(d, 0.5, 1), lambda d: f.log_probs(d, torch.zeros(2, dtype=torch.int64)),

@@ -67,6 +67,7 @@ CASES = {
     "dropout": lambda: _dropout((77, 130), torch.bfloat16),
     "log_probs, team": lambda: _log_probs(200, 70, 4, True),
     "log_probs, block": lambda: _log_probs(600, 3000, 4, True),
+    "log_probs, long rows": lambda: _log_probs(600, 5000, 4, True),
     "log_probs, parts": lambda: _log_probs(2, 50000, 20, True),
     "mixture, one row": lambda: _mixture(1, 300, 200, 8),
     "mixture, few rows": lambda: _mixture(7, 300, 200, 8),

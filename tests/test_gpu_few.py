@@ -104,6 +104,15 @@ def test_wide_layers():
         check(x, gate, coeffs, 2)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 20])
+def test_large_gates(rows):
+    """Gates of more than 2^16 entries, whose logits a launch of their own makes."""
+    for in_dim, experts, dtype in ((1100, 64, F32), (130, 512, BF16), (3001, 24, F32)):
+        x, gate, coeffs = make(rows, in_dim, 20, 3, experts, F32, dtype, F32, in_dim)
+        assert in_dim * experts > 1 << 16
+        check(x, gate, coeffs, 3)
+
+
 def test_many_rows_and_gradients_take_the_parts():
     x, gate, coeffs = (t.cuda() for t in make(300, 40, 30, 4, 4, F32, F32, F32, 6))
     with torch.no_grad():

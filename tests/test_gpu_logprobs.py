@@ -117,6 +117,16 @@ def test_masks_ties_and_rows_of_nothing(classes, dtype):
         compare(l, t, top)
 
 
+@pytest.mark.parametrize("classes", [2050, 3001, 4088, 4095, 4096, 4097, 4104])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_where_rows_leave_the_registers(classes, dtype):
+    for rows, top in ((1, 64), (7, 10), (530, 3)):
+        l, t = logits(rows, classes, dtype, classes + rows)
+        l[0, classes - 9:] = 20.0  # equal ones in a row's last chunks
+        l[rows - 1] = torch.sort(l[rows - 1]).values
+        compare(l, t, top)
+
+
 def test_sure_rows_keep_their_relative_precision():
     """exp(-d) for d up to 80 beside the largest: log p and entropy to a few half steps of themselves."""
     for classes in (16, 900, 5000):
