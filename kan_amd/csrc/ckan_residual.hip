@@ -848,6 +848,16 @@ int64_t team_blocks(const ResidualArgs& a, int teams, int block, int waves, int 
   const int64_t all = ceil_div(a.rows, teams), most = (int64_t)per_cu * kNumCUs;
   return all < most ? all : most;
 }
+// The forward's, which leave no sums: four times as many in fp32 where their teams keep four rows each. A
+// chip of blocks that begin and end apart spreads reads and writes better than one that runs in step (65536 x
+// 512 111 -> 103 us, 131072 x 256 111 -> 105); in bf16, with half of the bytes a row, filling the parameters
+// costs more (56.8 -> 58.6), with fewer rows too (8192 x 1000 16.0 -> 22.9), and of a wider row's parameters (8192 x
+// 4096 101.9 -> 103.7).
+template <typename TX, typename TY>
+int64_t forward_blocks(const ResidualArgs& a, int teams, int block, int lds) {
+  const int64_t blocks = team_blocks(a, teams, block, 4, lds);
+  return sizeof(TX) + sizeof(TY) == 8 && block == 256 && a.rows >= 16 * teams * blocks ? 4 * blocks : blocks;
+}
 constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
 
 // The team of a width, WIDE that of the widest rows: in the backward half as many lanes, whose 256
@@ -887,7 +897,7 @@ void forward_typed(const ResidualArgs& a, hipStream_t st) {
 #define CKAN_FORWARD(L, NN, B)                                                                           \
   static std::atomic<uint32_t> done;                                                                     \
   const int lds = team_lds(a, false, L, NN, B);                                                          \
-  launch_team(k_residual_rows<TX, TY, L, NN, B>, a, team_blocks(a, B / L, B, 4, lds), B, lds, st, done); \
+  launch_team(k_residual_rows<TX, TY, L, NN, B>, a, forward_blocks<TX, TY>(a, B / L, B, lds), B, lds, st, done); \
   return;
     CKAN_TEAM(a.dim, CKAN_FORWARD, CKAN_FORWARD(1024, 1, 1024));
 #undef CKAN_FORWARD
