@@ -398,7 +398,9 @@ class ResidualKAN(nn.Module):
     ``final_norm``, else x.
 
     ``dropout`` is drawn in training mode from the buffer ``dropout_state`` (seed, offset): a forward uses one
-    call a layer and moves the offset on, on the device, so that replays of a captured step draw anew."""
+    call a layer and moves the offset on, on the device, so that replays of a captured step draw anew. A forward
+    made again for its backward (activation checkpointing) would draw other masks: checkpoint the layers, not the
+    stack. Ranks of a data-parallel run draw different masks only if their buffers are not broadcast."""
 
     def __init__(self, layers: Iterable[nn.Module], dim: int, *, norm: str = "rms", post: bool = True,
                  gate: Optional[float] = 0.1, scale: float = 1.0, dropout: float = 0.0, eps: float = 1e-6,

@@ -52,8 +52,10 @@ void launch_gate(const FewArgs& a, hipStream_t st) {
 void few_plan(FewArgs* a) {
   const int64_t rows = a->route.rows, S = rows * a->route.top_k, E = a->route.E;
   const int64_t active = E < S ? E : S;
-  // as few slots as the experts' coefficients are streamed for: 16 an expert on average
-  a->few = rows > 0 && S <= kFewMaxSlots && S <= 16 * active;
+  // fewer than 64 slots an expert on average, two passes of kFewRows: 240 rows, two of 8 experts of 1024 -> 1024, degree
+  // 8, 105 us in bf16 and 174 in fp32 (the parts' entry points, which pack the coefficients, 173 and 279), 64 rows 53 and 88
+  // (110 and 137); 500 rows of 512 -> 512, two of 16, 76 and 118 (111 and 162)
+  a->few = rows > 0 && S <= kFewMaxSlots && S < 64 * active;
   if (!a->few) return;
   a->S = (int)S;
   a->active = (int)active;
@@ -62,10 +64,10 @@ void few_plan(FewArgs* a) {
   a->apart = E * a->I > (1 << 16);
   a->gated = rows == 1 && !a->apart;
   const bool by_row = rows <= kRowsMax;
-  // chunks of inputs: a block of k_few_rows a CU, eight of k_few_stream's, at least an input a
+  // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's, at least an input a
   // wave, at most what a block holds
   const int64_t oc = ceil_div(a->O, by_row && a->coeff_bf16 ? 128 : 64), hold = by_row ? kRowTanh : kFewInputs;
-  int64_t chunks = by_row ? ceil_div(kNumCUs, oc) : ceil_div(8 * kNumCUs, active * oc);
+  int64_t chunks = by_row ? ceil_div(kNumCUs, oc) : ceil_div(4 * kNumCUs, active * oc);
   if (chunks > ceil_div(a->I, 16)) chunks = ceil_div(a->I, 16);
   if (chunks < ceil_div(a->I, hold)) chunks = ceil_div(a->I, hold);
   a->chunk_inputs = (int)ceil_div(a->I, chunks);

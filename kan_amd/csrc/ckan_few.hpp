@@ -283,25 +283,60 @@ __global__ __launch_bounds__(256) void k_few_rows_sum(FewArgs a) {
   if (wave == 0 && q < n) ((TX*)a.y)[q] = (TX)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
 }
 
-// More rows: a block takes one of the chosen experts, 64 outputs (a lane
-// each) and a chunk of inputs, and leaves part[chunk, slot, o]. It finds its expert and that expert's
-// slots itself; the first coefficients are on their way while it makes the basis values of up to
-// kFewRows rows in LDS (read as broadcasts).
-constexpr int kFewMaxSlots = 1024, kFewInputs = 64, kFewRows = 8;
+// More rows: a block takes one of the chosen experts, 64 outputs and a chunk of inputs, and leaves part[chunk,
+// slot, o] of up to kFewRows rows at a time. It finds its expert and that expert's slots itself.
+//
+// The products run on the matrix cores: on the vector ALU 64 rows, two of 8 experts of 1024 -> 1024, degree 8, took 112 us
+// in bf16 and 131 in fp32 (here 52 and 85, of which the coefficients' stream is 29 and 59 and the launches of gate and sum
+// 13); 20 rows, one of 8 of 2048 -> 2048, degree 4, 75 and 139 (57 and 131). In an instruction of 16 outputs by 16 rows by 32 products a lane holds eight
+// coefficients of one input and output, as they lie, and against them eight basis values of that input for one
+// row, made in registers: bf16 coefficients are an operand as they are, fp32 ones and the basis values three bf16
+// planes (24 bits), of whose products those below 2^-24 are left out. T_0 = 1 is a sum of coefficients beside them;
+// degrees above 8 take a second run of eight basis values, padded with zeros.
+constexpr int kFewMaxSlots = 1024, kFewInputs = 128, kFewRows = 32;
 
-template <typename TX, typename TC, int D>
-__global__ __launch_bounds__(256) void k_few_stream(FewArgs a) {
-  constexpr int kDeg = D - 1, kW = (kDeg + 3) / 4 * 4, kU = D * sizeof(TC) <= 36 ? 4 : 2;
+// The eight coefficients of an output (its T_0 at `from`) from 8 G + 1 on as an operand.
+template <int D, int G>
+__device__ __forceinline__ Frag<kBf16> coef_frag(const __bf16* from) {
+  Frag<kBf16> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = 8 * G + j + 1 < D ? from[8 * G + j + 1 < D ? 8 * G + j + 1 : 0] : (__bf16)0.0f;
+  return f;
+}
+template <int D, int G>
+__device__ __forceinline__ Frag<kSplit> coef_frag(const float* from) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 8 * G + j + 1 < D ? from[8 * G + j + 1 < D ? 8 * G + j + 1 : 0] : 0.0f;
+  return make_frag_split_any(v);
+}
+__device__ __forceinline__ void add_products(f32x4_t& acc, const Frag<kBf16>& c, const Frag<kSplit>& b) {
+#pragma unroll
+  for (int k = 2; k >= 0; --k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c.v, b.p[k], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void add_products(f32x4_t& acc, const Frag<kSplit>& c, const Frag<kSplit>& b) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int k = 0; k <= s; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c.p[k], b.p[s - k], acc, 0, 0, 0);
+}
+
+// A lane's coefficients are those of P outputs next to each other, which go to tiles of their own: pairs in bf16, where
+// outputs are even, so that they begin at whole dwords (20 rows of the case above: 75 us, one by one 99).
+template <typename TX, typename TC, int D, int P>
+__global__ __launch_bounds__(256, sizeof(TC) == 2 || D <= 12 ? 3 : 2) void k_few_stream(FewArgs a) {
+  constexpr int kTiles = 4, kCols = kFewRows / 16, kPitch = 64 + 4;
   __shared__ int slots[kFewMaxSlots], counts[4];
   __shared__ unsigned chosen[kRouteMaxExperts / 32];
-  __shared__ __align__(16) float basis[kFewInputs * kFewRows * kW];
-  __shared__ float red[4][kFewRows][64];
+  __shared__ float t[kFewRows][kFewInputs + 1];
+  __shared__ __align__(16) float red[4][16][kPitch];
+  __shared__ float first[4][64];
   const int oc = (a.O + 63) / 64;
   int id = blockIdx.x;
   const int chunk = id % a.chunks;
   id /= a.chunks;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int o = id % oc * 64 + lane;
+  const int o0 = id % oc * 64;
   int nth = id / oc;
   if (tid < kRouteMaxExperts / 32) chosen[tid] = 0;
   __syncthreads();
@@ -338,55 +373,110 @@ __global__ __launch_bounds__(256) void k_few_stream(FewArgs a) {
     __syncthreads();
   }
   const int i0 = chunk * a.chunk_inputs, ni = a.I - i0 < a.chunk_inputs ? a.I - i0 : a.chunk_inputs;
-  const bool real = o < a.O;
   const int64_t pitch = (int64_t)a.O * D;
-  const TC* C = (const TC*)a.coeffs + (((int64_t)e * a.I + i0) * a.O + (real ? o : 0)) * D;
+  // a lane's outputs o0 + (16 q + lane % 16) P and on, its inputs i + lane / 16
+  const int col = lane & 15, sub = lane >> 4;
+  // (loads past the ends go to the last ones: a branch around a load makes the compiler wait for it at once)
+  const TC* C = (const TC*)a.coeffs + ((int64_t)e * a.I + i0) * pitch;
+  int off[kTiles / P];
+#pragma unroll
+  for (int q = 0; q < kTiles / P; ++q) {
+    const int o = o0 + (q * 16 + col) * P;
+    off[q] = (o < a.O ? o : a.O - P) * D;
+  }
   float* part = (float*)(a.ws + a.part_off) + (size_t)chunk * a.S * a.O;
   for (int r0 = 0; r0 < n; r0 += kFewRows) {
     const int nr = n - r0 < kFewRows ? n - r0 : kFewRows;
-    Coefs<TC, D> c[kU];
-    const auto fetch = [&](int i) {
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        if (i + 4 * u < ni) c[u] = *(const Coefs<TC, D>*)(C + (i + 4 * u) * pitch);
+    Coefs<TC, D * P> c[kTiles / P];
+    const auto fetch = [&](int i, int q) {  // inputs from i on
+      const TC* at = C + (int64_t)(i + sub < ni ? i + sub : ni - 1) * pitch;
+      c[q] = *(const Coefs<TC, D * P>*)(at + off[q]);
     };
-    fetch(wave);
+#pragma unroll
+    for (int q = 0; q < kTiles / P; ++q) fetch(wave * 4, q);
     for (int q = tid; q < ni * nr; q += 256) {
       const int r = q / ni, i = q - r * ni;
-      const float t = tanhf((float)((const TX*)a.x)[(int64_t)(slots[r0 + r] / a.route.top_k) * a.I + i0 + i]);
-      float* b = basis + (i * kFewRows + r) * kW;
-      float ta = 1.0f, tb = t;
-#pragma unroll
-      for (int d = 0; d < kDeg; ++d) {
-        b[d] = tb;
-        const float tc = fmaf(t + t, tb, -ta);
-        ta = tb;
-        tb = tc;
-      }
+      t[r][i] = tanhf((float)((const TX*)a.x)[(int64_t)(slots[r0 + r] / a.route.top_k) * a.I + i0 + i]);
     }
     __syncthreads();
-    float acc[kFewRows] = {};
-    for (int i = wave; i < ni; i += 4 * kU) {
+    f32x4_t acc[kTiles][kCols] = {};
+    float ones[kTiles] = {};
+    for (int i = wave * 4; i < ni; i += 16) {
+      // inputs past the end count as 0; rows past the end have columns of their own, which nobody reads
+      if (i + 4 > ni && i + sub >= ni)
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        if (i + 4 * u >= ni) break;
-        const float* b = basis + (i + 4 * u) * kFewRows * kW;
+        for (int q = 0; q < kTiles / P; ++q) c[q] = Coefs<TC, D * P>{};
+      float u[kCols], ta[kCols], tb[kCols];
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r) {
-          if (r >= nr) break;
-          float s = (float)c[u].v[0];
+      for (int k = 0; k < kCols; ++k) {
+        u[k] = i + sub < ni ? t[k * 16 + col][i + sub] : 0.0f;
+        ta[k] = 1.0f;
+        tb[k] = u[k];
+      }
+      const auto group = [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        Frag<kSplit> b[kCols];
 #pragma unroll
-          for (int d = 0; d < kDeg; ++d) s = fmaf((float)c[u].v[d + 1], b[r * kW + d], s);
-          acc[r] += s;
+        for (int k = 0; k < kCols; ++k) {
+          if (k && nr <= 16) break;
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = 0.0f;
+            if (8 * G + j + 1 >= D) continue;
+            v[j] = tb[k];
+            const float next = fmaf(u[k] + u[k], tb[k], -ta[k]);
+            ta[k] = tb[k];
+            tb[k] = next;
+          }
+          b[k] = make_frag_split(v);
+        }
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile) {
+          const TC* from = c[tile / P].v + tile % P * D;
+          const auto f = coef_frag<D, G>(from);
+          if (G == 0) ones[tile] += (float)from[0];
+          if (8 * G + 9 >= D && tile % P == P - 1) fetch(i + 16, tile / P);
+          add_products(acc[tile][0], f, b[0]);
+          if (nr > 16) add_products(acc[tile][1], f, b[1]);
+        }
+      };
+      group(std::integral_constant<int, 0>());
+      if constexpr (D > 9) group(std::integral_constant<int, 1>());
+    }
+#pragma unroll
+    for (int tile = 0; tile < kTiles; ++tile) {  // over the lanes of an output
+      auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(ones[tile]), __float_as_uint(ones[tile]), false, false);
+      const float v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      if (sub == 0) first[wave][(tile / P * 16 + col) * P + tile % P] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    // the waves' sums: a lane has outputs (16 (tile / P) + 4 sub + j) P + tile % P of row col
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+      if (k * 16 >= nr) break;
+      if (k) __syncthreads();
+#pragma unroll
+      for (int tile = 0; tile < kTiles; tile += P) {
+        f32x4_t* to = (f32x4_t*)&red[wave][col][(tile * 16 + sub * 4 * P)];
+        if constexpr (P == 1) {
+          to[0] = acc[tile][k];
+        } else {
+          const f32x4_t u = acc[tile][k], v = acc[tile + 1][k];
+          to[0] = f32x4_t{u[0], v[0], u[1], v[1]};
+          to[1] = f32x4_t{u[2], v[2], u[3], v[3]};
         }
       }
-      fetch(i + 4 * kU);
-    }
+      __syncthreads();
+      const int r = k * 16 + (tid >> 4);
 #pragma unroll
-    for (int r = 0; r < kFewRows; ++r) red[wave][r][lane] = acc[r];
-    __syncthreads();
-    for (int r = wave; r < nr; r += 4)
-      if (real) part[(size_t)slots[r0 + r] * a.O + o] = (red[0][r][lane] + red[1][r][lane]) + (red[2][r][lane] + red[3][r][lane]);
+      for (int j = 0; j < 4; ++j) {
+        const int o = j * 16 + (tid & 15);
+        const float v = (red[0][tid >> 4][o] + red[1][tid >> 4][o]) + (red[2][tid >> 4][o] + red[3][tid >> 4][o]) +
+                        ((first[0][o] + first[1][o]) + (first[2][o] + first[3][o]));
+        if (r < nr && o0 + o < a.O) part[(size_t)slots[r0 + r] * a.O + o0 + o] = v;
+      }
+    }
     __syncthreads();
   }
 }
@@ -418,7 +508,10 @@ template <typename TX, typename TC, int D>
 void launch_products(const FewArgs& a, hipStream_t st) {
   if (a.route.rows > kRowsMax) {
     const dim3 grid((unsigned)((int64_t)a.chunks * ceil_div(a.O, 64) * a.active));
-    hipLaunchKernelGGL((k_few_stream<TX, TC, D>), grid, dim3(256), 0, st, a);
+    if (sizeof(TC) == 2 && a.O % 2 == 0)
+      hipLaunchKernelGGL((k_few_stream<TX, TC, D, 4 / sizeof(TC)>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_few_stream<TX, TC, D, 1>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL((k_few_sum<TX>), dim3((unsigned)ceil_div(a.O, 64), (unsigned)a.route.rows), dim3(256), 0, st, a);
     return;
   }

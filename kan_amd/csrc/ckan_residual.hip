@@ -12,6 +12,12 @@
 //
 // out is made again from x and y, unrounded, so that no gradient sees its rounding: the
 // same bytes as reading out.  Sums over a row and over rows are in fp32, in a fixed order.
+//
+// Bound by the bytes: every tensor once, a row in the registers of a team of lanes between its sums (65536 x 512
+// in fp32, layer norms with biases and a gate a row: forward 130 us, backward 206, both 5.2 TB/s, the rate of a large
+// copy; 32768 x 1024 in bf16 60 and 98 us, 4.4 and 4.1 TB/s, by instructions too). Rows above 8192 values, whose sums
+// over rows and parameters fit neither registers nor LDS, and below 8 are read again for every sum (2048 x 16384 in fp32:
+// forward 175 us).
 #include <type_traits>
 
 #include "ckan_block.hpp"
@@ -860,7 +866,8 @@ int64_t forward_blocks(const ResidualArgs& a, int teams, int block, int lds) {
 }
 constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
 
-// The team of a width, WIDE that of the widest rows: in the backward half as many lanes, whose 256
+// The team of a width: a chunk a lane, so that a row is one batch of loads, up to eight rows a wave and 16 waves a
+// row. WIDE is that of the widest rows: in the backward half as many lanes, whose 256
 // registers hold two chunks and their sums (4096 x 8192 212 us in fp32 and 142 in bf16; 1024 lanes
 // of 128 registers 291 and 175).
 #define CKAN_TEAM(dim, F, WIDE)                 \

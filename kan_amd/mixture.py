@@ -267,7 +267,7 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
 
     ``x`` [rows, in], ``gate`` [experts, in] and ``coeffs`` [experts, in, out, degree+1] are fp32 or
     bf16 each; y [rows, out] has x's dtype, weights and indices are ``route``'s.  Few rows without a
-    gradient (up to 1024 slots, 16 an expert on average) take a form of their own: the gate's sums in 64
+    gradient (up to 1024 slots, fewer than 64 an expert on average) take a form of their own: the gate's sums in 64
     bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
     product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (on x in the coefficients'
     dtype), differentiable as they are in x, gate and coeffs."""

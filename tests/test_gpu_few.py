@@ -104,6 +104,28 @@ def test_wide_layers():
         check(x, gate, coeffs, 2)
 
 
+@pytest.mark.parametrize("degree", [1, 4, 7, 8, 9, 16])
+@pytest.mark.parametrize("c_dtype", [F32, BF16])
+def test_many_rows_an_expert(degree, c_dtype):
+    """Several passes over the rows of one expert, with 1 to 32 in the last; odd and even outputs, inputs past a chunk's end."""
+    for rows, in_dim, out_dim, lean in ((33, 130, 66, 0.0), (48, 37, 65, 0.0), (125, 64, 30, 4.0), (126, 259, 200, 0.5)):
+        x, gate, coeffs = make(rows, in_dim, out_dim, degree, 2, F32, F32, c_dtype, rows)
+        check(x, gate, coeffs, 1, bias=torch.tensor([0.1 * lean, 0.0]))
+
+
+def test_an_infinite_coefficient_stays_in_its_output():
+    for rows, c_dtype in ((1, F32), (5, BF16), (40, F32), (40, BF16)):
+        x, gate, coeffs = (t.cuda() for t in make(rows, 70, 34, 5, 4, F32, F32, c_dtype, 8))
+        with torch.no_grad():
+            want, _, idx = f.kan_mixture(x, gate, coeffs, 2)
+            coeffs[2, 11, 7, 3] = float("inf")
+            coeffs[2, 69, 33, 0] = float("nan")
+            got, _, again = f.kan_mixture(x, gate, coeffs, 2)
+        hit = torch.zeros_like(want, dtype=torch.bool)
+        hit[(idx == 2).any(1)[:, None] & torch.isin(torch.arange(34, device="cuda"), torch.tensor([7, 33], device="cuda"))] = True
+        assert torch.equal(idx, again) and torch.equal(got[~hit], want[~hit]) and not torch.isfinite(got[hit]).any()
+
+
 @pytest.mark.parametrize("rows", [1, 2, 20])
 def test_large_gates(rows):
     """Gates of more than 2^16 entries, whose logits a launch of their own makes."""
