@@ -41,6 +41,11 @@ def _pitch(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.stride(0)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """Dense memory of t's shape and type (empty_like takes a third less host time than empty)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _shaped(t: Optional[torch.Tensor], shape) -> Optional[torch.Tensor]:
     return t if t is None or len(shape) == 2 else t.view(shape)
 
@@ -95,7 +100,7 @@ class ResidualFunction(torch.autograd.Function):
             gate = _rows(gate, desc.dim)
         desc = _pitched(desc, x_ld=x.stride(0), y_ld=_pitch(y), gate_ld=gate.stride(0) if desc.gate_rows else 0)
         inputs = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip(inputs, need)]
+        grads = [_like(t) if n else None for t, n in zip(inputs, need)]
         if desc.rows == 0:
             return (*(None if g is None else g.zero_() for g in grads), None)
         lib = _lib.load()
@@ -124,8 +129,10 @@ def _residual_forward(tensors, call, keep):
     x, y, gate, post_weight, post_bias, next_weight, next_bias = tensors
     desc, dev, ptr = call.desc, x.device, _lib.ptr
     rows, dim = desc.rows, desc.dim
-    out = torch.empty(rows, dim, dtype=x.dtype, device=dev) if y is not None else None
-    h = torch.empty(rows, dim, dtype=call.h_dtype, device=dev) if next_weight is not None else None
+    out = _like(x) if y is not None else None
+    h = None
+    if next_weight is not None:  # of y's type where there is a y
+        h = _like(y) if y is not None else torch.empty(rows, dim, dtype=call.h_dtype, device=dev)
     stats = torch.empty(rows * 4 + 4, dtype=torch.float32, device=dev) if keep else None
     buffers = _lib.CkanResidualBuffers(
         x.data_ptr(), ptr(y), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(next_weight), ptr(next_bias),
@@ -243,7 +250,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", eps: f
 def _dropout_launch(x, p, state, seed, offset, keep):
     """(y, used) of x [rows, dim]."""
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _like(x)
     used = torch.empty(2, dtype=torch.int64, device=dev) if keep else None
     desc = _lib.CkanDropoutDesc(x.shape[0], max(x.shape[1], 1), x.stride(0), p, seed, offset, _DTYPES[x.dtype])
     with _on(dev):
@@ -336,7 +343,7 @@ class LogProbsFunction(torch.autograd.Function):
         desc = _pitched(ctx.desc, logits_ld=logits.stride(0))
         dlogp, dentropy = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
                            else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))
-        dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dl = _like(logits)
         _lib.check(_lib.load().ckan_log_probs_backward(desc, logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
                                                        _lib.ptr(dlogp), _lib.ptr(dentropy), dl.data_ptr(),
                                                        _stream(dl.device)))
