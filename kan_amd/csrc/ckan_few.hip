@@ -64,8 +64,9 @@ void few_plan(FewArgs* a) {
   a->apart = E * a->I > (1 << 16);
   a->gated = rows == 1 && !a->apart;
   const bool by_row = rows <= kRowsMax;
-  // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's, at least an input a
-  // wave, at most what a block holds
+  // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's (64 rows, two of 8 experts of 1024 -> 1024 in
+  // bf16: four 52 us, six 58, eight 55; 2048 -> 700, degree 16, 121, 128 and 127), at least an input a wave, at most
+  // what a block holds
   const int64_t oc = ceil_div(a->O, by_row && a->coeff_bf16 ? 128 : 64), hold = by_row ? kRowTanh : kFewInputs;
   int64_t chunks = by_row ? ceil_div(kNumCUs, oc) : ceil_div(4 * kNumCUs, active * oc);
   if (chunks > ceil_div(a->I, 16)) chunks = ceil_div(a->I, 16);

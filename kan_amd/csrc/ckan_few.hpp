@@ -288,8 +288,8 @@ __global__ __launch_bounds__(256) void k_few_rows_sum(FewArgs a) {
 //
 // The products run on the matrix cores: on the vector ALU 64 rows, two of 8 experts of 1024 -> 1024, degree 8, took 112 us
 // in bf16 and 131 in fp32 (here 52 and 85, of which the coefficients' stream is 29 and 59 and the launches of gate and sum
-// 13); 20 rows, one of 8 of 2048 -> 2048, degree 4, 75 and 139 (57 and 131). In an instruction of 16 outputs by 16 rows by 32 products a lane holds eight
-// coefficients of one input and output, as they lie, and against them eight basis values of that input for one
+// 13); 20 rows, one of 8 of 2048 -> 2048, degree 4, 75 and 139 (57 and 131). In an instruction of 16 outputs by 16
+// rows by 32 products a lane holds eight coefficients of one input and output, as they lie, and against them eight basis values of that input for one
 // row, made in registers: bf16 coefficients are an operand as they are, fp32 ones and the basis values three bf16
 // planes (24 bits), of whose products those below 2^-24 are left out. T_0 = 1 is a sum of coefficients beside them;
 // degrees above 8 take a second run of eight basis values, padded with zeros.

@@ -114,8 +114,8 @@ class RouteFunction(torch.autograd.Function):
         dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         logits, ld = _logit_rows(logits)
         # the engine runs a node on its device and stream
-        _lib.check(_lib.load().ckan_route_backward(_pitched(ctx.desc, logits_ld=ld), logits.data_ptr(), ctx.idx.data_ptr(), dw.data_ptr(),
-                                                   dl.data_ptr(), _stream(dl.device)))
+        _lib.check(_lib.load().ckan_route_backward(_pitched(ctx.desc, logits_ld=ld), logits.data_ptr(), ctx.idx.data_ptr(),
+                                                   dw.data_ptr(), dl.data_ptr(), _stream(dl.device)))
         return dl, None, None, None
 
 
