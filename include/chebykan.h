@@ -416,8 +416,8 @@ int ckan_mixture_forward(const ckan_mixture_desc* desc, const void* x, const voi
 /*   u = drop(post(y)),  out = x + scale gate u,  h = next(out)
  * over rows of `dim` values, post and next being (v - mean) r w + b with
  * r = 1 / sqrt(mean((v - mean)^2) + eps), mean taken as 0 in the RMS form.  A NULL
- * post_weight or next_weight leaves that norm (and h) out, a NULL gate is 1, a NULL y
- * leaves only h = next(x).  gate is [dim] or, with gate_rows, [rows, dim].
+ * post_weight or next_weight leaves that norm (and h) out, a NULL gate is 1 (gate_rows then
+ * says nothing), a NULL y leaves only h = next(x).  gate is [dim] or, with gate_rows, [rows, dim].
  * x, out, dout and dx have x_dtype, y, h, dh and dy have y_dtype; parameters, row gates
  * and their gradients have a dtype each.  Rows are contiguous, `*_ld` elements apart (out, h and
  * the gradients dense).  Arithmetic in fp32, results rounded once; h comes from out

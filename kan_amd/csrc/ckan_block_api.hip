@@ -105,7 +105,7 @@ int residual_args(const ckan_residual_desc* d, const ckan_residual_buffers* b, b
   a->x_bf16 = d->x_dtype == CKAN_DTYPE_BF16;
   a->y_bf16 = d->y_dtype == CKAN_DTYPE_BF16;
   a->layer = d->norm == CKAN_NORM_LAYER;
-  a->gate_rows = d->gate_rows;
+  a->gate_rows = d->gate_rows && b->gate;  // a NULL gate is 1 in either form
   a->eps = d->eps;
   a->scale = d->scale;
   a->x = b->x;
