@@ -269,8 +269,8 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
     bf16 each; y [rows, out] has x's dtype, weights and indices are ``route``'s.  Few rows without a
     gradient (up to 1024 slots, fewer than 64 an expert on average) take a form of their own: the gate's sums in 64
     bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
-    product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (on x in the coefficients'
-    dtype), differentiable as they are in x, gate and coeffs."""
+    product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (in fp32 unless x and coeffs
+    are both bf16), differentiable as they are in x, gate and coeffs."""
     if score not in _SCORES:
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
     _lib.refuse_tangents("kan_mixture", x, gate, coeffs)
@@ -296,7 +296,9 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
     if trains or not lib.ckan_mixture_few(desc):
         weights, indices = route(_gate_logits(x.to(torch.float32), gate.to(torch.float32)), top_k, score=score, bias=bias,
                                  groups=groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
-        return kan_experts(x.to(coeffs.dtype), coeffs, indices, weights).to(x.dtype), weights, indices
+        # in the wider of the two types, so that fp32 rows keep fp32's accuracy on bf16 coefficients in either form
+        dtype = torch.promote_types(x.dtype, coeffs.dtype)
+        return kan_experts(x.to(dtype), coeffs.to(dtype), indices, weights).to(x.dtype), weights, indices
     dev = x.device
     x, gate, coeffs = _aligned(x), _aligned(gate), _aligned(coeffs)
     if bias is not None:
