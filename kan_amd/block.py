@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .mixture import _on, _once, _pitched, _stream
+from .mixture import _dense, _on, _once, _pitched, _stream
 
 _NORMS = {"rms": _lib.CKAN_NORM_RMS, "layer": _lib.CKAN_NORM_LAYER}
 _DTYPES = {torch.float32: _lib.CKAN_DTYPE_F32, torch.bfloat16: _lib.CKAN_DTYPE_BF16}
@@ -89,15 +89,15 @@ class ResidualFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dout is None and dh is None:
             return (None,) * 8
-        x, y, gate, post_weight, post_bias, next_weight, next_bias, stats = ctx.saved_tensors
+        x, y, gate, *vectors, stats = ctx.saved_tensors
+        post_weight, post_bias, next_weight, next_bias, stats = map(_dense, (*vectors, stats))
         desc, dev = ctx.desc, x.device
         if dout is not None:
             dout = _rows(dout if dout.dtype == x.dtype else dout.to(x.dtype), desc.dim)
         if dh is not None:
             dh = _rows(dh if dh.dtype == ctx.h_dtype else dh.to(ctx.h_dtype), desc.dim)
         x, y = _rows(x, desc.dim), y if y is None else _rows(y, desc.dim)
-        if desc.gate_rows:
-            gate = _rows(gate, desc.dim)
+        gate = _rows(gate, desc.dim) if desc.gate_rows else _dense(gate)
         desc = _pitched(desc, x_ld=x.stride(0), y_ld=_pitch(y), gate_ld=gate.stride(0) if desc.gate_rows else 0)
         inputs = (x, y, gate, post_weight, post_bias, next_weight, next_bias)
         grads = [_like(t) if n else None for t, n in zip(inputs, need)]
@@ -339,7 +339,7 @@ class LogProbsFunction(torch.autograd.Function):
         if dlogp is None and dentropy is None:
             return None, None, None, None
         logits, targets, stats = ctx.saved_tensors
-        logits = _rows(logits, ctx.desc.classes)
+        logits, targets, stats = _rows(logits, ctx.desc.classes), _dense(targets), _dense(stats)
         desc = _pitched(ctx.desc, logits_ld=logits.stride(0))
         dlogp, dentropy = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
                            else g.to(torch.float32).contiguous() for g in (dlogp, dentropy))

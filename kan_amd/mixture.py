@@ -72,6 +72,11 @@ def _once(name: str) -> None:
         raise RuntimeError(f"{name} is differentiable once (create_graph is not supported)")
 
 
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A saved tensor as its kernel reads it, whatever layout a hook returned it in."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _pitched(desc, **pitches):
     """desc with these row pitches: a hook on saved tensors may have returned them in another layout
     than they were saved in."""
@@ -188,7 +193,7 @@ class ExpertsFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _once("kan_experts")
-        saved, indices, weights = ctx.saved_tensors
+        saved, indices, weights = map(_dense, ctx.saved_tensors)
         desc = ctx.desc
         xs, cs, dtype = ctx.shapes
         need_x, need_c, need_w = ctx.needs_input_grad[:3]
