@@ -54,11 +54,12 @@ void few_plan(FewArgs* a) {
   const int64_t active = E < S ? E : S;
   // fewer than 64 slots an expert on average, two passes of kFewRows: 240 rows, two of 8 experts of 1024 -> 1024, degree
   // 8, 105 us in bf16 and 174 in fp32 (the parts' entry points, which pack the coefficients, 173 and 279), 64 rows 53 and 88
-  // (110 and 137); 500 rows of 512 -> 512, two of 16, 76 and 118 (111 and 162)
+  // (110 and 137); 500 rows of 512 -> 512, two of 16, 73 and 108 (111 and 161), all on the same two 61 and 85 (103 and 150)
   a->few = rows > 0 && S <= kFewMaxSlots && S < 64 * active;
   if (!a->few) return;
   a->S = (int)S;
-  a->active = (int)active;
+  // runs of kFewUnit slots of one expert: at most one begun an expert and one for every kFewUnit slots
+  a->runs = (int)(rows > kFewUnit ? active + S / kFewUnit : active);
   // a gate of 2^16 entries: one launch 20.0 us (1 row) to 26.8 (64 rows), two 22.3 to 26.9; of 2^18
   // entries 22.6 to 41.7 and 22.1 to 35.4
   a->apart = E * a->I > (1 << 16);
@@ -74,7 +75,7 @@ void few_plan(FewArgs* a) {
   a->chunk_inputs = (int)ceil_div(a->I, chunks);
   a->chunks = (int)ceil_div(a->I, a->chunk_inputs);
   // a launch holds fewer than 2^32 threads
-  if (!by_row && a->chunks * oc * active >= ((int64_t)1 << 24)) a->few = false;
+  if (!by_row && a->chunks * oc * a->runs >= ((int64_t)1 << 24)) a->few = false;
   a->part_off = align256(a->apart ? (size_t)rows * E * sizeof(float) : 1);
   a->ws_bytes = a->part_off + align256((size_t)a->chunks * (by_row ? rows : S) * a->O * sizeof(float));
 }

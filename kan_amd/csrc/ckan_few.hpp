@@ -283,8 +283,11 @@ __global__ __launch_bounds__(256) void k_few_rows_sum(FewArgs a) {
   if (wave == 0 && q < n) ((TX*)a.y)[q] = (TX)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
 }
 
-// More rows: a block takes one of the chosen experts, 64 outputs and a chunk of inputs, and leaves part[chunk,
-// slot, o] of up to kFewRows rows at a time. It finds its expert and that expert's slots itself.
+// More rows: a block takes up to kFewUnit slots of one of the chosen experts, 64 outputs and a chunk of inputs, and leaves
+// part[chunk, slot, o] of up to kFewRows rows at a time. It finds its expert and that expert's slots itself. Rows that crowd
+// on few experts thus spread over more blocks: 500 rows on two of 16 experts of 512 -> 512, degree 8, 85 us in fp32 and 61 in
+// bf16 (a block an expert, however many its slots: 216 and 165), 200 on two of 8 of 1024 -> 1024 113 and 78 (180 and 132);
+// where no expert has more than kFewUnit slots nothing changes.
 //
 // The products run on the matrix cores: on the vector ALU 64 rows, two of 8 experts of 1024 -> 1024, degree 8, took 112 us
 // in bf16 and 131 in fp32 (here 52 and 85, of which the coefficients' stream is 29 and 59 and the launches of gate and sum
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(256) void k_few_rows_sum(FewArgs a) {
 // row, made in registers: bf16 coefficients are an operand as they are, fp32 ones and the basis values three bf16
 // planes (24 bits), of whose products those below 2^-24 are left out. T_0 = 1 is a sum of coefficients beside them;
 // degrees above 8 take a second run of eight basis values, padded with zeros.
-constexpr int kFewMaxSlots = 1024, kFewInputs = 128, kFewRows = 32;
+constexpr int kFewMaxSlots = 1024, kFewInputs = 128, kFewRows = 32, kFewUnit = 2 * kFewRows;
 
 // The eight coefficients of an output (its T_0 at `from`) from 8 G + 1 on as an operand.
 template <int D, int G>
@@ -326,7 +329,7 @@ __device__ __forceinline__ void add_products(f32x4_t& acc, const Frag<kSplit>& c
 template <typename TX, typename TC, int D, int P>
 __global__ __launch_bounds__(256, sizeof(TC) == 2 || D <= 12 ? 3 : 2) void k_few_stream(FewArgs a) {
   constexpr int kTiles = 4, kCols = kFewRows / 16, kPitch = 64 + 4;
-  __shared__ int slots[kFewMaxSlots], counts[4];
+  __shared__ int slots[kFewMaxSlots], counts[4], mine_e, mine_r;
   __shared__ unsigned chosen[kRouteMaxExperts / 32];
   __shared__ float t[kFewRows][kFewInputs + 1];
   __shared__ __align__(16) float red[4][16][kPitch];
@@ -338,26 +341,59 @@ __global__ __launch_bounds__(256, sizeof(TC) == 2 || D <= 12 ? 3 : 2) void k_few
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int o0 = id % oc * 64;
   int nth = id / oc;
-  if (tid < kRouteMaxExperts / 32) chosen[tid] = 0;
-  __syncthreads();
-  for (int s = tid; s < a.S; s += 256) {
-    const int64_t e = a.route.indices[s];
-    if (e >= 0 && e < a.route.E) atomicOr(&chosen[e >> 5], 1u << (e & 31));
-  }
-  __syncthreads();
-  // the nth of the chosen experts
-  int e = -1;
-  for (int w = 0; w < (a.route.E + 31) / 32; ++w) {
-    unsigned bits = chosen[w];
-    const int n = __popc(bits);
-    if (nth < n) {
-      for (; nth; --nth) bits &= bits - 1;
-      e = w * 32 + __ffs(bits) - 1;
-      break;
+  // the nth run of kFewUnit slots of an expert, and where it begins among them
+  int e = -1, begin = 0;
+  if (a.route.rows <= kFewUnit) {  // one an expert: the nth of the chosen experts
+    if (tid < kRouteMaxExperts / 32) chosen[tid] = 0;
+    __syncthreads();
+    for (int s = tid; s < a.S; s += 256) {
+      const int64_t x = a.route.indices[s];
+      if (x >= 0 && x < a.route.E) atomicOr(&chosen[x >> 5], 1u << (x & 31));
     }
-    nth -= n;
+    __syncthreads();
+    for (int w = 0; w < (a.route.E + 31) / 32; ++w) {
+      unsigned bits = chosen[w];
+      const int n = __popc(bits);
+      if (nth < n) {
+        for (; nth; --nth) bits &= bits - 1;
+        e = w * 32 + __ffs(bits) - 1;
+        break;
+      }
+      nth -= n;
+    }
+  } else {
+    static_assert(kRouteMaxExperts == 2 * 256);
+    int* load = (int*)&red[0][0][0];  // an expert's slots, until the first sums
+    load[tid] = load[tid + 256] = 0;
+    if (tid == 0) mine_e = -1;
+    __syncthreads();
+    for (int s = tid; s < a.S; s += 256) {
+      const int64_t x = a.route.indices[s];
+      if (x >= 0 && x < a.route.E) atomicAdd(&load[x], 1);
+    }
+    __syncthreads();
+    // the runs of the experts before this thread's two
+    const int own = (load[2 * tid] + kFewUnit - 1) / kFewUnit, both = own + (load[2 * tid + 1] + kFewUnit - 1) / kFewUnit;
+    int before = both;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int o = __shfl_up(before, w);
+      before += lane >= w ? o : 0;
+    }
+    if (lane == 63) counts[wave] = before;
+    __syncthreads();
+    before -= both;
+    for (int w = 0; w < wave; ++w) before += counts[w];
+    if (nth >= before && nth < before + both) {
+      const int q = nth >= before + own;
+      mine_e = 2 * tid + q;
+      mine_r = (nth - before - (q ? own : 0)) * kFewUnit;
+    }
+    __syncthreads();
+    e = mine_e;
+    begin = mine_r;
   }
-  if (e < 0) return;  // uniform: fewer are chosen than there are blocks for
+  if (e < 0) return;  // uniform: fewer runs than there are blocks for
   e = __builtin_amdgcn_readfirstlane(e);
   int n = 0;
   for (int s0 = 0; s0 < a.S; s0 += 256) {
@@ -385,7 +421,8 @@ __global__ __launch_bounds__(256, sizeof(TC) == 2 || D <= 12 ? 3 : 2) void k_few
     off[q] = (o < a.O ? o : a.O - P) * D;
   }
   float* part = (float*)(a.ws + a.part_off) + (size_t)chunk * a.S * a.O;
-  for (int r0 = 0; r0 < n; r0 += kFewRows) {
+  if (n > begin + kFewUnit) n = begin + kFewUnit;
+  for (int r0 = begin; r0 < n; r0 += kFewRows) {
     const int nr = n - r0 < kFewRows ? n - r0 : kFewRows;
     Coefs<TC, D * P> c[kTiles / P];
     const auto fetch = [&](int i, int q) {  // inputs from i on
@@ -507,7 +544,7 @@ __global__ __launch_bounds__(256) void k_few_sum(FewArgs a) {
 template <typename TX, typename TC, int D>
 void launch_products(const FewArgs& a, hipStream_t st) {
   if (a.route.rows > kRowsMax) {
-    const dim3 grid((unsigned)((int64_t)a.chunks * ceil_div(a.O, 64) * a.active));
+    const dim3 grid((unsigned)((int64_t)a.chunks * ceil_div(a.O, 64) * a.runs));
     if (sizeof(TC) == 2 && a.O % 2 == 0)
       hipLaunchKernelGGL((k_few_stream<TX, TC, D, 4 / sizeof(TC)>), grid, dim3(256), 0, st, a);
     else

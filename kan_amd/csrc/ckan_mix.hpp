@@ -148,7 +148,7 @@ struct FewArgs {
   bool few;            // whether this form takes the call
   bool apart;          // logits by a launch of their own
   bool gated;          // the choice made by the products' launch
-  int active, chunks, chunk_inputs;
+  int runs, chunks, chunk_inputs;
   size_t part_off, ws_bytes;
 };
 void few_plan(FewArgs* a);
