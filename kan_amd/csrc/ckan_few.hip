@@ -62,7 +62,10 @@ void few_plan(FewArgs* a) {
   a->runs = (int)(rows > kFewUnit ? active + S / kFewUnit : active);
   // a gate of 2^16 entries: one launch 20.0 us (1 row) to 26.8 (64 rows), two 22.3 to 26.9; of 2^18
   // entries 22.6 to 41.7 and 22.1 to 35.4
-  a->apart = E * a->I > (1 << 16);
+  // and where a block's waves would take their four experts in two rounds or more, the GPU's time in one launch and in two: 128
+  // experts of 128 inputs 14.1 and 12.6 (2 rows), 17.2 and 16.2 (64), 512 of 128 28.0 and 14.2, 32.1 and 21.5; 96 of 128 9.7 and
+  // 11.3 (1 row), 12.7 and 12.5, 15.7 and 15.8
+  a->apart = E * a->I > (1 << 16) || E >= 2 * kGateWaves * kGateExperts;
   a->gated = rows == 1 && !a->apart;
   const bool by_row = rows <= kRowsMax;
   // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's (64 rows, two of 8 experts of 1024 -> 1024 in

@@ -44,10 +44,25 @@ __device__ __forceinline__ void gate_dots(const FewArgs& a, int64_t row, int e0,
     }
   }
 }
+// The sum over a wave, in every lane, by butterflies on the vector ALU as lanes_sum's. Through LDS (__shfl_xor) the exchanges
+// of many experts' sums share a CU's one LDS: 128 rows of 128 inputs by 512 experts 13.5 -> 10.2 us.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
+  return v + __hiloint2double(hi, lo);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
-  return v;
+  v = dpp_add<0xb1>(v);
+  v = dpp_add<0x4e>(v);
+  v = dpp_add<0x141>(v);
+  v = dpp_add<0x140>(v);
+  auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+  v = __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+  lo = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+  hi = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+  return __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
 }
 
 struct GateShared {

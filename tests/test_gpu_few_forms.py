@@ -1,0 +1,45 @@
+"""Few-row mixtures on either side of the rules between the forms of the gate and of the products.
+
+Bounds as the other tests of the few-row form: weights 1e-6, y 5e-6 of its norm against the 64-bit sum, and half a step more of
+each value of a y in bf16."""
+import numpy as np
+import pytest
+import torch
+
+import kan_amd
+from kan_amd import _lib
+from oracle import mixture_oracle as orc
+
+pytestmark = pytest.mark.gpu
+f = kan_amd.functional
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def check(rows, in_dim, out_dim, degree, experts, top_k, x_dtype=F32, g_dtype=F32, c_dtype=F32, few=1):
+    g = torch.Generator().manual_seed(rows + experts)
+    x = torch.randn(rows, in_dim, generator=g).to(x_dtype)
+    gate = (2 * torch.randn(experts, in_dim, generator=g) / in_dim ** 0.5).to(g_dtype)
+    coeffs = (torch.randn(experts, in_dim, out_dim, degree + 1, generator=g) / (in_dim * (degree + 1))).to(c_dtype)
+    code = {F32: 0, BF16: 1}
+    desc = _lib.CkanMixtureDesc(rows, experts, top_k, in_dim, out_dim, degree, 0, 1, 1, 1, code[x_dtype], code[g_dtype],
+                                code[c_dtype], 1.0)
+    assert _lib.load().ckan_mixture_few(desc) == few
+    with torch.no_grad():
+        y, w, idx = (t.cpu() for t in f.kan_mixture(x.cuda(), gate.cuda(), coeffs.cuda(), top_k))
+    if few:
+        logits = (x.double() @ gate.double().t()).float()
+        want_w, want_idx = orc.route(logits.double().numpy(), top_k)
+        assert np.array_equal(idx.numpy(), want_idx)
+        assert np.abs(w.numpy() - want_w).max() <= 1e-6
+    want = orc.kan_experts(x.double().numpy(), coeffs.double().numpy(), idx.numpy(), w.double().numpy())
+    err = np.abs(y.double().numpy() - want)
+    if x_dtype == BF16:
+        err = np.maximum(err - 2.0 ** -8 * np.abs(want), 0)
+    assert np.linalg.norm(err) <= 5e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 9, 70])
+@pytest.mark.parametrize("experts,in_dim", [(127, 40), (128, 40), (128, 7), (129, 65), (300, 12), (512, 24), (64, 1024), (64, 1025)])
+def test_gates_of_many_experts(rows, experts, in_dim):
+    for x_dtype, g_dtype in ((F32, F32), (BF16, F32), (BF16, BF16)):
+        check(rows, in_dim, 18, 2, experts, 3, x_dtype, g_dtype)
