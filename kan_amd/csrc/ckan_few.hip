@@ -67,7 +67,11 @@ void few_plan(FewArgs* a) {
   // 11.3 (1 row), 12.7 and 12.5, 15.7 and 15.8
   a->apart = E * a->I > (1 << 16) || E >= 2 * kGateWaves * kGateExperts;
   a->gated = rows == 1 && !a->apart;
-  const bool by_row = rows <= kRowsMax;
+  // a block of k_few_rows visits every chosen expert in turn, some 0.5 us each where its coefficients are few: 8 rows of 16 of 128
+  // experts of 64 -> 64, degree 3, 57 us (k_few_stream 26), 5 rows of 16 of 384 of 128 -> 128, degree 4, 55 (40), but 8 rows of 16 of
+  // 128 of 512 -> 512, degree 4, 87 (107), in bf16 79 (57), of 12 of 32 of 1024 -> 1024 122 (151), in bf16 81 (87)
+  const int64_t expert_bytes = (int64_t)a->I * a->O * a->D * (a->coeff_bf16 ? 2 : 4);
+  const bool by_row = a->by_row = rows <= kRowsMax && (S <= 64 || expert_bytes >= 5 << 20);
   // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's (64 rows, two of 8 experts of 1024 -> 1024 in
   // bf16: four 52 us, six 58, eight 55; 2048 -> 700, degree 16, 121, 128 and 127), at least an input a wave, at most
   // what a block holds

@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256) void k_few_sum(FewArgs a) {
 
 template <typename TX, typename TC, int D>
 void launch_products(const FewArgs& a, hipStream_t st) {
-  if (a.route.rows > kRowsMax) {
+  if (!a.by_row) {
     const dim3 grid((unsigned)((int64_t)a.chunks * ceil_div(a.O, 64) * a.runs));
     if (sizeof(TC) == 2 && a.O % 2 == 0)
       hipLaunchKernelGGL((k_few_stream<TX, TC, D, 4 / sizeof(TC)>), grid, dim3(256), 0, st, a);

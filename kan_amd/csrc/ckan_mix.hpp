@@ -148,6 +148,7 @@ struct FewArgs {
   bool few;            // whether this form takes the call
   bool apart;          // logits by a launch of their own
   bool gated;          // the choice made by the products' launch
+  bool by_row;         // the products by k_few_rows
   int runs, chunks, chunk_inputs;
   size_t part_off, ws_bytes;
 };

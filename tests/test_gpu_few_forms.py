@@ -43,3 +43,13 @@ def check(rows, in_dim, out_dim, degree, experts, top_k, x_dtype=F32, g_dtype=F3
 def test_gates_of_many_experts(rows, experts, in_dim):
     for x_dtype, g_dtype in ((F32, F32), (BF16, F32), (BF16, BF16)):
         check(rows, in_dim, 18, 2, experts, 3, x_dtype, g_dtype)
+
+
+@pytest.mark.parametrize("c_dtype", [F32, BF16])
+@pytest.mark.parametrize("case", [
+    (4, 30, 34, 5, 40, 16), (5, 30, 34, 5, 40, 16), (8, 30, 33, 3, 64, 8), (8, 30, 33, 3, 64, 9), (2, 20, 70, 9, 64, 33),
+    (8, 17, 16, 16, 100, 64), (5, 640, 700, 2, 14, 13), (5, 640, 700, 5, 14, 13)], ids=lambda c: "-".join(map(str, c)))
+def test_few_rows_of_many_slots(case, c_dtype):
+    """64 slots and more of up to 8 rows, in experts of few and of many coefficients."""
+    for x_dtype in (F32, BF16):
+        check(*case, x_dtype, F32, c_dtype)
