@@ -72,6 +72,14 @@ void few_plan(FewArgs* a) {
   // 128 of 512 -> 512, degree 4, 87 (107), in bf16 79 (57), of 12 of 32 of 1024 -> 1024 122 (151), in bf16 81 (87)
   const int64_t expert_bytes = (int64_t)a->I * a->O * a->D * (a->coeff_bf16 ? 2 : 4);
   const bool by_row = a->by_row = rows <= kRowsMax && (S <= 64 || expert_bytes >= 5 << 20);
+  // k_few_stream makes fp32 coefficients of degree 9 and more operands in two runs of three planes, whether two rows or 32 meet them:
+  // where few do and the coefficients are many, the parts' vector ALU is as fast or faster (12 rows, three of 12 experts of 300 ->
+  // 700, degree 16, 62 us and 56, 24 rows 72 and 62, 48 rows 75 and 84; 16 rows, two of 32 of 700 -> 300, 92 and 75; two of 8 of 512 ->
+  // 512 52 and 48). Of fewer coefficients their launches take longer (two of 8 of 512 -> 512, degree 12, 43 and 45)
+  if (!by_row && !a->coeff_bf16 && a->D > 9 && S < 8 * active && active * a->I * a->O * a->D >= (int64_t)1 << 25) {
+    a->few = false;
+    return;
+  }
   // chunks of inputs: a block of k_few_rows a CU, four of k_few_stream's (64 rows, two of 8 experts of 1024 -> 1024 in
   // bf16: four 52 us, six 58, eight 55; 2048 -> 700, degree 16, 121, 128 and 127), at least an input a wave, at most
   // what a block holds

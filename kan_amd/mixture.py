@@ -272,8 +272,9 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
 
     ``x`` [rows, in], ``gate`` [experts, in] and ``coeffs`` [experts, in, out, degree+1] are fp32 or
     bf16 each; y [rows, out] has x's dtype, weights and indices are ``route``'s.  Few rows without a
-    gradient (up to 1024 slots, fewer than 64 an expert on average) take a form of their own: the gate's sums in 64
-    bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
+    gradient (up to 1024 slots, fewer than 64 an expert on average; of many fp32 coefficients of degree
+    9 and more up to 8 rows, or from 8 slots an expert on) take a form of their own: the gate's sums in
+    64 bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
     product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (in fp32 unless x and coeffs
     are both bf16), differentiable as they are in x, gate and coeffs."""
     if score not in _SCORES:
@@ -377,11 +378,13 @@ class MixtureKANLayer(nn.Module):
         return y
 
     def _few(self, x: torch.Tensor) -> bool:
-        """Whether ``kan_mixture`` would take its own form for x."""
+        """Whether x is few rows as ``kan_mixture`` counts them: by its rule for bf16 coefficients, which has no limit for high
+        degrees (past that one its parts run in fp32 too, and casting all coefficients takes longer)."""
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
             return False
         desc = _lib.CkanMixtureDesc(x.shape[0], self.experts, self.top_k, self.input_dim, self.output_dim, self.degree,
-                                    _SCORES[self.score], self.groups, self.top_groups, 1, 0, 0, 0, self.scale)
+                                    _SCORES[self.score], self.groups, self.top_groups, 1, 0, 0, _lib.CKAN_DTYPE_BF16,
+                                    self.scale)
         return bool(_lib.load().ckan_mixture_few(desc))
 
     @torch.no_grad()
