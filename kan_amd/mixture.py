@@ -7,6 +7,7 @@ Tensors on the CPU are rejected: there is no CPU path.
 from __future__ import annotations
 
 from contextlib import nullcontext
+from functools import lru_cache
 from typing import Any, Dict, Optional, Tuple
 
 import torch
@@ -322,6 +323,14 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
     return y, weights, indices
 
 
+@lru_cache(maxsize=4096)
+def _few_rows(rows, experts, top_k, in_dim, out_dim, degree, score, groups, top_groups, coeff_code) -> bool:
+    """The library's rule by sizes; asking it takes 4 us."""
+    desc = _lib.CkanMixtureDesc(rows, experts, top_k, in_dim, out_dim, degree, score, groups, top_groups, 1, 0, 0, coeff_code,
+                                1.0)
+    return bool(_lib.load().ckan_mixture_few(desc))
+
+
 class MixtureKANLayer(nn.Module):
     """A mixture of ChebyKAN layers: each row goes to ``top_k`` of ``experts`` layers of
     ``ChebyKANLayer(input_dim, output_dim, degree)`` (kan/layers/chebykan.py:21-51), chosen
@@ -369,8 +378,11 @@ class MixtureKANLayer(nn.Module):
         x = x.reshape(-1, self.input_dim).to(torch.float32)
         how = dict(score=self.score, bias=self.balance_bias, groups=self.groups, top_groups=self.top_groups,
                    renormalize=self.renormalize, scale=self.scale)
-        if self.compute == "fp32" or self._few(x):
+        if self._few(x):
             y, _, indices = kan_mixture(x, self.gate, self.cheby_coeffs, self.top_k, **how)
+        elif self.compute == "fp32":  # what kan_mixture does, without its checks (10 us of the host's time)
+            weights, indices = route(_gate_logits(x, self.gate.to(torch.float32)), self.top_k, **how)
+            y = kan_experts(x, self.cheby_coeffs.to(torch.float32), indices, weights)
         else:
             weights, indices = route(_gate_logits(x, self.gate), self.top_k, **how)
             y = kan_experts(x.bfloat16(), self.cheby_coeffs.bfloat16(), indices, weights).to(torch.float32)
@@ -378,14 +390,13 @@ class MixtureKANLayer(nn.Module):
         return y
 
     def _few(self, x: torch.Tensor) -> bool:
-        """Whether x is few rows as ``kan_mixture`` counts them: by its rule for bf16 coefficients, which has no limit for high
-        degrees (past that one its parts run in fp32 too, and casting all coefficients takes longer)."""
-        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+        """Whether x is for ``kan_mixture``. In bf16 mode by its rule for bf16 coefficients, which has no limit for high degrees: past
+        that one its parts run in fp32 too, and casting all coefficients takes longer."""
+        if torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or self.cheby_coeffs.requires_grad):
             return False
-        desc = _lib.CkanMixtureDesc(x.shape[0], self.experts, self.top_k, self.input_dim, self.output_dim, self.degree,
-                                    _SCORES[self.score], self.groups, self.top_groups, 1, 0, 0, _lib.CKAN_DTYPE_BF16,
-                                    self.scale)
-        return bool(_lib.load().ckan_mixture_few(desc))
+        code = _lib.CKAN_DTYPE_F32 if self.compute == "fp32" else _lib.CKAN_DTYPE_BF16
+        return _few_rows(x.shape[0], self.experts, self.top_k, self.input_dim, self.output_dim, self.degree,
+                         _SCORES[self.score], self.groups, self.top_groups, code)
 
     @torch.no_grad()
     def update_balance(self, speed: float = 1e-3) -> None:
