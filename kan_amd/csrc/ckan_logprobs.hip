@@ -11,9 +11,10 @@
 //   dl_j = dlogp (delta_jt - p_j) - dH p_j (log p_j + H).
 //
 // Bound by the bytes of the logits, read once (the likeliest classes' few chunks twice), the backward reading and
-// writing them once: 4000 rows of 50001 classes in bf16 82 us (4.9 TB/s) without and 90 with five likeliest classes, backward 169
-// (4.7); 65536 x 1000 in fp32 56 and 95 us (4.7 and 5.5 TB/s). One row of 131072 is two launches of a few microseconds
-// each: parts of the row, and their join.
+// writing them once. Four tensors in turn: 4000 rows of 50001 classes in bf16 78 to 86 us (4.7 to 5.1 TB/s) without and 87 with five
+// likeliest classes, backward 161 to 170 (4.7 to 5.0); in training steps, where it follows a backward that has just written 400
+// MB, the forward takes 117 to 119 (3.4). 65536 x 1000 in fp32 63 and 92 us (4.2 and 5.7 TB/s), in bf16 48 and 53 (2.7 and
+// 5.0). One row of 131072 is two launches of a few microseconds each: parts of the row, and their join.
 #include "ckan_block.hpp"
 #include "ckan_mix.hpp"
 
@@ -125,9 +126,10 @@ __device__ __forceinline__ void write_top(const LogpArgs& a, int64_t row, int j,
 }
 
 constexpr int kThreads = 256;
-// 16384 rows by a team and by a block: 3000 classes in fp32 59.5 and 61 us, with five likeliest 71 and 92, with twenty 111
-// and 129; 4096 classes in bf16 60.9 and 67.9, 70 and 85, 111 and 116. Only 4096 classes in fp32 without any are
-// better by a block (75.9 and 64.2; with five 82.6 and 94.5).
+// 16384 rows, one tensor again and again, by a team and by a block: 3000 classes in fp32 59.5 and 61 us, with five likeliest 71
+// and 92, with twenty 111 and 129; 4096 classes in bf16 60.9 and 67.9, 70 and 85, 111 and 116. Only 4096 classes in fp32 without
+// any are better by a block (75.9 and 64.2; with five 82.6 and 94.5). Four tensors in turn by a team: 74, 87 and 120 (3000 in
+// fp32), 59, 73 and 114 (4096 in bf16).
 constexpr int kTeamMaxClasses = 4096;
 
 // ---- up to kTeamMaxClasses: a row in the registers of a team of lanes ----------------

@@ -15,9 +15,9 @@
 //
 // Bound by the bytes: every tensor once, a row in the registers of a team of lanes between its sums (65536 x 512
 // in fp32, layer norms with biases and a gate a row: forward 130 us, backward 206, both 5.2 TB/s, the rate of a large
-// copy; 32768 x 1024 in bf16 60 and 98 us, 4.4 and 4.1 TB/s, by instructions too). Rows above 8192 values, whose sums
-// over rows and parameters fit neither registers nor LDS, and below 8 are read again for every sum (2048 x 16384 in fp32:
-// forward 175 us).
+// copy; 32768 x 1024 in bf16 60 and 98 us, 4.4 and 4.1 TB/s, by instructions too). Rows above 8192 values, a forward with
+// five parameters from 8153 on, and rows below 8 values are read again for every sum (2048 x 16384 in fp32: forward 170 to 178
+// us, backward 318 + 118; 65536 x 4, a block a row and one thread of it at work: 343 and 591 + 434).
 #include <type_traits>
 
 #include "ckan_block.hpp"
@@ -254,8 +254,8 @@ __global__ __launch_bounds__(kAnyThreads) void k_residual_any_dx(ResidualArgs a)
   }
 }
 
-// Sums over rows of the parameters' gradients: a thread a column chunk, a block 64
-// chunks by four rows at a time of its slab; partial sums [slab, 5, dim].
+// Sums over rows of the parameters' gradients: a thread a column chunk, the rows of its slab one
+// after another; partial sums [slab, 5, dim].
 constexpr int kSums = 5;  // dpost_w, dpost_b, dgate, dnext_w, dnext_b
 constexpr int kAnySlabs = 256;
 
@@ -412,8 +412,8 @@ struct RowAny {
 enum Param { kPostW, kPostB, kGate, kNextW, kNextB, kParams };
 //
 // A parameter takes two runs of 16 bytes a chunk: a chunk for every lane of the team, or, PACKED, the
-// row's chunks and one of zeros for the lanes past it, which lets five parameters of up to 6500 values
-// fit (and costs the backward registers that it does not have).
+// row's chunks and one of zeros for the lanes past it, which lets five parameters of up to 8152 values
+// fit into 159.5 KiB (and costs the backward registers that it does not have).
 template <int LANES, int N, bool PACKED>
 struct ParamTable {
   float* lds;
@@ -629,7 +629,9 @@ __global__ __launch_bounds__(BLOCK, 4) void k_residual_rows(ResidualArgs a) {
   }
 }
 
-// Waves a SIMD that the backward's registers leave room for.
+// Waves a SIMD that the backward's registers leave room for. The five sums over rows take 8 N registers each whether a call
+// has them all or not, and some forms keep values in scratch for it: of 4097 to 8192 values (512 lanes, N = 2) 304 to 384 bytes a lane, in
+// bf16 of 64 to 512 lanes 16 to 72, with a bf16 stream and an fp32 branch of 512 lanes 40, in fp32 of 512 lanes 24.
 __host__ __device__ constexpr int backward_waves(int lanes, int n) { return lanes < 64 || n > 1 ? 2 : 3; }
 
 // Its sums over rows a block leaves as a part of each, [block, 5, dim].
@@ -877,8 +879,8 @@ constexpr int kPartBlocks = 4;  // at most a CU: each leaves a part of every sum
 
 // The team of a width: a chunk a lane, so that a row is one batch of loads, up to eight rows a wave and 16 waves a
 // row. WIDE is that of the widest rows: in the backward half as many lanes, whose 256
-// registers hold two chunks and their sums (4096 x 8192 212 us in fp32 and 142 in bf16; 1024 lanes
-// of 128 registers 291 and 175).
+// registers hold two chunks and their sums, but for what goes to scratch (4096 x 8192 212 to 224 us in fp32 and 132 to 142 in
+// bf16; 1024 lanes of 128 registers 291 and 175).
 #define CKAN_TEAM(dim, F, WIDE)                 \
   do {                                          \
     if ((dim) <= 64) { F(8, 1, 256) }           \
