@@ -395,8 +395,8 @@ int ckan_experts_backward(const ckan_experts_desc* desc, const int64_t* indices,
 /* logits = x gate^T, ckan_route's choice and weights on them, and ckan_experts_forward's
  * sum, without a backward, for as few rows as the experts' coefficients are streamed for
  * (ckan_mixture_few: at most 1024 slots, fewer than 64 an expert on average, and of many fp32
- * coefficients of degree 9 and more at most 8 rows or at least 8 slots an expert).  The logits
- * are summed in 64 bits and rounded once to fp32, so that the choice does not hang on an order
+ * coefficients of degree 9 and more at most 8 rows of 64 slots or at least 8 slots an expert).
+ * The logits are summed in 64 bits and rounded once to fp32, so that the choice does not hang on an order
  * of sums.  x [rows, in] and y have x_dtype, gate [experts, in] and coeffs [experts, in, out,
  * degree + 1] a dtype each;
  * bias fp32 [experts] or NULL; weights fp32 and indices [rows, top_k] are outputs.  Buffers need

@@ -274,7 +274,7 @@ def kan_mixture(x: torch.Tensor, gate: torch.Tensor, coeffs: torch.Tensor, top_k
     ``x`` [rows, in], ``gate`` [experts, in] and ``coeffs`` [experts, in, out, degree+1] are fp32 or
     bf16 each; y [rows, out] has x's dtype, weights and indices are ``route``'s.  Few rows without a
     gradient (up to 1024 slots, fewer than 64 an expert on average; of many fp32 coefficients of degree
-    9 and more up to 8 rows, or from 8 slots an expert on) take a form of their own: the gate's sums in
+    9 and more up to 8 rows of 64 slots, or from 8 slots an expert on) take a form of their own: the gate's sums in
     64 bits, the chosen experts' coefficients read as they lie, x unrounded.  Otherwise the gate's
     product is torch's in fp32 and the rest is ``route`` and ``kan_experts`` (in fp32 unless x and coeffs
     are both bf16), differentiable as they are in x, gate and coeffs."""

@@ -27,6 +27,7 @@ def test_slots(args, taken):
     ((32, 12, 3, 300, 700, 16), 1), ((9, 12, 3, 300, 700, 16, 1), 1), ((9, 12, 3, 300, 700, 8), 1),
     ((16, 8, 2, 512, 512, 16), 0), ((16, 8, 2, 512, 512, 15), 0), ((16, 8, 2, 512, 512, 14), 1),
     ((16, 64, 2, 512, 512, 9), 0), ((16, 64, 2, 200, 200, 9), 1),
+    ((8, 128, 8, 256, 256, 16), 1), ((8, 128, 9, 256, 256, 16), 0), ((8, 128, 9, 300, 300, 16), 1),  # 64 slots, experts of 5 MiB
 ])
 def test_high_degrees(args, taken):
     assert few(*args) == taken
